@@ -36,9 +36,9 @@ def listed():
         dict(name="linear_1", op="linear", m=1, n=5120, k=8192, act="none", bias=False, residual=True, out="bf16"),
         # a serving batch through the query projection
         dict(name="linear_24", op="linear", m=24, n=32768, k=1280, act="none", bias=False, residual=False, out="bf16"),
-        # a small odd head: bias and activation, scores in 32 bits, nothing a multiple of a tile
+        # a small odd head: bias and activation, nothing a multiple of a tile
         dict(name="linear_301_odd", op="linear", m=301, n=1001, k=5120 - 96, act="gelu", bias=True, residual=False,
-             out="fp32"),
+             out="bf16"),
         # a prefill chunk's output projection with the residual
         dict(name="linear_4096", op="linear", m=4096, n=5120, k=8192, act="none", bias=False, residual=True, out="bf16"),
         # one token through the gate and up projections
@@ -63,7 +63,7 @@ def draw(rng):
         return dict(op=op, m=_log(rng, 1, 8192), d=32 * _log(rng, 4, 160), residual=rng.random() < 0.6)
     m, k = _log(rng, 1, 4096), 32 * _log(rng, 16, 256)
     if op == "linear":
-        out = rng.choice(["bf16", "bf16", "bf16", "fp32", "a8"])
+        out = rng.choice(["bf16", "bf16", "bf16", "a8"])
         n = _log(rng, 100, min(32768, 8192 * 5120 // k))
         if out == "a8" or rng.random() < 0.5:
             n = 32 * max(1, n // 32)
@@ -190,7 +190,7 @@ def _plain(s):
         y = _act(y, c["act"])
         if s["residual"] is not None:
             y = y + s["residual"].float()
-        return dict(zip(("codes", "scales"), _quant(y))) if c["out"] == "a8" else dict(y=y if c["out"] == "fp32" else y.to(BF))
+        return dict(zip(("codes", "scales"), _quant(y))) if c["out"] == "a8" else dict(y=y.to(BF))
     if c["op"] == "gated":
         y = _gated(_activation(s["a8"], s["s8"]), s["gate"], s["up"], c["act"], c["limit"])
         return dict(zip(("codes", "scales"), _quant(y))) if c["out"] == "a8" else dict(y=y.to(BF))
@@ -219,7 +219,7 @@ def run(s):
         return dict(_parts(q), h=h)
     if c["op"] == "linear":
         y = linear_a8(A8(s["a8"], s["s8"]), W8(*s["w"], permuted=True), bias=s["bias"], act=c["act"],
-                      residual=s["residual"], out={"bf16": BF, "fp32": torch.float32, "a8": A8}[c["out"]])
+                      residual=s["residual"], out=A8 if c["out"] == "a8" else BF)
         return _parts(y) if c["out"] == "a8" else dict(y=y)
     if c["op"] == "gated":
         y = gated_a8(A8(s["a8"], s["s8"]), W8(*s["gate"], permuted=True), W8(*s["up"], permuted=True), act=c["act"],
@@ -240,7 +240,7 @@ def work(case):
         return dict(bytes=m * d * (6 if case["residual"] else 2) + a8(m, d) + 2 * d, flops=6 * m * d)
     n, k = case["n"], case["k"]
     if op == "linear":
-        size = {"bf16": 2, "fp32": 4, "a8": 33 / 32}[case["out"]]
+        size = 33 / 32 if case["out"] == "a8" else 2
         by = a8(m, k) + w8(n, k) + m * n * (size + 2 * case["residual"]) + 2 * n * case["bias"]
         return dict(bytes=by, flops=2 * m * n * k)
     if op == "gated":
