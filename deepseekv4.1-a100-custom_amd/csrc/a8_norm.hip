@@ -1,0 +1,151 @@
+// norm_quant8: the residual's addition, the root-mean-square norm and the block quantisation in one pass,
+//   h = bf16(x + r);  y = h / sqrt(mean(h^2) + eps) * w;  codes and scales of y (a8_core.h).
+// y stays in 32 bits up to its one rounding, to 8 bits (norm_quant rounds to bf16 in between, as the reference does);
+// the norm is that of the bf16 stream, whose readers see what was normed.  Without w: the quantisation alone.
+//
+// Bound: HBM, 2 bytes a value in (4 with r) and 1 + 1/32 out (3 + 1/32 with h).  A lane holds 8 adjacent values (16-byte
+// loads, all of a row's in flight at once), so a row is read once and a block is 4 lanes; its codes leave as 8 bytes a
+// lane after one exchange with the neighbour.
+#include "a8_core.h"
+#include "rowop.h"
+
+namespace {
+
+struct NormArgs {
+  const uint16_t *x, *r, *w;
+  float eps;
+  uint16_t* h;
+  uint8_t *a8, *s8;
+  long rows;
+  int D;
+};
+
+
+DSV41_DEV void norm_unpack(uint4 q, float (&v)[8]) {
+  const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(u[i] << 16);
+    v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+  }
+}
+
+// One row by nt lanes (t: this lane's number); red: the workgroup's exchange, null where a row is one wave's.
+template <int IT, bool BLOCK>
+DSV41_DEV void norm_row(const NormArgs& a, long row, bool live, int t, int nt, float* red) {
+  const int nc = a.D / 8;
+  const long base = row * a.D;
+  uint4 xq[IT], rq[IT], wq[IT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    const int c = min(t + i * nt, nc - 1);  // (lanes past the row load its last chunk and store nothing)
+    xq[i] = ((const uint4*)(a.x + base))[c];
+    if (a.r) rq[i] = ((const uint4*)(a.r + base))[c];
+    if (a.w) wq[i] = ((const uint4*)a.w)[c];
+  }
+  float v[IT][8];
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    const bool in = live && t + i * nt < nc;
+    norm_unpack(xq[i], v[i]);
+    if (a.r) {
+      float r[8];
+      norm_unpack(rq[i], r);
+      uint32_t u[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) u[k] = a8_bf16x2(v[i][2 * k] + r[2 * k], v[i][2 * k + 1] + r[2 * k + 1]);
+      const uint4 hq = make_uint4(u[0], u[1], u[2], u[3]);
+      if (in) ((uint4*)(a.h + base))[t + i * nt] = hq;
+      norm_unpack(hq, v[i]);
+    }
+    if (in) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) ss = __builtin_fmaf(v[i][k], v[i][k], ss);
+    }
+  }
+  if (a.w) {
+    ss = wave_sum(ss);
+    if constexpr (BLOCK) {
+      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = ss;
+      __syncthreads();
+      ss = 0.0f;
+      for (int k = 0; k < nt / 64; ++k) ss += red[k];
+    }
+    const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)a.D) + a.eps));
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      float w[8];
+      norm_unpack(wq[i], w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[i][k] = v[i][k] * inv * w[k];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    const int c = t + i * nt;
+    int top = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = max(top, a8_abs_bits(v[i][k]));
+    top = max(top, dpp_movi<0xB1>(top));
+    top = max(top, dpp_movi<0x4E>(top));
+    const int s = a8_scale(top);
+    const float inv = a8_inv(s);
+    const uint32_t lo = a8_pack4(v[i][0], v[i][1], v[i][2], v[i][3], inv, s == 255);
+    const uint32_t hi = a8_pack4(v[i][4], v[i][5], v[i][6], v[i][7], inv, s == 255);
+    // words of 16 codes in the byte order: {0 1 8 9} {2 3 10 11} {4 5 12 13} {6 7 14 15}; the even lane has 0..7 and
+    // writes the first two, the odd one 8..15 and the last two
+    const bool odd = t & 1;
+    const uint32_t got = (uint32_t)dpp_movi<0xB1>((int)(odd ? lo : hi));
+    const uint32_t p = odd ? got : lo, q = odd ? hi : got;  // codes 0..3 or 4..7, and 8..11 or 12..15
+    if (live && c < nc) {
+      *(uint2*)(a.a8 + base + 8 * c) = make_uint2((p & 0xffffu) | (q << 16), (p >> 16) | (q & 0xffff0000u));
+      if ((c & 3) == 0) {
+        const int b = c >> 2;
+        uint8_t* sp = a.s8 + ((long)(b >> 2) * a.rows + row) * 4 + (b & 3);
+        *sp = (uint8_t)s;
+        if (b == nc / 4 - 1)
+          for (int k = (b & 3) + 1; k < 4; ++k) *++sp = 127;
+      }
+    }
+  }
+}
+
+// A row a workgroup (its threads: the row's chunks, rounded up to whole waves, at most 1024).
+template <int IT>
+__global__ void __launch_bounds__(1024) norm_quant8_block_kernel(const NormArgs a) {
+  __shared__ float red[16];
+  norm_row<IT, true>(a, blockIdx.x, true, threadIdx.x, blockDim.x, red);
+}
+
+// A row a wave, four to a workgroup.
+template <int IT>
+__global__ void __launch_bounds__(256) norm_quant8_wave_kernel(const NormArgs a) {
+  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  norm_row<IT, false>(a, min(row, a.rows - 1), row < a.rows, threadIdx.x & 63, 64, nullptr);
+}
+
+}  // namespace
+
+extern "C" int dsv41_norm_quant8(const void* x, const void* residual, const void* w, float eps, void* h, void* a8,
+                                 void* s8, long n_rows, int D, void* stream) {
+  if (n_rows <= 0) return 0;
+  if (D <= 0 || D % 32 != 0 || D > 16384 || n_rows > 0x7fffffffl || (residual && !h)) return (int)hipErrorInvalidValue;
+  if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)w | (uintptr_t)h | (uintptr_t)a8) & 15)
+    return (int)hipErrorInvalidValue;
+  const NormArgs a{(const uint16_t*)x, (const uint16_t*)residual, (const uint16_t*)w, eps, (uint16_t*)h,
+                   (uint8_t*)a8, (uint8_t*)s8, n_rows, D};
+  const hipStream_t st = (hipStream_t)stream;
+  if (D <= 2048) {
+    const dim3 g((unsigned)((n_rows + 3) / 4));
+    if (D <= 512) norm_quant8_wave_kernel<1><<<g, 256, 0, st>>>(a);
+    else if (D <= 1024) norm_quant8_wave_kernel<2><<<g, 256, 0, st>>>(a);
+    else norm_quant8_wave_kernel<4><<<g, 256, 0, st>>>(a);
+  } else {
+    const int nc = D / 8, nt = nc <= 1024 ? (nc + 63) / 64 * 64 : (nc / 2 + 63) / 64 * 64;
+    if (nc <= 1024) norm_quant8_block_kernel<1><<<(unsigned)n_rows, nt, 0, st>>>(a);
+    else norm_quant8_block_kernel<2><<<(unsigned)n_rows, nt, 0, st>>>(a);
+  }
+  DSV41_CHECK_LAUNCH();
+  return 0;
+}

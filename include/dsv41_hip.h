@@ -319,6 +319,39 @@ int dsv41_fp8_gemm(const void* x, long ldx, const void* w8, const void* s8, int 
 int dsv41_fp8_gemv_m1_pre(const void* x_raw, const void* norm_w, float eps, int mode, const void* w8, const void* s8,
                           int N, int K, int Kc, void* out, void* ws, long ws_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------------ 8-bit activations */
+
+/* Activations in 8 bits (the twin of the W8 weights): codes e4m3 [rows, K], every 16 of a row in the PERM_K byte order;
+ * scales E8M0 [ceil(K / 128)][rows][4], byte j of word (c, row) for values 128 c + 32 j .. + 31 of the row, 127 behind
+ * the last block.  Per block s = 2^ceil(log2(max(amax, 1e-4) / 448)), code = e4m3(v / s) (the grid of fake_quant_fp8,
+ * dsv41/quant.py:45-72); a block with an infinity or a NaN: scale 255, NaN codes.  Codes 16-byte, scales 4-byte aligned.
+ *
+ * norm_quant8: h = bf16(x + residual) (residual null: h = x, nothing stored), y = h / sqrt(mean(h^2) + eps) * w (w null:
+ * y = h) in fp32, codes and scales of y.  x, residual, h bf16 [n_rows, D] and w bf16 [D], 16-byte aligned, D % 32 == 0,
+ * D <= 16384.  The residual's addition and rmsnorm in front of fused2.norm_quant (dsv41/fused2.py:251-272). */
+int dsv41_norm_quant8(const void* x, const void* residual, const void* w, float eps, void* h, void* a8, void* s8,
+                      long n_rows, int D, void* stream);
+
+/* Workspace bytes of dsv41_linear_a8 (gated 0) or dsv41_gated_a8 (gated 1): 0, or the fp32 partials of K slices.  It
+ * need not be initialised and holds nothing between calls; 16-byte aligned. */
+long dsv41_a8_workspace_bytes(int M, int N, int K, int gated);
+
+/* y[m, n] = act(sum_k x[m, k] w[n, k] + bias[n]) + residual[m, n]: x 8-bit activations [M, K], w e4m3 [N, K] in the
+ * PERM_K byte order (16-byte aligned) with E8M0 scales [ceil(N / 32), Kc], Kc >= K / 32 (dsv41/w8.py:39-60); K % 32 == 0.
+ * bias bf16 or (bias_f32) fp32 [N] or null; act 0 none, 1 relu, 2 silu, 3 gelu (erf), 4 gelu by tanh; residual bf16
+ * [M, N] or null.  Exactly one output: out bf16 [M, N], or (out null) out_a8 / out_s8, the result as 8-bit activations,
+ * N % 32 == 0.  fp32 sums on the block-scaled fp8 matrix instructions (2^-16 relative), rounded once.  Replaces
+ * cukern.fp8_gemm_tc (dsv41/cukern.py:164-200) where x is held in 8 bits. */
+int dsv41_linear_a8(const void* a8, const void* s8, const void* w8, const void* ws8, int M, int N, int K, int Kc,
+                    const void* bias, int bias_f32, int act, const void* residual, void* out, void* out_a8,
+                    void* out_s8, void* ws, long ws_bytes, void* stream);
+
+/* y = act(min(x Wg^T, limit)) * clamp(x Wu^T, -limit, limit) (limit 0: as they are), operands, act and outputs as
+ * dsv41_linear_a8; wg8, wu8 [N, K] with scales of Kcg and Kcu columns. */
+int dsv41_gated_a8(const void* a8, const void* s8, const void* wg8, const void* wgs8, const void* wu8,
+                   const void* wus8, int M, int N, int K, int Kcg, int Kcu, int act, float limit, void* out,
+                   void* out_a8, void* out_s8, void* ws, long ws_bytes, void* stream);
+
 /* ------------------------------------------------------------------------------------------------ numerics */
 
 /* norm_quant (dsv41/fused2.py:251-272): per row of D bf16 values (D % 32 == 0, D <= 16384; x and y 16-byte aligned,

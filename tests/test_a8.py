@@ -1,0 +1,126 @@
+"""8-bit activations without a GPU: the container, the refusals of the shims and of the C entry points."""
+import ctypes
+
+import pytest
+import torch
+
+from dsv41_amd import A8, GatedFeedForward, gated_a8, linear_a8, norm_quant8
+from dsv41_amd._lib import lib
+from dsv41_amd.w8 import W8
+
+import _a8_ref as R
+
+
+def _a8(rows, k, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    y = torch.randn(rows, k, generator=g, dtype=torch.float64)
+    codes, s = R.quantised(y)
+    return A8(R.permuted(codes), R.pack_scales(s))
+
+
+def _w8(n, k):
+    return W8(torch.zeros(n, k, dtype=torch.uint8), torch.full(((n + 31) // 32, k // 32), 127, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("k", [32, 96, 128, 160, 512])
+def test_container_values(k):
+    q = _a8(5, k)
+    assert q.shape == (5, k) and q.s8.shape == ((k + 127) // 128, 5, 4)
+    v = R.a8_values(q.a8, q.s8)
+    assert torch.equal(q.float().double(), v) and torch.equal(q.bf16().double(), v)
+    assert torch.equal(q.scales(), R.unpack_scales(q.s8, k))
+
+
+def test_container_keeps_leading_sizes_and_nan_blocks():
+    q = _a8(6, 64)
+    q.s8[0, 2, 1] = 255
+    r = A8(q.a8, q.s8, (2, 3, 64))
+    v = r.float()
+    assert v.shape == (2, 3, 64) and v[0, 2, 32:].isnan().all() and v.isnan().sum() == 32
+
+
+def test_container_refusals():
+    u = lambda *s: torch.zeros(*s, dtype=torch.uint8)  # noqa: E731
+    for a, s in [(u(4, 40), u(1, 4, 4)), (u(4, 64), u(4, 2)), (u(4, 64), u(2, 4, 4)), (u(4, 64).float(), u(1, 4, 4)),
+                 (u(64), u(1, 1, 4)), (u(4, 64), u(1, 4, 4).int())]:
+        with pytest.raises(ValueError):
+            A8(a, s)
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="GPU"):
+        norm_quant8(x, x[0], 1e-6)
+    with pytest.raises(RuntimeError, match="GPU"):
+        linear_a8(_a8(2, 64), _w8(32, 64))
+    with pytest.raises(RuntimeError, match="GPU"):
+        gated_a8(_a8(2, 64), _w8(32, 64), _w8(32, 64))
+    with pytest.raises(TypeError):
+        linear_a8(x, _w8(32, 64))
+    with pytest.raises(TypeError):
+        linear_a8(_a8(2, 64), x)
+
+
+def test_feed_forward_refuses_sizes_that_do_not_fit():
+    n = torch.ones(64)
+    GatedFeedForward(n, _w8(96, 64), _w8(96, 64), _w8(64, 96))
+    for bad in [(n, _w8(96, 64), _w8(32, 64), _w8(64, 96)), (n, _w8(96, 64), _w8(96, 64), _w8(96, 64)),
+                (n[:32], _w8(96, 64), _w8(96, 64), _w8(64, 96)), (n, _w8(100, 64), _w8(100, 64), _w8(64, 100 // 32 * 32))]:
+        with pytest.raises(ValueError):
+            GatedFeedForward(*bad)
+    with pytest.raises(ValueError):
+        GatedFeedForward(n, _w8(96, 64), _w8(96, 64), _w8(64, 96), act="swish")
+
+
+# Addresses are never read by a refused call: any aligned number will do.
+P = 1 << 20
+
+
+def _norm(x=P, r=None, w=P, h=None, a8=P, s8=P, rows=4, D=64):
+    return lib().dsv41_norm_quant8(x, r, w, 1e-6, h, a8, s8, rows, D, None)
+
+
+def test_norm_entry_refusals():
+    assert _norm(rows=0) == 0
+    for bad in [dict(D=0), dict(D=48), dict(D=16416), dict(D=-32), dict(x=P + 8), dict(w=P + 2), dict(a8=P + 4),
+                dict(r=P), dict(r=P + 8, h=P), dict(r=P, h=P + 2), dict(rows=1 << 40)]:
+        assert _norm(**bad) == 1, bad
+
+
+def _linear(x=P, xs=P, w=P, ws=P, M=4, N=64, K=64, Kc=2, bias=None, bf=0, act=0, res=None, out=P, oa=None, os=None,
+            work=None, n=0):
+    return lib().dsv41_linear_a8(x, xs, w, ws, M, N, K, Kc, bias, bf, act, res, out, oa, os, work, n, None)
+
+
+def _gated(x=P, xs=P, g=P, gs=P, u=P, us=P, M=4, N=64, K=64, Kg=2, Ku=2, act=2, limit=0.0, out=P, oa=None, os=None,
+           work=None, n=0):
+    return lib().dsv41_gated_a8(x, xs, g, gs, u, us, M, N, K, Kg, Ku, act, limit, out, oa, os, work, n, None)
+
+
+def test_product_entry_refusals():
+    for f in (_linear, _gated):
+        assert f(M=0) == 0 and f(N=0) == 0
+        for bad in [dict(M=-1), dict(N=-1), dict(K=0), dict(K=48), dict(x=P + 8), dict(xs=P + 1), dict(act=5),
+                    dict(act=-1), dict(out=None), dict(out=None, oa=P), dict(out=None, oa=P, os=P, N=40),
+                    dict(out=None, oa=P + 8, os=P)]:
+            assert f(**bad) == 1, (f.__name__, bad)
+    for bad in [dict(w=P + 8), dict(Kc=1)]:
+        assert _linear(**bad) == 1, bad
+    for bad in [dict(g=P + 8), dict(u=P + 8), dict(u=None), dict(us=None), dict(Kg=1), dict(Ku=1), dict(limit=-1.0),
+                dict(limit=float("nan"))]:
+        assert _gated(**bad) == 1, bad
+
+
+def test_workspace_is_of_the_call_and_asked_for():
+    """K slices need their partials: whole rows of 32-column blocks (twice for gate and up), none for few or many rows."""
+    L = lib()
+    assert L.dsv41_a8_workspace_bytes(1, 5120, 8192, 0) == 0 and L.dsv41_a8_workspace_bytes(0, 5120, 8192, 0) == 0
+    assert L.dsv41_a8_workspace_bytes(8192, 5120, 8192, 0) == 0
+    for gated in (0, 1):
+        n = L.dsv41_a8_workspace_bytes(130, 1000, 5120, gated)
+        assert n > 0 and n % (130 * 1024 * (1 + gated) * 4) == 0
+    n = L.dsv41_a8_workspace_bytes(130, 1000, 5120, 0)
+    args = dict(M=130, N=1000, K=5120, Kc=160)
+    for bad in [dict(work=None, n=n), dict(work=P, n=n - 1), dict(work=P + 4, n=n)]:
+        assert _linear(**args, **bad) == 1, bad
+    assert isinstance(n, int) and ctypes.sizeof(ctypes.c_long) == 8
