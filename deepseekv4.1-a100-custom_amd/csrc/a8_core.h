@@ -42,13 +42,9 @@ DSV41_DEV uint32_t a8_bf16x2(float a, float b) {  // nearest, ties to even
 // ---- activations
 constexpr int kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4;
 
-// exp(x) to about 2 ulp: 2^(x log2 e) with the product's rounding error carried into the result.
-DSV41_DEV float a8_exp(float x) {
-  const float t = x * kLog2e;
-  const float lo = __builtin_fmaf(x, kLog2e, -t) + x * 1.925963033e-8f;  // (log2 e = kLog2e + 1.92596e-8)
-  const float e = __builtin_amdgcn_exp2f(t);
-  return fabsf(t) < 126.0f ? __builtin_fmaf(e, lo * 0.6931471806f, e) : e;  // (beyond: e is or nears 0 or infinity)
-}
+// e^x: the argument's rounding makes it |x| 2^-24 off (5e-6 at the ends of the range), far below half a step of the
+// outputs, bf16 and e4m3.
+DSV41_DEV float a8_exp(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 // silu(v) = v / (1 + e^-v); gelu_tanh(v) = v / (1 + e^(-2 c (v + 0.044715 v^3))), c = sqrt(2 / pi): 1/2 (1 + tanh z) is
 // 1 / (1 + e^-2z).  gelu(v) = v Phi(v), Phi(-a) = e^(-a^2 / 2) R(1 / (1 + 0.35 a)): R a polynomial of degree 7 fitted to
 // erfcx(a / sqrt 2) / 2 over a <= 14 for the relative error (3.1e-7), so that the tail keeps its digits.
@@ -75,6 +71,7 @@ DSV41_DEV float a8_act(float v, int act) {
 }
 
 // ---- epilogue: y = act(sum + bias) + residual, or act(min(gate, limit)) * clamp(up, -limit, limit)
+// A lane has 8 adjacent columns of a row, n % 8 == 0: 16 bytes of bf16, 8 of codes, a quarter of a block.
 struct A8Epi {
   const void* bias;  // [N] or null
   int bias_f32;
@@ -84,67 +81,67 @@ struct A8Epi {
   uint16_t* out;      // bf16 [M, N], or null:
   uint8_t *oa8, *os8; // codes [M, N] and scales
   int M, N;
-  int vec;            // N % 4 == 0, out / res 8-byte aligned, fp32 bias 16-byte
+  int vec;            // rows of out and res in whole 16-byte units
+};
+struct alignas(16) A8x8 {
+  float v[8];
 };
 
-DSV41_DEV float a8_gate(const A8Epi& e, float g, float u) {
-  if (e.limit > 0.0f) {  // (comparisons, not fminf: a NaN stays)
-    g = g > e.limit ? e.limit : g;
-    u = u > e.limit ? e.limit : u < -e.limit ? -e.limit : u;
+DSV41_DEV void a8_unpack8(uint4 q, float (&v)[8]) {
+  const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(u[i] << 16);
+    v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
   }
-  return a8_act(g, e.act) * u;
 }
-
-// Columns n .. n + 3 of row m (m < M), bias, activation and residual applied.
-template <bool GATED>
-DSV41_DEV f32x4_t a8_finish4(const A8Epi& e, f32x4_t v, f32x4_t u, int m, int n) {
-  if constexpr (GATED) {
+DSV41_DEV uint4 a8_pack8(const float (&v)[8]) {
+  return make_uint4(a8_bf16x2(v[0], v[1]), a8_bf16x2(v[2], v[3]), a8_bf16x2(v[4], v[5]), a8_bf16x2(v[6], v[7]));
+}
+// Columns n .. n + 7 of the bias, 0 behind the last and without one.
+DSV41_DEV A8x8 a8_bias8(const A8Epi& e, int n) {
+  A8x8 b;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = a8_gate(e, v[i], u[i]);
-    return v;
-  }
-  const bool whole = e.vec && n < e.N;
-  if (e.bias) {
-    if (whole && e.bias_f32) {
-      v += *(const f32x4_t*)((const float*)e.bias + n);
-    } else if (whole) {
-      const uint2 b = *(const uint2*)((const uint16_t*)e.bias + n);
-      v += f32x4_t{__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u), __uint_as_float(b.y << 16),
-                   __uint_as_float(b.y & 0xffff0000u)};
-    } else {
+  for (int i = 0; i < 8; ++i)
+    b.v[i] = !e.bias || n + i >= e.N ? 0.0f : e.bias_f32 ? ((const float*)e.bias)[n + i] : bf2f(((const uint16_t*)e.bias)[n + i]);
+  return b;
+}
+// The residual's columns n .. n + 7 of row m, as loaded (a conversion here would wait for it).
+DSV41_DEV uint4 a8_res8(const A8Epi& e, int m, int n) {
+  uint4 q = make_uint4(0, 0, 0, 0);
+  if (!e.res || m >= e.M || n >= e.N) return q;
+  const uint16_t* r = e.res + (long)m * e.N + n;
+  if (e.vec) return *(const uint4*)r;
+  uint32_t u[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < e.N) v[i] += e.bias_f32 ? ((const float*)e.bias)[n + i] : bf2f(((const uint16_t*)e.bias)[n + i]);
-    }
-  }
+  for (int i = 0; i < 8; ++i)
+    if (n + i < e.N) u[i >> 1] |= (uint32_t)r[i] << (16 * (i & 1));
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+DSV41_DEV void a8_linear8(const A8Epi& e, A8x8& y, const A8x8& bias, uint4 res) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y.v[i] += bias.v[i];
   if (e.act != kActNone) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = a8_act(v[i], e.act);
+    for (int i = 0; i < 8; ++i) y.v[i] = a8_act(y.v[i], e.act);
   }
   if (e.res) {
-    const uint16_t* r = e.res + (long)m * e.N + n;
-    if (whole) {
-      const uint2 b = *(const uint2*)r;
-      v += f32x4_t{__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u), __uint_as_float(b.y << 16),
-                   __uint_as_float(b.y & 0xffff0000u)};
-    } else {
+    float r[8];
+    a8_unpack8(res, r);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < e.N) v[i] += bf2f(r[i]);
+    for (int i = 0; i < 8; ++i) y.v[i] += r[i];
+  }
+}
+DSV41_DEV void a8_gated8(const A8Epi& e, A8x8& g, A8x8& u) {
+  if (e.limit > 0.0f) {  // (comparisons, not fminf: a NaN stays)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      g.v[i] = g.v[i] > e.limit ? e.limit : g.v[i];
+      u.v[i] = u.v[i] > e.limit ? e.limit : u.v[i] < -e.limit ? -e.limit : u.v[i];
     }
   }
-  return v;
-}
-
-DSV41_DEV void a8_store4(const A8Epi& e, f32x4_t v, int m, int n) {
-  uint16_t* o = e.out + (long)m * e.N + n;
-  if (e.vec && n < e.N) {
-    *(uint2*)o = make_uint2(a8_bf16x2(v[0], v[1]), a8_bf16x2(v[2], v[3]));
-  } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < e.N) o[i] = (uint16_t)a8_bf16x2(v[i], 0.0f);
-  }
+  for (int i = 0; i < 8; ++i) g.v[i] = a8_act(g.v[i], e.act) * u.v[i];
 }
 
 DSV41_DEV long a8_scale_at(int M, int m, int block) { return ((long)(block >> 2) * M + m) * 4 + (block & 3); }
@@ -156,22 +153,48 @@ DSV41_DEV void a8_store_scale(const A8Epi& e, int m, int block, int byte) {
     for (int b = (block & 3) + 1; b < 4; ++b) *++s = 127;
 }
 
-// Codes and scale of a block of 32 columns held by 8 adjacent lanes (lane a: columns 4 a .. 4 a + 3 from n).  Every lane
-// of the group must call it; valid is the group's.  In the byte order a lane's first two codes and those of the lane two
-// on are one word, its last two and theirs another: lane a of four writes word 2 (a & 1) + (a >> 1).
-DSV41_DEV void a8_store_block8(const A8Epi& e, f32x4_t v, int m, int n, bool valid) {
-  int top = max(max(a8_abs_bits(v[0]), a8_abs_bits(v[1])), max(a8_abs_bits(v[2]), a8_abs_bits(v[3])));
-  top = max(top, dpp_movi<0xB1>(top));
-  top = max(top, dpp_movi<0x4E>(top));
-  top = max(top, dpp_movi<0x141>(top));
-  const int s = a8_scale(top);
-  const uint32_t c = a8_pack4(v[0], v[1], v[2], v[3], a8_inv(s), s == 255);
-  const uint32_t p = (uint32_t)dpp_movi<0x4E>((int)c);  // lane a ^ 2
-  const int a = (n >> 2) & 3;
-  const uint32_t w = a < 2 ? (c & 0xffffu) | (p << 16) : (p >> 16) | (c & 0xffff0000u);
-  if (!valid) return;
-  *(uint32_t*)(e.oa8 + (long)m * e.N + (n & ~15) + 4 * (2 * (a & 1) + (a >> 1))) = w;
-  if (((n >> 2) & 7) == 0) a8_store_scale(e, m, n >> 5, s);
+// The codes of a lane's 8 of 16 values in the byte order's words {0 1 8 9} {2 3 10 11} {4 5 12 13} {6 7 14 15}: the even
+// lane has 0..7 and gets the first two words, the odd one 8..15 and the last two; one exchange with the neighbour.
+DSV41_DEV uint2 a8_words(uint32_t lo, uint32_t hi, bool odd) {
+  const uint32_t got = (uint32_t)dpp_movi<0xB1>((int)(odd ? lo : hi));
+  const uint32_t p = odd ? got : lo, q = odd ? hi : got;
+  return make_uint2((p & 0xffffu) | (q << 16), (p >> 16) | (q & 0xffff0000u));
+}
+// Codes and scale byte of 8 of a block's 32 values, the block in 4 adjacent lanes (all of them must call it).
+DSV41_DEV uint2 a8_quant8(const float (&v)[8], bool odd, int* scale) {
+  float top = 0.0f;  // (the maximum that keeps a NaN)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = __builtin_elementwise_maximum(top, fabsf(v[i]));
+  int t = __float_as_int(top) & 0x7fffffff;
+  t = max(t, dpp_movi<0xB1>(t));
+  t = max(t, dpp_movi<0x4E>(t));
+  const int s = a8_scale(t);
+  const float inv = a8_inv(s);
+  *scale = s;
+  return a8_words(a8_pack4(v[0], v[1], v[2], v[3], inv, s == 255), a8_pack4(v[4], v[5], v[6], v[7], inv, s == 255), odd);
+}
+
+// A lane's 8 columns n .. n + 7 of row m to the output.  Every lane of a wave calls it; live: m < M and n < N.
+DSV41_DEV void a8_store8(const A8Epi& e, const A8x8& y, int m, int n, bool live) {
+  if (e.out) {
+    if (!live) return;
+    uint16_t* o = e.out + (long)m * e.N + n;
+    const uint4 q = a8_pack8(y.v);
+    if (e.vec) {
+      *(uint4*)o = q;
+    } else {
+      const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n + i < e.N) o[i] = (uint16_t)(u[i >> 1] >> (16 * (i & 1)));
+    }
+    return;
+  }
+  int s;
+  const uint2 w = a8_quant8(y.v, (n >> 3) & 1, &s);
+  if (!live) return;
+  *(uint2*)(e.oa8 + (long)m * e.N + n) = w;
+  if ((n & 31) == 0) a8_store_scale(e, m, n >> 5, s);
 }
 
 }  // namespace

@@ -10,11 +10,11 @@
 // Sums over k are fp32, in a fixed order.
 //
 // The weights are the instruction's row operand: a lane ends with 4 adjacent columns of a row of y.
+#include <type_traits>
+
 #include "a8_core.h"
 
 namespace {
-
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 struct A8Args {
   const uint8_t *x, *xs;      // codes [M, K], scales [ceil(K / 128)][M][4]
@@ -23,6 +23,7 @@ struct A8Args {
   int M, N, K, Kc, Kc2;
   A8Epi e;
   int mtiles, ntiles;
+  int words;                  // weight scales in whole words: K % 128 == 0, rows 4-byte aligned
   int splits, kslice;         // K slices of kslice steps of 128 k; more than one: partials
   float* part;                // [splits][M][ldp], ldp = ceil(N / 32) * 32 (gated: twice, up behind gate)
   long ldp;
@@ -128,22 +129,26 @@ __global__ void __launch_bounds__(512) a8_stream_kernel(const A8Args a) {
 #pragma unroll
     for (int j = 0; j < MT; ++j) *(f32x4_t*)(red + (((long)wave * WT + i) * MT + j) * 256 + lane * 4) = acc[i][j];
   __syncthreads();
-  constexpr int QN = 4 * CT;  // lanes of a row: 4 columns each
-  for (int t = tid; t < QN * 16 * MT; t += blockDim.x) {
-    const int c = t % QN, m = t / QN, n = n0 + 4 * c;
-    const float* p = red + ((c >> 2) * MT + (m >> 4)) * 256 + ((c & 3) * 16 + (m & 15)) * 4;
-    f32x4_t v = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, u = v;
-    for (int w = 0; w < nw; ++w) {
-      v += *(const f32x4_t*)(p + w * (WT * MT * 256));
-      if constexpr (GATED) u += *(const f32x4_t*)(p + (w * WT + CT) * MT * 256);
-    }
+  constexpr int QN = 2 * CT;  // lanes of a row: 8 columns each
+  for (int t = tid; t < QN * 16 * MT; t += blockDim.x) {  // (in whole quads of lanes: a block of 32 columns with CT 2)
+    const int c = t % QN, m = t / QN, n = n0 + 8 * c;
+    const float* p = red + ((c >> 1) * MT + (m >> 4)) * 256 + ((c & 1) * 32 + (m & 15)) * 4;  // the next 4: lanes on 16
     const bool live = m < a.M && n < a.N;
-    if (live) v = a8_finish4<GATED>(a.e, v, u, m, n);
-    if (a.e.out) {
-      if (live) a8_store4(a.e, v, m, n);
-    } else if constexpr (CT == 2) {  // (whole groups of 8 lanes run the loop together: 8 * 16 * MT of them, N % 32 == 0)
-      a8_store_block8(a.e, v, m, n, live);
+    const uint4 res = a8_res8(a.e, m, n);
+    const A8x8 bias = a8_bias8(a.e, n);
+    A8x8 y, u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y.v[i] = u.v[i] = 0.0f;
+    for (int w = 0; w < nw; ++w) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y.v[i] += p[w * (WT * MT * 256) + (i >> 2) * 64 + (i & 3)];
+        if constexpr (GATED) u.v[i] += p[(w * WT + CT) * MT * 256 + (i >> 2) * 64 + (i & 3)];
+      }
     }
+    if constexpr (GATED) a8_gated8(a.e, y, u);
+    else a8_linear8(a.e, y, bias, res);
+    a8_store8(a.e, y, m, n, live);
   }
 }
 
@@ -158,85 +163,86 @@ DSV41_DEV void a8_dma4(const void* base, uint32_t off, uint32_t lds_addr) {
   asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory", "m0");
 }
 
+constexpr int kA8Strip = 4;
 constexpr int kA8SliceSteps = 128;  // a K slice's steps of 128 k at most: its weight scales are held in LDS
 
-// One 32 x 32 block of sums: lane (m = lane & 31, g = lane >> 5) holds row m, columns 8 q + 4 g + i in v[4 q + i].
-template <bool GATED>
-DSV41_DEV void a8_tile_out(const A8Args& a, const f32x16_t& v, const f32x16_t& u, int m, int n, int g) {
-  if (a.splits > 1) {
-    if (m < a.M && n < a.N) {
-      float* p = a.part + ((long)blockIdx.y * a.M + m) * a.ldp + n + 4 * g;
+// Output of a wave's ROWS x OCW block of sums from LDS (fp32, row stride LD bytes): rolled, so that bias, activation and
+// quantisation stand there once (unrolled over the accumulators they were 100 KB of code); the residual of U passes is
+// loaded before any of them is stored.
+template <int ROWS, int LD, int OCW, bool GATED>
+DSV41_DEV void a8_wave_out(const A8Args& a, const uint8_t* s, int m0, int n0) {
+  constexpr int QN = OCW / 8, RP = 64 / QN, PASSES = ROWS / RP, U = PASSES < 8 ? PASSES : 8;  // lanes of a row, rows of a pass
+  static_assert(ROWS % RP == 0 && PASSES % U == 0, "whole passes");
+  const int lane = threadIdx.x & 63, c = lane % QN * 8, n = n0 + c;
+  s += (lane / QN) * LD + (GATED ? (c / 32 * 64 + c % 32) * 4 : c * 4);
+  const A8x8 bias = a8_bias8(a.e, n);
+#pragma unroll 1
+  for (int r0 = 0; r0 < ROWS; r0 += U * RP) {
+    uint4 res[U];
+    if constexpr (!GATED) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        *(f32x4_t*)(p + 8 * q) = f32x4_t{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-        if constexpr (GATED)
-          *(f32x4_t*)(p + a.ldp / 2 + 8 * q) = f32x4_t{u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]};
+      for (int k = 0; k < U; ++k) res[k] = a8_res8(a.e, m0 + r0 + k * RP + lane / QN, n);
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int m = m0 + r0 + k * RP + lane / QN;
+      const uint8_t* p = s + (r0 + k * RP) * LD;
+      A8x8 y = *(const A8x8*)p, u = y;
+      if constexpr (GATED) u = *(const A8x8*)(p + 128);
+      if (a.splits > 1) {
+        float* o = a.part + ((long)blockIdx.y * a.M + m) * a.ldp + n;
+        if (m < a.M && n < (a.N + 31) / 32 * 32) {
+          *(A8x8*)o = y;
+          if constexpr (GATED) *(A8x8*)(o + a.ldp / 2) = u;
+        }
+      } else {
+        if constexpr (GATED) a8_gated8(a.e, y, u);
+        else a8_linear8(a.e, y, bias, res[k]);
+        a8_store8(a.e, y, m, n, m < a.M && n < a.N);
       }
     }
-    return;
   }
-  if (m >= a.M || n >= a.N) return;  // (a block's two lanes go together)
-  f32x4_t y[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    f32x4_t vq, uq;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      vq[i] = v[4 * q + i];
-      uq[i] = u[4 * q + i];
-    }
-    y[q] = a8_finish4<GATED>(a.e, vq, uq, m, n + 8 * q + 4 * g);
-  }
-  if (a.e.out) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) a8_store4(a.e, y[q], m, n + 8 * q + 4 * g);
-    return;
-  }
-  int top = 0;
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, a8_abs_bits(y[q][i]));
-  const auto sw = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-  top = max((int)sw[0], (int)sw[1]);
-  const int s = a8_scale(top);
-  const float inv = a8_inv(s);
-  // the byte order's words of 16 codes are {0 1 8 9} {2 3 10 11} | {4 5 12 13} {6 7 14 15}: this lane's own pairs
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t p = a8_pack4(y[2 * h][0], y[2 * h][1], y[2 * h + 1][0], y[2 * h + 1][1], inv, s == 255);
-    const uint32_t q = a8_pack4(y[2 * h][2], y[2 * h][3], y[2 * h + 1][2], y[2 * h + 1][3], inv, s == 255);
-    *(uint2*)(a.e.oa8 + (long)m * a.N + n + 16 * h + 8 * g) = make_uint2(p, q);
-  }
-  if (g == 0) a8_store_scale(a.e, m, n >> 5, s);
 }
 
-// BM rows of x by BN rows of weights in WM x WN waves of (BM / WM) x (BN / WN); steps of 128 k through NBUF LDS buffers.
+// BM rows of x by BN rows of weights in WM x WN waves of (BM / WM) x (BN / WN); stages of 128 k through NBUF LDS buffers.
 // A gated tile has BN / 2 output columns: of a wave's 32-row weight blocks the even ones are gate rows, the odd ones the
-// up rows of the same columns, so that a lane ends with both.
+// up rows of the same columns.
 template <int BM, int BN, int WM, int WN, int NBUF, bool GATED>
 __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   constexpr int NT = 64 * WM * WN;
-  constexpr int MT = BM / WM / 32, CT = BN / WN / 32;  // 32-row blocks of a wave
+  constexpr int MT = BM / WM / 16, CT = BN / WN / 16;  // 16-row blocks of a wave
   constexpr int XB = BM * 128, WB = BN * 128, SB = (BM < 64 ? 64 : BM) * 4, STAGE = XB + WB + SB;
   constexpr int XL = XB / 16 / NT, WL = WB / 16 / NT, LPT = XL + WL + 1;  // loads per thread and stage
   constexpr int OC = GATED ? BN / 2 : BN;                                 // output columns
-  static_assert(XL * NT * 16 == XB && WL * NT * 16 == WB && MT * WM * 32 == BM && CT * WN * 32 == BN, "tile shape");
-  static_assert(!GATED || CT % 2 == 0, "gate and up blocks in pairs");
-  static_assert((NBUF - 2) * LPT < 64, "vmcnt immediate");
+  // A stage is MT steps: x block t with the CT weight blocks.  x of a step is read AHEAD steps before, across the stage's
+  // end too: the barrier stands in step ENTER, where the first of the next stage is read.  A weight block is read for the
+  // next stage behind its last product.
+    constexpr int RING = MT >= 4 ? 4 : 2, AHEAD = RING / 2, ENTER = MT - AHEAD;
+  // A stage's loads are issued between the products from that barrier on, in the first POS of the MT CT places; FIRST of
+  // them fall into the stage in which they begin.
+  constexpr int POS = MT * CT * 3 / 4;
+  constexpr auto upto = [](int z) constexpr { return z >= POS ? LPT : z * LPT / POS; };
+  constexpr int FIRST = upto(AHEAD * CT);
+  static_assert(XL * NT * 16 == XB && WL * NT * 16 == WB && MT * WM * 16 == BM && CT * WN * 16 == BN, "tile shape");
+  static_assert(!GATED || CT % 4 == 0, "gate and up blocks in pairs");
+  static_assert(MT % RING == 0, "ring");
+  static_assert((NBUF - 2) * LPT + FIRST < 64, "vmcnt immediate");
   __shared__ __align__(16) uint8_t buf[NBUF * STAGE];
-  __shared__ __align__(16) uint8_t scl[BN / 32][kA8SliceSteps * 4];
+  __shared__ __align__(16) uint8_t scl[BN / 32][kA8SliceSteps * 4 + 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int l32 = lane & 31, g = lane >> 5;
+  const int l16 = lane & 15, g = lane >> 4;
   const int wm = wave / WN, wn = wave - wm * WN;
-  // contiguous tile ranges per XCD, rows fastest: the x rows stay in the XCD's L2 while its weights stream once
+  // contiguous tile ranges per XCD, in strips of kA8Strip row tiles: the tiles that run on an XCD together share rows and
+  // weights in its L2
   const int per = gridDim.x / kXcds;
   const int id = (blockIdx.x % kXcds) * per + blockIdx.x / kXcds;
   if (id >= a.mtiles * a.ntiles) return;
-  const int m0 = id % a.mtiles * BM, n0 = id / a.mtiles * OC;
+  const int strip = id / (kA8Strip * a.ntiles), sm = min(kA8Strip, a.mtiles - strip * kA8Strip);
+  const int in = id - strip * kA8Strip * a.ntiles;
+  const int m0 = (strip * kA8Strip + in % sm) * BM, n0 = in / sm * OC;
   const int s0 = blockIdx.y * a.kslice;
-  const int nk = min((a.K + 127) / 128 - s0, a.kslice);
-  const int kb = (a.K - s0 * 128) / 32 < nk * 4 ? (a.K - s0 * 128) / 32 : nk * 4;  // blocks of 32 k in the slice
+  const int nk = min(a.K / 128 - s0, a.kslice);  // whole stages of the slice
+  const int tail = a.K / 128 < s0 + a.kslice ? a.K % 128 : 0;  // k behind them, in the slice of that step
 
   // weight row r of the tile: output column (from n0) and matrix
   auto column = [&](int r) { return GATED ? (r / 64) * 32 + (r & 31) : r; };
@@ -247,7 +253,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   const uint8_t* xsb = a.xs + ((long)s0 * a.M + m0) * 4;
   // Load u of a thread brings 16 bytes of row u NT / 8 + tid / 8 (rows past the end repeat the last and are not stored).
   // Chunk c of a 128-byte row r sits at c ^ (r & 7): the 8 lanes of an LDS read cycle (8 rows, one chunk) then hit 8
-  // different 16-byte bank groups.  Offsets are made anew each time: as registers they would spill.
+  // different 16-byte bank groups.
   const int r0 = tid >> 3, ch = ((tid & 7) ^ (r0 & 7)) * 16;
   const int xlim = a.M - 1 - m0, wlim = a.N - 1 - n0;
   const int sr = min((wave % (SB / 256)) * 64 + lane, BM - 1);
@@ -255,118 +261,170 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   const uint32_t lds0 = lds_addr_of(buf);
   const uint32_t ldsw = lds0 + (uint32_t)wave * 1024, ldss = lds0 + XB + WB + (uint32_t)(wave % (SB / 256)) * 256;
   const int klast = a.K - s0 * 128 - 16;  // the last 16 codes of a row, from the slice's start
-  auto issue = [&](int kt, int b) {
+  uint32_t xo[XL], wo[WL];
+#pragma unroll
+  for (int u = 0; u < XL; ++u) xo[u] = (uint32_t)min(u * (NT / 8) + r0, xlim) * (uint32_t)a.K;
+#pragma unroll
+  for (int u = 0; u < WL; ++u) wo[u] = (uint32_t)min(column(u * (NT / 8) + r0), wlim) * (uint32_t)a.K;
+  // Load q of stage kt (past the last: the last again, into a buffer that is read no more, so that counts stay the same)
+  auto dma = [&](int kt, int b, int q) {
     const uint32_t l = (uint32_t)(b * STAGE);
     const uint32_t k = (uint32_t)min(kt * 128 + ch, klast);  // (chunks past K load the last one and are zeroed below)
-#pragma unroll
-    for (int u = 0; u < XL; ++u)
-      a8_dma16(xb, (uint32_t)min(u * (NT / 8) + r0, xlim) * (uint32_t)a.K + k, ldsw + l + u * NT * 16);
-#pragma unroll
-    for (int u = 0; u < WL; ++u)  // (a wave's 8 rows are of one matrix)
-      a8_dma16(is_up(u * (NT / 8) + wave * 8) ? wb2 : wb,
-               (uint32_t)min(column(u * (NT / 8) + r0), wlim) * (uint32_t)a.K + k, ldsw + l + XB + u * NT * 16);
-    a8_dma4(xsb + (long)kt * a.M * 4, so, ldss + l);
+    if (q < XL) {
+      a8_dma16(xb, xo[q] + k, ldsw + l + q * NT * 16);
+    } else if (q < XL + WL) {  // (a wave's 8 rows are of one matrix)
+      const int u = q - XL;
+      a8_dma16(is_up(u * (NT / 8) + wave * 8) ? wb2 : wb, wo[u] + k, ldsw + l + XB + u * NT * 16);
+    } else {
+      a8_dma4(xsb + (long)kt * a.M * 4, so, ldss + l);
+    }
   };
-#pragma unroll
-  for (int p = 0; p < NBUF - 1; ++p)
-    if (p < nk) issue(p, p);
-  {  // the slice's weight scales, by bytes (a row's may start at any address); 127 behind the last
-    const int nb = (a.N + 31) / 32;
-    for (int e = tid; e < BN / 32 * nk * 4; e += NT) {
-      const int b = e / (nk * 4), k = e - b * (nk * 4);
+  {  // the slice's weight scales
+    const int nb = (a.N + 31) / 32, kb = (nk * 128 + tail) / 32;
+    auto scales = [&](int b) {
       const int row = min((n0 + column(b * 32)) / 32, nb - 1);
-      const uint8_t* p = is_up(b * 32) ? a.ws2 + (long)row * a.Kc2 : a.ws + (long)row * a.Kc;
-      scl[b][k] = k < kb ? p[s0 * 4 + k] : 127;
+      return (is_up(b * 32) ? a.ws2 + (long)row * a.Kc2 : a.ws + (long)row * a.Kc) + s0 * 4;
+    };
+    if (a.words) {  // whole words: by direct loads, ahead of the stages'
+      for (int b = wave; b < BN / 32; b += WM * WN)
+        for (int c = 0; c < nk; c += 64)
+          a8_dma4(scales(b), (uint32_t)min(c + lane, nk - 1) * 4, lds_addr_of(&scl[b][0]) + c * 4);
+    } else {  // by bytes, 127 behind the last
+      for (int b = wave; b < BN / 32; b += WM * WN) {
+        const uint8_t* p = scales(b);
+        for (int k = lane; k < (nk + 1) * 4; k += 64) scl[b][k] = k < kb ? p[k] : 127;
+      }
     }
   }
+#pragma unroll
+  for (int p = 0; p < NBUF; ++p)
+#pragma unroll
+    for (int q = 0; q < (p < NBUF - 1 ? LPT : FIRST); ++q) dma(max(min(p, nk - 1), 0), p, q);
 
-  f32x16_t acc[MT][CT];
+  f32x4_t acc[MT][CT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < CT; ++j)
+    for (int j = 0; j < CT; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  const int xr = wm * (BM / WM) + l16, wr = wn * (BN / WN) + l16;  // (16-row steps keep the swizzle's row bits)
+  const int c0 = (g ^ (l16 & 7)) * 16, c1 = c0 ^ 64;                // chunks g and 4 + g
+  auto operand = [&](const uint8_t* p) { return a8_operand(*(const uint4*)(p + c0), *(const uint4*)(p + c1)); };
+  // The next stage has landed for every wave (`later` younger loads may not have), and every wave has read this one.
+  auto enter = [&](auto later) {
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(decltype(later)::value));
+    lds_barrier();
+  };
+  i32x8_t xf[RING], wf[CT];
+  int xs[RING], ws[CT];  // (bytes: a shift of a word would wait for it where it is read)
+  auto fetch_w = [&](int j, int kt, int b) {
+    wf[j] = operand(buf + b * STAGE + XB + (wr + 16 * j) * 128);
+    ws[j] = scl[wn * (CT / 2) + j / 2][kt * 4 + g];  // (kt may be one past the slice: the row is longer)
+  };
+  auto fetch_x = [&](int t, int b) {
+    const uint8_t* st = buf + b * STAGE;
+    xf[t % RING] = operand(st + (xr + 16 * t) * 128);
+    xs[t % RING] = st[XB + WB + (xr + 16 * t) * 4 + g];
+  };
+  if (nk > 0) {
+    int bi = 0;
+    enter(std::integral_constant<int, (NBUF - 2) * LPT + FIRST>{});
 #pragma unroll
-      for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.0f;
-  const int xr = wm * (BM / WM) + l32, wr = wn * (BN / WN) + l32;  // (32-row steps keep the swizzle's row bits)
-  const int xsw = xr & 7, wsw = wr & 7;
-  int bi = 0;
+    for (int j = 0; j < CT; ++j) fetch_w(j, 0, 0);
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t) fetch_x(t, 0);
 #pragma unroll 1
-  for (int kt = 0; kt < nk; ++kt) {
-    // this wave's loads of stage kt have landed (the NBUF - 2 stages after it may not)
-    if (NBUF > 2 && kt + NBUF - 2 < nk) __builtin_amdgcn_s_waitcnt(vmcnt_imm((NBUF - 2) * LPT));
-    else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-    lds_barrier();  // stage kt is there for every wave, and every wave has read stage kt - 1
-    if (kt + NBUF - 1 < nk) issue(kt + NBUF - 1, bi == 0 ? NBUF - 1 : bi - 1);
-    uint8_t* st = buf + bi * STAGE;
-    if (kt * 4 + 4 > kb) {  // K ends inside this stage: zeros from there on
-      const int first = (kb - kt * 4) * 2;
-      for (int e = tid; e < (BM + BN) * 8; e += NT)
-        if ((e & 7) >= first) *(uint4*)(st + (e >> 3) * 128 + (((e & 7) ^ ((e >> 3) & 7)) * 16)) = make_uint4(0, 0, 0, 0);
-      lds_barrier();
-    }
-    int xs[MT], ws[CT];
+    for (int kt = 0; kt < nk; ++kt) {  // (what the last stage reads and loads ahead is the last again, and not used)
+      const int b0 = bi;
+      bi = bi + 1 == NBUF ? 0 : bi + 1;
+      const int bp = b0 == 0 ? NBUF - 1 : b0 - 1;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) xs[i] = *(const int*)(st + XB + WB + (xr + 32 * i) * 4) >> (8 * g);
+      for (int t = 0; t < MT; ++t) {
+        if (t < ENTER) {
+          fetch_x(t + AHEAD, b0);
+        } else {
+          if (t == ENTER) enter(std::integral_constant<int, (NBUF - 2) * LPT>{});
+          fetch_x(t - ENTER, bi);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int j = 0; j < CT; ++j) ws[j] = *(const int*)(&scl[wn * CT + j][kt * 4]) >> (8 * g);
+        for (int j = 0; j < CT; ++j) {
+          acc[t][j] = a8_mfma16(wf[j], xf[t % RING], acc[t][j], ws[j], xs[t % RING]);
+          if (t == MT - 1) fetch_w(j, kt + 1, bi);
+          const int z = (t < ENTER ? t + AHEAD : t - ENTER) * CT + j;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {  // 64 k each
-      i32x8_t xf[MT], wf[CT];
-#pragma unroll
-      for (int j = 0; j < CT; ++j) {
-        const uint8_t* p = st + XB + (wr + 32 * j) * 128;
-        wf[j] = a8_operand(*(const uint4*)(p + ((4 * h + g) ^ wsw) * 16), *(const uint4*)(p + ((4 * h + 2 + g) ^ wsw) * 16));
+          for (int q = upto(z); q < upto(z + 1); ++q) dma(min(t < ENTER ? kt + NBUF - 1 : kt + NBUF, nk - 1), t < ENTER ? bp : b0, q);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const uint8_t* p = st + (xr + 32 * i) * 128;
-        xf[i] = a8_operand(*(const uint4*)(p + ((4 * h + g) ^ xsw) * 16), *(const uint4*)(p + ((4 * h + 2 + g) ^ xsw) * 16));
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < CT; ++j)
-          acc[i][j] = h == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[j], xf[i], acc[i][j], 0, 0, 0, ws[j], 0, xs[i])
-                             : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[j], xf[i], acc[i][j], 0, 0, 2, ws[j], 2, xs[i]);
     }
-    bi = bi + 1 == NBUF ? 0 : bi + 1;
   }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  lds_barrier();  // every wave has read its last stage, and no load is on its way
+  if (tail) {     // K ends inside a stage of its own: zeros behind it
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int m = m0 + wm * (BM / WM) + 32 * i + l32;
-    if constexpr (GATED) {
+    for (int q = 0; q < LPT; ++q) dma(nk, 0, q);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    lds_barrier();
+    for (int e = tid; e < (BM + BN) * 8; e += NT)
+      if ((e & 7) * 16 >= tail) *(uint4*)(buf + (e >> 3) * 128 + (((e & 7) ^ ((e >> 3) & 7)) * 16)) = make_uint4(0, 0, 0, 0);
+    lds_barrier();
 #pragma unroll
-      for (int j = 0; j < CT; j += 2) a8_tile_out<true>(a, acc[i][j], acc[i][j + 1], m, n0 + wn * (BN / WN / 2) + 16 * j, g);
-    } else {
+    for (int j = 0; j < CT; ++j) fetch_w(j, nk, 0);
 #pragma unroll
-      for (int j = 0; j < CT; ++j) a8_tile_out<false>(a, acc[i][j], acc[i][j], m, n0 + wn * (BN / WN) + 32 * j, g);
+    for (int t = 0; t < MT; ++t) {
+      fetch_x(t, 0);
+#pragma unroll
+      for (int j = 0; j < CT; ++j) acc[t][j] = a8_mfma16(wf[j], xf[t % RING], acc[t][j], ws[j], xs[t % RING]);
     }
+    lds_barrier();
+  }
+
+  // A lane (l16, g) has row l16, columns 4 g .. 4 g + 3 of a block: PM blocks of rows at a time through the wave's part of
+  // the LDS (rows padded by 16 bytes: 8 lanes write 8 different bank groups)
+  constexpr int LD = BN / WN * 4 + 16;
+  constexpr int PM = MT * 16 * LD * WM * WN <= NBUF * STAGE ? MT : MT * 8 * LD * WM * WN <= NBUF * STAGE ? MT / 2 : MT / 4;
+  static_assert(PM * 16 * LD * WM * WN <= NBUF * STAGE && MT % PM == 0 && PM % 2 == 0, "output staging");
+  uint8_t* own = buf + wave * (PM * 16 * LD);
+#pragma unroll
+  for (int p = 0; p < MT; p += PM) {
+#pragma unroll
+    for (int i = 0; i < PM; ++i)
+#pragma unroll
+      for (int j = 0; j < CT; ++j) *(f32x4_t*)(own + (16 * i + l16) * LD + (16 * j + 4 * g) * 4) = acc[p + i][j];
+    a8_wave_out<PM * 16, LD, OC / WN, GATED>(a, own, m0 + wm * (BM / WM) + 16 * p, n0 + wn * (OC / WN));
   }
 }
 
-// The K slices' partials summed in slice order and finished: 4 columns a thread, 8 adjacent lanes a block of 32.
+// The K slices' partials summed in slice order and finished: 8 columns a thread, 4 adjacent lanes a block of 32.
 template <bool GATED>
 __global__ void __launch_bounds__(256) a8_sum_kernel(const A8Args a) {
-  const int q = (a.N + 31) / 32 * 8;  // threads of a row
+  const int q = (a.N + 31) / 32 * 4;  // threads of a row
   const long t = (long)blockIdx.x * 256 + threadIdx.x;
   const long m = t / q;
-  const int n = (int)(t - m * q) * 4;
+  const int n = (int)(t - m * q) * 8;
   const bool live = m < a.M && n < a.N;
-  f32x4_t v = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, u = v;
+  A8x8 y, u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y.v[i] = u.v[i] = 0.0f;
   if (live) {
+    const uint4 res = a8_res8(a.e, (int)m, n);
+    const A8x8 bias = a8_bias8(a.e, n);
     const float* p = a.part + m * a.ldp + n;
 #pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
-      v += *(const f32x4_t*)(p + (long)s * a.M * a.ldp);
-      if constexpr (GATED) u += *(const f32x4_t*)(p + (long)s * a.M * a.ldp + a.ldp / 2);
+      const A8x8 v = *(const A8x8*)(p + (long)s * a.M * a.ldp);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y.v[i] += v.v[i];
+      if constexpr (GATED) {
+        const A8x8 w = *(const A8x8*)(p + (long)s * a.M * a.ldp + a.ldp / 2);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u.v[i] += w.v[i];
+      }
     }
-    v = a8_finish4<GATED>(a.e, v, u, (int)m, n);
+    if constexpr (GATED) a8_gated8(a.e, y, u);
+    else a8_linear8(a.e, y, bias, res);
   }
-  if (a.e.out) {
-    if (live) a8_store4(a.e, v, (int)m, n);
-  } else {
-    a8_store_block8(a.e, v, (int)m, n, live);
-  }
+  a8_store8(a.e, y, (int)m, n, live);
 }
 
 // ------------------------------------------------------------------------------------------------ plan
@@ -414,8 +472,8 @@ int a8_run(A8Args& a, void* ws, long ws_bytes, hipStream_t st) {
   if (!a.e.out && (!a.e.oa8 || !a.e.os8 || a.N % 32 != 0 || (uintptr_t)a.e.oa8 & 15)) return (int)hipErrorInvalidValue;
   a.e.M = a.M;
   a.e.N = a.N;
-  a.e.vec = a.N % 4 == 0 && (((uintptr_t)a.e.out | (uintptr_t)a.e.res) & 7) == 0 &&
-            ((uintptr_t)a.e.bias & (a.e.bias_f32 ? 15 : 7)) == 0;
+  a.e.vec = a.N % 8 == 0 && (((uintptr_t)a.e.out | (uintptr_t)a.e.res) & 15) == 0;
+  a.words = a.K % 128 == 0 && ((a.Kc | a.Kc2 | (uintptr_t)a.ws | (uintptr_t)a.ws2) & 3) == 0;
   const A8Plan p = a8_plan(a.M, a.N, a.K, GATED);
   a.splits = p.splits;
   a.kslice = p.kslice;
@@ -442,12 +500,12 @@ int a8_run(A8Args& a, void* ws, long ws_bytes, hipStream_t st) {
   a.mtiles = (a.M + p.rows - 1) / p.rows;
   a.ntiles = (a.N + oc - 1) / oc;
   const dim3 g((unsigned)((a.mtiles * a.ntiles + kXcds - 1) / kXcds * kXcds), (unsigned)p.splits);
-  if (p.rows == 64) a8_tile_kernel<64, 128, 2, 2, 3, GATED><<<g, 256, 0, st>>>(a);
+  if (p.rows == 64) a8_tile_kernel<64, 128, 2, 2, 2, GATED><<<g, 256, 0, st>>>(a);
   else if (p.rows == 128) a8_tile_kernel<128, 128, 2, 2, 2, GATED><<<g, 256, 0, st>>>(a);
   else a8_tile_kernel<256, 256, 2, 4, 2, GATED><<<g, 512, 0, st>>>(a);
   DSV41_CHECK_LAUNCH();
   if (p.splits > 1) {
-    const long t = (long)a.M * ((a.N + 31) / 32 * 8);
+    const long t = (long)a.M * ((a.N + 31) / 32 * 4);
     a8_sum_kernel<GATED><<<(unsigned)((t + 255) / 256), 256, 0, st>>>(a);
     DSV41_CHECK_LAUNCH();
   }

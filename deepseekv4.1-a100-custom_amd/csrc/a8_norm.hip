@@ -21,15 +21,6 @@ struct NormArgs {
 };
 
 
-DSV41_DEV void norm_unpack(uint4 q, float (&v)[8]) {
-  const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(u[i] << 16);
-    v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-  }
-}
-
 // One row by nt lanes (t: this lane's number); red: the workgroup's exchange, null where a row is one wave's.
 template <int IT, bool BLOCK>
 DSV41_DEV void norm_row(const NormArgs& a, long row, bool live, int t, int nt, float* red) {
@@ -48,16 +39,15 @@ DSV41_DEV void norm_row(const NormArgs& a, long row, bool live, int t, int nt, f
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
     const bool in = live && t + i * nt < nc;
-    norm_unpack(xq[i], v[i]);
+    a8_unpack8(xq[i], v[i]);
     if (a.r) {
       float r[8];
-      norm_unpack(rq[i], r);
-      uint32_t u[4];
+      a8_unpack8(rq[i], r);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) u[k] = a8_bf16x2(v[i][2 * k] + r[2 * k], v[i][2 * k + 1] + r[2 * k + 1]);
-      const uint4 hq = make_uint4(u[0], u[1], u[2], u[3]);
+      for (int k = 0; k < 8; ++k) r[k] += v[i][k];
+      const uint4 hq = a8_pack8(r);
       if (in) ((uint4*)(a.h + base))[t + i * nt] = hq;
-      norm_unpack(hq, v[i]);
+      a8_unpack8(hq, v[i]);
     }
     if (in) {
 #pragma unroll
@@ -76,7 +66,7 @@ DSV41_DEV void norm_row(const NormArgs& a, long row, bool live, int t, int nt, f
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       float w[8];
-      norm_unpack(wq[i], w);
+      a8_unpack8(wq[i], w);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[i][k] = v[i][k] * inv * w[k];
     }
@@ -84,22 +74,10 @@ DSV41_DEV void norm_row(const NormArgs& a, long row, bool live, int t, int nt, f
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
     const int c = t + i * nt;
-    int top = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) top = max(top, a8_abs_bits(v[i][k]));
-    top = max(top, dpp_movi<0xB1>(top));
-    top = max(top, dpp_movi<0x4E>(top));
-    const int s = a8_scale(top);
-    const float inv = a8_inv(s);
-    const uint32_t lo = a8_pack4(v[i][0], v[i][1], v[i][2], v[i][3], inv, s == 255);
-    const uint32_t hi = a8_pack4(v[i][4], v[i][5], v[i][6], v[i][7], inv, s == 255);
-    // words of 16 codes in the byte order: {0 1 8 9} {2 3 10 11} {4 5 12 13} {6 7 14 15}; the even lane has 0..7 and
-    // writes the first two, the odd one 8..15 and the last two
-    const bool odd = t & 1;
-    const uint32_t got = (uint32_t)dpp_movi<0xB1>((int)(odd ? lo : hi));
-    const uint32_t p = odd ? got : lo, q = odd ? hi : got;  // codes 0..3 or 4..7, and 8..11 or 12..15
+    int s;
+    const uint2 q = a8_quant8(v[i], t & 1, &s);
     if (live && c < nc) {
-      *(uint2*)(a.a8 + base + 8 * c) = make_uint2((p & 0xffffu) | (q << 16), (p >> 16) | (q & 0xffff0000u));
+      *(uint2*)(a.a8 + base + 8 * c) = q;
       if ((c & 3) == 0) {
         const int b = c >> 2;
         uint8_t* sp = a.s8 + ((long)(b >> 2) * a.rows + row) * 4 + (b & 3);

@@ -18,12 +18,16 @@ OBJ = PKG.parent / "_build"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Xclang", "-target-feature", "-Xclang",
-         "-packed-fp32-ops", "-mllvm", "-amdgpu-mfma-vgpr-form=1", f"-I{INCLUDE}", f"-I{CSRC}"]
+         "-packed-fp32-ops", f"-I{INCLUDE}", f"-I{CSRC}"]
+# Matrix results in the VGPRs their epilogues read; not where a kernel's sums take the accumulation registers.
+VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+ACC_FORM = {"a8_gemm"}
 
 
 def _compile(src: Path, extra=(), tag: str = "") -> Path:
     obj = OBJ / (src.stem + tag + ".o")
-    cmd = [HIPCC, *FLAGS, *extra, "-c", str(src), "-o", str(obj)]
+    form = [] if src.stem in ACC_FORM else VGPR_FORM
+    cmd = [HIPCC, *FLAGS, *form, *extra, "-c", str(src), "-o", str(obj)]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed for {src.name}:\n{r.stderr}")
