@@ -24,9 +24,6 @@ struct A8Args {
   A8Epi e;
   int mtiles, ntiles;
   int words;                  // weight scales in whole words: K % 128 == 0, rows 4-byte aligned
-  int splits, kslice;         // K slices of kslice steps of 128 k; more than one: partials
-  float* part;                // [splits][M][ldp], ldp = ceil(N / 32) * 32 (gated: twice, up behind gate)
-  long ldp;
 };
 
 DSV41_DEV i32x8_t a8_operand(uint4 lo, uint4 hi) {
@@ -38,108 +35,186 @@ DSV41_DEV f32x4_t a8_mfma16(i32x8_t a, i32x8_t b, f32x4_t c, int sa, int sb) {
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
-// Up to 16 MT rows: a stream of the weights.  A workgroup has 16 CT output columns, its waves take the steps of 128 k in
-// turn (wave v: steps v, v + waves, ...), so that together they read whole rows in order; sums meet in LDS.  The weights
-// go from memory into the instruction's registers, a step ahead; x comes from the L2, in the same lanes.
-template <int MT, int CT, bool GATED>
-__global__ void __launch_bounds__(512) a8_stream_kernel(const A8Args a) {
-  extern __shared__ __align__(16) float red[];  // [waves][WT * MT][64 lanes][4]
-  constexpr int WT = GATED ? 2 * CT : CT;       // weight tiles of 16 rows: gate tiles, then up tiles
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nw = blockDim.x >> 6;
+DSV41_DEV float a8_e8m0(int s) { return s == 255 ? __builtin_nanf("") : s ? __int_as_float(s << 23) : __int_as_float(0x00400000); }
+// 8 codes (two words) times their scale, exact in bf16.
+DSV41_DEV uint4 a8_decode(uint32_t a, uint32_t b, float sc) {
+  return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, sc, false)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, sc, true)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, sc, false)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, sc, true)));
+}
+
+// Direct-to-LDS load of 16 (4) bytes a lane from base + off to lds_addr + 16 (4) i; callers wait with vmcnt counts.
+DSV41_DEV void a8_dma16(const void* base, uint32_t off, uint32_t lds_addr) {
+  const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory", "m0");
+}
+DSV41_DEV void a8_dma4(const void* base, uint32_t off, uint32_t lds_addr) {
+  const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory", "m0");
+}
+
+// 16 MT rows by 16 CT output columns a workgroup: a stream of the weights.  Its NW waves take the steps of 128 k in turn
+// (wave v: steps v, v + NW, ...), so that together they read whole rows in order, each through a ring of D steps in LDS
+// that only it fills and reads: no barrier until the sums meet, and D steps of loads on the way in every wave.  (Loads
+// into registers a step ahead were 16 us where this is 11: 24 rows of 1280 k, 32768 columns.)
+// EXACT: the codes and scales as bf16 (exact), products and sums as the bf16 matrix units have them, in fp32: the time is
+// the weights' anyway, and the few blocks of a small output show single codes that fall to the other side of a border.
+// A lane's 32 codes are then k 32 g .. 32 g + 31, one scale block.
+constexpr int kStreamMaxK = 32768;  // (the weight scales of all of K are held in LDS)
+
+template <int MT, int CT, int NW, int D, bool GATED, bool EXACT>
+__global__ void __launch_bounds__(64 * NW) a8_stream_kernel(const A8Args a) {
+  constexpr int WT = GATED ? 2 * CT : CT;  // weight tiles of 16 rows: gate tiles, then up tiles
+  constexpr int STEP = (WT + MT) * 2048 + 256, LPS = 2 * (WT + MT) + 1;
+  constexpr int RING = NW * D * STEP, SUMS = NW * WT * MT * 1024;
+  static_assert((D - 1) * LPS < 64, "vmcnt immediate");
+  __shared__ __align__(16) uint8_t lds[RING > SUMS ? RING : SUMS];
+  __shared__ __align__(16) uint8_t scl[GATED ? 2 : 1][kStreamMaxK / 32];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16 * CT;
-  const int steps = (a.K + 127) / 128, last = a.K / 32 - 1;
-  const uint8_t *wp[WT], *sp[WT], *xp[MT], *xsp[MT];
+  const int n0 = blockIdx.x * 16 * CT, m0 = blockIdx.y * 16 * MT;
+  const int steps = (a.K + 127) / 128;
+  const int mine = (steps - wave + NW - 1) / NW;  // this wave's steps (none where K is short)
+  // 16 bytes of row (lane / 8) of 8: chunk c of a 128-byte row r sits at c ^ (r & 7)
+  const int r8 = lane >> 3, ch = ((lane & 7) ^ r8) * 16;
+  uint32_t wo[WT][2], xo[MT][2];
 #pragma unroll
-  for (int t = 0; t < WT; ++t) {
-    const int n = min(n0 + 16 * (t % CT) + l16, a.N - 1);  // (columns past N repeat the last and are not stored)
-    const bool up = GATED && t >= CT;
-    wp[t] = (up ? a.w2 : a.w) + (long)n * a.K;
-    sp[t] = up ? a.ws2 + (long)(n >> 5) * a.Kc2 : a.ws + (long)(n >> 5) * a.Kc;
+  for (int t = 0; t < WT; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)  // (columns past N repeat the last and are not stored)
+      wo[t][u] = (uint32_t)min(16 * (t % CT) + 8 * u + r8, a.N - 1 - n0) * (uint32_t)a.K;
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) xo[t][u] = (uint32_t)min(16 * t + 8 * u + r8, a.M - 1 - m0) * (uint32_t)a.K;
+  const uint8_t* wb = a.w + (long)n0 * a.K;
+  const uint8_t* wb2 = GATED ? a.w2 + (long)n0 * a.K : nullptr;
+  const uint8_t* xb = a.x + (long)m0 * a.K;
+  const uint8_t* xsb = a.xs + 4l * m0;
+  const uint32_t so = (uint32_t)min(min(lane, 16 * MT - 1), a.M - 1 - m0) * 4;
+  uint8_t* ring = lds + wave * (D * STEP);
+  const uint32_t ring0 = lds_addr_of(lds) + (uint32_t)wave * (D * STEP);
+  auto issue = [&](int i, int b) {  // step i of this wave (past the last: the last again, not used) into slot b
+    const int s = min(wave + i * NW, steps - 1);
+    const uint32_t k = (uint32_t)min(s * 128 + ch, a.K - 16);  // (chunks past K load the last one and are zeroed below)
+    const uint32_t l = ring0 + (uint32_t)(b * STEP);
+#pragma unroll
+    for (int t = 0; t < WT; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) a8_dma16(GATED && t >= CT ? wb2 : wb, wo[t][u] + k, l + t * 2048 + u * 1024);
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) a8_dma16(xb, xo[t][u] + k, l + (WT + t) * 2048 + u * 1024);
+    a8_dma4(xsb + (long)s * a.M * 4, so, l + (WT + MT) * 2048);
+  };
+  {  // the weight scales of the columns' block, in whole words or by bytes
+    const int row = n0 >> 5, nb = a.K / 32;
+    for (int q = wave; q < (GATED ? 2 : 1); q += NW) {
+      const uint8_t* p = q ? a.ws2 + (long)row * a.Kc2 : a.ws + (long)row * a.Kc;
+      if (a.words)
+        for (int c = 0; c < nb / 4; c += 64)
+          a8_dma4(p, (uint32_t)min(c + lane, nb / 4 - 1) * 4, lds_addr_of(&scl[q][0]) + c * 4);
+      else
+        for (int k = lane; k < nb; k += 64) scl[q][k] = p[k];
+    }
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int m = min(16 * t + l16, a.M - 1);
-    xp[t] = a.x + (long)m * a.K;
-    xsp[t] = a.xs + 4l * m + g;
-  }
-  struct Step {
-    uint4 w[WT][2], x[MT][2];
-    int ws[WT], xs[MT];
-  };
-  auto load = [&](int s, Step& o) {
-    const int k = min(s, steps - 1) * 128;
-    const int p = k + 16 * g < a.K ? k + 16 * g : k, q = k + 64 + 16 * g < a.K ? k + 64 + 16 * g : k;
-    const int b = min(k / 32 + g, last);
-#pragma unroll
-    for (int t = 0; t < WT; ++t) {
-      o.w[t][0] = *(const uint4*)(wp[t] + p);
-      o.w[t][1] = *(const uint4*)(wp[t] + q);
-      o.ws[t] = sp[t][b];
-    }
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      o.x[t][0] = *(const uint4*)(xp[t] + p);
-      o.x[t][1] = *(const uint4*)(xp[t] + q);
-      o.xs[t] = xsp[t][(long)(k / 128) * a.M * 4];
-    }
-  };
+  for (int i = 0; i < D - 1; ++i) issue(i, i);
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm((D - 1) * LPS));  // the scales are there (they were first)
+  lds_barrier();
+
   f32x4_t acc[WT][MT];
 #pragma unroll
   for (int i = 0; i < WT; ++i)
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  auto mul = [&](int s, Step& o) {
-    if (s * 128 + 128 > a.K) {  // K ends inside this step: codes past it are zero on both sides
-      const bool p = s * 128 + 16 * g < a.K, q = s * 128 + 64 + 16 * g < a.K;
-      const uint4 z = make_uint4(0, 0, 0, 0);
+  const int c0 = EXACT ? (2 * g) ^ (l16 & 7) : g ^ (l16 & 7), c1 = EXACT ? c0 ^ 1 : c0 ^ 4;  // a lane's two chunks
+  const int last = a.K / 32 - 1;
+  int bi = 0;
+#pragma unroll 1
+  for (int i = 0; i < mine; ++i) {
+    issue(i + D - 1, bi == 0 ? D - 1 : bi - 1);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm((D - 1) * LPS));
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    uint8_t* st = ring + bi * STEP;
+    const int s = wave + i * NW;
+    if (s * 128 + 128 > a.K) {  // K ends inside this step: zeros from there on
+      const int first = (a.K - s * 128) / 16;
+      for (int e = lane; e < (WT + MT) * 128; e += 64)
+        if ((e & 7) >= first) *(uint4*)(st + (e >> 3) * 128 + (((e & 7) ^ ((e >> 3) & 7)) * 16)) = make_uint4(0, 0, 0, 0);
+    }
+    auto operand = [&](int t, uint4& p, uint4& q) {
+      const uint8_t* r = st + t * 2048 + l16 * 128;
+      p = *(const uint4*)(r + c0 * 16);
+      q = *(const uint4*)(r + c1 * 16);
+    };
+    const int blk = min(4 * s + g, last);  // (behind the last: any scale that is a number, the codes are zero)
+    int ws[GATED ? 2 : 1], xs[MT];
+    ws[0] = scl[0][blk];
+    if constexpr (GATED) ws[1] = scl[1][blk];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) xs[j] = st[(WT + MT) * 2048 + (16 * j + l16) * 4 + (blk & 3)];
+    uint4 x[MT][2];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) operand(WT + j, x[j][0], x[j][1]);
+    if constexpr (EXACT) {
+      uint4 xd[MT][4];
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        const float sc = a8_e8m0(xs[j]);
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+          xd[j][h] = h & 1 ? a8_decode(x[j][h >> 1].z, x[j][h >> 1].w, sc) : a8_decode(x[j][h >> 1].x, x[j][h >> 1].y, sc);
+      }
 #pragma unroll
       for (int t = 0; t < WT; ++t) {
-        if (!p) o.w[t][0] = z;
-        if (!q) o.w[t][1] = z;
-        if (s * 4 + g > last) o.ws[t] = 127;
-      }
+        const float sc = a8_e8m0(ws[t / CT]);
+        uint4 c[2];
+        operand(t, c[0], c[1]);
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        if (!p) o.x[t][0] = z;
-        if (!q) o.x[t][1] = z;
+        for (int h = 0; h < 4; ++h) {
+          const uint4 w = h & 1 ? a8_decode(c[h >> 1].z, c[h >> 1].w, sc) : a8_decode(c[h >> 1].x, c[h >> 1].y, sc);
+#pragma unroll
+          for (int j = 0; j < MT; ++j) acc[t][j] = mfma_bf16_16x16x32(w, xd[j][h], acc[t][j]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < WT; ++t) {
+        uint4 c[2];
+        operand(t, c[0], c[1]);
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+          acc[t][j] = a8_mfma16(a8_operand(c[0], c[1]), a8_operand(x[j][0], x[j][1]), acc[t][j], ws[t / CT], xs[j]);
       }
     }
-#pragma unroll
-    for (int j = 0; j < MT; ++j)
-#pragma unroll
-      for (int i = 0; i < WT; ++i)
-        acc[i][j] = a8_mfma16(a8_operand(o.w[i][0], o.w[i][1]), a8_operand(o.x[j][0], o.x[j][1]), acc[i][j], o.ws[i],
-                              o.xs[j]);
-  };
-  Step s0, s1;
-  load(wave, s0);
-#pragma unroll 1
-  for (int s = wave; s < steps; s += 2 * nw) {
-    load(s + nw, s1);
-    mul(s, s0);
-    if (s + nw < steps) {
-      load(s + 2 * nw, s0);
-      mul(s + nw, s1);
-    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this slot is read: the next issue may fill it
+    bi = bi + 1 == D ? 0 : bi + 1;
   }
   // lane (l16, g): row l16 of x, columns 4 g .. 4 g + 3 of the tile
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  lds_barrier();  // no load is on its way into the LDS, and every wave has read its last step
+  float* red = (float*)lds;  // [waves][WT * MT][64 lanes][4]
 #pragma unroll
   for (int i = 0; i < WT; ++i)
 #pragma unroll
-    for (int j = 0; j < MT; ++j) *(f32x4_t*)(red + (((long)wave * WT + i) * MT + j) * 256 + lane * 4) = acc[i][j];
+    for (int j = 0; j < MT; ++j) *(f32x4_t*)(red + ((wave * WT + i) * MT + j) * 256 + lane * 4) = acc[i][j];
   __syncthreads();
   constexpr int QN = 2 * CT;  // lanes of a row: 8 columns each
-  for (int t = tid; t < QN * 16 * MT; t += blockDim.x) {  // (in whole quads of lanes: a block of 32 columns with CT 2)
-    const int c = t % QN, m = t / QN, n = n0 + 8 * c;
-    const float* p = red + ((c >> 1) * MT + (m >> 4)) * 256 + ((c & 1) * 32 + (m & 15)) * 4;  // the next 4: lanes on 16
+  for (int t = tid; t < QN * 16 * MT; t += 64 * NW) {  // (in whole quads of lanes: a block of 32 columns with CT 2)
+    const int c = t % QN, r = t / QN, m = m0 + r, n = n0 + 8 * c;
+    const float* p = red + ((c >> 1) * MT + (r >> 4)) * 256 + ((c & 1) * 32 + (r & 15)) * 4;  // the next 4: lanes on 16
     const bool live = m < a.M && n < a.N;
     const uint4 res = a8_res8(a.e, m, n);
     const A8x8 bias = a8_bias8(a.e, n);
     A8x8 y, u;
 #pragma unroll
     for (int i = 0; i < 8; ++i) y.v[i] = u.v[i] = 0.0f;
-    for (int w = 0; w < nw; ++w) {
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         y.v[i] += p[w * (WT * MT * 256) + (i >> 2) * 64 + (i & 3)];
@@ -153,53 +228,36 @@ __global__ void __launch_bounds__(512) a8_stream_kernel(const A8Args a) {
 }
 
 // ------------------------------------------------------------------------------------------------ tiles
-// Direct-to-LDS load of 16 (4) bytes a lane from base + off to lds_addr + 16 (4) i; callers wait with vmcnt counts.
-DSV41_DEV void a8_dma16(const void* base, uint32_t off, uint32_t lds_addr) {
-  const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory", "m0");
-}
-DSV41_DEV void a8_dma4(const void* base, uint32_t off, uint32_t lds_addr) {
-  const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory", "m0");
-}
-
 constexpr int kA8Strip = 4;
-constexpr int kA8SliceSteps = 128;  // a K slice's steps of 128 k at most: its weight scales are held in LDS
+constexpr int kTileMaxK = 16384;  // (the weight scales of a tile are held in LDS)
 
 // Output of a wave's ROWS x OCW block of sums from LDS (fp32, row stride LD bytes): rolled, so that bias, activation and
 // quantisation stand there once (unrolled over the accumulators they were 100 KB of code); the residual of U passes is
 // loaded before any of them is stored.
 template <int ROWS, int LD, int OCW, bool GATED>
 DSV41_DEV void a8_wave_out(const A8Args& a, const uint8_t* s, int m0, int n0) {
-  constexpr int QN = OCW / 8, RP = 64 / QN, PASSES = ROWS / RP, U = PASSES < 8 ? PASSES : 8;  // lanes of a row, rows of a pass
-  static_assert(ROWS % RP == 0 && PASSES % U == 0, "whole passes");
-  const int lane = threadIdx.x & 63, c = lane % QN * 8, n = n0 + c;
-  s += (lane / QN) * LD + (GATED ? (c / 32 * 64 + c % 32) * 4 : c * 4);
+  constexpr int QN = OCW / 8, RP = 64 / QN;  // lanes of a row, rows of a pass
+  constexpr int PASSES = (ROWS + RP - 1) / RP, U = PASSES % 8 == 0 ? 8 : PASSES % 4 == 0 ? 4 : PASSES % 6 == 0 ? 6 : 1;
+  const int lane = threadIdx.x & 63, c = lane % QN * 8, n = n0 + c, row = lane / QN;
+  s += row * LD + (GATED ? (c / 32 * 64 + c % 32) * 4 : c * 4);
   const A8x8 bias = a8_bias8(a.e, n);
 #pragma unroll 1
   for (int r0 = 0; r0 < ROWS; r0 += U * RP) {
     uint4 res[U];
     if constexpr (!GATED) {
 #pragma unroll
-      for (int k = 0; k < U; ++k) res[k] = a8_res8(a.e, m0 + r0 + k * RP + lane / QN, n);
+      for (int k = 0; k < U; ++k) res[k] = a8_res8(a.e, m0 + r0 + k * RP + row, n);
     }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const int m = m0 + r0 + k * RP + lane / QN;
-      const uint8_t* p = s + (r0 + k * RP) * LD;
+      const int r = r0 + k * RP + row, m = m0 + r;
+      const bool in = (64 % QN == 0 || row < RP) && (ROWS % RP == 0 || r < ROWS);  // (a row's lanes may not fill the wave)
+      const uint8_t* p = s + (in ? (r0 + k * RP) * LD : 0);
       A8x8 y = *(const A8x8*)p, u = y;
       if constexpr (GATED) u = *(const A8x8*)(p + 128);
-      if (a.splits > 1) {
-        float* o = a.part + ((long)blockIdx.y * a.M + m) * a.ldp + n;
-        if (m < a.M && n < (a.N + 31) / 32 * 32) {
-          *(A8x8*)o = y;
-          if constexpr (GATED) *(A8x8*)(o + a.ldp / 2) = u;
-        }
-      } else {
-        if constexpr (GATED) a8_gated8(a.e, y, u);
-        else a8_linear8(a.e, y, bias, res[k]);
-        a8_store8(a.e, y, m, n, m < a.M && n < a.N);
-      }
+      if constexpr (GATED) a8_gated8(a.e, y, u);
+      else a8_linear8(a.e, y, bias, res[k]);
+      a8_store8(a.e, y, m, n, in && m < a.M && n < a.N);
     }
   }
 }
@@ -217,7 +275,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   // A stage is MT steps: x block t with the CT weight blocks.  x of a step is read AHEAD steps before, across the stage's
   // end too: the barrier stands in step ENTER, where the first of the next stage is read.  A weight block is read for the
   // next stage behind its last product.
-    constexpr int RING = MT >= 4 ? 4 : 2, AHEAD = RING / 2, ENTER = MT - AHEAD;
+    constexpr int RING = MT % 4 == 0 ? 4 : 2, AHEAD = RING / 2, ENTER = MT - AHEAD;
   // A stage's loads are issued between the products from that barrier on, in the first POS of the MT CT places; FIRST of
   // them fall into the stage in which they begin.
   constexpr int POS = MT * CT * 3 / 4;
@@ -228,7 +286,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   static_assert(MT % RING == 0, "ring");
   static_assert((NBUF - 2) * LPT + FIRST < 64, "vmcnt immediate");
   __shared__ __align__(16) uint8_t buf[NBUF * STAGE];
-  __shared__ __align__(16) uint8_t scl[BN / 32][kA8SliceSteps * 4 + 16];
+  __shared__ __align__(16) uint8_t scl[BN / 32][kTileMaxK / 32 + 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
   const int wm = wave / WN, wn = wave - wm * WN;
@@ -236,21 +294,19 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   // weights in its L2
   const int per = gridDim.x / kXcds;
   const int id = (blockIdx.x % kXcds) * per + blockIdx.x / kXcds;
-  if (id >= a.mtiles * a.ntiles) return;
+  if (id >= a.mtiles * a.ntiles) return;  // (the grid is a multiple of the XCDs)
   const int strip = id / (kA8Strip * a.ntiles), sm = min(kA8Strip, a.mtiles - strip * kA8Strip);
   const int in = id - strip * kA8Strip * a.ntiles;
   const int m0 = (strip * kA8Strip + in % sm) * BM, n0 = in / sm * OC;
-  const int s0 = blockIdx.y * a.kslice;
-  const int nk = min(a.K / 128 - s0, a.kslice);  // whole stages of the slice
-  const int tail = a.K / 128 < s0 + a.kslice ? a.K % 128 : 0;  // k behind them, in the slice of that step
+  const int nk = a.K / 128, tail = a.K % 128;  // whole stages, and the k behind them
 
   // weight row r of the tile: output column (from n0) and matrix
   auto column = [&](int r) { return GATED ? (r / 64) * 32 + (r & 31) : r; };
   auto is_up = [&](int r) { return GATED && (r & 32) != 0; };
-  const uint8_t* xb = a.x + (long)m0 * a.K + s0 * 128l;
-  const uint8_t* wb = a.w + (long)n0 * a.K + s0 * 128l;
-  const uint8_t* wb2 = GATED ? a.w2 + (long)n0 * a.K + s0 * 128l : nullptr;
-  const uint8_t* xsb = a.xs + ((long)s0 * a.M + m0) * 4;
+  const uint8_t* xb = a.x + (long)m0 * a.K;
+  const uint8_t* wb = a.w + (long)n0 * a.K;
+  const uint8_t* wb2 = GATED ? a.w2 + (long)n0 * a.K : nullptr;
+  const uint8_t* xsb = a.xs + 4l * m0;
   // Load u of a thread brings 16 bytes of row u NT / 8 + tid / 8 (rows past the end repeat the last and are not stored).
   // Chunk c of a 128-byte row r sits at c ^ (r & 7): the 8 lanes of an LDS read cycle (8 rows, one chunk) then hit 8
   // different 16-byte bank groups.
@@ -260,7 +316,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   const uint32_t so = (uint32_t)min(sr, xlim) * 4;
   const uint32_t lds0 = lds_addr_of(buf);
   const uint32_t ldsw = lds0 + (uint32_t)wave * 1024, ldss = lds0 + XB + WB + (uint32_t)(wave % (SB / 256)) * 256;
-  const int klast = a.K - s0 * 128 - 16;  // the last 16 codes of a row, from the slice's start
+  const int klast = a.K - 16;  // the last 16 codes of a row
   uint32_t xo[XL], wo[WL];
 #pragma unroll
   for (int u = 0; u < XL; ++u) xo[u] = (uint32_t)min(u * (NT / 8) + r0, xlim) * (uint32_t)a.K;
@@ -279,11 +335,11 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
       a8_dma4(xsb + (long)kt * a.M * 4, so, ldss + l);
     }
   };
-  {  // the slice's weight scales
-    const int nb = (a.N + 31) / 32, kb = (nk * 128 + tail) / 32;
+  {  // the tile's weight scales
+    const int nb = (a.N + 31) / 32, kb = a.K / 32;
     auto scales = [&](int b) {
       const int row = min((n0 + column(b * 32)) / 32, nb - 1);
-      return (is_up(b * 32) ? a.ws2 + (long)row * a.Kc2 : a.ws + (long)row * a.Kc) + s0 * 4;
+      return (is_up(b * 32) ? a.ws2 + (long)row * a.Kc2 : a.ws + (long)row * a.Kc);
     };
     if (a.words) {  // whole words: by direct loads, ahead of the stages'
       for (int b = wave; b < BN / 32; b += WM * WN)
@@ -318,7 +374,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   int xs[RING], ws[CT];  // (bytes: a shift of a word would wait for it where it is read)
   auto fetch_w = [&](int j, int kt, int b) {
     wf[j] = operand(buf + b * STAGE + XB + (wr + 16 * j) * 128);
-    ws[j] = scl[wn * (CT / 2) + j / 2][kt * 4 + g];  // (kt may be one past the slice: the row is longer)
+    ws[j] = scl[(wn * CT + j) / 2][kt * 4 + g];  // (kt may be one past the last: the row is longer)
   };
   auto fetch_x = [&](int t, int b) {
     const uint8_t* st = buf + b * STAGE;
@@ -382,8 +438,9 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   // A lane (l16, g) has row l16, columns 4 g .. 4 g + 3 of a block: PM blocks of rows at a time through the wave's part of
   // the LDS (rows padded by 16 bytes: 8 lanes write 8 different bank groups)
   constexpr int LD = BN / WN * 4 + 16;
-  constexpr int PM = MT * 16 * LD * WM * WN <= NBUF * STAGE ? MT : MT * 8 * LD * WM * WN <= NBUF * STAGE ? MT / 2 : MT / 4;
-  static_assert(PM * 16 * LD * WM * WN <= NBUF * STAGE && MT % PM == 0 && PM % 2 == 0, "output staging");
+  constexpr int ROOM = NBUF * STAGE / (16 * LD * WM * WN);  // blocks of rows a wave has LDS for
+  constexpr int PM = ROOM >= MT ? MT : ROOM >= MT / 2 && MT % 2 == 0 ? MT / 2 : ROOM >= MT / 3 && MT % 3 == 0 ? MT / 3 : MT / 4;
+  static_assert(PM > 0 && PM <= ROOM && MT % PM == 0, "output staging");
   uint8_t* own = buf + wave * (PM * 16 * LD);
 #pragma unroll
   for (int p = 0; p < MT; p += PM) {
@@ -395,77 +452,61 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   }
 }
 
-// The K slices' partials summed in slice order and finished: 8 columns a thread, 4 adjacent lanes a block of 32.
-template <bool GATED>
-__global__ void __launch_bounds__(256) a8_sum_kernel(const A8Args a) {
-  const int q = (a.N + 31) / 32 * 4;  // threads of a row
-  const long t = (long)blockIdx.x * 256 + threadIdx.x;
-  const long m = t / q;
-  const int n = (int)(t - m * q) * 8;
-  const bool live = m < a.M && n < a.N;
-  A8x8 y, u;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y.v[i] = u.v[i] = 0.0f;
-  if (live) {
-    const uint4 res = a8_res8(a.e, (int)m, n);
-    const A8x8 bias = a8_bias8(a.e, n);
-    const float* p = a.part + m * a.ldp + n;
-#pragma unroll 4
-    for (int s = 0; s < a.splits; ++s) {
-      const A8x8 v = *(const A8x8*)(p + (long)s * a.M * a.ldp);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y.v[i] += v.v[i];
-      if constexpr (GATED) {
-        const A8x8 w = *(const A8x8*)(p + (long)s * a.M * a.ldp + a.ldp / 2);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) u.v[i] += w.v[i];
-      }
-    }
-    if constexpr (GATED) a8_gated8(a.e, y, u);
-    else a8_linear8(a.e, y, bias, res);
-  }
-  a8_store8(a.e, y, (int)m, n, live);
-}
-
 // ------------------------------------------------------------------------------------------------ plan
+// Up to 32 rows: the stream of one row block, exact.  16 columns a workgroup (one token, 8192 k, 5120 columns 10.6 us
+// against 13.3 of 32) unless the output is in blocks of 32 or there are columns enough to fill the card twice over (32768
+// columns of 1280 k 10.5 against 9.1 us, in workgroups of 2 waves, 10.3 in 4); 8 waves where a workgroup of 4 to every CU
+// would leave half of them idle (512 columns of 5120 k 5.3 against 6.1 us).
+// More rows: the least of the estimates below, microseconds a round of the card (measured over 10 to 64 steps; the
+// partly filled last round counted as a whole one, which it is within a tenth: 512 to 4096 rows of the layer's widths).
 constexpr int kCus = 256;
+enum A8Kernel { kStream16, kStream32, kStream64, kTile64x128, kTile64x256, kTile128, kTile192, kTile256 };
 struct A8Plan {
-  int rows;  // 0: the stream
-  int cols;  // weight rows of a tile (stream: output columns of a workgroup)
-  int splits, kslice, waves;
+  A8Kernel kernel;
+  int rows, cols, waves;  // a workgroup's rows of x, weight rows, and (streams) waves
 };
 
-A8Plan a8_plan(int M, int N, int K, bool gated) {
-  const int steps = (K + 127) / 128;
-  A8Plan p{0, 32, 1, steps, 8};
+A8Plan a8_plan(int M, int N, int K, bool gated, bool a8_out) {
   if (M <= 32) {
-    if (!gated && M <= 16 && N % 32 != 0) p.cols = 16;
-    return p;
+    const bool wide = N > 16384;
+    const int cols = a8_out || wide || (M > 16 && gated) ? 32 : 16;
+    return A8Plan{M <= 16 ? kStream16 : kStream32, M <= 16 ? 16 : 32, cols,
+                  wide ? 2 : M <= 16 && cols == 16 && N <= 16 * kCus / 2 ? 8 : 4};
   }
-  p.rows = M <= 64 ? 64 : M <= 2048 ? 128 : 256;
-  p.cols = M <= 2048 ? 128 : 256;
-  const long tiles = (long)((M + p.rows - 1) / p.rows) * ((N * (gated ? 2l : 1l) + p.cols - 1) / p.cols);
-  int s = (int)(2 * kCus / tiles);
-  s = s < 1 ? 1 : s > steps / 2 ? (steps / 2 < 1 ? 1 : steps / 2) : s;
-  const int least = (steps + kA8SliceSteps - 1) / kA8SliceSteps;
-  if (s < least) s = least;
-  p.kslice = (steps + s - 1) / s;
-  p.splits = (steps + p.kslice - 1) / p.kslice;
-  return p;
-}
-
-long a8_ldp(int N, bool gated) { return (long)(N + 31) / 32 * 32 * (gated ? 2 : 1); }
-
-long a8_workspace(int M, int N, int K, bool gated) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const A8Plan p = a8_plan(M, N, K, gated);
-  return p.rows == 0 || p.splits == 1 ? 0 : (long)p.splits * M * a8_ldp(N, gated) * 4;
+  struct Cost {
+    A8Plan plan;
+    float fixed, step;  // us of a round: launch, first loads and output; 128 k
+    int slots;
+  };
+  const Cost costs[] = {
+      {{kStream64, 64, gated ? 64 : 32, 4}, 3.0f, gated ? 0.28f : 0.155f, kCus},
+      {{kTile64x128, 64, 128, 4}, 5.0f, 0.33f, kCus},       // one workgroup a CU
+      {{kTile64x128, 64, 128, 4}, 8.3f, 0.53f, 2 * kCus},   // two
+      {{kTile64x256, 64, 256, 8}, 10.0f, 0.49f, kCus},
+      {{kTile128, 128, 256, 8}, 13.4f, 0.74f, kCus},
+      {{kTile192, 192, 256, 8}, 14.5f, 1.1f, kCus},
+      {{kTile256, 256, 256, 8}, 22.0f, 1.33f, kCus},
+  };
+  const float steps = (float)((K + 127) / 128);
+  const long wrows = (long)N * (gated ? 2 : 1);
+  A8Plan best = costs[0].plan;
+  float least = 0.0f;
+  for (const Cost& c : costs) {
+    if (c.plan.kernel != kStream64 && K > kTileMaxK) break;
+    const long groups = ((M + c.plan.rows - 1l) / c.plan.rows) * ((wrows + c.plan.cols - 1) / c.plan.cols);
+    const float us = (float)((groups + c.slots - 1) / c.slots) * (c.fixed + steps * c.step);
+    if (least == 0.0f || us < least) {
+      least = us;
+      best = c.plan;
+    }
+  }
+  return best;
 }
 
 template <bool GATED>
-int a8_run(A8Args& a, void* ws, long ws_bytes, hipStream_t st) {
+int a8_run(A8Args& a, hipStream_t st) {
   if (a.M == 0 || a.N == 0) return 0;
-  if (a.M < 0 || a.N < 0 || a.K <= 0 || a.K % 32 != 0 || a.Kc < a.K / 32 || (GATED && a.Kc2 < a.K / 32))
+  if (a.M < 0 || a.N < 0 || a.K <= 0 || a.K % 32 != 0 || a.K > kStreamMaxK || a.Kc < a.K / 32 || (GATED && a.Kc2 < a.K / 32))
     return (int)hipErrorInvalidValue;
   if (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.w2) & 15 || (uintptr_t)a.xs & 3) return (int)hipErrorInvalidValue;
   if (a.e.act < kActNone || a.e.act > kActGeluTanh || !(a.e.limit >= 0.0f)) return (int)hipErrorInvalidValue;
@@ -474,41 +515,36 @@ int a8_run(A8Args& a, void* ws, long ws_bytes, hipStream_t st) {
   a.e.N = a.N;
   a.e.vec = a.N % 8 == 0 && (((uintptr_t)a.e.out | (uintptr_t)a.e.res) & 15) == 0;
   a.words = a.K % 128 == 0 && ((a.Kc | a.Kc2 | (uintptr_t)a.ws | (uintptr_t)a.ws2) & 3) == 0;
-  const A8Plan p = a8_plan(a.M, a.N, a.K, GATED);
-  a.splits = p.splits;
-  a.kslice = p.kslice;
-  if (p.rows == 0) {
-    const dim3 g((unsigned)((a.N + p.cols - 1) / p.cols)), b((unsigned)(64 * p.waves));
-    const int mt = a.M <= 16 ? 1 : 2;
-    const size_t lds = (size_t)p.waves * (p.cols / 16) * (GATED ? 2 : 1) * mt * 1024;
-    if (p.cols == 16) {
-      if constexpr (!GATED) a8_stream_kernel<1, 1, false><<<g, b, lds, st>>>(a);
-    } else if (mt == 1) {
-      a8_stream_kernel<1, 2, GATED><<<g, b, lds, st>>>(a);
-    } else {
-      a8_stream_kernel<2, 2, GATED><<<g, b, lds, st>>>(a);
-    }
-    DSV41_CHECK_LAUNCH();
-    return 0;
-  }
-  if (p.splits > 1) {
-    a.ldp = a8_ldp(a.N, GATED);
-    a.part = (float*)ws;
-    if (!ws || ((uintptr_t)ws & 15) != 0 || ws_bytes < a8_workspace(a.M, a.N, a.K, GATED)) return (int)hipErrorInvalidValue;
-  }
-  const int oc = GATED ? p.cols / 2 : p.cols;
+  const A8Plan p = a8_plan(a.M, a.N, a.K, GATED, a.e.out == nullptr);
+  // (a stream's columns are the output's up to 32 rows, and in its 64-row form as in the tiles the weights' rows)
+  const int oc = GATED && a.M > 32 ? p.cols / 2 : p.cols;
   a.mtiles = (a.M + p.rows - 1) / p.rows;
   a.ntiles = (a.N + oc - 1) / oc;
-  const dim3 g((unsigned)((a.mtiles * a.ntiles + kXcds - 1) / kXcds * kXcds), (unsigned)p.splits);
-  if (p.rows == 64) a8_tile_kernel<64, 128, 2, 2, 2, GATED><<<g, 256, 0, st>>>(a);
-  else if (p.rows == 128) a8_tile_kernel<128, 128, 2, 2, 2, GATED><<<g, 256, 0, st>>>(a);
-  else a8_tile_kernel<256, 256, 2, 4, 2, GATED><<<g, 512, 0, st>>>(a);
-  DSV41_CHECK_LAUNCH();
-  if (p.splits > 1) {
-    const long t = (long)a.M * ((a.N + 31) / 32 * 4);
-    a8_sum_kernel<GATED><<<(unsigned)((t + 255) / 256), 256, 0, st>>>(a);
-    DSV41_CHECK_LAUNCH();
+  const dim3 gs((unsigned)a.ntiles, (unsigned)a.mtiles), gt((unsigned)((a.mtiles * a.ntiles + kXcds - 1) / kXcds * kXcds));
+  switch (p.kernel) {
+    case kStream16:
+      if (p.cols == 16 && p.waves == 8) a8_stream_kernel<1, 1, 8, 2, GATED, true><<<gs, 512, 0, st>>>(a);
+      else if (p.cols == 16) a8_stream_kernel<1, 1, 4, 2, GATED, true><<<gs, 256, 0, st>>>(a);
+      else if (p.waves == 2) a8_stream_kernel<1, 2, 2, 2, GATED, true><<<gs, 128, 0, st>>>(a);
+      else a8_stream_kernel<1, 2, 4, 2, GATED, true><<<gs, 256, 0, st>>>(a);
+      break;
+    case kStream32:
+      if (p.cols == 16) {
+        if constexpr (!GATED) a8_stream_kernel<2, 1, 4, 2, false, true><<<gs, 256, 0, st>>>(a);
+      } else if (p.waves == 2) {
+        a8_stream_kernel<2, 2, 2, 2, GATED, true><<<gs, 128, 0, st>>>(a);
+      } else {
+        a8_stream_kernel<2, 2, 4, 2, GATED, true><<<gs, 256, 0, st>>>(a);
+      }
+      break;
+    case kStream64: a8_stream_kernel<4, 2, 4, 2, GATED, false><<<gs, 256, 0, st>>>(a); break;
+    case kTile64x128: a8_tile_kernel<64, 128, 2, 2, 3, GATED><<<gt, 256, 0, st>>>(a); break;
+    case kTile64x256: a8_tile_kernel<64, 256, 2, 4, 3, GATED><<<gt, 512, 0, st>>>(a); break;
+    case kTile128: a8_tile_kernel<128, 256, 2, 4, 3, GATED><<<gt, 512, 0, st>>>(a); break;
+    case kTile192: a8_tile_kernel<192, 256, 2, 4, 2, GATED><<<gt, 512, 0, st>>>(a); break;
+    case kTile256: a8_tile_kernel<256, 256, 2, 4, 2, GATED><<<gt, 512, 0, st>>>(a); break;
   }
+  DSV41_CHECK_LAUNCH();
   return 0;
 }
 
@@ -516,11 +552,15 @@ int a8_run(A8Args& a, void* ws, long ws_bytes, hipStream_t st) {
 
 extern "C" {
 
-long dsv41_a8_workspace_bytes(int M, int N, int K, int gated) { return a8_workspace(M, N, K, gated != 0); }
+int dsv41_a8_plan(int M, int N, int K, int gated, int a8_out) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const A8Plan p = a8_plan(M, N, K, gated != 0, a8_out != 0);
+  return (p.kernel >= kTile64x128 ? 1 << 30 : 0) | p.rows << 16 | p.cols << 4 | p.waves;
+}
 
 int dsv41_linear_a8(const void* a8, const void* s8, const void* w8, const void* ws8, int M, int N, int K, int Kc,
                     const void* bias, int bias_f32, int act, const void* residual, void* out, void* out_a8,
-                    void* out_s8, void* ws, long ws_bytes, void* stream) {
+                    void* out_s8, void* stream) {
   A8Args a{};
   a.x = (const uint8_t*)a8;
   a.xs = (const uint8_t*)s8;
@@ -537,12 +577,12 @@ int dsv41_linear_a8(const void* a8, const void* s8, const void* w8, const void* 
   a.e.out = (uint16_t*)out;
   a.e.oa8 = (uint8_t*)out_a8;
   a.e.os8 = (uint8_t*)out_s8;
-  return a8_run<false>(a, ws, ws_bytes, (hipStream_t)stream);
+  return a8_run<false>(a, (hipStream_t)stream);
 }
 
 int dsv41_gated_a8(const void* a8, const void* s8, const void* wg8, const void* wgs8, const void* wu8,
                    const void* wus8, int M, int N, int K, int Kcg, int Kcu, int act, float limit, void* out,
-                   void* out_a8, void* out_s8, void* ws, long ws_bytes, void* stream) {
+                   void* out_a8, void* out_s8, void* stream) {
   A8Args a{};
   a.x = (const uint8_t*)a8;
   a.xs = (const uint8_t*)s8;
@@ -561,7 +601,7 @@ int dsv41_gated_a8(const void* a8, const void* s8, const void* wg8, const void* 
   a.e.oa8 = (uint8_t*)out_a8;
   a.e.os8 = (uint8_t*)out_s8;
   if (!wu8 || !wus8) return (int)hipErrorInvalidValue;
-  return a8_run<true>(a, ws, ws_bytes, (hipStream_t)stream);
+  return a8_run<true>(a, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import call, lib, ptr, require_gpu, stream
+from ._lib import call, ptr, require_gpu, stream
 from .w8 import W8, unpermute_k
 
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
@@ -134,15 +134,12 @@ def _operands(name: str, x: A8, act: str, out, *ws: W8):
     return dev, M, N, K
 
 
-def _product(name, x, out, dev, M, N, K, gated, head, tail):
-    """The launch: head arguments, sizes, tail arguments, the output's three pointers, workspace."""
+def _product(name, x, out, dev, M, N, K, head, tail):
+    """The launch: head arguments, sizes, tail arguments, the output's three pointers."""
     shape = (*x.shape[:-1], N)
     y = _new(M, N, dev, shape) if out is A8 else torch.empty(shape, dtype=torch.bfloat16, device=dev)
-    n = lib().dsv41_a8_workspace_bytes(M, N, K, gated)
-    # a call's own: the allocator keeps it to this stream, and a captured call to its graph
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n > 0 else None
     o = (None, ptr(y.a8), ptr(y.s8)) if out is A8 else (ptr(y), None, None)
-    _launch(name, dev, *head, M, N, K, *tail, *o, ptr(ws), n)
+    _launch(name, dev, *head, M, N, K, *tail, *o)
     return y
 
 
@@ -166,7 +163,7 @@ def linear_a8(x: A8, w: W8, bias: torch.Tensor | None = None, act: str = "none",
         residual = residual.contiguous()
     xa, wa = _aligned(x.a8), _aligned(w.w8)
     xs = _aligned(x.s8, 4)
-    return _product("dsv41_linear_a8", x, out, dev, M, N, K, 0, (ptr(xa), ptr(xs), ptr(wa), ptr(w.s8)),
+    return _product("dsv41_linear_a8", x, out, dev, M, N, K, (ptr(xa), ptr(xs), ptr(wa), ptr(w.s8)),
                     (w.s8.shape[1], ptr(bias), int(bias is not None and bias.dtype == torch.float32), ACTS[act],
                      ptr(residual)))
 
@@ -181,6 +178,6 @@ def gated_a8(x: A8, w_gate: W8, w_up: W8, act: str = "silu", limit: float = 0.0,
         raise ValueError(f"gated_a8: limit {limit} (0: none)")
     xa, ga, ua = _aligned(x.a8), _aligned(w_gate.w8), _aligned(w_up.w8)
     xs = _aligned(x.s8, 4)
-    return _product("dsv41_gated_a8", x, out, dev, M, N, K, 1,
+    return _product("dsv41_gated_a8", x, out, dev, M, N, K,
                     (ptr(xa), ptr(xs), ptr(ga), ptr(w_gate.s8), ptr(ua), ptr(w_up.s8)),
                     (w_gate.s8.shape[1], w_up.s8.shape[1], ACTS[act], float(limit)))

@@ -332,25 +332,25 @@ int dsv41_fp8_gemv_m1_pre(const void* x_raw, const void* norm_w, float eps, int 
 int dsv41_norm_quant8(const void* x, const void* residual, const void* w, float eps, void* h, void* a8, void* s8,
                       long n_rows, int D, void* stream);
 
-/* Workspace bytes of dsv41_linear_a8 (gated 0) or dsv41_gated_a8 (gated 1): 0, or the fp32 partials of K slices.  It
- * need not be initialised and holds nothing between calls; 16-byte aligned. */
-long dsv41_a8_workspace_bytes(int M, int N, int K, int gated);
-
 /* y[m, n] = act(sum_k x[m, k] w[n, k] + bias[n]) + residual[m, n]: x 8-bit activations [M, K], w e4m3 [N, K] in the
- * PERM_K byte order (16-byte aligned) with E8M0 scales [ceil(N / 32), Kc], Kc >= K / 32 (dsv41/w8.py:39-60); K % 32 == 0.
+ * PERM_K byte order (16-byte aligned) with E8M0 scales [ceil(N / 32), Kc], Kc >= K / 32 (dsv41/w8.py:39-60); K % 32 == 0, K <= 32768.
  * bias bf16 or (bias_f32) fp32 [N] or null; act 0 none, 1 relu, 2 silu, 3 gelu (erf), 4 gelu by tanh; residual bf16
  * [M, N] or null.  Exactly one output: out bf16 [M, N], or (out null) out_a8 / out_s8, the result as 8-bit activations,
  * N % 32 == 0.  fp32 sums on the block-scaled fp8 matrix instructions (2^-16 relative), rounded once.  Replaces
  * cukern.fp8_gemm_tc (dsv41/cukern.py:164-200) where x is held in 8 bits. */
 int dsv41_linear_a8(const void* a8, const void* s8, const void* w8, const void* ws8, int M, int N, int K, int Kc,
                     const void* bias, int bias_f32, int act, const void* residual, void* out, void* out_a8,
-                    void* out_s8, void* ws, long ws_bytes, void* stream);
+                    void* out_s8, void* stream);
+
+/* The kernel that a product of these sizes (a8_out: with 8-bit output) runs on: rows << 16 | columns << 4 | waves of its
+ * workgroups, with bit 30 set for the tile kernels (columns of weights) and clear for the streams. */
+int dsv41_a8_plan(int M, int N, int K, int gated, int a8_out);
 
 /* y = act(min(x Wg^T, limit)) * clamp(x Wu^T, -limit, limit) (limit 0: as they are), operands, act and outputs as
  * dsv41_linear_a8; wg8, wu8 [N, K] with scales of Kcg and Kcu columns. */
 int dsv41_gated_a8(const void* a8, const void* s8, const void* wg8, const void* wgs8, const void* wu8,
                    const void* wus8, int M, int N, int K, int Kcg, int Kcu, int act, float limit, void* out,
-                   void* out_a8, void* out_s8, void* ws, long ws_bytes, void* stream);
+                   void* out_a8, void* out_s8, void* stream);
 
 /* ------------------------------------------------------------------------------------------------ numerics */
 

@@ -1,6 +1,4 @@
 """8-bit activations without a GPU: the container, the refusals of the shims and of the C entry points."""
-import ctypes
-
 import pytest
 import torch
 
@@ -87,20 +85,18 @@ def test_norm_entry_refusals():
         assert _norm(**bad) == 1, bad
 
 
-def _linear(x=P, xs=P, w=P, ws=P, M=4, N=64, K=64, Kc=2, bias=None, bf=0, act=0, res=None, out=P, oa=None, os=None,
-            work=None, n=0):
-    return lib().dsv41_linear_a8(x, xs, w, ws, M, N, K, Kc, bias, bf, act, res, out, oa, os, work, n, None)
+def _linear(x=P, xs=P, w=P, ws=P, M=4, N=64, K=64, Kc=2, bias=None, bf=0, act=0, res=None, out=P, oa=None, os=None):
+    return lib().dsv41_linear_a8(x, xs, w, ws, M, N, K, Kc, bias, bf, act, res, out, oa, os, None)
 
 
-def _gated(x=P, xs=P, g=P, gs=P, u=P, us=P, M=4, N=64, K=64, Kg=2, Ku=2, act=2, limit=0.0, out=P, oa=None, os=None,
-           work=None, n=0):
-    return lib().dsv41_gated_a8(x, xs, g, gs, u, us, M, N, K, Kg, Ku, act, limit, out, oa, os, work, n, None)
+def _gated(x=P, xs=P, g=P, gs=P, u=P, us=P, M=4, N=64, K=64, Kg=2, Ku=2, act=2, limit=0.0, out=P, oa=None, os=None):
+    return lib().dsv41_gated_a8(x, xs, g, gs, u, us, M, N, K, Kg, Ku, act, limit, out, oa, os, None)
 
 
 def test_product_entry_refusals():
     for f in (_linear, _gated):
         assert f(M=0) == 0 and f(N=0) == 0
-        for bad in [dict(M=-1), dict(N=-1), dict(K=0), dict(K=48), dict(x=P + 8), dict(xs=P + 1), dict(act=5),
+        for bad in [dict(M=-1), dict(N=-1), dict(K=0), dict(K=48), dict(K=32800, Kc=1025) if f is _linear else dict(K=32800, Kg=1025, Ku=1025), dict(x=P + 8), dict(xs=P + 1), dict(act=5),
                     dict(act=-1), dict(out=None), dict(out=None, oa=P), dict(out=None, oa=P, os=P, N=40),
                     dict(out=None, oa=P + 8, os=P)]:
             assert f(**bad) == 1, (f.__name__, bad)
@@ -109,18 +105,3 @@ def test_product_entry_refusals():
     for bad in [dict(g=P + 8), dict(u=P + 8), dict(u=None), dict(us=None), dict(Kg=1), dict(Ku=1), dict(limit=-1.0),
                 dict(limit=float("nan"))]:
         assert _gated(**bad) == 1, bad
-
-
-def test_workspace_is_of_the_call_and_asked_for():
-    """K slices need their partials: whole rows of 32-column blocks (twice for gate and up), none for few or many rows."""
-    L = lib()
-    assert L.dsv41_a8_workspace_bytes(1, 5120, 8192, 0) == 0 and L.dsv41_a8_workspace_bytes(0, 5120, 8192, 0) == 0
-    assert L.dsv41_a8_workspace_bytes(8192, 5120, 8192, 0) == 0
-    for gated in (0, 1):
-        n = L.dsv41_a8_workspace_bytes(130, 1000, 5120, gated)
-        assert n > 0 and n % (130 * 1024 * (1 + gated) * 4) == 0
-    n = L.dsv41_a8_workspace_bytes(130, 1000, 5120, 0)
-    args = dict(M=130, N=1000, K=5120, Kc=160)
-    for bad in [dict(work=None, n=n), dict(work=P, n=n - 1), dict(work=P + 4, n=n)]:
-        assert _linear(**args, **bad) == 1, bad
-    assert isinstance(n, int) and ctypes.sizeof(ctypes.c_long) == 8

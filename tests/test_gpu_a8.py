@@ -173,7 +173,25 @@ def test_norm_quant8_views_and_sizes():
 SIZES = [(1, 1, 32), (1, 33, 64), (2, 100, 96), (5, 512, 128), (15, 257, 160), (16, 64, 1280), (17, 96, 1312), (31, 130, 224),
          (32, 2080, 512), (33, 64, 32), (40, 129, 96), (64, 257, 1280), (65, 1000, 160), (127, 128, 2080), (129, 384, 640),
          (200, 511, 5120), (257, 260, 352), (300, 1280, 288)]
-LARGE = [(2049, 513, 288), (2100, 1056, 1184), (4097, 256, 128)]
+LARGE = [(2049, 513, 288), (2100, 1056, 1184), (4097, 256, 128), (1, 16416, 128), (20, 17000, 160), (3, 4096, 8224),
+         (30, 2080, 4128), (1100, 2080, 160), (450, 4640, 6176), (1024, 8160, 640), (2049, 4096, 1312), (4090, 4064, 1280),
+         (70, 64, 20000), (40, 33, 32768)]
+
+
+def plan(m, n, k, gated=False, a8=False):
+    from dsv41_amd._lib import lib
+    return lib().dsv41_a8_plan(m, n, k, int(gated), int(a8))
+
+
+def test_sizes_reach_every_kernel():
+    """(rows, columns, waves) of the streams and tiles that the sizes below run on."""
+    kinds = lambda ps: {(p >> 30, p >> 16 & 0x3fff, p >> 4 & 0xfff, p & 15) for p in ps}  # noqa: E731
+    tiles = {(1, 64, 128, 4), (1, 64, 256, 8), (1, 128, 256, 8), (1, 192, 256, 8), (1, 256, 256, 8)}
+    assert kinds(plan(*s, a8=a) for s in SIZES + LARGE for a in (False, True) if not a or s[1] % 32 == 0) == tiles | {
+        (0, 16, 16, 8), (0, 16, 16, 4), (0, 16, 32, 4), (0, 16, 32, 2), (0, 32, 16, 4), (0, 32, 32, 4), (0, 32, 32, 2),
+        (0, 64, 32, 4)}
+    assert kinds(plan(*s, gated=True, a8=a) for s in GATED + GATED_LARGE for a in (False, True)) == tiles | {
+        (0, 16, 16, 8), (0, 16, 16, 4), (0, 16, 32, 4), (0, 16, 32, 2), (0, 32, 32, 4), (0, 32, 32, 2), (0, 64, 64, 4)}
 
 
 @pytest.mark.parametrize("m,n,k", SIZES + LARGE)
@@ -181,7 +199,7 @@ def test_linear_a8_whole_numbers(m, n, k):
     g = gen("whole", m, n, k)
     (x, xv), (w, wv) = whole_a8(g, m, k), whole_w8(g, n, k)
     y = linear_a8(x, w)
-    want = xv @ wv.t()
+    want = (xv.to(DEV) @ wv.to(DEV).t()).cpu()
     assert y.shape == (m, n) and y.dtype == BF and torch.equal(y.cpu(), want.to(BF))
     if n % 32 == 0:
         q = linear_a8(x, w, out=A8)
@@ -310,6 +328,8 @@ def test_refusals():
 # ------------------------------------------------------------------------------------------------ gated_a8
 GATED = [(1, 32, 32), (2, 96, 96), (16, 512, 1280), (17, 64, 160), (32, 224, 512), (33, 32, 64), (64, 160, 1280),
          (100, 1024, 352), (129, 416, 5120), (300, 288, 160), (2049, 288, 224)]
+GATED_LARGE = [(2, 16416, 96), (5, 2080, 4128), (18, 16896, 64), (1100, 1056, 160), (450, 2336, 6176), (1024, 4064, 640),
+               (2049, 2048, 1312), (4090, 2016, 1280)]
 
 
 @pytest.mark.parametrize("m,n,k", GATED)
@@ -329,6 +349,18 @@ def test_gated_a8(m, n, k, act, limit):
     check_a8(q, want, err)
     again = gated_a8(x, wg, wu, act=act, limit=limit)
     assert torch.equal(q.a8, again.a8) and torch.equal(q.s8, again.s8)
+
+
+@pytest.mark.parametrize("m,n,k", GATED_LARGE)
+def test_gated_a8_large(m, n, k):
+    g = gen("gated large", m, n, k)
+    (x, xv), (wg, gv), (wu, uv) = whole_a8(g, m, k), whole_w8(g, n, k), whole_w8(g, n, k)
+    wg, wu = W8(wg.w8, wg.s8 - 6, permuted=True), W8(wu.w8, wu.s8 - 4, permuted=True)
+    gate, up = ((xv.to(DEV) @ v.to(DEV).t()).cpu() / d for v, d in ((gv, 64), (uv, 16)))
+    want = R.act(gate, "silu") * up
+    err = want.abs() * (ACT_ERR + 2.0 ** -23) + 1e-30
+    check_bf16(gated_a8(x, wg, wu, out=BF), want, err)
+    check_a8(gated_a8(x, wg, wu), want, err)
 
 
 def test_gated_a8_odd_columns_in_bf16():
