@@ -135,6 +135,11 @@ def stream(dev: torch.device) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
 
 
+def stream_of(index: int) -> int:
+    """The raw handle of the current stream of GPU `index`."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def require_gpu(*ts: torch.Tensor | None) -> torch.device:
     dev = None
     for t in ts:

@@ -11,9 +11,11 @@ matrix instructions.  What stands between the attention layer and the next one i
 Forward only, as everything here: inputs that require a gradient are refused while gradients are recorded."""
 from __future__ import annotations
 
+import math
+
 import torch
 
-from ._lib import call, ptr, require_gpu, stream
+from ._lib import as_bf16, call, ptr, require_gpu, stream_of
 from .w8 import W8, unpermute_k
 
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
@@ -34,6 +36,8 @@ class A8:
             raise ValueError(f"A8: scales {tuple(s8.shape)} for codes {tuple(a8.shape)}: [ceil(K / 128), rows, 4] expected")
         if s8.device != a8.device:
             raise RuntimeError(f"A8: codes on {a8.device}, scales on {s8.device}")
+        if shape is not None and (shape[-1] != k or math.prod(shape[:-1]) != rows):
+            raise ValueError(f"A8: shape {tuple(shape)} for codes {tuple(a8.shape)}")
         self.a8, self.s8 = a8.contiguous(), s8.contiguous()
         self.shape = tuple(a8.shape) if shape is None else tuple(shape)
 
@@ -59,18 +63,28 @@ class A8:
         return self.float().to(torch.bfloat16)
 
 
-def _no_grad(name: str, *ts) -> None:
-    if torch.is_grad_enabled():
-        for t in ts:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{name}: forward only (an input requires a gradient)")
+def _index(*ts: torch.Tensor | None) -> int:
+    """The index of the GPU that the tensors are on (the first is one); raises as require_gpu does."""
+    i = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != i:
+            require_gpu(*ts)
+    if i < 0:
+        require_gpu(*ts)
+    return i
+
+
+def _no_grad(name: str, *ts: torch.Tensor | None) -> None:
+    for t in ts:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name}: forward only (an input requires a gradient)")
 
 
 def _aligned(t: torch.Tensor, n: int = 16) -> torch.Tensor:
     return t if t.data_ptr() % n == 0 else t.clone()
 
 
-def _new(rows: int, k: int, dev, shape) -> A8:
+def _codes(rows: int, k: int, dev: torch.device, shape: tuple) -> A8:
     q = A8.__new__(A8)
     q.a8 = torch.empty(rows, k, dtype=torch.uint8, device=dev)
     q.s8 = torch.empty((k + 127) // 128, rows, 4, dtype=torch.uint8, device=dev)
@@ -78,13 +92,13 @@ def _new(rows: int, k: int, dev, shape) -> A8:
     return q
 
 
-def _launch(name: str, dev: torch.device, *args) -> None:
-    """The call on dev's current stream, with dev current."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        call(name, *args, stream(dev))
+def _launch(name: str, index: int, *args) -> None:
+    """The call on the current stream of GPU `index`, with that GPU current."""
+    if index == torch.cuda.current_device():
+        call(name, *args, stream_of(index))
     else:
-        with torch.cuda.device(dev):
-            call(name, *args, stream(dev))
+        with torch.cuda.device(index):
+            call(name, *args, stream_of(index))
 
 
 def norm_quant8(x: torch.Tensor, w: torch.Tensor | None, eps: float, residual: torch.Tensor | None = None):
@@ -93,54 +107,59 @@ def norm_quant8(x: torch.Tensor, w: torch.Tensor | None, eps: float, residual: t
     x, residual: bf16 [..., D], D % 32 == 0, D <= 16384; w: [D] or None (no norm: the quantisation alone).  Returns the
     A8, with a residual (A8, h): h = bf16(x + residual), the stream that the norm is of.  The normed value is rounded
     once, to 8 bits (norm_quant rounds to bf16 in between, as the reference does, so single codes differ from its)."""
-    dev = require_gpu(x, residual, w)
+    index = _index(x, residual, w)
     _no_grad("norm_quant8", x, residual, w)
-    D = x.shape[-1] if x.dim() else 0
+    shape = x.shape
+    D = shape[-1] if shape else 0
     if x.dtype != torch.bfloat16 or (residual is not None and residual.dtype != torch.bfloat16):
         raise RuntimeError("norm_quant8: bf16 rows expected")
     if D == 0 or D % 32 or D > 16384:
         raise RuntimeError(f"norm_quant8: rows of {D} (a multiple of 32, at most 16384)")
-    if residual is not None and residual.shape != x.shape:
-        raise RuntimeError(f"norm_quant8: residual {tuple(residual.shape)} for x {tuple(x.shape)}")
-    if w is not None and w.shape != (D,):
-        raise RuntimeError(f"norm_quant8: weight {tuple(w.shape)} for rows of {D}")
-    xc = _aligned(x.contiguous())
-    rows = xc.numel() // D
-    wc = None if w is None else _aligned(w.to(torch.bfloat16).contiguous())
-    q = _new(rows, D, dev, tuple(x.shape))
-    h = rc = None
-    if residual is not None:
-        rc = _aligned(residual.contiguous())
-        h = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
-    _launch("dsv41_norm_quant8", dev, ptr(xc), ptr(rc), ptr(wc), float(eps), ptr(h), ptr(q.a8), ptr(q.s8), rows, D)
-    return q if residual is None else (q, h)
+    if residual is not None and residual.shape != shape:
+        raise RuntimeError(f"norm_quant8: residual {tuple(residual.shape)} for x {tuple(shape)}")
+    if w is not None:
+        if w.dim() != 1 or w.shape[0] != D:
+            raise RuntimeError(f"norm_quant8: weight {tuple(w.shape)} for rows of {D}")
+        w = _aligned(as_bf16(w))
+    x = _aligned(x.contiguous())
+    rows = x.numel() // D
+    q = _codes(rows, D, x.device, shape)
+    if residual is None:
+        _launch("dsv41_norm_quant8", index, x.data_ptr(), None, ptr(w), eps, None, q.a8.data_ptr(), q.s8.data_ptr(), rows, D)
+        return q
+    residual = _aligned(residual.contiguous())
+    h = torch.empty_like(x)
+    _launch("dsv41_norm_quant8", index, x.data_ptr(), residual.data_ptr(), ptr(w), eps, h.data_ptr(), q.a8.data_ptr(),
+            q.s8.data_ptr(), rows, D)
+    return q, h
 
 
-def _operands(name: str, x: A8, act: str, out, *ws: W8):
-    if not isinstance(x, A8) or not all(isinstance(w, W8) for w in ws):
+def _operands(name: str, x: A8, act: str, out, w: W8):
+    """Checks of one weight; its columns and K."""
+    if not isinstance(x, A8) or not isinstance(w, W8):
         raise TypeError(f"{name}: an A8 and W8 weights expected")
-    dev = require_gpu(x.a8, x.s8, *(t for w in ws for t in (w.w8, w.s8)))
     if act not in ACTS:
         raise ValueError(f"{name}: act {act!r} (one of {', '.join(ACTS)})")
     if out is not A8 and out is not torch.bfloat16:
         raise ValueError(f"{name}: out {out} (torch.bfloat16 or A8; fp32 sums: w8.fp8_gemm_tc)")
-    M, K = x.a8.shape
-    N = ws[0].shape[0]
-    for w in ws:
-        if w.w8.shape != (N, K) or w.s8.dim() != 2 or w.s8.shape[0] < (N + 31) // 32 or w.s8.shape[1] < K // 32:
-            raise RuntimeError(f"{name}: weight {tuple(w.w8.shape)}, scales {tuple(w.s8.shape)} for x {x.shape}")
+    K = x.shape[-1]
+    N, Kw = w.shape
+    s = w.s8.shape
+    if Kw != K or K > 32768 or len(s) != 2 or s[0] < (N + 31) // 32 or s[1] < K // 32:
+        raise RuntimeError(f"{name}: weight {(N, Kw)}, scales {tuple(s)} for x {tuple(x.shape)} (K at most 32768)")
     if out is A8 and N % 32:
         raise RuntimeError(f"{name}: {N} columns in 8 bits (a multiple of 32)")
-    return dev, M, N, K
+    return N, K
 
 
-def _product(name, x, out, dev, M, N, K, head, tail):
-    """The launch: head arguments, sizes, tail arguments, the output's three pointers."""
+def _output(x: A8, N: int, out, dev: torch.device):
+    """The result, and its three pointers."""
     shape = (*x.shape[:-1], N)
-    y = _new(M, N, dev, shape) if out is A8 else torch.empty(shape, dtype=torch.bfloat16, device=dev)
-    o = (None, ptr(y.a8), ptr(y.s8)) if out is A8 else (ptr(y), None, None)
-    _launch(name, dev, *head, M, N, K, *tail, *o)
-    return y
+    if out is A8:
+        y = _codes(x.a8.shape[0], N, dev, shape)
+        return y, None, y.a8.data_ptr(), y.s8.data_ptr()
+    y = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    return y, y.data_ptr(), None, None
 
 
 def linear_a8(x: A8, w: W8, bias: torch.Tensor | None = None, act: str = "none", residual: torch.Tensor | None = None,
@@ -149,23 +168,27 @@ def linear_a8(x: A8, w: W8, bias: torch.Tensor | None = None, act: str = "none",
 
     x: A8 [..., K]; w: W8 [N, K]; bias: [N] bf16 or fp32; act: none, relu, silu, gelu (erf), gelu_tanh; residual: bf16
     [..., N].  fp32 sums; bias, activation and residual are applied to them and the result is rounded once."""
-    dev, M, N, K = _operands("linear_a8", x, act, out, w)
-    _no_grad("linear_a8", bias, residual)
+    N, K = _operands("linear_a8", x, act, out, w)
+    xa, xs, wa, ws = x.a8, x.s8, w.w8, w.s8
+    index = _index(xa, xs, wa, ws, bias, residual)
+    bias_f32 = 0
     if bias is not None:
         if bias.shape != (N,) or bias.dtype not in (torch.bfloat16, torch.float32):
             raise RuntimeError(f"linear_a8: bias {tuple(bias.shape)} {bias.dtype} (bf16 or fp32 [{N}])")
-        require_gpu(x.a8, bias)
+        _no_grad("linear_a8", bias)
+        bias_f32 = int(bias.dtype == torch.float32)
         bias = bias.contiguous()
     if residual is not None:
         if residual.shape != (*x.shape[:-1], N) or residual.dtype != torch.bfloat16:
             raise RuntimeError(f"linear_a8: residual {tuple(residual.shape)} {residual.dtype} (bf16 {(*x.shape[:-1], N)})")
-        require_gpu(x.a8, residual)
+        _no_grad("linear_a8", residual)
         residual = residual.contiguous()
-    xa, wa = _aligned(x.a8), _aligned(w.w8)
-    xs = _aligned(x.s8, 4)
-    return _product("dsv41_linear_a8", x, out, dev, M, N, K, (ptr(xa), ptr(xs), ptr(wa), ptr(w.s8)),
-                    (w.s8.shape[1], ptr(bias), int(bias is not None and bias.dtype == torch.float32), ACTS[act],
-                     ptr(residual)))
+    if (xa.data_ptr() | wa.data_ptr()) & 15 or xs.data_ptr() & 3:
+        xa, xs, wa = _aligned(xa), _aligned(xs, 4), _aligned(wa)
+    y, o, oa, os = _output(x, N, out, xa.device)
+    _launch("dsv41_linear_a8", index, xa.data_ptr(), xs.data_ptr(), wa.data_ptr(), ws.data_ptr(), xa.shape[0], N, K,
+            ws.shape[1], ptr(bias), bias_f32, ACTS[act], ptr(residual), o, oa, os)
+    return y
 
 
 def gated_a8(x: A8, w_gate: W8, w_up: W8, act: str = "silu", limit: float = 0.0, out=A8):
@@ -173,11 +196,16 @@ def gated_a8(x: A8, w_gate: W8, w_up: W8, act: str = "silu", limit: float = 0.0,
 
     x: A8 [..., K]; w_gate, w_up: W8 [N, K]; act as linear_a8's.  limit > 0: the gate's sum is held to at most limit and
     the up sum to [-limit, limit] first.  Both sums stay in registers; the result is rounded once."""
-    dev, M, N, K = _operands("gated_a8", x, act, out, w_gate, w_up)
+    N, K = _operands("gated_a8", x, act, out, w_gate)
+    if _operands("gated_a8", x, act, out, w_up) != (N, K):
+        raise RuntimeError(f"gated_a8: gate {w_gate.shape}, up {w_up.shape}")
     if not limit >= 0.0:
         raise ValueError(f"gated_a8: limit {limit} (0: none)")
-    xa, ga, ua = _aligned(x.a8), _aligned(w_gate.w8), _aligned(w_up.w8)
-    xs = _aligned(x.s8, 4)
-    return _product("dsv41_gated_a8", x, out, dev, M, N, K,
-                    (ptr(xa), ptr(xs), ptr(ga), ptr(w_gate.s8), ptr(ua), ptr(w_up.s8)),
-                    (w_gate.s8.shape[1], w_up.s8.shape[1], ACTS[act], float(limit)))
+    xa, xs, ga, gs, ua, us = x.a8, x.s8, w_gate.w8, w_gate.s8, w_up.w8, w_up.s8
+    index = _index(xa, xs, ga, gs, ua, us)
+    if (xa.data_ptr() | ga.data_ptr() | ua.data_ptr()) & 15 or xs.data_ptr() & 3:
+        xa, xs, ga, ua = _aligned(xa), _aligned(xs, 4), _aligned(ga), _aligned(ua)
+    y, o, oa, os = _output(x, N, out, xa.device)
+    _launch("dsv41_gated_a8", index, xa.data_ptr(), xs.data_ptr(), ga.data_ptr(), gs.data_ptr(), ua.data_ptr(),
+            us.data_ptr(), xa.shape[0], N, K, gs.shape[1], us.shape[1], ACTS[act], limit, o, oa, os)
+    return y

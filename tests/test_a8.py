@@ -43,6 +43,9 @@ def test_container_refusals():
                  (u(64), u(1, 1, 4)), (u(4, 64), u(1, 4, 4).int())]:
         with pytest.raises(ValueError):
             A8(a, s)
+    for shape in [(4, 32), (2, 3, 64), (64,), (4, 2, 64)]:
+        with pytest.raises(ValueError):
+            A8(u(4, 64), u(1, 4, 4), shape)
 
 
 def test_cpu_tensors_are_refused():
