@@ -48,7 +48,8 @@ DSV41_DEV float a8_exp(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 // silu(v) = v / (1 + e^-v); gelu_tanh(v) = v / (1 + e^(-2 c (v + 0.044715 v^3))), c = sqrt(2 / pi): 1/2 (1 + tanh z) is
 // 1 / (1 + e^-2z).  gelu(v) = v Phi(v), Phi(-a) = e^(-a^2 / 2) R(1 / (1 + 0.35 a)): R a polynomial of degree 7 fitted to
 // erfcx(a / sqrt 2) / 2 over a <= 14 for the relative error (3.1e-7), so that the tail keeps its digits.
-DSV41_DEV float a8_act(float v, int act) {
+template <int act>
+DSV41_DEV float a8_act(float v) {
   if (act == kActRelu) return v < 0.0f ? 0.0f : v;  // (NaN stays)
   if (act == kActSilu || act == kActGeluTanh) {
     const float z = act == kActSilu ? v : v * __builtin_fmaf(0.07135481283f, v * v, 1.595769122f);
@@ -118,13 +119,22 @@ DSV41_DEV uint4 a8_res8(const A8Epi& e, int m, int n) {
     if (n + i < e.N) u[i >> 1] |= (uint32_t)r[i] << (16 * (i & 1));
   return make_uint4(u[0], u[1], u[2], u[3]);
 }
+template <int ACT>
+DSV41_DEV void a8_act8(A8x8& y) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y.v[i] = a8_act<ACT>(y.v[i]);
+}
+// (one branch for the 8 of them)
+DSV41_DEV void a8_act8(A8x8& y, int act) {
+  if (act == kActSilu) a8_act8<kActSilu>(y);
+  else if (act == kActRelu) a8_act8<kActRelu>(y);
+  else if (act == kActGelu) a8_act8<kActGelu>(y);
+  else if (act == kActGeluTanh) a8_act8<kActGeluTanh>(y);
+}
 DSV41_DEV void a8_linear8(const A8Epi& e, A8x8& y, const A8x8& bias, uint4 res) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) y.v[i] += bias.v[i];
-  if (e.act != kActNone) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y.v[i] = a8_act(y.v[i], e.act);
-  }
+  a8_act8(y, e.act);
   if (e.res) {
     float r[8];
     a8_unpack8(res, r);
@@ -140,8 +150,9 @@ DSV41_DEV void a8_gated8(const A8Epi& e, A8x8& g, A8x8& u) {
       u.v[i] = u.v[i] > e.limit ? e.limit : u.v[i] < -e.limit ? -e.limit : u.v[i];
     }
   }
+  a8_act8(g, e.act);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) g.v[i] = a8_act(g.v[i], e.act) * u.v[i];
+  for (int i = 0; i < 8; ++i) g.v[i] *= u.v[i];
 }
 
 DSV41_DEV long a8_scale_at(int M, int m, int block) { return ((long)(block >> 2) * M + m) * 4 + (block & 3); }

@@ -3,8 +3,8 @@
 //   gated:  y[m, n] = act(min(g, limit)) clamp(u, -limit, limit),  g = sum_k x wg, u = sum_k x wu
 // x and y: A8 (a8_core.h), y also bf16; w: e4m3 codes [N, K] and E8M0 scales per [32 x 32] block (dsv41/w8.py:39-60).
 // Both operands keep their bytes: the block-scaled matrix instructions take the codes and the scales of 32 k of a row as
-// they are.  A lane's 32 codes of such an instruction (R = 16 or 32 rows, KI = 128 or 64 k, lane group g = lane / R) are
-// k 16 g .. 16 g + 15 and KI / 2 + 16 g .. KI / 2 + 16 g + 15, and the scale it gives is that of k 32 g .. 32 g + 31.
+// they are.  A lane's 32 codes of the instruction (16 rows, 128 k; lane group g = lane / 16) are k 16 g .. 16 g + 15 and
+// 64 + 16 g .. 64 + 16 g + 15, and the scale it gives is that of k 32 g .. 32 g + 31.
 // The instruction adds its products with about 2^-16 of relative error (measured 1.5e-5 in the 2-norm at every K, random
 // in sign), well below half a step of bf16 (2^-9 of a value) or of e4m3; outputs are therefore bf16 or A8, not fp32.
 // Sums over k are fp32, in a fixed order.
@@ -277,8 +277,9 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   // next stage behind its last product.
     constexpr int RING = MT % 4 == 0 ? 4 : 2, AHEAD = RING / 2, ENTER = MT - AHEAD;
   // A stage's loads are issued between the products from that barrier on, in the first POS of the MT CT places; FIRST of
-  // them fall into the stage in which they begin.
-  constexpr int POS = MT * CT * 3 / 4;
+  // them fall into the stage in which they begin.  With two buffers they have less than a stage to land and go out early
+  // (3/8 of the places against 3/4: 291 and 318 us for the gated 4096 x 8192 x 5120); with three, 3/4 is as good or better.
+  constexpr int POS = MT * CT * (NBUF == 2 ? 3 : 6) / 8;
   constexpr auto upto = [](int z) constexpr { return z >= POS ? LPT : z * LPT / POS; };
   constexpr int FIRST = upto(AHEAD * CT);
   static_assert(XL * NT * 16 == XB && WL * NT * 16 == WB && MT * WM * 16 == BM && CT * WN * 16 == BN, "tile shape");
@@ -483,9 +484,9 @@ A8Plan a8_plan(int M, int N, int K, bool gated, bool a8_out) {
       {{kTile64x128, 64, 128, 4}, 5.0f, 0.33f, kCus},       // one workgroup a CU
       {{kTile64x128, 64, 128, 4}, 8.3f, 0.53f, 2 * kCus},   // two
       {{kTile64x256, 64, 256, 8}, 10.0f, 0.49f, kCus},
-      {{kTile128, 128, 256, 8}, 13.4f, 0.74f, kCus},
-      {{kTile192, 192, 256, 8}, 14.5f, 1.1f, kCus},
-      {{kTile256, 256, 256, 8}, 22.0f, 1.33f, kCus},
+      {{kTile128, 128, 256, 8}, 13.4f, 0.69f, kCus},
+      {{kTile192, 192, 256, 8}, 13.5f, 1.02f, kCus},
+      {{kTile256, 256, 256, 8}, 21.0f, 1.25f, kCus},
   };
   const float steps = (float)((K + 127) / 128);
   const long wrows = (long)N * (gated ? 2 : 1);
