@@ -459,9 +459,11 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
 // columns of 1280 k 10.5 against 9.1 us, in workgroups of 2 waves, 10.3 in 4); 8 waves where a workgroup of 4 to every CU
 // would leave half of them idle (512 columns of 5120 k 5.3 against 6.1 us).
 // More rows: the least of the estimates below, microseconds a round of the card (measured over 10 to 64 steps; the
-// partly filled last round counted as a whole one, which it is within a tenth: 512 to 4096 rows of the layer's widths).
+// partly filled last round counted as a whole one, which it is within a tenth: 33 to 4096 rows of the layer's widths).
+// Streams of 32, 48 and 64 rows at 5120 k, us: 64 rows of 2048 columns 6.6, 7.4, 8.9; 130 rows 9.7, 7.7, 8.6; 200 rows
+// 10.3, 12.9, 8.8; and the smallest tile 20.
 constexpr int kCus = 256;
-enum A8Kernel { kStream16, kStream32, kStream64, kTile64x128, kTile64x256, kTile128, kTile192, kTile256 };
+enum A8Kernel { kStream16, kStream32, kStream48, kStream64, kTile64x128, kTile64x256, kTile128, kTile192, kTile256 };
 struct A8Plan {
   A8Kernel kernel;
   int rows, cols, waves;  // a workgroup's rows of x, weight rows, and (streams) waves
@@ -479,10 +481,14 @@ A8Plan a8_plan(int M, int N, int K, bool gated, bool a8_out) {
     float fixed, step;  // us of a round: launch, first loads and output; 128 k
     int slots;
   };
+  const int sc = gated ? 64 : 32;  // weight rows of a stream
   const Cost costs[] = {
-      {{kStream64, 64, gated ? 64 : 32, 4}, 3.0f, gated ? 0.28f : 0.155f, kCus},
-      {{kTile64x128, 64, 128, 4}, 5.0f, 0.33f, kCus},       // one workgroup a CU
-      {{kTile64x128, 64, 128, 4}, 8.3f, 0.53f, 2 * kCus},   // two
+      {{kStream32, 32, sc, 4}, gated ? 2.6f : 3.0f, gated ? 0.16f : 0.09f, kCus},  // one workgroup a CU
+      {{kStream32, 32, sc, 4}, 3.2f, gated ? 0.32f : 0.18f, 2 * kCus},             // two
+      {{kStream48, 48, sc, 4}, 2.8f, gated ? 0.215f : 0.125f, kCus},
+      {{kStream64, 64, sc, 4}, 3.0f, gated ? 0.25f : 0.157f, kCus},
+      {{kTile64x128, 64, 128, 4}, 5.0f, 0.37f, kCus},      // one workgroup a CU
+      {{kTile64x128, 64, 128, 4}, 8.3f, 0.53f, 2 * kCus},  // two
       {{kTile64x256, 64, 256, 8}, 10.0f, 0.49f, kCus},
       {{kTile128, 128, 256, 8}, 13.4f, 0.69f, kCus},
       {{kTile192, 192, 256, 8}, 13.5f, 1.02f, kCus},
@@ -493,7 +499,7 @@ A8Plan a8_plan(int M, int N, int K, bool gated, bool a8_out) {
   A8Plan best = costs[0].plan;
   float least = 0.0f;
   for (const Cost& c : costs) {
-    if (c.plan.kernel != kStream64 && K > kTileMaxK) break;
+    if (c.plan.kernel >= kTile64x128 && K > kTileMaxK) break;
     const long groups = ((M + c.plan.rows - 1l) / c.plan.rows) * ((wrows + c.plan.cols - 1) / c.plan.cols);
     const float us = (float)((groups + c.slots - 1) / c.slots) * (c.fixed + steps * c.step);
     if (least == 0.0f || us < least) {
@@ -517,7 +523,7 @@ int a8_run(A8Args& a, hipStream_t st) {
   a.e.vec = a.N % 8 == 0 && (((uintptr_t)a.e.out | (uintptr_t)a.e.res) & 15) == 0;
   a.words = a.K % 128 == 0 && ((a.Kc | a.Kc2 | (uintptr_t)a.ws | (uintptr_t)a.ws2) & 3) == 0;
   const A8Plan p = a8_plan(a.M, a.N, a.K, GATED, a.e.out == nullptr);
-  // (a stream's columns are the output's up to 32 rows, and in its 64-row form as in the tiles the weights' rows)
+  // (a plan's columns are the output's up to 32 rows, the weights' rows above)
   const int oc = GATED && a.M > 32 ? p.cols / 2 : p.cols;
   a.mtiles = (a.M + p.rows - 1) / p.rows;
   a.ntiles = (a.N + oc - 1) / oc;
@@ -530,7 +536,9 @@ int a8_run(A8Args& a, hipStream_t st) {
       else a8_stream_kernel<1, 2, 4, 2, GATED, true><<<gs, 256, 0, st>>>(a);
       break;
     case kStream32:
-      if (p.cols == 16) {
+      if (a.M > 32) {
+        a8_stream_kernel<2, 2, 4, 2, GATED, false><<<gs, 256, 0, st>>>(a);
+      } else if (p.cols == 16) {
         if constexpr (!GATED) a8_stream_kernel<2, 1, 4, 2, false, true><<<gs, 256, 0, st>>>(a);
       } else if (p.waves == 2) {
         a8_stream_kernel<2, 2, 2, 2, GATED, true><<<gs, 128, 0, st>>>(a);
@@ -538,6 +546,7 @@ int a8_run(A8Args& a, hipStream_t st) {
         a8_stream_kernel<2, 2, 4, 2, GATED, true><<<gs, 256, 0, st>>>(a);
       }
       break;
+    case kStream48: a8_stream_kernel<3, 2, 4, 2, GATED, false><<<gs, 256, 0, st>>>(a); break;
     case kStream64: a8_stream_kernel<4, 2, 4, 2, GATED, false><<<gs, 256, 0, st>>>(a); break;
     case kTile64x128: a8_tile_kernel<64, 128, 2, 2, 3, GATED><<<gt, 256, 0, st>>>(a); break;
     case kTile64x256: a8_tile_kernel<64, 256, 2, 4, 3, GATED><<<gt, 512, 0, st>>>(a); break;

@@ -184,14 +184,14 @@ def plan(m, n, k, gated=False, a8=False):
 
 
 def test_sizes_reach_every_kernel():
-    """(rows, columns, waves) of the streams and tiles that the sizes below run on."""
-    kinds = lambda ps: {(p >> 30, p >> 16 & 0x3fff, p >> 4 & 0xfff, p & 15) for p in ps}  # noqa: E731
-    tiles = {(1, 64, 128, 4), (1, 64, 256, 8), (1, 128, 256, 8), (1, 192, 256, 8), (1, 256, 256, 8)}
-    assert kinds(plan(*s, a8=a) for s in SIZES + LARGE for a in (False, True) if not a or s[1] % 32 == 0) == tiles | {
-        (0, 16, 16, 8), (0, 16, 16, 4), (0, 16, 32, 4), (0, 16, 32, 2), (0, 32, 16, 4), (0, 32, 32, 4), (0, 32, 32, 2),
-        (0, 64, 32, 4)}
-    assert kinds(plan(*s, gated=True, a8=a) for s in GATED + GATED_LARGE for a in (False, True)) == tiles | {
-        (0, 16, 16, 8), (0, 16, 16, 4), (0, 16, 32, 4), (0, 16, 32, 2), (0, 32, 32, 4), (0, 32, 32, 2), (0, 64, 64, 4)}
+    """(exact sums, tile, rows, columns, waves) of the streams and tiles that the sizes below run on."""
+    kind = lambda m, p: (m <= 32, p >> 30, p >> 16 & 0x3fff, p >> 4 & 0xfff, p & 15)  # noqa: E731
+    tiles = {(False, 1, *t) for t in ((64, 128, 4), (64, 256, 8), (128, 256, 8), (192, 256, 8), (256, 256, 8))}
+    exact = {(True, 0, *t) for t in ((16, 16, 8), (16, 16, 4), (16, 32, 4), (16, 32, 2), (32, 32, 4), (32, 32, 2))}
+    linear = {kind(s[0], plan(*s, a8=a)) for s in SIZES + LARGE for a in (False, True) if not a or s[1] % 32 == 0}
+    assert linear == tiles | exact | {(True, 0, 32, 16, 4)} | {(False, 0, r, 32, 4) for r in (32, 48, 64)}
+    gated = {kind(s[0], plan(*s, gated=True, a8=a)) for s in GATED + GATED_LARGE for a in (False, True)}
+    assert gated == tiles | exact | {(False, 0, r, 64, 4) for r in (32, 48, 64)}
 
 
 @pytest.mark.parametrize("m,n,k", SIZES + LARGE)
@@ -327,7 +327,7 @@ def test_refusals():
 
 # ------------------------------------------------------------------------------------------------ gated_a8
 GATED = [(1, 32, 32), (2, 96, 96), (16, 512, 1280), (17, 64, 160), (32, 224, 512), (33, 32, 64), (64, 160, 1280),
-         (100, 1024, 352), (129, 416, 5120), (300, 288, 160), (2049, 288, 224)]
+         (100, 1024, 352), (140, 1952, 160), (200, 2016, 352), (129, 416, 5120), (300, 288, 160), (2049, 288, 224)]
 GATED_LARGE = [(2, 16416, 96), (5, 2080, 4128), (18, 16896, 64), (1100, 1056, 160), (450, 2336, 6176), (1024, 4064, 640),
                (2049, 2048, 1312), (4090, 2016, 1280)]
 
