@@ -430,6 +430,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
       fetch_x(t, 0);
+      xs[t % RING] = buf[XB + WB + (xr + 16 * t) * 4 + min(g, tail / 32 - 1)];  // (bytes behind the last may be anything)
 #pragma unroll
       for (int j = 0; j < CT; ++j) acc[t][j] = a8_mfma16(wf[j], xf[t % RING], acc[t][j], ws[j], xs[t % RING]);
     }
@@ -463,6 +464,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
 // Streams of 32, 48 and 64 rows at 5120 k, us: 64 rows of 2048 columns 6.6, 7.4, 8.9; 130 rows 9.7, 7.7, 8.6; 200 rows
 // 10.3, 12.9, 8.8; and the smallest tile 20.
 constexpr int kCus = 256;
+constexpr int kMaxRows = 0x7fffff00;  // (a workgroup's rows are counted to its end)
 enum A8Kernel { kStream16, kStream32, kStream48, kStream64, kTile64x128, kTile64x256, kTile128, kTile192, kTile256 };
 struct A8Plan {
   A8Kernel kernel;
@@ -494,13 +496,14 @@ A8Plan a8_plan(int M, int N, int K, bool gated, bool a8_out) {
       {{kTile192, 192, 256, 8}, 13.5f, 1.02f, kCus},
       {{kTile256, 256, 256, 8}, 21.0f, 1.25f, kCus},
   };
-  const float steps = (float)((K + 127) / 128);
+  const float steps = (float)((K + 127) / 128);  // (a stream's row blocks are the grid's y: up to 65535 of them)
   const long wrows = (long)N * (gated ? 2 : 1);
-  A8Plan best = costs[0].plan;
+  A8Plan best = costs[3].plan;
   float least = 0.0f;
   for (const Cost& c : costs) {
-    if (c.plan.kernel >= kTile64x128 && K > kTileMaxK) break;
-    const long groups = ((M + c.plan.rows - 1l) / c.plan.rows) * ((wrows + c.plan.cols - 1) / c.plan.cols);
+    const bool tile = c.plan.kernel >= kTile64x128;
+    const long rows = (M + c.plan.rows - 1l) / c.plan.rows, groups = rows * ((wrows + c.plan.cols - 1) / c.plan.cols);
+    if (tile ? K > kTileMaxK : rows > 65535) continue;
     const float us = (float)((groups + c.slots - 1) / c.slots) * (c.fixed + steps * c.step);
     if (least == 0.0f || us < least) {
       least = us;
@@ -513,8 +516,9 @@ A8Plan a8_plan(int M, int N, int K, bool gated, bool a8_out) {
 template <bool GATED>
 int a8_run(A8Args& a, hipStream_t st) {
   if (a.M == 0 || a.N == 0) return 0;
-  if (a.M < 0 || a.N < 0 || a.K <= 0 || a.K % 32 != 0 || a.K > kStreamMaxK || a.Kc < a.K / 32 || (GATED && a.Kc2 < a.K / 32))
+  if (a.M < 0 || a.N < 0 || a.M > kMaxRows || a.N > kMaxRows || a.K <= 0 || a.K % 32 != 0 || a.K > kStreamMaxK || a.Kc < a.K / 32 || (GATED && a.Kc2 < a.K / 32))
     return (int)hipErrorInvalidValue;
+  if (!a.x || !a.xs || !a.w || !a.ws || (GATED && (!a.w2 || !a.ws2))) return (int)hipErrorInvalidValue;
   if (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.w2) & 15 || (uintptr_t)a.xs & 3) return (int)hipErrorInvalidValue;
   if (a.e.act < kActNone || a.e.act > kActGeluTanh || !(a.e.limit >= 0.0f)) return (int)hipErrorInvalidValue;
   if (!a.e.out && (!a.e.oa8 || !a.e.os8 || a.N % 32 != 0 || (uintptr_t)a.e.oa8 & 15)) return (int)hipErrorInvalidValue;
@@ -525,9 +529,12 @@ int a8_run(A8Args& a, hipStream_t st) {
   const A8Plan p = a8_plan(a.M, a.N, a.K, GATED, a.e.out == nullptr);
   // (a plan's columns are the output's up to 32 rows, the weights' rows above)
   const int oc = GATED && a.M > 32 ? p.cols / 2 : p.cols;
-  a.mtiles = (a.M + p.rows - 1) / p.rows;
-  a.ntiles = (a.N + oc - 1) / oc;
-  const dim3 gs((unsigned)a.ntiles, (unsigned)a.mtiles), gt((unsigned)((a.mtiles * a.ntiles + kXcds - 1) / kXcds * kXcds));
+  a.mtiles = (int)((a.M + p.rows - 1l) / p.rows);
+  a.ntiles = (int)((a.N + oc - 1l) / oc);
+  const bool tile = p.kernel >= kTile64x128;
+  const long tiles = ((long)a.mtiles * a.ntiles + kXcds - 1) / kXcds * kXcds, threads = 64 * p.waves;
+  if ((tile ? tiles : a.ntiles) * threads > 0xffffffffl || (!tile && a.mtiles > 65535)) return (int)hipErrorInvalidValue;
+  const dim3 gs((unsigned)a.ntiles, (unsigned)a.mtiles), gt((unsigned)tiles);
   switch (p.kernel) {
     case kStream16:
       if (p.cols == 16 && p.waves == 8) a8_stream_kernel<1, 1, 8, 2, GATED, true><<<gs, 512, 0, st>>>(a);
@@ -610,7 +617,6 @@ int dsv41_gated_a8(const void* a8, const void* s8, const void* wg8, const void* 
   a.e.out = (uint16_t*)out;
   a.e.oa8 = (uint8_t*)out_a8;
   a.e.os8 = (uint8_t*)out_s8;
-  if (!wu8 || !wus8) return (int)hipErrorInvalidValue;
   return a8_run<true>(a, (hipStream_t)stream);
 }
 

@@ -18,10 +18,9 @@ struct NormArgs {
   float eps;
   uint16_t* h;
   uint8_t *a8, *s8;
-  long rows;
+  long rows, first;  // all of them; the launch's first
   int D;
 };
-
 
 // One row by nt lanes (t: this lane's number); red: the workgroup's exchange, null where a row is one wave's.
 template <int IT, bool BLOCK>
@@ -104,13 +103,13 @@ DSV41_DEV void norm_row(const NormArgs& a, long row, bool live, int t, int nt, f
 template <int IT>
 __global__ void __launch_bounds__(1024) norm_quant8_block_kernel(const NormArgs a) {
   __shared__ float red[16];
-  norm_row<IT, true>(a, blockIdx.x, true, threadIdx.x, blockDim.x, red);
+  norm_row<IT, true>(a, a.first + blockIdx.x, true, threadIdx.x, blockDim.x, red);
 }
 
 // A row a wave, four to a workgroup.
 template <int IT>
 __global__ void __launch_bounds__(256) norm_quant8_wave_kernel(const NormArgs a) {
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long row = a.first + (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   norm_row<IT, false>(a, min(row, a.rows - 1), row < a.rows, threadIdx.x & 63, 64, nullptr);
 }
 
@@ -120,21 +119,27 @@ extern "C" int dsv41_norm_quant8(const void* x, const void* residual, const void
                                  void* s8, long n_rows, int D, void* stream) {
   if (n_rows <= 0) return 0;
   if (D <= 0 || D % 32 != 0 || D > 16384 || n_rows > 0x7fffffffl || (residual && !h)) return (int)hipErrorInvalidValue;
+  if (!x || !a8 || !s8) return (int)hipErrorInvalidValue;
   if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)w | (uintptr_t)h | (uintptr_t)a8) & 15)
     return (int)hipErrorInvalidValue;
-  const NormArgs a{(const uint16_t*)x, (const uint16_t*)residual, (const uint16_t*)w, eps, (uint16_t*)h,
-                   (uint8_t*)a8, (uint8_t*)s8, n_rows, D};
+  NormArgs a{(const uint16_t*)x, (const uint16_t*)residual, (const uint16_t*)w, eps, (uint16_t*)h,
+             (uint8_t*)a8, (uint8_t*)s8, n_rows, 0, D};
   const hipStream_t st = (hipStream_t)stream;
-  if (D <= 2048) {
-    const dim3 g((unsigned)((n_rows + 3) / 4));
-    if (D <= 512) norm_quant8_wave_kernel<1><<<g, 256, 0, st>>>(a);
-    else if (D <= 1024) norm_quant8_wave_kernel<2><<<g, 256, 0, st>>>(a);
-    else if (D <= 1536) norm_quant8_wave_kernel<3><<<g, 256, 0, st>>>(a);
-    else norm_quant8_wave_kernel<4><<<g, 256, 0, st>>>(a);
-  } else {
-    const int nc = D / 8, nt = nc <= 1024 ? (nc + 63) / 64 * 64 : (nc / 2 + 63) / 64 * 64;
-    if (nc <= 1024) norm_quant8_block_kernel<1><<<(unsigned)n_rows, nt, 0, st>>>(a);
-    else norm_quant8_block_kernel<2><<<(unsigned)n_rows, nt, 0, st>>>(a);
+  // (a launch has fewer than 2^32 threads: 64 a row, or up to 1024)
+  const long most = D <= 2048 ? 1l << 25 : 1l << 21;
+  for (; a.first < n_rows; a.first += most) {
+    const long rows = min(n_rows - a.first, most);
+    if (D <= 2048) {
+      const dim3 g((unsigned)((rows + 3) / 4));
+      if (D <= 512) norm_quant8_wave_kernel<1><<<g, 256, 0, st>>>(a);
+      else if (D <= 1024) norm_quant8_wave_kernel<2><<<g, 256, 0, st>>>(a);
+      else if (D <= 1536) norm_quant8_wave_kernel<3><<<g, 256, 0, st>>>(a);
+      else norm_quant8_wave_kernel<4><<<g, 256, 0, st>>>(a);
+    } else {
+      const int nc = D / 8, nt = nc <= 1024 ? (nc + 63) / 64 * 64 : (nc / 2 + 63) / 64 * 64;
+      if (nc <= 1024) norm_quant8_block_kernel<1><<<(unsigned)rows, nt, 0, st>>>(a);
+      else norm_quant8_block_kernel<2><<<(unsigned)rows, nt, 0, st>>>(a);
+    }
   }
   DSV41_CHECK_LAUNCH();
   return 0;

@@ -18,6 +18,7 @@ import torch
 from ._lib import as_bf16, call, ptr, require_gpu, stream_of
 from .w8 import W8, unpermute_k
 
+MOST = 0x7fffff00  # rows and columns of a product
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 
@@ -36,7 +37,7 @@ class A8:
             raise ValueError(f"A8: scales {tuple(s8.shape)} for codes {tuple(a8.shape)}: [ceil(K / 128), rows, 4] expected")
         if s8.device != a8.device:
             raise RuntimeError(f"A8: codes on {a8.device}, scales on {s8.device}")
-        if shape is not None and (shape[-1] != k or math.prod(shape[:-1]) != rows):
+        if shape is not None and (len(shape) == 0 or shape[-1] != k or math.prod(shape[:-1]) != rows):
             raise ValueError(f"A8: shape {tuple(shape)} for codes {tuple(a8.shape)}")
         self.a8, self.s8 = a8.contiguous(), s8.contiguous()
         self.shape = tuple(a8.shape) if shape is None else tuple(shape)
@@ -147,6 +148,8 @@ def _operands(name: str, x: A8, act: str, out, w: W8):
     s = w.s8.shape
     if Kw != K or K > 32768 or len(s) != 2 or s[0] < (N + 31) // 32 or s[1] < K // 32:
         raise RuntimeError(f"{name}: weight {(N, Kw)}, scales {tuple(s)} for x {tuple(x.shape)} (K at most 32768)")
+    if N > MOST or x.a8.shape[0] > MOST:
+        raise RuntimeError(f"{name}: {x.a8.shape[0]} rows, {N} columns (at most {MOST})")
     if out is A8 and N % 32:
         raise RuntimeError(f"{name}: {N} columns in 8 bits (a multiple of 32)")
     return N, K

@@ -84,7 +84,7 @@ def _norm(x=P, r=None, w=P, h=None, a8=P, s8=P, rows=4, D=64):
 def test_norm_entry_refusals():
     assert _norm(rows=0) == 0
     for bad in [dict(D=0), dict(D=48), dict(D=16416), dict(D=-32), dict(x=P + 8), dict(w=P + 2), dict(a8=P + 4),
-                dict(r=P), dict(r=P + 8, h=P), dict(r=P, h=P + 2), dict(rows=1 << 40)]:
+                dict(x=None), dict(a8=None), dict(s8=None), dict(r=P), dict(r=P + 8, h=P), dict(r=P, h=P + 2), dict(rows=1 << 40)]:
         assert _norm(**bad) == 1, bad
 
 
@@ -99,12 +99,37 @@ def _gated(x=P, xs=P, g=P, gs=P, u=P, us=P, M=4, N=64, K=64, Kg=2, Ku=2, act=2, 
 def test_product_entry_refusals():
     for f in (_linear, _gated):
         assert f(M=0) == 0 and f(N=0) == 0
-        for bad in [dict(M=-1), dict(N=-1), dict(K=0), dict(K=48), dict(K=32800, Kc=1025) if f is _linear else dict(K=32800, Kg=1025, Ku=1025), dict(x=P + 8), dict(xs=P + 1), dict(act=5),
+        for bad in [dict(M=-1), dict(N=-1), dict(M=0x7fffff01), dict(N=0x7fffff01), dict(x=None), dict(xs=None), dict(K=0), dict(K=48), dict(K=32800, Kc=1025) if f is _linear else dict(K=32800, Kg=1025, Ku=1025), dict(x=P + 8), dict(xs=P + 1), dict(act=5),
                     dict(act=-1), dict(out=None), dict(out=None, oa=P), dict(out=None, oa=P, os=P, N=40),
                     dict(out=None, oa=P + 8, os=P)]:
             assert f(**bad) == 1, (f.__name__, bad)
-    for bad in [dict(w=P + 8), dict(Kc=1)]:
+    for bad in [dict(w=P + 8), dict(w=None), dict(ws=None), dict(Kc=1)]:
         assert _linear(**bad) == 1, bad
-    for bad in [dict(g=P + 8), dict(u=P + 8), dict(u=None), dict(us=None), dict(Kg=1), dict(Ku=1), dict(limit=-1.0),
+    for bad in [dict(g=P + 8), dict(u=P + 8), dict(g=None), dict(gs=None), dict(u=None), dict(us=None), dict(Kg=1), dict(Ku=1), dict(limit=-1.0),
                 dict(limit=float("nan"))]:
         assert _gated(**bad) == 1, bad
+
+
+def test_products_of_more_rows_than_a_grid_holds():
+    """A stream's row blocks are a grid's second size, at most 65535: more go to the tiles, and where K keeps them out the
+    call is refused; so is one of more threads than a launch has."""
+    plan = lib().dsv41_a8_plan
+    for gated in (0, 1):
+        for rows in (65535 * 64 + 1, 5000000, 1 << 26):
+            assert plan(rows, 32, 32, gated, 0) >> 30 == 1
+        assert plan(65535 * 32 + 1, 32, 20000, gated, 0) >> 16 in (48, 64)
+    assert _linear(M=65535 * 64 + 1, K=20000, Kc=625) == 1
+    assert _gated(M=65535 * 64 + 1, K=20000, Kg=625, Ku=625) == 1
+    assert _linear(M=1 << 30, N=4096) == 1 and _linear(N=1 << 30) == 1
+
+
+def test_counts_past_32_bits_are_refused():
+    rows = (1 << 32) + 4
+    meta = lambda *s: torch.empty(*s, dtype=torch.uint8, device="meta")  # noqa: E731
+    x = A8(meta(rows, 64), meta(1, rows, 4))
+    with pytest.raises(RuntimeError, match="at most"):
+        linear_a8(x, _w8(32, 64))
+    with pytest.raises(RuntimeError, match="at most"):
+        gated_a8(x, _w8(32, 64), _w8(32, 64))
+    with pytest.raises(ValueError):
+        A8(meta(1, 64), meta(1, 1, 4), ())

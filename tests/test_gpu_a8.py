@@ -480,3 +480,25 @@ def test_offsets_past_32_bits():
     assert torch.equal(A8(q.a8[-71:], q.s8[:, -71:]).bf16(), linear_a8(x, w, out=A8).bf16())
     t = norm_quant8(torch.ones(70001, 1, dtype=BF, device=DEV).expand(-1, 32768)[:, :16384].contiguous(), None, 0.0)
     assert (t.s8 == 119).all() and (t.a8[-1] == 0x78).all()
+
+
+@pytest.mark.parametrize("rows,d", [((1 << 25) + 5, 32), ((1 << 21) + 3, 2080)])
+def test_norm_quant8_of_more_rows_than_a_launch_has(rows, d):
+    """The rows of a second launch against the same rows alone."""
+    g = gen("launches", d)
+    x = torch.ones(rows, d, dtype=BF, device=DEV)
+    x[-9:] = bf(g, 9, d).to(DEV)
+    w = (torch.rand(d, generator=g) + 0.5).to(BF).to(DEV)
+    q, last, first = norm_quant8(x, w, EPS), norm_quant8(x[-9:], w, EPS), norm_quant8(x[:1], w, EPS)
+    assert torch.equal(q.a8[-9:], last.a8) and torch.equal(q.s8[:, -9:], last.s8)
+    assert (q.a8[:-9] == first.a8).all() and (q.s8[:, :-9] == first.s8).all()
+
+
+@pytest.mark.parametrize("m", [1, 40, 300, 2049])
+def test_bytes_behind_a_rows_last_scale_do_not_count(m):
+    g = gen("behind", m)
+    (x, _), (w, _) = random_a8(g, m, 1184), random_w8(g, 1056, 1184)
+    y = linear_a8(x, w)
+    s = x.s8.clone()
+    s[-1, :, 1:] = 255  # K = 9 * 128 + 32
+    assert torch.equal(linear_a8(A8(x.a8, s), w), y)
