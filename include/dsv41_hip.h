@@ -333,10 +333,12 @@ int dsv41_norm_quant8(const void* x, const void* residual, const void* w, float 
                       long n_rows, int D, void* stream);
 
 /* y[m, n] = act(sum_k x[m, k] w[n, k] + bias[n]) + residual[m, n]: x 8-bit activations [M, K], w e4m3 [N, K] in the
- * PERM_K byte order (16-byte aligned) with E8M0 scales [ceil(N / 32), Kc], Kc >= K / 32 (dsv41/w8.py:39-60); K % 32 == 0, K <= 32768.
+ * PERM_K byte order (16-byte aligned) with E8M0 scales [ceil(N / 32), Kc], Kc >= K / 32 (dsv41/w8.py:39-60);
+ * K % 32 == 0, K <= 32768.
  * bias bf16 or (bias_f32) fp32 [N] or null; act 0 none, 1 relu, 2 silu, 3 gelu (erf), 4 gelu by tanh; residual bf16
  * [M, N] or null.  Exactly one output: out bf16 [M, N], or (out null) out_a8 / out_s8, the result as 8-bit activations,
- * N % 32 == 0.  fp32 sums on the block-scaled fp8 matrix instructions (2^-16 relative), rounded once.  Replaces
+ * N % 32 == 0.  fp32 sums, of exact bf16 products up to 32 rows and on the block-scaled fp8 matrix instructions (2^-16
+ * relative) above, rounded once.  Streams (K > 16384 always) take up to 65535 blocks of rows.  Replaces
  * cukern.fp8_gemm_tc (dsv41/cukern.py:164-200) where x is held in 8 bits. */
 int dsv41_linear_a8(const void* a8, const void* s8, const void* w8, const void* ws8, int M, int N, int K, int Kc,
                     const void* bias, int bias_f32, int act, const void* residual, void* out, void* out_a8,
