@@ -463,10 +463,13 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
 // More rows: the least of the estimates below, microseconds a round of the card (measured over 10 to 64 steps; the
 // partly filled last round counted as a whole one, which it is within a tenth: 33 to 4096 rows of the layer's widths).
 // Streams of 32, 48 and 64 rows at 5120 k, us: 64 rows of 2048 columns 6.6, 7.4, 8.9; 130 rows 9.7, 7.7, 8.6; 200 rows
-// 10.3, 12.9, 8.8; and the smallest tile 20.
+// 10.3, 12.9, 8.8; and the smallest tile 17.
+// Of a tile and the same one with rows and columns exchanged the one with more rows was the faster: the same areas
+// the other way, us: 64 x 128 for 128 x 64 at 1000 rows of 2048 columns and 5120 k 22 for 19; 64 x 256 for 128 x 128 at 512
+// rows of 2 x 4096 gated 27 to 32 for 24 to 28; 128 x 256 for 256 x 128 at 4096 rows of 2 x 8192 gated 330 for 297.
 constexpr int kCus = 256;
 constexpr int kMaxRows = 0x7fffff00;  // (a workgroup's rows are counted to its end)
-enum A8Kernel { kStream16, kStream32, kStream48, kStream64, kTile64x128, kTile64x256, kTile128, kTile192, kTile256 };
+enum A8Kernel { kStream16, kStream32, kStream48, kStream64, kTile128x64, kTile128x128, kTile256x128, kTile192x256, kTile256x256 };
 struct A8Plan {
   A8Kernel kernel;
   int rows, cols, waves;  // a workgroup's rows of x, weight rows, and (streams) waves
@@ -490,19 +493,19 @@ A8Plan a8_plan(int M, int N, int K, bool gated, bool a8_out) {
       {{kStream32, 32, sc, 4}, 3.2f, gated ? 0.32f : 0.18f, 2 * kCus},             // two
       {{kStream48, 48, sc, 4}, 2.8f, gated ? 0.215f : 0.125f, kCus},
       {{kStream64, 64, sc, 4}, 3.0f, gated ? 0.25f : 0.157f, kCus},
-      {{kTile64x128, 64, 128, 4}, 5.0f, 0.37f, kCus},      // one workgroup a CU
-      {{kTile64x128, 64, 128, 4}, 8.3f, 0.6f, 2 * kCus},   // two
-      {{kTile64x256, 64, 256, 8}, 10.0f, 0.49f, kCus},
-      {{kTile128, 128, 256, 8}, 13.4f, 0.69f, kCus},
-      {{kTile192, 192, 256, 8}, 13.5f, 1.02f, kCus},
-      {{kTile256, 256, 256, 8}, 21.0f, 1.25f, kCus},
+      {{kTile128x64, 128, 64, 4}, 5.5f, 0.32f, kCus},      // one workgroup a CU
+      {{kTile128x64, 128, 64, 4}, 8.0f, 0.58f, 2 * kCus},  // two
+      {{kTile128x128, 128, 128, 8}, 7.5f, 0.47f, kCus},
+      {{kTile256x128, 256, 128, 8}, 11.0f, 0.68f, kCus},
+      {{kTile192x256, 192, 256, 8}, 13.5f, 1.05f, kCus},
+      {{kTile256x256, 256, 256, 8}, 19.0f, 1.22f, kCus},
   };
   const float steps = (float)((K + 127) / 128);  // (a stream's row blocks are the grid's y: up to 65535 of them)
   const long wrows = (long)N * (gated ? 2 : 1);
   A8Plan best = costs[3].plan;
   float least = 0.0f;
   for (const Cost& c : costs) {
-    const bool tile = c.plan.kernel >= kTile64x128;
+    const bool tile = c.plan.kernel >= kTile128x64;
     const long rows = (M + c.plan.rows - 1l) / c.plan.rows, groups = rows * ((wrows + c.plan.cols - 1) / c.plan.cols);
     if (tile ? K > kTileMaxK : rows > 65535) continue;
     const float us = (float)((groups + c.slots - 1) / c.slots) * (c.fixed + steps * c.step);
@@ -532,7 +535,7 @@ int a8_run(A8Args& a, hipStream_t st) {
   const int oc = GATED && a.M > 32 ? p.cols / 2 : p.cols;
   a.mtiles = (int)((a.M + p.rows - 1l) / p.rows);
   a.ntiles = (int)((a.N + oc - 1l) / oc);
-  const bool tile = p.kernel >= kTile64x128;
+  const bool tile = p.kernel >= kTile128x64;
   const long tiles = ((long)a.mtiles * a.ntiles + kXcds - 1) / kXcds * kXcds, threads = 64 * p.waves;
   if ((tile ? tiles : a.ntiles) * threads > 0xffffffffl || (!tile && a.mtiles > 65535)) return (int)hipErrorInvalidValue;
   const dim3 gs((unsigned)a.ntiles, (unsigned)a.mtiles), gt((unsigned)tiles);
@@ -556,11 +559,11 @@ int a8_run(A8Args& a, hipStream_t st) {
       break;
     case kStream48: a8_stream_kernel<3, 2, 4, 2, GATED, false><<<gs, 256, 0, st>>>(a); break;
     case kStream64: a8_stream_kernel<4, 2, 4, 2, GATED, false><<<gs, 256, 0, st>>>(a); break;
-    case kTile64x128: a8_tile_kernel<64, 128, 2, 2, 3, GATED><<<gt, 256, 0, st>>>(a); break;
-    case kTile64x256: a8_tile_kernel<64, 256, 2, 4, 3, GATED><<<gt, 512, 0, st>>>(a); break;
-    case kTile128: a8_tile_kernel<128, 256, 2, 4, 3, GATED><<<gt, 512, 0, st>>>(a); break;
-    case kTile192: a8_tile_kernel<192, 256, 2, 4, 2, GATED><<<gt, 512, 0, st>>>(a); break;
-    case kTile256: a8_tile_kernel<256, 256, 2, 4, 2, GATED><<<gt, 512, 0, st>>>(a); break;
+    case kTile128x64: a8_tile_kernel<128, 64, 4, 1, 3, GATED><<<gt, 256, 0, st>>>(a); break;
+    case kTile128x128: a8_tile_kernel<128, 128, 4, 2, 3, GATED><<<gt, 512, 0, st>>>(a); break;
+    case kTile256x128: a8_tile_kernel<256, 128, 4, 2, 3, GATED><<<gt, 512, 0, st>>>(a); break;
+    case kTile192x256: a8_tile_kernel<192, 256, 2, 4, 2, GATED><<<gt, 512, 0, st>>>(a); break;
+    case kTile256x256: a8_tile_kernel<256, 256, 2, 4, 2, GATED><<<gt, 512, 0, st>>>(a); break;
   }
   DSV41_CHECK_LAUNCH();
   return 0;
@@ -573,7 +576,7 @@ extern "C" {
 int dsv41_a8_plan(int M, int N, int K, int gated, int a8_out) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   const A8Plan p = a8_plan(M, N, K, gated != 0, a8_out != 0);
-  return (p.kernel >= kTile64x128 ? 1 << 30 : 0) | p.rows << 16 | p.cols << 4 | p.waves;
+  return (p.kernel >= kTile128x64 ? 1 << 30 : 0) | p.rows << 16 | p.cols << 4 | p.waves;
 }
 
 int dsv41_linear_a8(const void* a8, const void* s8, const void* w8, const void* ws8, int M, int N, int K, int Kc,
