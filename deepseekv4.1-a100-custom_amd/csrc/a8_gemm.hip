@@ -22,7 +22,7 @@ struct A8Args {
   const uint8_t *w2, *ws2;    // the up weights of a gated product
   int M, N, K, Kc, Kc2;
   A8Epi e;
-  int mtiles, ntiles;
+  int mtiles, ntiles, first;  // tiles: of the columns from `first` on
   int words;                  // weight scales in whole words: K % 128 == 0, rows 4-byte aligned
 };
 
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   if (id >= a.mtiles * a.ntiles) return;  // (the grid is a multiple of the XCDs)
   const int strip = id / (kA8Strip * a.ntiles), sm = min(kA8Strip, a.mtiles - strip * kA8Strip);
   const int in = id - strip * kA8Strip * a.ntiles;
-  const int m0 = (strip * kA8Strip + in % sm) * BM, n0 = in / sm * OC;
+  const int m0 = (strip * kA8Strip + in % sm) * BM, n0 = a.first + in / sm * OC;
   const int nk = a.K / 128, tail = a.K % 128;  // whole stages, and the k behind them
 
   // weight row r of the tile: output column (from n0) and matrix
@@ -469,18 +469,26 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
 // rows of 2 x 4096 gated 27 to 32 for 24 to 28; 128 x 256 for 256 x 128 at 4096 rows of 2 x 8192 gated 330 for 297.
 constexpr int kCus = 256;
 constexpr int kMaxRows = 0x7fffff00;  // (a workgroup's rows are counted to its end)
-enum A8Kernel { kStream16, kStream32, kStream48, kStream64, kTile128x64, kTile128x128, kTile256x128, kTile192x256, kTile256x256 };
+enum A8Kernel {
+  kStream16, kStream32, kStream48, kStream64,
+  kTile128x64, kTile128x128, kTile256x128, kTile192x256, kTile256x256
+};
 struct A8Plan {
   A8Kernel kernel;
   int rows, cols, waves;  // a workgroup's rows of x, weight rows, and (streams) waves
 };
+struct A8Parts {
+  A8Plan plan, rest;
+  int columns;  // output columns on `plan`, and from there on those on `rest`
+};
 
-A8Plan a8_plan(int M, int N, int K, bool gated, bool a8_out) {
+A8Parts a8_plan(int M, int N, int K, bool gated, bool a8_out) {
   if (M <= 32) {
     const bool wide = N > 16384;
     const int cols = a8_out || wide || (M > 16 && gated) ? 32 : 16;
-    return A8Plan{M <= 16 ? kStream16 : kStream32, M <= 16 ? 16 : 32, cols,
-                  wide ? 2 : M <= 16 && cols == 16 && N <= 16 * kCus / 2 ? 8 : 4};
+    const A8Plan p{M <= 16 ? kStream16 : kStream32, M <= 16 ? 16 : 32, cols,
+                   wide ? 2 : M <= 16 && cols == 16 && N <= 16 * kCus / 2 ? 8 : 4};
+    return A8Parts{p, p, N};
   }
   struct Cost {
     A8Plan plan;
@@ -500,41 +508,52 @@ A8Plan a8_plan(int M, int N, int K, bool gated, bool a8_out) {
       {{kTile192x256, 192, 256, 8}, 13.5f, 1.05f, kCus},
       {{kTile256x256, 256, 256, 8}, 19.0f, 1.22f, kCus},
   };
-  const float steps = (float)((K + 127) / 128);  // (a stream's row blocks are the grid's y: up to 65535 of them)
-  const long wrows = (long)N * (gated ? 2 : 1);
-  A8Plan best = costs[3].plan;
-  float least = 0.0f;
-  for (const Cost& c : costs) {
-    const bool tile = c.plan.kernel >= kTile128x64;
-    const long rows = (M + c.plan.rows - 1l) / c.plan.rows, groups = rows * ((wrows + c.plan.cols - 1) / c.plan.cols);
-    if (tile ? K > kTileMaxK : rows > 65535) continue;
-    const float us = (float)((groups + c.slots - 1) / c.slots) * (c.fixed + steps * c.step);
-    if (least == 0.0f || us < least) {
-      least = us;
-      best = c.plan;
+  const float steps = (float)((K + 127) / 128);
+  const long wr = gated ? 2 : 1;
+  // The least estimate for n columns on one kernel (`any`, or a tile kernel)
+  auto least = [&](long n, bool any, A8Plan* plan) {
+    float best = 0.0f;
+    for (const Cost& c : costs) {
+      const bool tile = c.plan.kernel >= kTile128x64;
+      const long rows = (M + c.plan.rows - 1l) / c.plan.rows, groups = rows * ((n * wr + c.plan.cols - 1) / c.plan.cols);
+      if (tile ? K > kTileMaxK : !any || rows > 65535) continue;  // (a stream's row blocks are the grid's y)
+      const float us = (float)((groups + c.slots - 1) / c.slots) * (c.fixed + steps * c.step);
+      if (best == 0.0f || us < best) {
+        best = us;
+        *plan = c.plan;
+      }
+    }
+    return best;
+  };
+  A8Parts p{costs[3].plan, costs[3].plan, N};
+  float best = least(N, true, &p.plan);
+  // Or the columns that fill whole rounds of a tile kernel, and a second launch for the others (4096 rows of 5120 columns,
+  // 8192 k: one round of 256 x 256 and one of 128 x 128 155 us, 3 rounds of 256 x 128, half the last empty, 165)
+  if (K <= kTileMaxK) {
+    for (const Cost& c : costs) {
+      if (c.plan.kernel < kTile128x64) continue;
+      const long rows = (M + c.plan.rows - 1l) / c.plan.rows, per = c.plan.cols / wr, rounds = rows * (N / per) / c.slots;
+      const long columns = rounds * c.slots / rows * per;
+      if (columns == 0 || columns >= N) continue;
+      A8Plan rest;
+      const float us = (float)rounds * (c.fixed + steps * c.step) + least(N - columns, false, &rest);
+      if (us < 0.97f * best) {
+        best = us;
+        p = A8Parts{c.plan, rest, (int)columns};
+      }
     }
   }
-  return best;
+  return p;
 }
 
+// Columns first .. end - 1 by the kernel of p.
 template <bool GATED>
-int a8_run(A8Args& a, hipStream_t st) {
-  if (a.M == 0 || a.N == 0) return 0;
-  if (a.M < 0 || a.N < 0 || a.M > kMaxRows || a.N > kMaxRows || a.K <= 0 || a.K % 32 != 0 || a.K > kStreamMaxK || a.Kc < a.K / 32 || (GATED && a.Kc2 < a.K / 32))
-    return (int)hipErrorInvalidValue;
-  if (!a.x || !a.xs || !a.w || !a.ws || (GATED && (!a.w2 || !a.ws2))) return (int)hipErrorInvalidValue;
-  if (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.w2) & 15 || (uintptr_t)a.xs & 3) return (int)hipErrorInvalidValue;
-  if (a.e.act < kActNone || a.e.act > kActGeluTanh || !(a.e.limit >= 0.0f)) return (int)hipErrorInvalidValue;
-  if (!a.e.out && (!a.e.oa8 || !a.e.os8 || a.N % 32 != 0 || (uintptr_t)a.e.oa8 & 15)) return (int)hipErrorInvalidValue;
-  a.e.M = a.M;
-  a.e.N = a.N;
-  a.e.vec = a.N % 8 == 0 && (((uintptr_t)a.e.out | (uintptr_t)a.e.res) & 15) == 0;
-  a.words = a.K % 128 == 0 && ((a.Kc | a.Kc2 | (uintptr_t)a.ws | (uintptr_t)a.ws2) & 3) == 0;
-  const A8Plan p = a8_plan(a.M, a.N, a.K, GATED, a.e.out == nullptr);
+int a8_launch(A8Args& a, const A8Plan& p, int first, int end, hipStream_t st) {
   // (a plan's columns are the output's up to 32 rows, the weights' rows above)
-  const int oc = GATED && a.M > 32 ? p.cols / 2 : p.cols;
+  const long oc = GATED && a.M > 32 ? p.cols / 2 : p.cols;
   a.mtiles = (int)((a.M + p.rows - 1l) / p.rows);
-  a.ntiles = (int)((a.N + oc - 1l) / oc);
+  a.first = first;
+  a.ntiles = (int)((end - first + oc - 1l) / oc);
   const bool tile = p.kernel >= kTile128x64;
   const long tiles = ((long)a.mtiles * a.ntiles + kXcds - 1) / kXcds * kXcds, threads = 64 * p.waves;
   if ((tile ? tiles : a.ntiles) * threads > 0xffffffffl || (!tile && a.mtiles > 65535)) return (int)hipErrorInvalidValue;
@@ -569,14 +588,35 @@ int a8_run(A8Args& a, hipStream_t st) {
   return 0;
 }
 
+template <bool GATED>
+int a8_run(A8Args& a, hipStream_t st) {
+  if (a.M == 0 || a.N == 0) return 0;
+  if (a.M < 0 || a.N < 0 || a.M > kMaxRows || a.N > kMaxRows || a.K <= 0 || a.K % 32 != 0 || a.K > kStreamMaxK ||
+      a.Kc < a.K / 32 || (GATED && a.Kc2 < a.K / 32))
+    return (int)hipErrorInvalidValue;
+  if (!a.x || !a.xs || !a.w || !a.ws || (GATED && (!a.w2 || !a.ws2))) return (int)hipErrorInvalidValue;
+  if (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)a.w2) & 15 || (uintptr_t)a.xs & 3) return (int)hipErrorInvalidValue;
+  if (a.e.act < kActNone || a.e.act > kActGeluTanh || !(a.e.limit >= 0.0f)) return (int)hipErrorInvalidValue;
+  if (!a.e.out && (!a.e.oa8 || !a.e.os8 || a.N % 32 != 0 || (uintptr_t)a.e.oa8 & 15)) return (int)hipErrorInvalidValue;
+  a.e.M = a.M;
+  a.e.N = a.N;
+  a.e.vec = a.N % 8 == 0 && (((uintptr_t)a.e.out | (uintptr_t)a.e.res) & 15) == 0;
+  a.words = a.K % 128 == 0 && ((a.Kc | a.Kc2 | (uintptr_t)a.ws | (uintptr_t)a.ws2) & 3) == 0;
+  const A8Parts p = a8_plan(a.M, a.N, a.K, GATED, a.e.out == nullptr);
+  const int rc = a8_launch<GATED>(a, p.plan, 0, p.columns, st);
+  return rc != 0 || p.columns == a.N ? rc : a8_launch<GATED>(a, p.rest, p.columns, a.N, st);
+}
+
 }  // namespace
 
 extern "C" {
 
-int dsv41_a8_plan(int M, int N, int K, int gated, int a8_out) {
+int dsv41_a8_plan(int M, int N, int K, int gated, int a8_out, int rest) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const A8Plan p = a8_plan(M, N, K, gated != 0, a8_out != 0);
-  return (p.kernel >= kTile128x64 ? 1 << 30 : 0) | p.rows << 16 | p.cols << 4 | p.waves;
+  const A8Parts p = a8_plan(M, N, K, gated != 0, a8_out != 0);
+  const A8Plan& k = rest ? p.rest : p.plan;
+  if (rest && p.columns == N) return 0;
+  return (k.kernel >= kTile128x64 ? 1 << 30 : 0) | k.rows << 16 | k.cols << 4 | k.waves;
 }
 
 int dsv41_linear_a8(const void* a8, const void* s8, const void* w8, const void* ws8, int M, int N, int K, int Kc,

@@ -57,7 +57,7 @@ SIGNATURES = {
     "dsv41_fp8_gemv_m1_pre": [_P, _P, _F, _I, _P, _P, _I, _I, _I, _P, _P, _L, _P],
     "dsv41_fp8_gemm": [_P, _L, _P, _P, _I, _I, _I, _I, _I, _P, _L, _P, _P, _L, _P],
     "dsv41_norm_quant8": [_P, _P, _P, _F, _P, _P, _P, _L, _I, _P],
-    "dsv41_a8_plan": [_I, _I, _I, _I, _I],
+    "dsv41_a8_plan": [_I, _I, _I, _I, _I, _I],
     "dsv41_linear_a8": [_P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _I, _P, _P, _P, _P, _P],
     "dsv41_gated_a8": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P],
     "dsv41_f32_proj2": [_P, _L, _P, _P, _I, _I, _I, _P, _P, _P],

@@ -345,8 +345,9 @@ int dsv41_linear_a8(const void* a8, const void* s8, const void* w8, const void* 
                     void* out_s8, void* stream);
 
 /* The kernel that a product of these sizes (a8_out: with 8-bit output) runs on: rows << 16 | columns << 4 | waves of its
- * workgroups, with bit 30 set for the tile kernels (columns of weights) and clear for the streams. */
-int dsv41_a8_plan(int M, int N, int K, int gated, int a8_out);
+ * workgroups, with bit 30 set for the tile kernels (columns of weights) and clear for the streams.  Where the columns behind
+ * the last whole round of the card's CUs run on another kernel, in a second launch, that one with rest set (else 0). */
+int dsv41_a8_plan(int M, int N, int K, int gated, int a8_out, int rest);
 
 /* y = act(min(x Wg^T, limit)) * clamp(x Wu^T, -limit, limit) (limit 0: as they are), operands, act and outputs as
  * dsv41_linear_a8; wg8, wu8 [N, K] with scales of Kcg and Kcu columns. */

@@ -116,8 +116,8 @@ def test_products_of_more_rows_than_a_grid_holds():
     plan = lib().dsv41_a8_plan
     for gated in (0, 1):
         for rows in (65535 * 64 + 1, 5000000, 1 << 26):
-            assert plan(rows, 32, 32, gated, 0) >> 30 == 1
-        assert plan(65535 * 32 + 1, 32, 20000, gated, 0) >> 16 in (48, 64)
+            assert plan(rows, 32, 32, gated, 0, 0) >> 30 == 1
+        assert plan(65535 * 32 + 1, 32, 20000, gated, 0, 0) >> 16 in (48, 64)
     assert _linear(M=65535 * 64 + 1, K=20000, Kc=625) == 1
     assert _gated(M=65535 * 64 + 1, K=20000, Kg=625, Ku=625) == 1
     assert _linear(M=1 << 30, N=4096) == 1 and _linear(N=1 << 30) == 1

@@ -175,12 +175,12 @@ SIZES = [(1, 1, 32), (1, 33, 64), (2, 100, 96), (5, 512, 128), (15, 257, 160), (
          (200, 511, 5120), (257, 260, 352), (300, 1280, 288)]
 LARGE = [(2049, 513, 288), (2100, 1056, 1184), (4097, 256, 128), (1, 16416, 128), (20, 17000, 160), (3, 4096, 8224),
          (30, 2080, 4128), (1100, 2080, 160), (450, 4640, 6176), (1024, 8160, 640), (2049, 4096, 1312), (4090, 4064, 1280),
-         (70, 64, 20000), (40, 33, 32768)]
+         (70, 64, 20000), (40, 33, 32768), (2049, 7233, 160), (4090, 4928, 160)]
 
 
-def plan(m, n, k, gated=False, a8=False):
+def plan(m, n, k, gated=False, a8=False, rest=False):
     from dsv41_amd._lib import lib
-    return lib().dsv41_a8_plan(m, n, k, int(gated), int(a8))
+    return lib().dsv41_a8_plan(m, n, k, int(gated), int(a8), int(rest))
 
 
 def test_sizes_reach_every_kernel():
@@ -192,6 +192,8 @@ def test_sizes_reach_every_kernel():
     assert linear == tiles | exact | {(True, 0, 32, 16, 4)} | {(False, 0, r, 32, 4) for r in (32, 48, 64)}
     gated = {kind(s[0], plan(*s, gated=True, a8=a)) for s in GATED + GATED_LARGE for a in (False, True)}
     assert gated == tiles | exact | {(False, 0, r, 64, 4) for r in (32, 48, 64)}
+    for sizes, g in ((LARGE, False), (GATED_LARGE, True)):  # columns behind the last whole round on another kernel
+        assert sum(plan(*s, gated=g, rest=True) != 0 for s in sizes) >= 2
 
 
 @pytest.mark.parametrize("m,n,k", SIZES + LARGE)
@@ -329,7 +331,7 @@ def test_refusals():
 GATED = [(1, 32, 32), (2, 96, 96), (16, 512, 1280), (17, 64, 160), (32, 224, 512), (33, 32, 64), (64, 160, 1280),
          (100, 1024, 352), (140, 1952, 160), (200, 2016, 352), (129, 416, 5120), (300, 288, 160), (2049, 288, 224)]
 GATED_LARGE = [(2, 16416, 96), (5, 2080, 4128), (18, 16896, 64), (1100, 1056, 160), (450, 2336, 6176), (1024, 4064, 640),
-               (2049, 2048, 1312), (4090, 2016, 1280)]
+               (2049, 2048, 1312), (4090, 2016, 1280), (1100, 6560, 160), (4090, 2528, 160)]
 
 
 @pytest.mark.parametrize("m,n,k", GATED)
