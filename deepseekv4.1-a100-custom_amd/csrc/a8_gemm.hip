@@ -232,34 +232,29 @@ __global__ void __launch_bounds__(64 * NW) a8_stream_kernel(const A8Args a) {
 constexpr int kA8Strip = 4;
 constexpr int kTileMaxK = 16384;  // (the weight scales of a tile are held in LDS)
 
-// Output of a wave's ROWS x OCW block of sums from LDS (fp32, row stride LD bytes): rolled, so that bias, activation and
-// quantisation stand there once (unrolled over the accumulators they were 100 KB of code); the residual of U passes is
-// loaded before any of them is stored.
+// Output of a wave's ROWS x OCW block of sums from LDS (fp32, row stride LD bytes), not from the accumulators: unrolled over
+// those, bias, activation and quantisation were 100 KB of code.  The residual is loaded before any of it is stored.
 template <int ROWS, int LD, int OCW, bool GATED>
 DSV41_DEV void a8_wave_out(const A8Args& a, const uint8_t* s, int m0, int n0) {
-  constexpr int QN = OCW / 8, RP = 64 / QN;  // lanes of a row, rows of a pass
-  constexpr int PASSES = (ROWS + RP - 1) / RP, U = PASSES % 8 == 0 ? 8 : PASSES % 4 == 0 ? 4 : PASSES % 6 == 0 ? 6 : 1;
-  const int lane = threadIdx.x & 63, c = lane % QN * 8, n = n0 + c, row = lane / QN;
-  s += row * LD + (GATED ? (c / 32 * 64 + c % 32) * 4 : c * 4);
+  constexpr int QN = OCW / 8, RP = 64 / QN, PASSES = ROWS / RP;  // lanes of a row, rows of a pass
+  static_assert(64 % QN == 0 && ROWS % RP == 0 && PASSES <= 8, "whole passes, residuals in registers");
+  static_assert(!GATED || OCW == 32, "a gate block and its up block");
+  const int lane = threadIdx.x & 63, c = lane % QN * 8, n = n0 + c, m = m0 + lane / QN;
+  s += lane / QN * LD + c * 4;
   const A8x8 bias = a8_bias8(a.e, n);
-#pragma unroll 1
-  for (int r0 = 0; r0 < ROWS; r0 += U * RP) {
-    uint4 res[U];
-    if constexpr (!GATED) {
+  uint4 res[PASSES];
+  if constexpr (!GATED) {
 #pragma unroll
-      for (int k = 0; k < U; ++k) res[k] = a8_res8(a.e, m0 + r0 + k * RP + row, n);
-    }
+    for (int k = 0; k < PASSES; ++k) res[k] = a8_res8(a.e, m + k * RP, n);
+  }
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int r = r0 + k * RP + row, m = m0 + r;
-      const bool in = (64 % QN == 0 || row < RP) && (ROWS % RP == 0 || r < ROWS);  // (a row's lanes may not fill the wave)
-      const uint8_t* p = s + (in ? (r0 + k * RP) * LD : 0);
-      A8x8 y = *(const A8x8*)p, u = y;
-      if constexpr (GATED) u = *(const A8x8*)(p + 128);
-      if constexpr (GATED) a8_gated8(a.e, y, u);
-      else a8_linear8(a.e, y, bias, res[k]);
-      a8_store8(a.e, y, m, n, in && m < a.M && n < a.N);
-    }
+  for (int k = 0; k < PASSES; ++k) {
+    const uint8_t* p = s + k * RP * LD;
+    A8x8 y = *(const A8x8*)p, u = y;
+    if constexpr (GATED) u = *(const A8x8*)(p + 128);
+    if constexpr (GATED) a8_gated8(a.e, y, u);
+    else a8_linear8(a.e, y, bias, res[k]);
+    a8_store8(a.e, y, m + k * RP, n, m + k * RP < a.M && n < a.N);
   }
 }
 
@@ -270,7 +265,7 @@ template <int BM, int BN, int WM, int WN, int NBUF, bool GATED>
 __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   constexpr int NT = 64 * WM * WN;
   constexpr int MT = BM / WM / 16, CT = BN / WN / 16;  // 16-row blocks of a wave
-  constexpr int XB = BM * 128, WB = BN * 128, SB = (BM < 64 ? 64 : BM) * 4, STAGE = XB + WB + SB;
+  constexpr int XB = BM * 128, WB = BN * 128, SB = BM * 4, STAGE = XB + WB + SB;
   constexpr int XL = XB / 16 / NT, WL = WB / 16 / NT, LPT = XL + WL + 1;  // loads per thread and stage
   constexpr int OC = GATED ? BN / 2 : BN;                                 // output columns
   // A stage is MT steps: x block t with the CT weight blocks.  x of a step is read AHEAD steps before, across the stage's
@@ -285,7 +280,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   constexpr int FIRST = upto(AHEAD * CT);
   static_assert(XL * NT * 16 == XB && WL * NT * 16 == WB && MT * WM * 16 == BM && CT * WN * 16 == BN, "tile shape");
   static_assert(!GATED || CT % 4 == 0, "gate and up blocks in pairs");
-  static_assert(MT % RING == 0, "ring");
+  static_assert(MT % RING == 0 && BM % 64 == 0, "ring, scales of 64 rows a wave");
   static_assert((NBUF - 2) * LPT + FIRST < 64, "vmcnt immediate");
   __shared__ __align__(16) uint8_t buf[NBUF * STAGE];
   __shared__ __align__(16) uint8_t scl[BN / 32][kTileMaxK / 32 + 16];
@@ -314,8 +309,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   // different 16-byte bank groups.
   const int r0 = tid >> 3, ch = ((tid & 7) ^ (r0 & 7)) * 16;
   const int xlim = a.M - 1 - m0, wlim = a.N - 1 - n0;
-  const int sr = min((wave % (SB / 256)) * 64 + lane, BM - 1);
-  const uint32_t so = (uint32_t)min(sr, xlim) * 4;
+  const uint32_t so = (uint32_t)min((wave % (SB / 256)) * 64 + lane, xlim) * 4;
   const uint32_t lds0 = lds_addr_of(buf);
   const uint32_t ldsw = lds0 + (uint32_t)wave * 1024, ldss = lds0 + XB + WB + (uint32_t)(wave % (SB / 256)) * 256;
   const int klast = a.K - 16;  // the last 16 codes of a row
@@ -442,7 +436,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   // the LDS (rows padded by 16 bytes: 8 lanes write 8 different bank groups)
   constexpr int LD = BN / WN * 4 + 16;
   constexpr int ROOM = NBUF * STAGE / (16 * LD * WM * WN);  // blocks of rows a wave has LDS for
-  constexpr int PM = ROOM >= MT ? MT : ROOM >= MT / 2 && MT % 2 == 0 ? MT / 2 : ROOM >= MT / 3 && MT % 3 == 0 ? MT / 3 : MT / 4;
+  constexpr int PM = ROOM >= MT ? MT : ROOM >= MT / 2 ? MT / 2 : MT / 4;
   static_assert(PM > 0 && PM <= ROOM && MT % PM == 0, "output staging");
   uint8_t* own = buf + wave * (PM * 16 * LD);
 #pragma unroll
