@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   // A stage is MT steps: x block t with the CT weight blocks.  x of a step is read AHEAD steps before, across the stage's
   // end too: the barrier stands in step ENTER, where the first of the next stage is read.  A weight block is read for the
   // next stage behind its last product.
-    constexpr int RING = MT % 4 == 0 ? 4 : 2, AHEAD = RING / 2, ENTER = MT - AHEAD;
+  constexpr int RING = MT % 4 == 0 ? 4 : 2, AHEAD = RING / 2, ENTER = MT - AHEAD;
   // A stage's loads are issued between the products from that barrier on, in the first POS of the MT CT places; FIRST of
   // them fall into the stage in which they begin.  With two buffers they have less than a stage to land and go out early
   // (3/8 of the places against 3/4: 291 and 318 us for the gated 4096 x 8192 x 5120); with three, 3/4 is as good or better.

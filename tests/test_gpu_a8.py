@@ -422,9 +422,9 @@ def test_feed_forward(rows, limit):
 
 
 def test_feed_forward_captured_on_two_streams():
-    """Two captured graphs and eager calls between their replays, on their own streams: workspaces are each call's own."""
+    """Two captured graphs and eager calls between their replays, on their own streams."""
     g = gen("cap")
-    dim, F, rows = 512, 256, 70  # (K slices, so a workspace)
+    dim, F, rows = 512, 256, 70
     norm = torch.ones(dim, dtype=BF)
     f = [GatedFeedForward(norm.to(DEV), random_w8(g, F, dim)[0], random_w8(g, F, dim)[0], random_w8(g, dim, F)[0])
          for _ in range(2)]
@@ -452,6 +452,28 @@ def test_feed_forward_captured_on_two_streams():
         torch.cuda.synchronize()
         for i in range(2):
             assert torch.equal(outs[i], eager[i]), (rep, i)
+
+
+def test_product_of_two_launches_captured():
+    g = gen("two parts")
+    m, n, k = 2049, 7232, 160
+    assert plan(m, n, k, rest=True)
+    (x, _), (w, _), (z, _) = random_a8(g, m, k), random_w8(g, n, k), random_a8(g, m, k)
+    r = bf(g, m, n).to(DEV)
+    linear_a8(x, w, residual=r)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = linear_a8(x, w, residual=r)
+        q = linear_a8(x, w, out=A8)
+    for rep in range(3):
+        if rep == 2:
+            x.a8.copy_(z.a8)
+            x.s8.copy_(z.s8)
+        graph.replay()
+        eager, codes = linear_a8(x, w, residual=r), linear_a8(x, w, out=A8)
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager) and torch.equal(q.a8, codes.a8) and torch.equal(q.s8, codes.s8), rep
 
 
 def test_results_do_not_depend_on_other_rows():
