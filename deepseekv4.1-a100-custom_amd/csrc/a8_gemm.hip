@@ -44,16 +44,6 @@ DSV41_DEV uint4 a8_decode(uint32_t a, uint32_t b, float sc) {
                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, sc, true)));
 }
 
-// Direct-to-LDS load of 16 (4) bytes a lane from base + off to lds_addr + 16 (4) i; callers wait with vmcnt counts.
-DSV41_DEV void a8_dma16(const void* base, uint32_t off, uint32_t lds_addr) {
-  const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory", "m0");
-}
-DSV41_DEV void a8_dma4(const void* base, uint32_t off, uint32_t lds_addr) {
-  const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory", "m0");
-}
-
 // 16 MT rows by 16 CT output columns a workgroup: a stream of the weights.  Its NW waves take the steps of 128 k in turn
 // (wave v: steps v, v + NW, ...), so that together they read whole rows in order, each through a ring of D steps in LDS
 // that only it fills and reads: no barrier until the sums meet, and D steps of loads on the way in every wave.  (Loads
@@ -103,12 +93,12 @@ __global__ void __launch_bounds__(64 * NW) a8_stream_kernel(const A8Args a) {
 #pragma unroll
     for (int t = 0; t < WT; ++t)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) a8_dma16(GATED && t >= CT ? wb2 : wb, wo[t][u] + k, l + t * 2048 + u * 1024);
+      for (int u = 0; u < 2; ++u) lds_dma16_off(GATED && t >= CT ? wb2 : wb, wo[t][u] + k, l + t * 2048 + u * 1024);
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) a8_dma16(xb, xo[t][u] + k, l + (WT + t) * 2048 + u * 1024);
-    a8_dma4(xsb + (long)s * a.M * 4, so, l + (WT + MT) * 2048);
+      for (int u = 0; u < 2; ++u) lds_dma16_off(xb, xo[t][u] + k, l + (WT + t) * 2048 + u * 1024);
+    lds_dma4_off(xsb + (long)s * a.M * 4, so, l + (WT + MT) * 2048);
   };
   {  // the weight scales of the columns' block, in whole words or by bytes
     const int row = n0 >> 5, nb = a.K / 32;
@@ -116,7 +106,7 @@ __global__ void __launch_bounds__(64 * NW) a8_stream_kernel(const A8Args a) {
       const uint8_t* p = q ? a.ws2 + (long)row * a.Kc2 : a.ws + (long)row * a.Kc;
       if (a.words)
         for (int c = 0; c < nb / 4; c += 64)
-          a8_dma4(p, (uint32_t)min(c + lane, nb / 4 - 1) * 4, lds_addr_of(&scl[q][0]) + c * 4);
+          lds_dma4_off(p, (uint32_t)min(c + lane, nb / 4 - 1) * 4, lds_addr_of(&scl[q][0]) + c * 4);
       else
         for (int k = lane; k < nb; k += 64) scl[q][k] = p[k];
     }
@@ -323,12 +313,12 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
     const uint32_t l = (uint32_t)(b * STAGE);
     const uint32_t k = (uint32_t)min(kt * 128 + ch, klast);  // (chunks past K load the last one and are zeroed below)
     if (q < XL) {
-      a8_dma16(xb, xo[q] + k, ldsw + l + q * NT * 16);
+      lds_dma16_off(xb, xo[q] + k, ldsw + l + q * NT * 16);
     } else if (q < XL + WL) {  // (a wave's 8 rows are of one matrix)
       const int u = q - XL;
-      a8_dma16(is_up(u * (NT / 8) + wave * 8) ? wb2 : wb, wo[u] + k, ldsw + l + XB + u * NT * 16);
+      lds_dma16_off(is_up(u * (NT / 8) + wave * 8) ? wb2 : wb, wo[u] + k, ldsw + l + XB + u * NT * 16);
     } else {
-      a8_dma4(xsb + (long)kt * a.M * 4, so, ldss + l);
+      lds_dma4_off(xsb + (long)kt * a.M * 4, so, ldss + l);
     }
   };
   {  // the tile's weight scales
@@ -340,7 +330,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
     if (a.words) {  // whole words: by direct loads, ahead of the stages'
       for (int b = wave; b < BN / 32; b += WM * WN)
         for (int c = 0; c < nk; c += 64)
-          a8_dma4(scales(b), (uint32_t)min(c + lane, nk - 1) * 4, lds_addr_of(&scl[b][0]) + c * 4);
+          lds_dma4_off(scales(b), (uint32_t)min(c + lane, nk - 1) * 4, lds_addr_of(&scl[b][0]) + c * 4);
     } else {  // by bytes, 127 behind the last
       for (int b = wave; b < BN / 32; b += WM * WN) {
         const uint8_t* p = scales(b);

@@ -220,16 +220,29 @@ __device__ long long g_dsv41_px[1024][32];
 constexpr int vmcnt_imm(int n) { return (n & 15) | ((n >> 4) << 14) | (0x7 << 4) | (0xf << 8); }
 DSV41_DEV void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// As lds_dma16, with the destination given as a wave-uniform LDS byte address (no generic-to-LDS conversion per
-// load: the caller computes the workgroup's LDS base once).
+// Direct-to-LDS loads: lane i writes 16 (4) bytes at lds_addr + 16 (4) i, lds_addr a wave-uniform LDS byte address.
+// Inline assembly, so that the compiler does not treat later LDS reads as dependent on them (it would wait for every
+// outstanding load before each); callers wait with counted vmcnt.  Compiler-tracked loads are unaffected: loads complete in
+// order, so the compiler's own waits only become stricter.  The load takes its LDS address from m0, and a scalar write of
+// m0 needs one wait state before a load to LDS reads it: the s_nop, which the compiler, blind to what an asm block holds,
+// does not insert.
+#define DSV41_LOAD_LDS(op) "s_mov_b32 m0, %0\n\ts_nop 0\n\t" op
 DSV41_DEV void lds_dma16_at(const void* src, uint32_t lds_addr) {
   const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);  // (an SGPR operand: uniform values may sit in VGPRs)
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m) : "memory", "m0");
+  asm volatile(DSV41_LOAD_LDS("global_load_lds_dwordx4 %1, off") ::"s"(m), "v"(src) : "memory", "m0");
 }
-// As lds_dma16_at, 4 bytes per lane (lane i writes lds_addr + 4 i).
 DSV41_DEV void lds_dma4_at(const void* src, uint32_t lds_addr) {
   const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(m) : "memory", "m0");
+  asm volatile(DSV41_LOAD_LDS("global_load_lds_dword %1, off") ::"s"(m), "v"(src) : "memory", "m0");
+}
+// The same from base + off, base wave-uniform.
+DSV41_DEV void lds_dma16_off(const void* base, uint32_t off, uint32_t lds_addr) {
+  const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
+  asm volatile(DSV41_LOAD_LDS("global_load_lds_dwordx4 %1, %2") ::"s"(m), "v"(off), "s"(base) : "memory", "m0");
+}
+DSV41_DEV void lds_dma4_off(const void* base, uint32_t off, uint32_t lds_addr) {
+  const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
+  asm volatile(DSV41_LOAD_LDS("global_load_lds_dword %1, %2") ::"s"(m), "v"(off), "s"(base) : "memory", "m0");
 }
 // The LDS-address-space view of a generic pointer to a __shared__ object (its low 32 bits): accesses through it
 // are LDS instructions (counted by lgkmcnt alone), not flat ones.
@@ -242,16 +255,9 @@ DSV41_DEV uint32_t lds_addr_of(const void* p) {
   return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p);
 }
 
-// 16-byte direct-to-LDS load: lane i writes lds_dst + 16 i (lds_dst is wave-uniform).  Issued as inline assembly
-// so the compiler does not treat later LDS reads as dependent on it (it would wait for every outstanding load
-// before them); callers wait for these loads with explicit vmcnt counts.  Compiler-tracked loads are unaffected:
-// loads complete in order, so the compiler's own waits only become stricter.
-// The LDS address is the low 32 bits of the flat address of an LDS object (the LDS aperture sits in the high
-// half), taken without the address-space conversion's null test.
-DSV41_DEV void lds_dma16(const void* src, void* lds_dst) {
-  const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds_dst);
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m) : "memory", "m0");
-}
+// As lds_dma16_at, to an LDS object by its pointer: its address is the low 32 bits of the flat one (the LDS aperture sits
+// in the high half), taken without the address-space conversion's null test.
+DSV41_DEV void lds_dma16(const void* src, void* lds_dst) { lds_dma16_at(src, (uint32_t)(uintptr_t)lds_dst); }
 
 // ---- scans
 // Inclusive prefix sum over the 64 lanes of a wave with DPP lane moves (no LDS traffic): shifts of 1, 2, 4, 8

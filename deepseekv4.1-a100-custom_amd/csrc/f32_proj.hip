@@ -27,11 +27,6 @@ struct F32ProjArgs {
   int M, N, K, mtiles;
 };
 
-DSV41_DEV void f32p_dma16(const void* base, uint32_t off, uint32_t lds_addr) {
-  const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory", "m0");
-}
-
 // The leading, middle and last 8 significant bits of a pair of weights.
 DSV41_DEV void split2(uint32_t u0, uint32_t u1, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
   hi = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
@@ -84,9 +79,9 @@ __global__ void __launch_bounds__(512) f32_proj_kernel(const F32ProjArgs a) {
   auto issue = [&](int kt, int b) {
     const uint32_t l = lds0 + (uint32_t)(b * UNIT);
 #pragma unroll
-    for (int u = 0; u < XL; ++u) f32p_dma16(xb + (long)kt * 128, xo[u], l + u * NT * 16);
+    for (int u = 0; u < XL; ++u) lds_dma16_off(xb + (long)kt * 128, xo[u], l + u * NT * 16);
 #pragma unroll
-    for (int u = 0; u < WL; ++u) f32p_dma16(wb + (long)kt * 256, wo[u], l + XB + u * NT * 16);
+    for (int u = 0; u < WL; ++u) lds_dma16_off(wb + (long)kt * 256, wo[u], l + XB + u * NT * 16);
   };
   auto landed = [&](int kt) {  // this wave's loads of stage kt have landed (the one after it may not)
     if (kt + 1 < nk) __builtin_amdgcn_s_waitcnt(vmcnt_imm(LPT));

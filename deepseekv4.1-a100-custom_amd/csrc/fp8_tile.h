@@ -34,12 +34,6 @@ DSV41_DEV uint32_t tile_pack(float a, float b) {  // two fp32 to bf16, round to 
   return __builtin_bit_cast(uint32_t, tile_bf2_t{(__bf16)a, (__bf16)b});
 }
 
-// Direct-to-LDS load of 16 bytes from base + off (lane i writes lds_addr + 16 i); callers wait with vmcnt counts.
-DSV41_DEV void tile_dma16(const void* base, uint32_t off, uint32_t lds_addr) {
-  const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory", "m0");
-}
-
 // 8 of a lane's 16 weight bytes (one 16-k group) as bf16, block scale applied; byte word i holds k (2i, 2i + 1) in its
 // low half and (2i + 8, 2i + 9) in its high half.  Part h of the k order of x: words' low (h = 0: k 0..7) or high
 // halves (k 8..15).  Part h of the byte order: words 2h and 2h + 1.
@@ -116,9 +110,9 @@ __global__ void __launch_bounds__(64 * WM * WN) fp8_tile_kernel(const TileArgs a
       const uint8_t* wp = wb + (long)(kt * KU + q) * 64;
       const uint32_t l = lds0 + (uint32_t)((b * KU + q) * UNIT);
 #pragma unroll
-      for (int u = 0; u < XL; ++u) tile_dma16(xp, xo[u], l + u * NT * 16);
+      for (int u = 0; u < XL; ++u) lds_dma16_off(xp, xo[u], l + u * NT * 16);
 #pragma unroll
-      for (int u = 0; u < WL; ++u) tile_dma16(wp, wo[u], l + XB + u * NT * 16);
+      for (int u = 0; u < WL; ++u) lds_dma16_off(wp, wo[u], l + XB + u * NT * 16);
     }
   };
   {
