@@ -2,12 +2,14 @@
 //   linear: y[m, n] = act(sum_k x[m, k] w[n, k] + bias[n]) + residual[m, n]
 //   gated:  y[m, n] = act(min(g, limit)) clamp(u, -limit, limit),  g = sum_k x wg, u = sum_k x wu
 // x and y: A8 (a8_core.h), y also bf16; w: e4m3 codes [N, K] and E8M0 scales per [32 x 32] block (dsv41/w8.py:39-60).
-// Both operands keep their bytes: the block-scaled matrix instructions take the codes and the scales of 32 k of a row as
-// they are.  A lane's 32 codes of the instruction (16 rows, 128 k; lane group g = lane / 16) are k 16 g .. 16 g + 15 and
-// 64 + 16 g .. 64 + 16 g + 15, and the scale it gives is that of k 32 g .. 32 g + 31.
-// The instruction adds its products with about 2^-16 of relative error (measured 1.5e-5 in the 2-norm at every K, random
-// in sign), well below half a step of bf16 (2^-9 of a value) or of e4m3; outputs are therefore bf16 or A8, not fp32.
-// Sums over k are fp32, in a fixed order.
+// Both operands keep their bytes up to the registers, where code times scale becomes bf16: exact (in bf16's range, past
+// which a value is infinite), and so are the bf16 matrix units' products; sums over k are fp32, in a fixed order (8.8e-8 of
+// relative error in the 2-norm at 5120 k, 1.2e-7 at 8192).  A lane's 32 codes of 128 k (16 rows; lane group g = lane / 16)
+// are k 32 g .. 32 g + 31: one scale.
+// The fp8 matrix instructions, block-scaled or not, take the bytes as they are at twice the rate, but drop what lies some
+// 2^-17 below an instruction's largest product: 1.5e-5 in the 2-norm for normal values, 4.5e-5 with a few large channels,
+// and where two large products cancel, all of the result.  That is not a sum in 32 bits, so they are not used (with them
+// 4096 x 5120 x 8192 took 161 us a pass for 301, gated 4096 x 2 x 8192 x 5120 290 for 541; up to 130 rows 3 % less).
 //
 // The weights are the instruction's row operand: a lane ends with 4 adjacent columns of a row of y.
 #include <type_traits>
@@ -26,16 +28,9 @@ struct A8Args {
   int words;                  // weight scales in whole words: K % 128 == 0, rows 4-byte aligned
 };
 
-DSV41_DEV i32x8_t a8_operand(uint4 lo, uint4 hi) {
-  return i32x8_t{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+DSV41_DEV float a8_e8m0(int s) {
+  return s == 255 ? __builtin_nanf("") : s ? __int_as_float(s << 23) : __int_as_float(0x00400000);
 }
-// (scales in the lowest byte)
-DSV41_DEV f32x4_t a8_mfma16(i32x8_t a, i32x8_t b, f32x4_t c, int sa, int sb) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
-}
-
-// ------------------------------------------------------------------------------------------------ few rows
-DSV41_DEV float a8_e8m0(int s) { return s == 255 ? __builtin_nanf("") : s ? __int_as_float(s << 23) : __int_as_float(0x00400000); }
 // 8 codes (two words) times their scale, exact in bf16.
 DSV41_DEV uint4 a8_decode(uint32_t a, uint32_t b, float sc) {
   return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, sc, false)),
@@ -44,17 +39,14 @@ DSV41_DEV uint4 a8_decode(uint32_t a, uint32_t b, float sc) {
                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, sc, true)));
 }
 
+// ------------------------------------------------------------------------------------------------ few rows
 // 16 MT rows by 16 CT output columns a workgroup: a stream of the weights.  Its NW waves take the steps of 128 k in turn
 // (wave v: steps v, v + NW, ...), so that together they read whole rows in order, each through a ring of D steps in LDS
 // that only it fills and reads: no barrier until the sums meet, and D steps of loads on the way in every wave.  (Loads
 // into registers a step ahead were 16 us where this is 11: 24 rows of 1280 k, 32768 columns.)
-// EXACT: the codes and scales as bf16 (exact), products and sums as the bf16 matrix units have them, in fp32: the time is
-// mostly the weights', and the few blocks of a small output show single codes that fall to the other side of a border
-// (24 rows of 8192 k, 5120 columns 15.5 us, of 5120 k, 2 x 4096 columns 14.7, against 14.0 and 11.9 without).
-// A lane's 32 codes are then k 32 g .. 32 g + 31, one scale block.
 constexpr int kStreamMaxK = 32768;  // (the weight scales of all of K are held in LDS)
 
-template <int MT, int CT, int NW, int D, bool GATED, bool EXACT>
+template <int MT, int CT, int NW, int D, bool GATED>
 __global__ void __launch_bounds__(64 * NW) a8_stream_kernel(const A8Args a) {
   constexpr int WT = GATED ? 2 * CT : CT;  // weight tiles of 16 rows: gate tiles, then up tiles
   constexpr int STEP = (WT + MT) * 2048 + 256, LPS = 2 * (WT + MT) + 1;
@@ -121,7 +113,7 @@ __global__ void __launch_bounds__(64 * NW) a8_stream_kernel(const A8Args a) {
   for (int i = 0; i < WT; ++i)
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  const int c0 = EXACT ? (2 * g) ^ (l16 & 7) : g ^ (l16 & 7), c1 = EXACT ? c0 ^ 1 : c0 ^ 4;  // a lane's two chunks
+  const int c0 = (2 * g) ^ (l16 & 7), c1 = c0 ^ 1;  // a lane's two chunks
   const int last = a.K / 32 - 1;
   int bi = 0;
 #pragma unroll 1
@@ -151,35 +143,24 @@ __global__ void __launch_bounds__(64 * NW) a8_stream_kernel(const A8Args a) {
     uint4 x[MT][2];
 #pragma unroll
     for (int j = 0; j < MT; ++j) operand(WT + j, x[j][0], x[j][1]);
-    if constexpr (EXACT) {
-      uint4 xd[MT][4];
+    uint4 xd[MT][4];
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const float sc = a8_e8m0(xs[j]);
+    for (int j = 0; j < MT; ++j) {
+      const float sc = a8_e8m0(xs[j]);
 #pragma unroll
-        for (int h = 0; h < 4; ++h)
-          xd[j][h] = h & 1 ? a8_decode(x[j][h >> 1].z, x[j][h >> 1].w, sc) : a8_decode(x[j][h >> 1].x, x[j][h >> 1].y, sc);
-      }
+      for (int h = 0; h < 4; ++h)
+        xd[j][h] = h & 1 ? a8_decode(x[j][h >> 1].z, x[j][h >> 1].w, sc) : a8_decode(x[j][h >> 1].x, x[j][h >> 1].y, sc);
+    }
 #pragma unroll
-      for (int t = 0; t < WT; ++t) {
-        const float sc = a8_e8m0(ws[t / CT]);
-        uint4 c[2];
-        operand(t, c[0], c[1]);
+    for (int t = 0; t < WT; ++t) {
+      const float sc = a8_e8m0(ws[t / CT]);
+      uint4 c[2];
+      operand(t, c[0], c[1]);
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const uint4 w = h & 1 ? a8_decode(c[h >> 1].z, c[h >> 1].w, sc) : a8_decode(c[h >> 1].x, c[h >> 1].y, sc);
+      for (int h = 0; h < 4; ++h) {
+        const uint4 w = h & 1 ? a8_decode(c[h >> 1].z, c[h >> 1].w, sc) : a8_decode(c[h >> 1].x, c[h >> 1].y, sc);
 #pragma unroll
-          for (int j = 0; j < MT; ++j) acc[t][j] = mfma_bf16_16x16x32(w, xd[j][h], acc[t][j]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < WT; ++t) {
-        uint4 c[2];
-        operand(t, c[0], c[1]);
-#pragma unroll
-        for (int j = 0; j < MT; ++j)
-          acc[t][j] = a8_mfma16(a8_operand(c[0], c[1]), a8_operand(x[j][0], x[j][1]), acc[t][j], ws[t / CT], xs[j]);
+        for (int j = 0; j < MT; ++j) acc[t][j] = mfma_bf16_16x16x32(w, xd[j][h], acc[t][j]);
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this slot is read: the next issue may fill it
@@ -249,6 +230,9 @@ DSV41_DEV void a8_wave_out(const A8Args& a, const uint8_t* s, int m0, int n0) {
 }
 
 // BM rows of x by BN rows of weights in WM x WN waves of (BM / WM) x (BN / WN); stages of 128 k through NBUF LDS buffers.
+// Bound: the bf16 matrix units under load.  256 x 256, gated 4096 x 2 x 8192 x 5120: 523 us, 1.31 PFLOP/s (a library bf16
+// product of 8192^3: 1.24); a wave's 96 decoding conversions of a half stand beside 64 products of 16 cycles.  Smaller tiles
+// decode more a product: 128 x 128, a wave of 32 x 64, 0.87.
 // A gated tile has BN / 2 output columns: of a wave's 32-row weight blocks the even ones are gate rows, the odd ones the
 // up rows of the same columns.
 template <int BM, int BN, int WM, int WN, int NBUF, bool GATED>
@@ -258,19 +242,19 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
   constexpr int XB = BM * 128, WB = BN * 128, SB = BM * 4, STAGE = XB + WB + SB;
   constexpr int XL = XB / 16 / NT, WL = WB / 16 / NT, LPT = XL + WL + 1;  // loads per thread and stage
   constexpr int OC = GATED ? BN / 2 : BN;                                 // output columns
-  // A stage is MT steps: x block t with the CT weight blocks.  x of a step is read AHEAD steps before, across the stage's
-  // end too: the barrier stands in step ENTER, where the first of the next stage is read.  A weight block is read for the
-  // next stage behind its last product.
-  constexpr int RING = MT % 4 == 0 ? 4 : 2, AHEAD = RING / 2, ENTER = MT - AHEAD;
-  // A stage's loads are issued between the products from that barrier on, in the first POS of the MT CT places; FIRST of
-  // them fall into the stage in which they begin.  With two buffers they have less than a stage to land and go out early
-  // (3/8 of the places against 3/4: 291 and 318 us for the gated 4096 x 8192 x 5120); with three, 3/4 is as good or better.
-  constexpr int POS = MT * CT * (NBUF == 2 ? 3 : 6) / 8;
+  // A stage is two halves (a lane's first and second 16 of its 32 codes) of MT steps each: 16 rows of x with the CT weight
+  // blocks.  The codes of a step are read two steps before it, across the stage's end too, and decoded one step before; the
+  // barrier stands in step ENTER, where the first of the next stage is read.  A half's weights are read in the step before
+  // the last of the half in front of it and decoded behind its last products.
+  constexpr int S = 2 * MT, ENTER = S - 2;
+  // A stage's loads are issued between the products from that barrier on, in the first POS of the S CT places; FIRST of
+  // them fall into the stage in which they begin.
+  constexpr int POS = S * CT * (NBUF == 2 ? 3 : 6) / 8;
   constexpr auto upto = [](int z) constexpr { return z >= POS ? LPT : z * LPT / POS; };
-  constexpr int FIRST = upto(AHEAD * CT);
+  constexpr int FIRST = upto(2 * CT);
   static_assert(XL * NT * 16 == XB && WL * NT * 16 == WB && MT * WM * 16 == BM && CT * WN * 16 == BN, "tile shape");
   static_assert(!GATED || CT % 4 == 0, "gate and up blocks in pairs");
-  static_assert(MT % RING == 0 && BM % 64 == 0, "ring, scales of 64 rows a wave");
+  static_assert(MT >= 2 && BM % 64 == 0, "two steps a half, scales of 64 rows a wave");
   static_assert((NBUF - 2) * LPT + FIRST < 64, "vmcnt immediate");
   __shared__ __align__(16) uint8_t buf[NBUF * STAGE];
   __shared__ __align__(16) uint8_t scl[BN / 32][kTileMaxK / 32 + 16];
@@ -349,52 +333,75 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
 #pragma unroll
     for (int j = 0; j < CT; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   const int xr = wm * (BM / WM) + l16, wr = wn * (BN / WN) + l16;  // (16-row steps keep the swizzle's row bits)
-  const int c0 = (g ^ (l16 & 7)) * 16, c1 = c0 ^ 64;                // chunks g and 4 + g
-  auto operand = [&](const uint8_t* p) { return a8_operand(*(const uint4*)(p + c0), *(const uint4*)(p + c1)); };
+  const int c0 = ((2 * g) ^ (l16 & 7)) * 16;                        // chunk 2 g; 2 g + 1 sits at c0 ^ 16
   // The next stage has landed for every wave (`later` younger loads may not have), and every wave has read this one.
   auto enter = [&](auto later) {
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(decltype(later)::value));
     lds_barrier();
   };
-  i32x8_t xf[RING], wf[CT];
-  int xs[RING], ws[CT];  // (bytes: a shift of a word would wait for it where it is read)
-  auto fetch_w = [&](int j, int kt, int b) {
-    wf[j] = operand(buf + b * STAGE + XB + (wr + 16 * j) * 128);
-    ws[j] = scl[(wn * CT + j) / 2][kt * 4 + g];  // (kt may be one past the last: the row is longer)
-  };
-  auto fetch_x = [&](int t, int b) {
+  uint4 xq[2], wq[CT], xd[2][2], wd[CT][2];  // codes as read; decoded
+  int xs[2], ws[CT / 2];                     // scale bytes
+  float wsc[CT / 2];
+  auto read_x = [&](int u, int b) {
     const uint8_t* st = buf + b * STAGE;
-    xf[t % RING] = operand(st + (xr + 16 * t) * 128);
-    xs[t % RING] = st[XB + WB + (xr + 16 * t) * 4 + g];
+    xq[u & 1] = *(const uint4*)(st + (xr + 16 * (u % MT)) * 128 + (c0 ^ (u / MT * 16)));
+    xs[u & 1] = st[XB + WB + (xr + 16 * (u % MT)) * 4 + g];
+  };
+  auto read_w = [&](int half, int kt, int b) {
+#pragma unroll
+    for (int j = 0; j < CT; ++j) wq[j] = *(const uint4*)(buf + b * STAGE + XB + (wr + 16 * j) * 128 + (c0 ^ (half * 16)));
+    if (half == 0) {
+#pragma unroll
+      for (int j = 0; j < CT / 2; ++j) ws[j] = scl[wn * (CT / 2) + j][kt * 4 + g];  // (kt may be one past the last: the row is longer)
+    }
+  };
+  auto decode_x = [&](int u) {
+    const float sc = a8_e8m0(xs[u & 1]);
+    xd[u & 1][0] = a8_decode(xq[u & 1].x, xq[u & 1].y, sc);
+    xd[u & 1][1] = a8_decode(xq[u & 1].z, xq[u & 1].w, sc);
+  };
+  auto decode_w = [&](int j) {
+    wd[j][0] = a8_decode(wq[j].x, wq[j].y, wsc[j / 2]);
+    wd[j][1] = a8_decode(wq[j].z, wq[j].w, wsc[j / 2]);
+  };
+  auto scales_w = [&] {
+#pragma unroll
+    for (int j = 0; j < CT / 2; ++j) wsc[j] = a8_e8m0(ws[j]);
+  };
+  auto product = [&](int u, int j) {
+    acc[u % MT][j] = mfma_bf16_16x16x32(wd[j][0], xd[u & 1][0], acc[u % MT][j]);
+    acc[u % MT][j] = mfma_bf16_16x16x32(wd[j][1], xd[u & 1][1], acc[u % MT][j]);
   };
   if (nk > 0) {
     int bi = 0;
     enter(std::integral_constant<int, (NBUF - 2) * LPT + FIRST>{});
+    read_w(0, 0, 0);
+    read_x(0, 0);
+    read_x(1, 0);
+    scales_w();
 #pragma unroll
-    for (int j = 0; j < CT; ++j) fetch_w(j, 0, 0);
-#pragma unroll
-    for (int t = 0; t < AHEAD; ++t) fetch_x(t, 0);
+    for (int j = 0; j < CT; ++j) decode_w(j);
+    decode_x(0);
 #pragma unroll 1
     for (int kt = 0; kt < nk; ++kt) {  // (what the last stage reads and loads ahead is the last again, and not used)
       const int b0 = bi;
       bi = bi + 1 == NBUF ? 0 : bi + 1;
       const int bp = b0 == 0 ? NBUF - 1 : b0 - 1;
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        if (t < ENTER) {
-          fetch_x(t + AHEAD, b0);
-        } else {
-          if (t == ENTER) enter(std::integral_constant<int, (NBUF - 2) * LPT>{});
-          fetch_x(t - ENTER, bi);
-        }
+      for (int u = 0; u < S; ++u) {
+        if (u == ENTER) enter(std::integral_constant<int, (NBUF - 2) * LPT>{});
+        if (u % MT == MT - 2) read_w(u < MT ? 1 : 0, u < MT ? kt : kt + 1, u < MT ? b0 : bi);
+        read_x((u + 2) % S, u < ENTER ? b0 : bi);
         __builtin_amdgcn_sched_barrier(0);
+        if (u == S - 1) scales_w();
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
-          acc[t][j] = a8_mfma16(wf[j], xf[t % RING], acc[t][j], ws[j], xs[t % RING]);
-          if (t == MT - 1) fetch_w(j, kt + 1, bi);
-          const int z = (t < ENTER ? t + AHEAD : t - ENTER) * CT + j;
+          product(u, j);
+          if (j == 0) decode_x((u + 1) % S);
+          if (u % MT == MT - 1) decode_w(j);
+          const int z = (u < ENTER ? u + 2 : u - ENTER) * CT + j;
 #pragma unroll
-          for (int q = upto(z); q < upto(z + 1); ++q) dma(min(t < ENTER ? kt + NBUF - 1 : kt + NBUF, nk - 1), t < ENTER ? bp : b0, q);
+          for (int q = upto(z); q < upto(z + 1); ++q) dma(min(u < ENTER ? kt + NBUF - 1 : kt + NBUF, nk - 1), u < ENTER ? bp : b0, q);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -411,13 +418,18 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
       if ((e & 7) * 16 >= tail) *(uint4*)(buf + (e >> 3) * 128 + (((e & 7) ^ ((e >> 3) & 7)) * 16)) = make_uint4(0, 0, 0, 0);
     lds_barrier();
 #pragma unroll
-    for (int j = 0; j < CT; ++j) fetch_w(j, nk, 0);
+    for (int u = 0; u < S; ++u) {
+      if (u % MT == 0) {
+        read_w(u / MT, nk, 0);
+        if (u == 0) scales_w();
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      fetch_x(t, 0);
-      xs[t % RING] = buf[XB + WB + (xr + 16 * t) * 4 + min(g, tail / 32 - 1)];  // (bytes behind the last may be anything)
+        for (int j = 0; j < CT; ++j) decode_w(j);
+      }
+      read_x(u, 0);
+      xs[u & 1] = buf[XB + WB + (xr + 16 * (u % MT)) * 4 + min(g, tail / 32 - 1)];  // (bytes behind the last may be anything)
+      decode_x(u);
 #pragma unroll
-      for (int j = 0; j < CT; ++j) acc[t][j] = a8_mfma16(wf[j], xf[t % RING], acc[t][j], ws[j], xs[t % RING]);
+      for (int j = 0; j < CT; ++j) product(u, j);
     }
     lds_barrier();
   }
@@ -444,13 +456,14 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
 // against 13.3 of 32) unless the output is in blocks of 32 or there are columns enough to fill the card twice over (32768
 // columns of 1280 k 10.5 against 9.1 us, in workgroups of 2 waves, 10.3 in 4); 8 waves where a workgroup of 4 to every CU
 // would leave half of them idle (512 columns of 5120 k 5.3 against 6.1 us).
-// More rows: the least of the estimates below, microseconds a round of the card (measured over 10 to 64 steps; the
-// partly filled last round counted as a whole one, which it is within a tenth: 33 to 4096 rows of the layer's widths).
-// Streams of 32, 48 and 64 rows at 5120 k, us: 64 rows of 2048 columns 6.6, 7.4, 8.9; 130 rows 9.7, 7.7, 8.6; 200 rows
-// 10.3, 12.9, 8.8; and the smallest tile 17.
-// Of a tile and the same one with rows and columns exchanged the one with more rows was the faster: the same areas
-// the other way, us: 64 x 128 for 128 x 64 at 1000 rows of 2048 columns and 5120 k 22 for 19; 64 x 256 for 128 x 128 at 512
-// rows of 2 x 4096 gated 27 to 32 for 24 to 28; 128 x 256 for 256 x 128 at 4096 rows of 2 x 8192 gated 330 for 297.
+// More rows: the least of the estimates below, microseconds (fitted to whole rounds of 640 to 8192 k; 33 to 4096 rows of
+// the layer's widths: within a tenth of the fastest kernel but for a few places between two rounds).  Of estimates within
+// half a microsecond of the least, which is as well as they are known, the one that reads the fewest operand bytes.
+// Streams of 32, 48 and 64 rows and the smallest tile at 5120 k and 2048 columns, us: 64 rows 9.3, 11.1, 12.8, 36; 130 rows
+// 12.4, 11.5, 13.4, 37; 500 rows 24.1, 31.5, 25.7, 38.  A stream's blocks of rows read the weights again, half of them past
+// the caches: 64 rows of 8192 columns and 8192 k 34 us in two blocks of 32 rows and 23 in one of 64.
+// A tile with rows and columns exchanged is as fast (64 x 128, 64 x 256, 128 x 256: within 3 %).  One round of 256 x 256
+// and one of 128 x 128 for the columns behind it: 4096 rows of 5120 columns, 8192 k 293 us for 323 in 2 rounds of 192 x 256.
 constexpr int kCus = 256;
 constexpr int kMaxRows = 0x7fffff00;  // (a workgroup's rows are counted to its end)
 enum A8Kernel {
@@ -476,51 +489,66 @@ A8Parts a8_plan(int M, int N, int K, bool gated, bool a8_out) {
   }
   struct Cost {
     A8Plan plan;
-    float fixed, step;  // us of a round: launch, first loads and output; 128 k
-    int slots;
+    float fixed, step;  // us of a round of kCus workgroups: launch, first loads and output; 128 k
+    int least;          // rounds at least (2: two workgroups a CU at once)
   };
-  const int sc = gated ? 64 : 32;  // weight rows of a stream
-  const Cost costs[] = {
-      {{kStream32, 32, sc, 4}, gated ? 2.6f : 3.0f, gated ? 0.16f : 0.09f, kCus},  // one workgroup a CU
-      {{kStream32, 32, sc, 4}, 3.2f, gated ? 0.32f : 0.18f, 2 * kCus},             // two
-      {{kStream48, 48, sc, 4}, 2.8f, gated ? 0.215f : 0.125f, kCus},
-      {{kStream64, 64, sc, 4}, 3.0f, gated ? 0.25f : 0.157f, kCus},
-      {{kTile128x64, 128, 64, 4}, 5.5f, 0.32f, kCus},      // one workgroup a CU
-      {{kTile128x64, 128, 64, 4}, 8.0f, 0.58f, 2 * kCus},  // two
-      {{kTile128x128, 128, 128, 8}, 7.5f, 0.47f, kCus},
-      {{kTile256x128, 256, 128, 8}, 11.0f, 0.68f, kCus},
-      {{kTile192x256, 192, 256, 8}, 13.5f, 1.05f, kCus},
-      {{kTile256x256, 256, 256, 8}, 19.0f, 1.22f, kCus},
+  const Cost linear[] = {
+      {{kStream32, 32, 32, 4}, 3.5f, 0.159f, 1},   {{kStream32, 32, 32, 4}, 1.9f, 0.120f, 2},
+      {{kStream48, 48, 32, 4}, 3.6f, 0.203f, 1},   {{kStream64, 64, 32, 4}, 4.0f, 0.250f, 1},
+      {{kTile128x64, 128, 64, 4}, 5.7f, 0.877f, 1}, {{kTile128x64, 128, 64, 4}, 3.4f, 0.690f, 2},
+      {{kTile128x128, 128, 128, 8}, 7.2f, 1.335f, 1}, {{kTile256x128, 256, 128, 8}, 10.5f, 2.110f, 1},
+      {{kTile192x256, 192, 256, 8}, 13.1f, 2.800f, 1}, {{kTile256x256, 256, 256, 8}, 16.4f, 3.520f, 1},
   };
+  const Cost gates[] = {  // (two 32-row streams do not fit a CU's LDS: 102400 bytes each)
+      {{kStream32, 32, 64, 4}, 4.0f, 0.250f, 1},
+      {{kStream48, 48, 64, 4}, 4.4f, 0.312f, 1},   {{kStream64, 64, 64, 4}, 5.0f, 0.372f, 1},
+      {{kTile128x64, 128, 64, 4}, 4.3f, 0.940f, 1}, {{kTile128x64, 128, 64, 4}, 2.4f, 0.703f, 2},
+      {{kTile128x128, 128, 128, 8}, 5.0f, 1.360f, 1}, {{kTile256x128, 256, 128, 8}, 7.0f, 2.160f, 1},
+      {{kTile192x256, 192, 256, 8}, 8.7f, 2.810f, 1}, {{kTile256x256, 256, 256, 8}, 11.3f, 3.520f, 1},
+  };
+  const Cost* const costs = gated ? gates : linear;
+  const int n_costs = gated ? sizeof(gates) / sizeof(Cost) : sizeof(linear) / sizeof(Cost);
   const float steps = (float)((K + 127) / 128);
   const long wr = gated ? 2 : 1;
-  // The least estimate for n columns on one kernel (`any`, or a tile kernel)
-  auto least = [&](long n, bool any, A8Plan* plan) {
-    float best = 0.0f;
-    for (const Cost& c : costs) {
-      const bool tile = c.plan.kernel >= kTile128x64;
-      const long rows = (M + c.plan.rows - 1l) / c.plan.rows, groups = rows * ((n * wr + c.plan.cols - 1) / c.plan.cols);
-      if (tile ? K > kTileMaxK : !any || rows > 65535) continue;  // (a stream's row blocks are the grid's y)
-      const float us = (float)((groups + c.slots - 1) / c.slots) * (c.fixed + steps * c.step);
-      if (best == 0.0f || us < best) {
-        best = us;
-        *plan = c.plan;
-      }
-    }
-    return best;
+  struct Estimate {
+    float us, bytes;  // bytes: operands read, a k
   };
-  A8Parts p{costs[3].plan, costs[3].plan, N};
-  float best = least(N, true, &p.plan);
-  // Or the columns that fill whole rounds of a tile kernel, and a second launch for the others (4096 rows of 5120 columns,
-  // 8192 k: one round of 256 x 256 and one of 128 x 128 155 us, 3 rounds of 256 x 128, half the last empty, 165)
+  auto estimate = [&](const Cost& c, long n) {
+    const long rows = (M + c.plan.rows - 1l) / c.plan.rows, cols = (n * wr + c.plan.cols - 1) / c.plan.cols;
+    const float rounds = fmaxf((float)((rows * cols + kCus - 1) / kCus), (float)c.least), weights = (float)(n * wr);
+    float us = rounds * (c.fixed + steps * c.step);
+    if (c.plan.kernel < kTile128x64) us = fmaxf(us, weights * (float)K * (0.5f + 0.5f * (float)rows) / 3.1e6f);
+    return Estimate{us, weights * (float)rows + (float)M * (float)cols};
+  };
+  // The plan of n columns on one kernel (`any`, or a tile kernel), and its estimate
+  auto choose = [&](long n, bool any, A8Plan* plan) {
+    float best = 1e30f;
+    auto open = [&](const Cost& c) {  // (a stream's row blocks are the grid's y)
+      return c.plan.kernel >= kTile128x64 ? K <= kTileMaxK : any && (M + c.plan.rows - 1l) / c.plan.rows <= 65535;
+    };
+    for (int i = 0; i < n_costs; ++i)
+      if (open(costs[i])) best = fminf(best, estimate(costs[i], n).us);
+    Estimate least{best, 1e30f};
+    for (int i = 0; i < n_costs; ++i) {
+      const Estimate e = estimate(costs[i], n);
+      if (!open(costs[i]) || e.us > best + 0.5f || e.bytes > least.bytes || (e.bytes == least.bytes && e.us >= least.us)) continue;
+      least = e;
+      *plan = costs[i].plan;
+    }
+    return least.us;
+  };
+  A8Parts p{linear[3].plan, linear[3].plan, N};
+  float best = choose(N, true, &p.plan);
+  // Or the columns that fill whole rounds of a tile kernel, and a second launch for the others
   if (K <= kTileMaxK) {
-    for (const Cost& c : costs) {
+    for (int i = 0; i < n_costs; ++i) {
+      const Cost& c = costs[i];
       if (c.plan.kernel < kTile128x64) continue;
-      const long rows = (M + c.plan.rows - 1l) / c.plan.rows, per = c.plan.cols / wr, rounds = rows * (N / per) / c.slots;
-      const long columns = rounds * c.slots / rows * per;
-      if (columns == 0 || columns >= N) continue;
+      const long rows = (M + c.plan.rows - 1l) / c.plan.rows, per = c.plan.cols / wr, rounds = rows * (N / per) / kCus;
+      const long columns = rounds * kCus / rows * per;
+      if (rounds < c.least || columns == 0 || columns >= N) continue;
       A8Plan rest;
-      const float us = (float)rounds * (c.fixed + steps * c.step) + least(N - columns, false, &rest);
+      const float us = (float)rounds * (c.fixed + steps * c.step) + choose(N - columns, false, &rest);
       if (us < 0.97f * best) {
         best = us;
         p = A8Parts{c.plan, rest, (int)columns};
@@ -544,24 +572,22 @@ int a8_launch(A8Args& a, const A8Plan& p, int first, int end, hipStream_t st) {
   const dim3 gs((unsigned)a.ntiles, (unsigned)a.mtiles), gt((unsigned)tiles);
   switch (p.kernel) {
     case kStream16:
-      if (p.cols == 16 && p.waves == 8) a8_stream_kernel<1, 1, 8, 2, GATED, true><<<gs, 512, 0, st>>>(a);
-      else if (p.cols == 16) a8_stream_kernel<1, 1, 4, 2, GATED, true><<<gs, 256, 0, st>>>(a);
-      else if (p.waves == 2) a8_stream_kernel<1, 2, 2, 2, GATED, true><<<gs, 128, 0, st>>>(a);
-      else a8_stream_kernel<1, 2, 4, 2, GATED, true><<<gs, 256, 0, st>>>(a);
+      if (p.cols == 16 && p.waves == 8) a8_stream_kernel<1, 1, 8, 2, GATED><<<gs, 512, 0, st>>>(a);
+      else if (p.cols == 16) a8_stream_kernel<1, 1, 4, 2, GATED><<<gs, 256, 0, st>>>(a);
+      else if (p.waves == 2) a8_stream_kernel<1, 2, 2, 2, GATED><<<gs, 128, 0, st>>>(a);
+      else a8_stream_kernel<1, 2, 4, 2, GATED><<<gs, 256, 0, st>>>(a);
       break;
     case kStream32:
-      if (a.M > 32) {
-        a8_stream_kernel<2, 2, 4, 2, GATED, false><<<gs, 256, 0, st>>>(a);
-      } else if (p.cols == 16) {
-        if constexpr (!GATED) a8_stream_kernel<2, 1, 4, 2, false, true><<<gs, 256, 0, st>>>(a);
+      if (p.cols == 16) {
+        if constexpr (!GATED) a8_stream_kernel<2, 1, 4, 2, false><<<gs, 256, 0, st>>>(a);
       } else if (p.waves == 2) {
-        a8_stream_kernel<2, 2, 2, 2, GATED, true><<<gs, 128, 0, st>>>(a);
+        a8_stream_kernel<2, 2, 2, 2, GATED><<<gs, 128, 0, st>>>(a);
       } else {
-        a8_stream_kernel<2, 2, 4, 2, GATED, true><<<gs, 256, 0, st>>>(a);
+        a8_stream_kernel<2, 2, 4, 2, GATED><<<gs, 256, 0, st>>>(a);
       }
       break;
-    case kStream48: a8_stream_kernel<3, 2, 4, 2, GATED, false><<<gs, 256, 0, st>>>(a); break;
-    case kStream64: a8_stream_kernel<4, 2, 4, 2, GATED, false><<<gs, 256, 0, st>>>(a); break;
+    case kStream48: a8_stream_kernel<3, 2, 4, 2, GATED><<<gs, 256, 0, st>>>(a); break;
+    case kStream64: a8_stream_kernel<4, 2, 4, 2, GATED><<<gs, 256, 0, st>>>(a); break;
     case kTile128x64: a8_tile_kernel<128, 64, 4, 1, 3, GATED><<<gt, 256, 0, st>>>(a); break;
     case kTile128x128: a8_tile_kernel<128, 128, 4, 2, 3, GATED><<<gt, 512, 0, st>>>(a); break;
     case kTile256x128: a8_tile_kernel<256, 128, 4, 2, 3, GATED><<<gt, 512, 0, st>>>(a); break;

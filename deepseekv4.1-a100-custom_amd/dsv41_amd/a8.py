@@ -1,8 +1,8 @@
 """Activations in 8 bits and the operators on them: the twin of the W8 weights (dsv41/w8.py:39-60) for x.
 
 fake_quant_fp8 / norm_quant put activations ON the fp8 grid and keep them in bf16; here they are held as the grid's own
-bytes -- e4m3 codes with one E8M0 scale per 32 values of a row -- and multiplied as they are by the block-scaled fp8
-matrix instructions.  What stands between the attention layer and the next one is then three launches:
+bytes -- e4m3 codes with one E8M0 scale per 32 values of a row -- which the products turn into bf16 in registers, exactly,
+beside the weights.  What stands between the attention layer and the next one is then three launches:
 
   q, h = norm_quant8(x, w, eps, residual=r)     h = x + r, q = rmsnorm(h) * w in 8 bits
   a    = gated_a8(q, w_gate, w_up)              silu(q Wg^T) * (q Wu^T) in 8 bits

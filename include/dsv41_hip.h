@@ -337,9 +337,11 @@ int dsv41_norm_quant8(const void* x, const void* residual, const void* w, float 
  * K % 32 == 0, K <= 32768.
  * bias bf16 or (bias_f32) fp32 [N] or null; act 0 none, 1 relu, 2 silu, 3 gelu (erf), 4 gelu by tanh; residual bf16
  * [M, N] or null.  Exactly one output: out bf16 [M, N], or (out null) out_a8 / out_s8, the result as 8-bit activations,
- * N % 32 == 0.  fp32 sums, of exact bf16 products up to 32 rows and on the block-scaled fp8 matrix instructions (2^-16
- * relative) above, rounded once.  Streams (K > 16384 always) take up to 65535 blocks of rows.  Replaces
- * cukern.fp8_gemm_tc (dsv41/cukern.py:164-200) where x is held in 8 bits. */
+ * N % 32 == 0.  Products are exact (values of x and w in bf16's range; past it they are infinite) and sums fp32, rounded
+ * once; their order depends on the kernel that the sizes take (dsv41_a8_plan), so a row's last bit may change with M.
+ * K > 16384 and M > 32: streams of at most 64 rows, which read the weights once for each (4096 rows take several times what
+ * the tiles would), up to 65535 blocks of rows.  Replaces cukern.fp8_gemm_tc (dsv41/cukern.py:164-200) where x is held in
+ * 8 bits; no block-diagonal form (group_cols). */
 int dsv41_linear_a8(const void* a8, const void* s8, const void* w8, const void* ws8, int M, int N, int K, int Kc,
                     const void* bias, int bias_f32, int act, const void* residual, void* out, void* out_a8,
                     void* out_s8, void* stream);
