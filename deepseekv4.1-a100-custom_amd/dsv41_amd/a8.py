@@ -204,6 +204,8 @@ def gated_a8(x: A8, w_gate: W8, w_up: W8, act: str = "silu", limit: float = 0.0,
         raise RuntimeError(f"gated_a8: gate {w_gate.shape}, up {w_up.shape}")
     if not limit >= 0.0:
         raise ValueError(f"gated_a8: limit {limit} (0: none)")
+    if limit > 0.0:
+        limit = max(limit, 2.0 ** -149)  # (fp32's smallest number: less would be 0, no limit)
     xa, xs, ga, gs, ua, us = x.a8, x.s8, w_gate.w8, w_gate.s8, w_up.w8, w_up.s8
     index = _index(xa, xs, ga, gs, ua, us)
     if (xa.data_ptr() | ga.data_ptr() | ua.data_ptr()) & 15 or xs.data_ptr() & 3:
