@@ -105,9 +105,10 @@ def _launch(name: str, index: int, *args) -> None:
 def norm_quant8(x: torch.Tensor, w: torch.Tensor | None, eps: float, residual: torch.Tensor | None = None):
     """rmsnorm(x + residual) * w in 8 bits, the residual's addition and the norm (dsv41/fused2.py:251-272) in one pass.
 
-    x, residual: bf16 [..., D], D % 32 == 0, D <= 16384; w: [D] or None (no norm: the quantisation alone).  Returns the
-    A8, with a residual (A8, h): h = bf16(x + residual), the stream that the norm is of.  The normed value is rounded
-    once, to 8 bits (norm_quant rounds to bf16 in between, as the reference does, so single codes differ from its)."""
+    x, residual: bf16 [..., D], D % 32 == 0, D <= 16384; w: [D], rounded to bf16 where it is not (as rmsnorm and
+    norm_quant do), or None (no norm: the quantisation alone).  Returns the A8, with a residual (A8, h): h = bf16(x +
+    residual), the stream that the norm is of.  The normed value is rounded once, to 8 bits (norm_quant rounds to bf16 in
+    between, as the reference does, so single codes differ from its)."""
     index = _index(x, residual, w)
     _no_grad("norm_quant8", x, residual, w)
     shape = x.shape
