@@ -11,8 +11,8 @@ from .w8 import W8
 class GatedFeedForward:
     """y = h + down(act(gate(q)) * up(q)), q = rmsnorm(h) * norm_w, h = x + residual (or x).
 
-    Weights: norm_w [dim] (rounded to bf16 where it is not), gate and up W8 [F, dim], down W8 [dim, F]; F % 32 == 0.  limit as gated_a8's.  Between
-    the launches the activations are A8: q once per value, the gated product once."""
+    Weights: norm_w [dim] (rounded to bf16 where it is not), gate and up W8 [F, dim], down W8 [dim, F]; F % 32 == 0.
+    limit as gated_a8's.  Between the launches the activations are A8: q once per value, the gated product once."""
 
     def __init__(self, norm_w: torch.Tensor, gate: W8, up: W8, down: W8, *, eps: float = 1e-6, act: str = "silu",
                  limit: float = 0.0):
