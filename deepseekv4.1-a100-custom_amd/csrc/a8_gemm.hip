@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
 }
 
 // ------------------------------------------------------------------------------------------------ plan
-// Up to 32 rows: the stream of one row block, exact.  16 columns a workgroup (one token, 8192 k, 5120 columns 10.6 us
+// Up to 32 rows: the stream of one row block, exact.  16 columns a workgroup (one token, 8192 k, 5120 columns 10.8 us
 // against 13.3 of 32) unless the output is in blocks of 32 or there are columns enough to fill the card twice over (32768
 // columns of 1280 k 10.5 against 9.1 us, in workgroups of 2 waves, 10.3 in 4); 8 waves where a workgroup of 4 to every CU
 // would leave half of them idle (512 columns of 5120 k 5.3 against 6.1 us).
