@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
     for (int j = 0; j < CT; ++j) wq[j] = *(const uint4*)(buf + b * STAGE + XB + (wr + 16 * j) * 128 + (c0 ^ (half * 16)));
     if (half == 0) {
 #pragma unroll
-      for (int j = 0; j < CT / 2; ++j) ws[j] = scl[wn * (CT / 2) + j][kt * 4 + g];  // (kt may be one past the last: the row is longer)
+      for (int j = 0; j < CT / 2; ++j) ws[j] = scl[wn * (CT / 2) + j][kt * 4 + g];  // (kt: to one past the last, in the row)
     }
   };
   auto decode_x = [&](int u) {
@@ -401,7 +401,8 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
           if (u % MT == MT - 1) decode_w(j);
           const int z = (u < ENTER ? u + 2 : u - ENTER) * CT + j;
 #pragma unroll
-          for (int q = upto(z); q < upto(z + 1); ++q) dma(min(u < ENTER ? kt + NBUF - 1 : kt + NBUF, nk - 1), u < ENTER ? bp : b0, q);
+          for (int q = upto(z); q < upto(z + 1); ++q)
+            dma(min(u < ENTER ? kt + NBUF - 1 : kt + NBUF, nk - 1), u < ENTER ? bp : b0, q);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
 }
 
 // ------------------------------------------------------------------------------------------------ plan
-// Up to 32 rows: the stream of one row block, exact.  16 columns a workgroup (one token, 8192 k, 5120 columns 10.8 us
+// Up to 32 rows: the stream of one row block.  16 columns a workgroup (one token, 8192 k, 5120 columns 10.8 us
 // against 13.3 of 32) unless the output is in blocks of 32 or there are columns enough to fill the card twice over (32768
 // columns of 1280 k 10.5 against 9.1 us, in workgroups of 2 waves, 10.3 in 4); 8 waves where a workgroup of 4 to every CU
 // would leave half of them idle (512 columns of 5120 k 5.3 against 6.1 us).
@@ -460,8 +461,9 @@ __global__ void __launch_bounds__(64 * WM * WN) a8_tile_kernel(const A8Args a) {
 // the layer's widths: within a tenth of the fastest kernel but for a few places between two rounds).  Of estimates within
 // half a microsecond of the least, which is as well as they are known, the one that reads the fewest operand bytes.
 // Streams of 32, 48 and 64 rows and the smallest tile at 5120 k and 2048 columns, us: 64 rows 9.3, 11.1, 12.8, 36; 130 rows
-// 12.4, 11.5, 13.4, 37; 500 rows 24.1, 31.5, 25.7, 38.  A stream's blocks of rows read the weights again, half of them past
-// the caches: 64 rows of 8192 columns and 8192 k 34 us in two blocks of 32 rows and 23 in one of 64.
+// 12.4, 11.5, 13.4, 37; 500 rows 24.1, 31.5, 25.7, 38.  A stream's blocks of rows read the weights again (3.1 TB/s, half
+// of each reading after the first from the caches): 64 rows of 8192 columns and 8192 k 34 us in two blocks of 32 rows and
+// 23 in one of 64.
 // A tile with rows and columns exchanged is as fast (64 x 128, 64 x 256, 128 x 256: within 3 %).  One round of 256 x 256
 // and one of 128 x 128 for the columns behind it: 4096 rows of 5120 columns, 8192 k 293 us for 323 in 2 rounds of 192 x 256.
 constexpr int kCus = 256;
@@ -493,18 +495,27 @@ A8Parts a8_plan(int M, int N, int K, bool gated, bool a8_out) {
     int least;          // rounds at least (2: two workgroups a CU at once)
   };
   const Cost linear[] = {
-      {{kStream32, 32, 32, 4}, 3.5f, 0.159f, 1},   {{kStream32, 32, 32, 4}, 1.9f, 0.120f, 2},
-      {{kStream48, 48, 32, 4}, 3.6f, 0.203f, 1},   {{kStream64, 64, 32, 4}, 4.0f, 0.250f, 1},
-      {{kTile128x64, 128, 64, 4}, 5.7f, 0.877f, 1}, {{kTile128x64, 128, 64, 4}, 3.4f, 0.690f, 2},
-      {{kTile128x128, 128, 128, 8}, 7.2f, 1.335f, 1}, {{kTile256x128, 256, 128, 8}, 10.5f, 2.110f, 1},
-      {{kTile192x256, 192, 256, 8}, 13.1f, 2.800f, 1}, {{kTile256x256, 256, 256, 8}, 16.4f, 3.520f, 1},
+      {{kStream32, 32, 32, 4}, 3.5f, 0.159f, 1},
+      {{kStream32, 32, 32, 4}, 1.9f, 0.120f, 2},
+      {{kStream48, 48, 32, 4}, 3.6f, 0.203f, 1},
+      {{kStream64, 64, 32, 4}, 4.0f, 0.250f, 1},
+      {{kTile128x64, 128, 64, 4}, 5.7f, 0.877f, 1},
+      {{kTile128x64, 128, 64, 4}, 3.4f, 0.690f, 2},
+      {{kTile128x128, 128, 128, 8}, 7.2f, 1.335f, 1},
+      {{kTile256x128, 256, 128, 8}, 10.5f, 2.110f, 1},
+      {{kTile192x256, 192, 256, 8}, 13.1f, 2.800f, 1},
+      {{kTile256x256, 256, 256, 8}, 16.4f, 3.520f, 1},
   };
   const Cost gates[] = {  // (two 32-row streams do not fit a CU's LDS: 102400 bytes each)
       {{kStream32, 32, 64, 4}, 4.0f, 0.250f, 1},
-      {{kStream48, 48, 64, 4}, 4.4f, 0.312f, 1},   {{kStream64, 64, 64, 4}, 5.0f, 0.372f, 1},
-      {{kTile128x64, 128, 64, 4}, 4.3f, 0.940f, 1}, {{kTile128x64, 128, 64, 4}, 2.4f, 0.703f, 2},
-      {{kTile128x128, 128, 128, 8}, 5.0f, 1.360f, 1}, {{kTile256x128, 256, 128, 8}, 7.0f, 2.160f, 1},
-      {{kTile192x256, 192, 256, 8}, 8.7f, 2.810f, 1}, {{kTile256x256, 256, 256, 8}, 11.3f, 3.520f, 1},
+      {{kStream48, 48, 64, 4}, 4.4f, 0.312f, 1},
+      {{kStream64, 64, 64, 4}, 5.0f, 0.372f, 1},
+      {{kTile128x64, 128, 64, 4}, 4.3f, 0.940f, 1},
+      {{kTile128x64, 128, 64, 4}, 2.4f, 0.703f, 2},
+      {{kTile128x128, 128, 128, 8}, 5.0f, 1.360f, 1},
+      {{kTile256x128, 256, 128, 8}, 7.0f, 2.160f, 1},
+      {{kTile192x256, 192, 256, 8}, 8.7f, 2.810f, 1},
+      {{kTile256x256, 256, 256, 8}, 11.3f, 3.520f, 1},
   };
   const Cost* const costs = gated ? gates : linear;
   const int n_costs = gated ? sizeof(gates) / sizeof(Cost) : sizeof(linear) / sizeof(Cost);
@@ -531,7 +542,8 @@ A8Parts a8_plan(int M, int N, int K, bool gated, bool a8_out) {
     Estimate least{best, 1e30f};
     for (int i = 0; i < n_costs; ++i) {
       const Estimate e = estimate(costs[i], n);
-      if (!open(costs[i]) || e.us > best + 0.5f || e.bytes > least.bytes || (e.bytes == least.bytes && e.us >= least.us)) continue;
+      if (!open(costs[i]) || e.us > best + 0.5f) continue;
+      if (e.bytes > least.bytes || (e.bytes == least.bytes && e.us >= least.us)) continue;
       least = e;
       *plan = costs[i].plan;
     }
