@@ -1,0 +1,500 @@
+// Sparse attention over window rows (bf16) and selected rows of the paged 4-bit cache.
+//
+// One workgroup of four waves: one query row, HB heads, a run of 64-key tiles (first the window's, then the cache's).
+// Each wave scores 16 of a tile's keys: S^T = K Q^T by 16x16x32 MFMAs, the keys' fragments straight from memory into
+// registers -- lane (key l % 16, quarter l / 16) holds 128 consecutive values of its key, 64 bytes of codes, which are
+// the operands of 16 k steps if Q is held in the same order.  The decoded rows go to LDS once, as the values; then each
+// wave multiplies the tile's probabilities by 128 of the 512 value columns, O^T += V^T P^T.
+//
+// Decoding is exact in fp16 (E2M1 times e4m3 has 6 significand bits), two packed instructions for two values; Q in fp16
+// is exact too, but for numbers under 2^-14 (off by 2^-25 at most, a logit by less than fp32's own rounding of the sum)
+// and for heads that reach 2^16, which are scaled by a power of two.  Window rows have bf16's range, so they stay in bf16.
+// Sums, the softmax's maximum and sum and O are fp32; the probabilities are rounded to fp16 (bf16 for window rows), the
+// operand type, and the output once, after the rotation.
+#include <type_traits>
+
+#include "kv4_core.h"
+
+namespace {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+struct Kv4AttnArgs {
+  const uint16_t* q;  // [R, H, DQK]
+  long q_rstride;
+  int R, H;
+  const uint16_t* win;  // window rows: slot stride, rows a slot
+  long win_sstride;
+  int win_rows, win_slots;
+  const int* widx;      // [R, wt] rows of win, or null: the ring by positions
+  int wt;
+  const uint8_t* pool;
+  Kv4Table map;
+  const int* idx;       // [R, t]
+  int t;
+  int rows_per_slot;    // query row r belongs to batch row r / rows_per_slot
+  const long* seq;      // per batch row: its sequence (null: itself)
+  const long* pos;      // ring: per row
+  const long* pmax;
+  const long* plim;
+  float scale;          // softmax scale times log2(e)
+  const float* sink;
+  const float* cos_t;
+  const float* sin_t;
+  long n_pos;           // rows of the tables
+  int rd;
+  uint16_t* out;        // [R, H, 512]
+  int wtiles, tiles, chunk, nsplit, groups;
+  float* part;          // splits: [R, H, nsplit, 2] maximum and sum, then [R, H, nsplit, 512]
+};
+
+__device__ __align__(16) uint8_t g_kv4_none[1152];  // what a key that is not there reads
+
+DSV41_DEV f32x4_t mfma_f16_16x16x32(uint4 a, uint4 b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8_t, a), __builtin_bit_cast(h16x8_t, b), c, 0, 0, 0);
+}
+
+typedef __bf16 b16x2_t __attribute__((ext_vector_type(2)));
+DSV41_DEV uint32_t pack_bf16(float a, float b) { return __builtin_bit_cast(uint32_t, b16x2_t{(__bf16)a, (__bf16)b}); }
+DSV41_DEV uint32_t pack_f16(float a, float b) { return __builtin_bit_cast(uint32_t, h16x2_t{(_Float16)a, (_Float16)b}); }
+
+// LDS transpose read: within 16 lanes, lane i receives element i % 4 of the 8 bytes of lanes i/4, i/4+4, i/4+8, i/4+12.
+DSV41_DEV uint2 lds_read_tr(uint32_t addr) {
+  typedef __attribute__((ext_vector_type(4))) short s4;
+  const s4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)addr);
+  return __builtin_bit_cast(uint2, v);
+}
+
+// The values in LDS: row `key` of 1024 bytes, its 16-byte unit u at u ^ swizzle(key), so that neither the writes (16 keys,
+// one unit each) nor the transpose reads (4 keys by 16 columns a group of lanes) meet in a bank.
+DSV41_DEV uint32_t v_swizzle(int key) { return ((key & 7) << 1) | ((key >> 3) & 1); }
+
+// Output of one (row, head, 4 columns from c on): the inverse rotation, one rounding.
+DSV41_DEV uint2 finish4(const Kv4AttnArgs& a, long pos, int c, float4 o) {
+  if (a.rd > 0 && c >= 512 - a.rd) {
+    if (pos < 0 || pos >= a.n_pos) return make_uint2(0x7fc07fc0u, 0x7fc07fc0u);  // (no angle: NaN)
+    const long j = pos * (a.rd / 2) + ((c - (512 - a.rd)) >> 1);
+    const float c0 = a.cos_t[j], s0 = a.sin_t[j], c1 = a.cos_t[j + 1], s1 = a.sin_t[j + 1];
+    o = make_float4(o.x * c0 + o.y * s0, o.y * c0 - o.x * s0, o.z * c1 + o.w * s1, o.w * c1 - o.z * s1);
+  }
+  return make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+}
+
+template <int HB, int DQK>
+__global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const Kv4AttnArgs a) {
+  constexpr int NB = HB / 16;              // head blocks
+  constexpr int TS = DQK == 576 ? 2 : 0;   // k steps of the last 64 columns
+  constexpr int RB = kv4_row_bytes(DQK);
+  __shared__ __align__(16) uint8_t s_v[64 * 1024];
+  __shared__ __align__(16) uint8_t s_p[HB * 128];
+  __shared__ __align__(16) float s_m[HB * 4];
+
+  const int b = blockIdx.x;
+  const int sp = b % a.nsplit, rh = b / a.nsplit;
+  const int hg = rh % a.groups, r = rh / a.groups;
+  const int h0 = hg * HB;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int l16 = lane & 15, g = lane >> 4;
+  const int slot = r / a.rows_per_slot;
+  const long seq = a.seq ? a.seq[slot] : slot;
+  const long pos = a.pos ? a.pos[r] : 0;
+  const int t0 = sp * a.chunk, t1 = min(t0 + a.chunk, a.tiles);
+
+  // Q: head l % 16 of each block, quarter l / 16 of the 512 columns, in k steps of 8
+  uint4 q[NB][16 + TS];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int h = h0 + 16 * n + l16;
+    const uint16_t* src = a.q + r * a.q_rstride + (long)(h < a.H ? h : a.H - 1) * DQK;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) q[n][k] = *(const uint4*)(src + 128 * g + 8 * k);
+#pragma unroll
+    for (int k = 0; k < TS; ++k) q[n][16 + k] = *(const uint4*)(src + 512 + 16 * g + 8 * k);
+  }
+  f32x4_t o[NB][8];
+  float m[NB], l[NB], cq[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    m[n] = -__builtin_inff();
+    l[n] = 0.0f;
+    cq[n] = a.scale;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) o[n][c] = f32x4_t{0, 0, 0, 0};
+  }
+
+  const uint32_t v_base = lds_addr_of(s_v), p_base = lds_addr_of(s_p), m_base = lds_addr_of(s_m);
+  const int key = wave * 16 + l16;  // this lane's key of a tile
+  const uint32_t v_row = v_base + key * 1024, v_sw = v_swizzle(key);
+
+  // the softmax of a tile's scores and the product with its values in LDS
+  auto attend = [&](f32x4_t (&s)[NB], bool valid, auto f16) {
+    constexpr bool F16 = decltype(f16)::value;
+    const uint32_t mask = (uint32_t)(__ballot(valid) & 0xffffu) >> (4 * g);
+    float mx[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] = (mask >> i & 1) ? s[n][i] * cq[n] : -__builtin_inff();
+      mx[n] = row_max4(fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3])));
+      if (g == 0) *(__attribute__((address_space(3))) float*)(m_base + ((16 * n + l16) * 4 + wave) * 4) = mx[n];
+    }
+    lds_barrier();
+    bool up = false;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const f32x4_t w = *(__attribute__((address_space(3))) f32x4_t*)(m_base + (16 * n + l16) * 16);
+      mx[n] = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+      up |= mx[n] > m[n] + 8.0f;
+    }
+    if (__any(up)) {  // (alike in every wave: all have the same maxima)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const float to = fmaxf(m[n], mx[n]);
+        const float f = to > m[n] ? exp2f(m[n] - to) : 1.0f;
+        m[n] = to;
+        l[n] *= f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) o[n][c] *= f;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const float ref = m[n] == -__builtin_inff() ? 0.0f : m[n];
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = exp2f(s[n][i] - ref);
+        l[n] += p[i];
+      }
+      const uint2 pk = F16 ? make_uint2(pack_f16(p[0], p[1]), pack_f16(p[2], p[3]))
+                           : make_uint2(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]));
+      *(__attribute__((address_space(3))) uint64_t*)(p_base + (16 * n + l16) * 128 +
+                                                     (((wave * 2 + (g >> 1)) ^ (l16 & 7)) << 4) + (g & 1) * 8) =
+          (uint64_t)pk.y << 32 | pk.x;
+    }
+    lds_barrier();
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      uint4 pb[NB];
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+        pb[n] = __builtin_bit_cast(uint4, *(__attribute__((address_space(3))) u32x4*)(p_base + (16 * n + l16) * 128 +
+                                                                                      (((kk * 4 + g) ^ (l16 & 7)) << 4)));
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint2 v[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int kr = kk * 32 + g * 8 + u * 4 + (l16 >> 2);
+          const int unit = (wave * 8 + c) * 2 + ((l16 & 3) >> 1);
+          v[u] = lds_read_tr(v_base + kr * 1024 + ((unit ^ v_swizzle(kr)) << 4) + (l16 & 1) * 8);
+        }
+        const uint4 av = make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+          o[n][c] = F16 ? mfma_f16_16x16x32(av, pb[n], o[n][c]) : mfma_bf16_16x16x32(av, pb[n], o[n][c]);
+      }
+    }
+  };
+  auto put_v = [&](int k, uint4 x) {
+    *(__attribute__((address_space(3))) u32x4*)(v_row + (((uint32_t)(16 * g + k) ^ v_sw) << 4)) = __builtin_bit_cast(u32x4, x);
+  };
+
+  // ---- window rows
+#pragma unroll 1
+  for (int t = t0; t < min(t1, a.wtiles); ++t) {
+    const int j = t * 64 + key;
+    long row = -1;
+    if (a.widx) {
+      if (j < a.wt) row = a.widx[(long)r * a.wt + j];
+      if (row >= a.win_rows) row = -1;
+    } else if (j < a.win_rows) {  // slot j of the ring holds the newest position of its residue
+      const long pmax = a.pmax[r], plim = a.plim ? a.plim[r] : pos;
+      int d = (int)(pmax - j) % a.win_rows;  // (positions fit in 31 bits)
+      if (d < 0) d += a.win_rows;
+      const long held = pmax - d;
+      if (held >= 0 && held <= plim && pos - held < a.win_rows && seq >= 0 && seq < a.win_slots) row = j;
+    }
+    const bool valid = row >= 0;
+    const uint16_t* src = valid ? a.win + (a.widx ? (long)slot : seq) * a.win_sstride + row * DQK : (const uint16_t*)g_kv4_none;
+    f32x4_t s[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) s[n] = f32x4_t{0, 0, 0, 0};
+    lds_barrier();  // (the last tile's values have been read)
+#pragma unroll
+    for (int k = 0; k < 16 + TS; ++k) {
+      const uint4 x = *(const uint4*)(src + (k < 16 ? 128 * g + 8 * k : 512 + 16 * g + 8 * (k - 16)));
+      if (k < 16) put_v(k, x);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) s[n] = mfma_bf16_16x16x32(x, q[n][k], s[n]);
+    }
+    attend(s, valid, std::false_type{});
+  }
+
+  // ---- rows of the cache
+  int t = max(t0, a.wtiles);
+  if (t < t1) {
+    // Q to fp16; a head that reaches 2^16 scaled to under 2^15, which its scores are multiplied by again
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      float top = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 16 + TS; ++k) {
+        const uint32_t w[4] = {q[n][k].x, q[n][k].y, q[n][k].z, q[n][k].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          top = fmaxf(fmaxf(top, fabsf(__uint_as_float(w[i] << 16))), fabsf(__uint_as_float(w[i] & 0xffff0000u)));
+      }
+      top = row_max4(top);
+      float down = 1.0f;
+      if (top >= 65536.0f) {  // (an infinity leaves zeros and infinities: its head's result is NaN)
+        const int e = min(((__float_as_int(top) >> 23) & 255) - 127, 127) - 14;
+        down = pow2i(-e);
+        cq[n] *= pow2i(e);
+      }
+#pragma unroll
+      for (int k = 0; k < 16 + TS; ++k) {
+        const uint32_t w[4] = {q[n][k].x, q[n][k].y, q[n][k].z, q[n][k].w};
+        uint32_t f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          f[i] = pack_f16(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down);
+        q[n][k] = make_uint4(f[0], f[1], f[2], f[3]);
+      }
+    }
+    const int* ids = a.idx + (long)r * a.t;
+    const long rows = (long)a.map.cols << a.map.shift;
+    const bool known = seq >= 0 && seq < a.map.slots;
+    const int* const pages = a.map.table + (known ? seq : 0) * a.map.cols;
+    // the index of this lane's key of tile u, -1: none
+    auto index = [&](int u) {
+      const int j = (u - a.wtiles) * 64 + key;
+      return j < a.t && u < t1 ? ids[j] : -1;
+    };
+    auto there = [&](int i) { return known && i >= 0 && i < rows; };
+    auto source = [&](int i, int p) -> const uint8_t* {
+      return there(i) && (unsigned)p < (unsigned)a.map.pages ? a.pool + kv4_offset(a.map, p, i, RB) : nullptr;
+    };
+    uint4 code[4];
+    uint2 sc, tail;
+    uint32_t tsc = 0;
+    auto load = [&](const uint8_t* row) {
+      const uint8_t* p = row ? row : g_kv4_none;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) code[k] = *(const uint4*)(p + 64 * g + 16 * k);
+      sc = *(const uint2*)(p + 256 + 8 * g);
+      if (TS) {
+        tail = *(const uint2*)(p + 288 + 8 * g);
+        tsc = p[320 + g];
+      }
+    };
+    int i0 = index(t), i1 = index(t + 1);
+    const uint8_t* row = source(i0, pages[there(i0) ? i0 >> a.map.shift : 0]);
+    load(row);
+#pragma unroll 1
+    for (; t < t1; ++t) {
+      const int p1 = pages[there(i1) ? i1 >> a.map.shift : 0];  // (the next tile's, and the index of the one behind it)
+      const int i2 = index(t + 2);
+      const h16x2_t s01 = kv4_scales<false>(sc.x), s23 = kv4_scales<true>(sc.x);
+      const h16x2_t s45 = kv4_scales<false>(sc.y), s67 = kv4_scales<true>(sc.y);
+      const _Float16 sv[9] = {s01[0], s01[1], s23[0], s23[1], s45[0], s45[1], s67[0], s67[1], kv4_scales<false>(tsc)[0]};
+      f32x4_t s[NB];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) s[n] = f32x4_t{0, 0, 0, 0};
+      lds_barrier();
+#pragma unroll
+      for (int k = 0; k < 16 + TS; ++k) {
+        const uint32_t w[4] = {code[(k / 4) % 4].x, code[(k / 4) % 4].y, code[(k / 4) % 4].z, code[(k / 4) % 4].w};
+        const uint4 x = kv4_values(k < 16 ? w[k % 4] : (k == 16 ? tail.x : tail.y), sv[k / 2]);
+        if (k < 16) put_v(k, x);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) s[n] = mfma_f16_16x16x32(x, q[n][k], s[n]);
+      }
+      const bool valid = row != nullptr;
+      row = source(i1, p1);
+      load(row);
+      i1 = i2;
+      attend(s, valid, std::true_type{});
+    }
+  }
+
+  // ---- sums of the waves' keys, output
+  lds_barrier();
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    l[n] = row_sum4(l[n]);
+    if (g == 0) *(__attribute__((address_space(3))) float*)(m_base + ((16 * n + l16) * 4 + wave) * 4) = l[n];
+  }
+  lds_barrier();
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const f32x4_t w = *(__attribute__((address_space(3))) f32x4_t*)(m_base + (16 * n + l16) * 16);
+    l[n] = (w[0] + w[1]) + (w[2] + w[3]);
+    const int h = h0 + 16 * n + l16;
+    if (h >= a.H) continue;
+    if (a.nsplit > 1) {
+      const long at = ((long)r * a.H + h) * a.nsplit + sp;
+      if (wave == 0 && g == 0) *(float2*)(a.part + 2 * at) = make_float2(m[n], l[n]);
+      float* dst = a.part + 2L * a.R * a.H * a.nsplit + at * 512 + wave * 128 + 4 * g;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) *(float4*)(dst + 16 * c) = make_float4(o[n][c][0], o[n][c][1], o[n][c][2], o[n][c][3]);
+    } else {
+      const float den = l[n] + exp2f(a.sink[h] * kLog2e - m[n]);
+      const float inv = m[n] == -__builtin_inff() ? 0.0f : 1.0f / den;  // (no key: zeros)
+      uint16_t* dst = a.out + ((long)r * a.H + h) * 512 + wave * 128 + 4 * g;
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        *(uint2*)(dst + 16 * c) = finish4(a, pos, wave * 128 + 16 * c + 4 * g,
+                                          make_float4(o[n][c][0] * inv, o[n][c][1] * inv, o[n][c][2] * inv, o[n][c][3] * inv));
+    }
+  }
+}
+
+// The splits of a (row, head), in order: one workgroup of 128 lanes, four columns each.
+__global__ void __launch_bounds__(128) kv4_combine_kernel(const Kv4AttnArgs a) {
+  const int r = blockIdx.x / a.H, h = blockIdx.x % a.H;
+  const long at = ((long)r * a.H + h) * a.nsplit;
+  const float* ml = a.part + 2 * at;
+  const float* src = a.part + 2L * a.R * a.H * a.nsplit + at * 512 + 4 * threadIdx.x;
+  float m = -__builtin_inff();
+  for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, ml[2 * s]);
+  const float ref = m == -__builtin_inff() ? 0.0f : m;  // (no key: zeros, but a NaN stays one)
+  float den = exp2f(a.sink[h] * kLog2e - ref);
+  float4 o = make_float4(0, 0, 0, 0);
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float w = exp2f(ml[2 * s] - ref);
+    const float4 v = *(const float4*)(src + 512L * s);
+    den += w * ml[2 * s + 1];
+    o = make_float4(o.x + w * v.x, o.y + w * v.y, o.z + w * v.z, o.w + w * v.w);
+  }
+  const float inv = m == -__builtin_inff() ? 0.0f : 1.0f / den;
+  o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  *(uint2*)(a.out + ((long)r * a.H + h) * 512 + 4 * threadIdx.x) =
+      finish4(a, a.pos ? a.pos[r] : 0, 4 * threadIdx.x, o);
+}
+
+struct Plan {
+  int hb, nsplit, chunk;
+};
+
+// Heads a workgroup, and splits of the tiles until the card's CUs have work.
+Plan plan_of(int R, int H, int tiles) {
+  Plan p{16, 1, tiles};
+  const long units = (long)R * ((H + p.hb - 1) / p.hb);
+  long ns = units >= 512 ? 1 : (512 + units - 1) / units;
+  if (ns > tiles) ns = tiles;
+  p.chunk = (int)((tiles + ns - 1) / ns);
+  p.nsplit = (tiles + p.chunk - 1) / p.chunk;
+  return p;
+}
+
+long part_bytes(int R, int H, int nsplit) { return nsplit > 1 ? 4L * R * H * nsplit * 514 : 0; }
+
+template <int HB, int DQK>
+void launch(const Kv4AttnArgs& a, hipStream_t st) {
+  kv4_attn_kernel<HB, DQK><<<(unsigned)((long)a.R * a.groups * a.nsplit), 256, 0, st>>>(a);
+}
+
+int run(Kv4AttnArgs& a, int dqk, void* ws, long ws_bytes, hipStream_t st) {
+  a.wtiles = a.widx ? (a.wt + 63) / 64 : (a.win_rows + 63) / 64;
+  a.tiles = a.wtiles + (a.t + 63) / 64;
+  if (a.tiles == 0) a.tiles = 1;  // (no key at all: zeros)
+  const Plan p = plan_of(a.R, a.H, a.tiles);
+  a.nsplit = p.nsplit;
+  a.chunk = p.chunk;
+  a.groups = (a.H + p.hb - 1) / p.hb;
+  if ((long)a.R * a.groups * a.nsplit >= (1L << 31) || (long)a.R * a.H >= (1L << 31)) return (int)hipErrorInvalidValue;
+  if (ws_bytes < part_bytes(a.R, a.H, a.nsplit) || (a.nsplit > 1 && (!ws || ((uintptr_t)ws & 15)))) return (int)hipErrorInvalidValue;
+  a.part = (float*)ws;
+  dqk == 512 ? launch<16, 512>(a, st) : launch<16, 576>(a, st);
+  DSV41_CHECK_LAUNCH();
+  if (a.nsplit > 1) {
+    kv4_combine_kernel<<<a.R * a.H, 128, 0, st>>>(a);
+    DSV41_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+bool attn_ok(const Kv4AttnArgs& a, int dim, const void* table, int slots, int cols, int pages, int page) {
+  return (dim == 512 || dim == 576) && a.q && a.H > 0 && a.sink && a.out && a.t >= 0 && (a.t == 0 || (a.idx && a.pool)) &&
+         (((uintptr_t)a.q | (uintptr_t)a.win | (uintptr_t)a.pool) & 15) == 0 && ((uintptr_t)a.out & 7) == 0 &&
+         a.win_sstride % 8 == 0 && kv4_map_ok(table, slots, cols, pages, page);
+}
+
+}  // namespace
+
+extern "C" {
+
+long dsv41_kv4_attn_workspace_bytes(int R, int H, int wt, int t) {
+  if (R <= 0 || H <= 0 || wt < 0 || t < 0) return 0;
+  const int tiles = (wt + 63) / 64 + (t + 63) / 64;
+  return part_bytes(R, H, plan_of(R, H, tiles > 0 ? tiles : 1).nsplit);
+}
+
+int dsv41_sattn4(const void* q, const void* kv_win, long win_sstride, int win_slots, int win, const void* pool, int pages, int page,
+                 int dim, const int* table, int slots, int cols, const int* idx, int t, const long* pos, const long* seq,
+                 const long* pmax, const long* plim, const float* sink, const float* cos_t, const float* sin_t,
+                 long n_pos, int rd, float scale, void* out, int B, int h, void* ws, long ws_bytes, void* stream) {
+  if (B <= 0) return B < 0 ? (int)hipErrorInvalidValue : 0;
+  Kv4AttnArgs a{};
+  a.q = (const uint16_t*)q;
+  a.q_rstride = (long)h * dim;
+  a.R = B;
+  a.H = h;
+  a.win = (const uint16_t*)kv_win;
+  a.win_sstride = win_sstride;
+  a.win_rows = win;
+  a.win_slots = win_slots;
+  a.pool = (const uint8_t*)pool;
+  a.idx = idx;
+  a.t = t;
+  a.rows_per_slot = 1;
+  a.seq = seq;
+  a.pos = pos;
+  a.pmax = pmax;
+  a.plim = plim;
+  a.scale = scale * kLog2e;
+  a.sink = sink;
+  a.cos_t = cos_t;
+  a.sin_t = sin_t;
+  a.n_pos = n_pos;
+  a.rd = rd;
+  a.out = (uint16_t*)out;
+  if (!attn_ok(a, dim, table, slots, cols, pages, page) || !kv_win || win <= 0 || !pos || !seq || !pmax || rd < 0 ||
+      rd > 512 || rd % 4 || (rd > 0 && (!cos_t || !sin_t)))
+    return (int)hipErrorInvalidValue;
+  a.map = kv4_map(table, slots, cols, pages, page);
+  return run(a, dim, ws, ws_bytes, (hipStream_t)stream);
+}
+
+int dsv41_sparse_attn4(const void* q, const void* kv, long kv_bstride, int n_kv, const int* widx, int wt,
+                       const void* pool, int pages, int page, int dim, const int* table, int slots, int cols,
+                       const int* idx, int t, const long* seq, const float* sink, float scale, void* out, int b, int s,
+                       int h, void* ws, long ws_bytes, void* stream) {
+  if (b <= 0 || s <= 0) return b < 0 || s < 0 ? (int)hipErrorInvalidValue : 0;
+  if ((long)b * s >= (1L << 31)) return (int)hipErrorInvalidValue;
+  Kv4AttnArgs a{};
+  a.q = (const uint16_t*)q;
+  a.q_rstride = (long)h * dim;
+  a.R = b * s;
+  a.H = h;
+  a.win = (const uint16_t*)kv;
+  a.win_sstride = kv_bstride;
+  a.win_rows = n_kv;
+  a.widx = widx;
+  a.wt = wt;
+  a.pool = (const uint8_t*)pool;
+  a.idx = idx;
+  a.t = t;
+  a.rows_per_slot = s;
+  a.seq = seq;
+  a.scale = scale * kLog2e;
+  a.sink = sink;
+  a.out = (uint16_t*)out;
+  if (!attn_ok(a, dim, table, slots, cols, pages, page) || wt < 0 || n_kv < 0 || (wt > 0 && (!kv || !widx)))
+    return (int)hipErrorInvalidValue;
+  a.map = kv4_map(table, slots, cols, pages, page);
+  return run(a, dim, ws, ws_bytes, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,443 @@
+// The pages of a 4-bit cache: sequences forked, rows made writable, sequences cut short, the pool compacted, pages
+// copied between pools.  Everything is kept on the device (a table of pages a sequence, a count of the table's entries
+// that name a page), so the calls are stream-ordered and may be captured.
+//
+// Free pages are handed out lowest first, in the order of the arguments, from prefix sums: no result depends on the
+// order in which workgroups run.  The counts are changed by integer atomics, whose order does not show.
+#include "kv4_core.h"
+
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPer = 8;              // counts a thread looks at in one round
+constexpr int kMostEntries = 4096;   // sequences of one reserve call
+
+struct PagesArgs {
+  int* table;
+  int slots, cols;
+  int* refs;
+  int pages, shift;
+  int* err;
+  uint8_t* pool;
+  long page_bytes;
+  const long* seq;    // (fork: the destinations)
+  const long* src;
+  const long* begin;  // (fork, release: rows kept)
+  const long* end;
+  int n;
+  int* ws;
+  int* live;
+};
+
+// Columns of a table that `rows` rows take.
+DSV41_DEV int columns(long rows, int shift, int cols) {
+  const long c = rows <= 0 ? 0 : ((rows - 1) >> shift) + 1;
+  return c < cols ? (int)c : cols;
+}
+
+DSV41_DEV void copy_bytes(uint8_t* dst, const uint8_t* src, long bytes) {  // by a workgroup, 16 bytes a lane
+  const uint4* s = (const uint4*)src;
+  uint4* d = (uint4*)dst;
+  const int n = (int)(bytes >> 4), nt = blockDim.x;
+  int i = threadIdx.x;
+  for (; i + 3 * nt < n; i += 4 * nt) {
+    const uint4 a = s[i], b = s[i + nt], c = s[i + 2 * nt], e = s[i + 3 * nt];
+    d[i] = a;
+    d[i + nt] = b;
+    d[i + 2 * nt] = c;
+    d[i + 3 * nt] = e;
+  }
+  for (; i < n; i += nt) d[i] = s[i];
+}
+
+// ---- release: the pages behind the first `rows` rows of a sequence are named no more
+__global__ void __launch_bounds__(256) release_kernel(const PagesArgs a) {
+  const long s = a.seq[blockIdx.x];
+  if (s < 0 || s >= a.slots) {
+    if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(a.err, kKv4Ignored);
+    return;
+  }
+  const int j = blockIdx.y * 256 + threadIdx.x;
+  if (j >= a.cols || j < columns(a.begin ? a.begin[blockIdx.x] : 0, a.shift, a.cols)) return;
+  const int p = atomicExch(a.table + s * a.cols + j, -1);  // (a sequence named twice gives a page up once)
+  if ((unsigned)p < (unsigned)a.pages) atomicSub(a.refs + p, 1);
+}
+
+// ---- fork: sequence dst names the pages of src's first `rows` rows instead of its own
+// A destination that is also a source, or that an earlier pair has, would be read and written at once: left out.
+__global__ void __launch_bounds__(256) fork_kernel(const PagesArgs a) {
+  const int i = blockIdx.x;
+  const long s = a.src[i], d = a.seq[i];
+  bool bad = s < 0 || s >= a.slots || d < 0 || d >= a.slots;
+  for (int k = threadIdx.x; k < a.n; k += 256) bad |= a.src[k] == d || (k < i && a.seq[k] == d);
+  if (__syncthreads_or(bad)) {
+    if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(a.err, kKv4Ignored);
+    return;
+  }
+  const int j = blockIdx.y * 256 + threadIdx.x;
+  if (j >= a.cols) return;
+  int* at = a.table + d * a.cols + j;
+  const int old = *at;
+  int p = j < columns(a.begin ? a.begin[i] : (1L << 62), a.shift, a.cols) ? a.table[s * a.cols + j] : -1;
+  if ((unsigned)p >= (unsigned)a.pages) p = -1;
+  if ((unsigned)old < (unsigned)a.pages) atomicSub(a.refs + old, 1);
+  if (p >= 0) atomicAdd(a.refs + p, 1);
+  *at = p;
+}
+
+// ---- reserve
+// Workspace (int32): owner [slots], entry [pages], column [pages], page [pages], copy from [n], copy to [n].
+DSV41_DEV int* ws_entry(const PagesArgs& a) { return a.ws + a.slots; }
+DSV41_DEV int* ws_from(const PagesArgs& a) { return a.ws + a.slots + 3L * a.pages; }
+
+// One workgroup: which columns of which entry need a page of their own (none there, or one that other entries name too),
+// counted in the order of the arguments; the lowest free pages in as many; then the table and the counts.
+__global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const PagesArgs a) {
+  __shared__ int offs[kMostEntries + 1];
+  __shared__ int tmp[kPlanThreads / 64];
+  const int t = threadIdx.x;
+  int* const owner = a.ws;
+  int* const entry = ws_entry(a);
+  int* const column = entry + a.pages;
+  int* const page = column + a.pages;
+  int* const from = ws_from(a);
+  int* const to = from + a.n;
+  for (int i = t; i < a.n; i += kPlanThreads) {
+    from[i] = -1;
+    const long s = a.seq[i];
+    if (s >= 0 && s < a.slots) __hip_atomic_store(owner + s, a.n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  for (int i = t; i < a.n; i += kPlanThreads) {
+    const long s = a.seq[i];
+    if (s >= 0 && s < a.slots) atomicMin(owner + s, i);
+  }
+  __syncthreads();
+  // columns of each entry, summed
+  int total = 0;
+  for (int i0 = 0; i0 < a.n; i0 += kPlanThreads) {
+    const int i = i0 + t;
+    int c = 0;
+    if (i < a.n) {
+      const long s = a.seq[i], b = a.begin[i], e = a.end[i];
+      const bool ok = s >= 0 && s < a.slots && b >= 0 && e <= ((long)a.cols << a.shift) &&
+                      __hip_atomic_load(owner + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == i;
+      if (!ok)
+        atomicOr(a.err, kKv4Ignored);
+      else if (b < e)
+        c = (int)(((e - 1) >> a.shift) - (b >> a.shift)) + 1;
+    }
+    int sum;
+    const int before = block_scan_dpp<kPlanThreads>(c, tmp, &sum);
+    if (i < a.n) offs[i] = total + before;
+    total += sum;
+  }
+  if (t == 0) offs[a.n] = total;
+  __syncthreads();
+  // the needs, in order
+  int needs = 0;
+  for (int f0 = 0; f0 < total; f0 += kPlanThreads) {
+    const int f = f0 + t;
+    int i = 0, j = 0;
+    bool need = false;
+    if (f < total) {
+      int hi = a.n;  // the last entry whose columns begin at f or before
+      while (hi - i > 1) {
+        const int mid = (i + hi) >> 1;
+        if (offs[mid] <= f)
+          i = mid;
+        else
+          hi = mid;
+      }
+      j = (int)(a.begin[i] >> a.shift) + f - offs[i];
+      const int p = a.table[a.seq[i] * a.cols + j];
+      need = (unsigned)p >= (unsigned)a.pages || a.refs[p] > 1;
+    }
+    int sum;
+    const int r = needs + block_scan_dpp<kPlanThreads>(need, tmp, &sum);
+    if (need && r < a.pages) {
+      entry[r] = i;
+      column[r] = j;
+    }
+    needs += sum;
+  }
+  // the lowest free pages
+  int found = 0;
+  for (int p0 = 0; p0 < a.pages && found < needs; p0 += kPlanThreads * kPer) {
+    const int p = p0 + t * kPer;
+    unsigned free = 0;
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) free |= (p + u < a.pages && a.refs[p + u] <= 0) ? 1u << u : 0u;
+    int sum;
+    int r = found + block_scan_dpp<kPlanThreads>(__popc(free), tmp, &sum);
+#pragma unroll
+    for (int u = 0; u < kPer; ++u)
+      if (free >> u & 1) {
+        if (r < needs) page[r] = p + u;
+        ++r;
+      }
+    found += sum;
+  }
+  if (t == 0 && found < needs) atomicOr(a.err, kKv4NoPages);
+  __syncthreads();
+  for (int r = t; r < (found < needs ? found : needs); r += kPlanThreads) {
+    const int i = entry[r], j = column[r], p = page[r];
+    int* at = a.table + a.seq[i] * a.cols + j;
+    const int old = *at;
+    *at = p;
+    a.refs[p] = 1;
+    if ((unsigned)old < (unsigned)a.pages) {
+      atomicSub(a.refs + old, 1);
+      if (j == (int)(a.begin[i] >> a.shift)) {
+        to[i] = p;
+        from[i] = old;
+      }
+    }
+  }
+}
+
+// What the first of an entry's new pages held before `begin` goes with it.
+__global__ void __launch_bounds__(256) reserve_copy_kernel(const PagesArgs a) {
+  const int i = blockIdx.x, from = ws_from(a)[i];
+  if (from < 0) return;
+  const long rows = a.begin[i] & ((1L << a.shift) - 1);
+  copy_bytes(a.pool + ws_from(a)[a.n + i] * a.page_bytes, a.pool + from * a.page_bytes, rows * (a.page_bytes >> a.shift));
+}
+
+// ---- compact
+// Workspace (int32): live, moves, from [pages], to [pages], where [pages] (of a moved page).
+// One workgroup: L live pages; the live ones of L and above go, in order, to the free ones below L.  Sources and
+// destinations do not meet, so the moves need no order.
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagesArgs a) {
+  __shared__ int tmp[kPlanThreads / 64];
+  const int t = threadIdx.x;
+  int* const from = a.ws + 2;
+  int* const to = from + a.pages;
+  int* const where = to + a.pages;
+  int live = 0;
+  for (int p0 = 0; p0 < a.pages; p0 += kPlanThreads * kPer) {
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int p = p0 + u * kPlanThreads + t;
+      live += p < a.pages && a.refs[p] > 0;
+    }
+  }
+  block_scan_dpp<kPlanThreads>(live, tmp, &live);
+  int ns = 0, nd = 0;
+  for (int p0 = 0; p0 < a.pages; p0 += kPlanThreads * kPer) {
+    const int p = p0 + t * kPer;
+    unsigned src = 0, dst = 0;
+#pragma unroll
+    for (int u = 0; u < kPer; ++u)
+      if (p + u < a.pages) {
+        const bool l = a.refs[p + u] > 0;
+        src |= l && p + u >= live ? 1u << u : 0u;
+        dst |= !l && p + u < live ? 1u << u : 0u;
+      }
+    int ss, sd;
+    int rs = ns + block_scan_dpp<kPlanThreads>(__popc(src), tmp, &ss);
+    int rd = nd + block_scan_dpp<kPlanThreads>(__popc(dst), tmp, &sd);
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      if (src >> u & 1) from[rs++] = p + u;
+      if (dst >> u & 1) to[rd++] = p + u;
+    }
+    ns += ss;
+    nd += sd;
+  }
+  __syncthreads();
+  for (int r = t; r < ns; r += kPlanThreads) where[from[r]] = to[r];
+  if (t == 0) {
+    a.ws[0] = live;
+    a.ws[1] = ns;
+    *a.live = live;
+  }
+}
+
+__global__ void __launch_bounds__(256) compact_move_kernel(const PagesArgs a) {
+  const int live = a.ws[0], moves = a.ws[1];
+  const int* const from = a.ws + 2;
+  const int* const to = from + a.pages;
+  const int* const where = to + a.pages;
+  const int entries = a.slots * a.cols;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < entries; i += gridDim.x * 256) {
+    const int p = a.table[i];
+    if (p >= live && p < a.pages) a.table[i] = where[p];
+  }
+  for (int r = blockIdx.x; r < moves; r += gridDim.x) {
+    const int s = from[r], d = to[r];
+    copy_bytes(a.pool + d * a.page_bytes, a.pool + s * a.page_bytes, a.page_bytes);
+    if (threadIdx.x == 0) {
+      a.refs[d] = a.refs[s];
+      a.refs[s] = 0;
+    }
+  }
+}
+
+// ---- copies between pools
+struct CopyArgs {
+  const uint8_t* src;
+  uint8_t* dst;
+  int src_pages, dst_pages, n;
+  long page_bytes;
+  const long* from;
+  const long* to;
+  int* err;
+  int* last;  // [dst_pages] or null
+};
+
+// The last pair that names a page as its destination (of many pairs, by one workgroup; of few every workgroup looks).
+__global__ void __launch_bounds__(kPlanThreads) copy_last_kernel(const CopyArgs a) {
+  for (int i = threadIdx.x; i < a.n; i += kPlanThreads) {
+    const long d = a.to[i];
+    if (d >= 0 && d < a.dst_pages) __hip_atomic_store(a.last + d, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.n; i += kPlanThreads) {
+    const long d = a.to[i], s = a.from[i];
+    if (d >= 0 && d < a.dst_pages && s >= 0 && s < a.src_pages) atomicMax(a.last + d, i);
+  }
+}
+
+__global__ void __launch_bounds__(256) copy_kernel(const CopyArgs a) {
+  const int i = blockIdx.x;
+  const long s = a.from[i], d = a.to[i];
+  if (s == -1 || d == -1) return;
+  if (s < 0 || s >= a.src_pages || d < 0 || d >= a.dst_pages) {
+    if (threadIdx.x == 0) atomicOr(a.err, kKv4Ignored);
+    return;
+  }
+  bool later = false;
+  if (a.last)
+    later = a.last[d] != i;
+  else
+    for (int k = i + 1 + threadIdx.x; k < a.n; k += 256) later |= a.to[k] == d && a.from[k] >= 0 && a.from[k] < a.src_pages;
+  if (__syncthreads_or(later)) {
+    if (threadIdx.x == 0) atomicOr(a.err, kKv4Ignored);
+    return;
+  }
+  copy_bytes(a.dst + d * a.page_bytes, a.src + s * a.page_bytes, a.page_bytes);
+}
+
+constexpr int kFewCopies = 1024;
+
+bool pages_args(PagesArgs& a, int* table, int slots, int cols, int* refs, int pages, int page, int* err) {
+  if (!kv4_map_ok(table, slots, cols, pages, page) || !refs) return false;
+  a = PagesArgs{};
+  a.table = table;
+  a.slots = slots;
+  a.cols = cols;
+  a.refs = refs;
+  a.pages = pages;
+  a.shift = kv4_shift(page);
+  a.err = err;
+  return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dsv41_kv4_fork(const long* src, const long* dst, const long* rows, int n, int* table, int slots, int cols, int* refs,
+                   int pages, int page, int* err, void* stream) {
+  PagesArgs a;
+  if (n < 0 || !pages_args(a, table, slots, cols, refs, pages, page, err) || !err || cols > 256 * 65535)
+    return (int)hipErrorInvalidValue;
+  if (n == 0) return 0;
+  if (!src || !dst) return (int)hipErrorInvalidValue;
+  a.src = src;
+  a.seq = dst;
+  a.begin = rows;
+  a.n = n;
+  fork_kernel<<<dim3(n, (cols + 255) / 256), 256, 0, (hipStream_t)stream>>>(a);
+  DSV41_CHECK_LAUNCH();
+  return 0;
+}
+
+int dsv41_kv4_release(const long* seq, const long* rows, int n, int* table, int slots, int cols, int* refs, int pages,
+                      int page, int* err, void* stream) {
+  PagesArgs a;
+  if (n < 0 || !pages_args(a, table, slots, cols, refs, pages, page, err) || !err || cols > 256 * 65535)
+    return (int)hipErrorInvalidValue;
+  if (n == 0) return 0;
+  if (!seq) return (int)hipErrorInvalidValue;
+  a.seq = seq;
+  a.begin = rows;
+  a.n = n;
+  release_kernel<<<dim3(n, (cols + 255) / 256), 256, 0, (hipStream_t)stream>>>(a);
+  DSV41_CHECK_LAUNCH();
+  return 0;
+}
+
+long dsv41_kv4_reserve_workspace_bytes(int n, int slots, int pages) {
+  return 4 * ((long)slots + 3L * pages + 2L * n);
+}
+
+int dsv41_kv4_reserve(const long* seq, const long* begin, const long* end, int n, void* pool, int dim, int* table,
+                      int slots, int cols, int* refs, int pages, int page, int* err, void* ws, long ws_bytes,
+                      void* stream) {
+  PagesArgs a;
+  if (n < 0 || n > kMostEntries || !pages_args(a, table, slots, cols, refs, pages, page, err) || !err || !pool ||
+      ((uintptr_t)pool & 15) || (dim != 512 && dim != 576))
+    return (int)hipErrorInvalidValue;
+  if (n == 0) return 0;
+  if (!seq || !begin || !end || !ws || ws_bytes < dsv41_kv4_reserve_workspace_bytes(n, slots, pages))
+    return (int)hipErrorInvalidValue;
+  a.seq = seq;
+  a.begin = begin;
+  a.end = end;
+  a.n = n;
+  a.pool = (uint8_t*)pool;
+  a.page_bytes = (long)kv4_row_bytes(dim) * page;
+  a.ws = (int*)ws;
+  reserve_plan_kernel<<<1, kPlanThreads, 0, (hipStream_t)stream>>>(a);
+  DSV41_CHECK_LAUNCH();
+  reserve_copy_kernel<<<n, 256, 0, (hipStream_t)stream>>>(a);
+  DSV41_CHECK_LAUNCH();
+  return 0;
+}
+
+long dsv41_kv4_compact_workspace_bytes(int pages) { return 4 * (2 + 3L * pages); }
+
+int dsv41_kv4_compact(void* pool, int dim, int* table, int slots, int cols, int* refs, int pages, int page, int* live,
+                      void* ws, long ws_bytes, void* stream) {
+  PagesArgs a;
+  if (!pages_args(a, table, slots, cols, refs, pages, page, nullptr) || !pool || ((uintptr_t)pool & 15) ||
+      (dim != 512 && dim != 576) || !live || !ws || ws_bytes < dsv41_kv4_compact_workspace_bytes(pages))
+    return (int)hipErrorInvalidValue;
+  a.pool = (uint8_t*)pool;
+  a.page_bytes = (long)kv4_row_bytes(dim) * page;
+  a.ws = (int*)ws;
+  a.live = live;
+  compact_plan_kernel<<<1, kPlanThreads, 0, (hipStream_t)stream>>>(a);
+  DSV41_CHECK_LAUNCH();
+  compact_move_kernel<<<pages < 2048 ? pages : 2048, 256, 0, (hipStream_t)stream>>>(a);
+  DSV41_CHECK_LAUNCH();
+  return 0;
+}
+
+long dsv41_kv4_copy_workspace_bytes(int n, int dst_pages) { return n > kFewCopies ? 4L * dst_pages : 0; }
+
+int dsv41_kv4_copy(const void* src_pool, int src_pages, void* dst_pool, int dst_pages, int page, int dim, const long* src,
+                   const long* dst, int n, int* err, void* ws, long ws_bytes, void* stream) {
+  if (n < 0 || kv4_shift(page) < 0 || (dim != 512 && dim != 576) || src_pages <= 0 || dst_pages <= 0)
+    return (int)hipErrorInvalidValue;
+  if (n == 0) return 0;
+  if (!src_pool || !dst_pool || (((uintptr_t)src_pool | (uintptr_t)dst_pool) & 15) || !src || !dst || !err ||
+      (n > kFewCopies && (!ws || ws_bytes < dsv41_kv4_copy_workspace_bytes(n, dst_pages))))
+    return (int)hipErrorInvalidValue;
+  const long pb = (long)kv4_row_bytes(dim) * page;
+  const char *s0 = (const char*)src_pool, *d0 = (const char*)dst_pool;
+  if (s0 < d0 + dst_pages * pb && d0 < s0 + src_pages * pb) return (int)hipErrorInvalidValue;  // (one memory)
+  CopyArgs a{(const uint8_t*)src_pool, (uint8_t*)dst_pool, src_pages, dst_pages, n, pb, src, dst, err,
+             n > kFewCopies ? (int*)ws : nullptr};
+  if (a.last) {
+    copy_last_kernel<<<1, kPlanThreads, 0, (hipStream_t)stream>>>(a);
+    DSV41_CHECK_LAUNCH();
+  }
+  copy_kernel<<<n, 256, 0, (hipStream_t)stream>>>(a);
+  DSV41_CHECK_LAUNCH();
+  return 0;
+}
+
+}  // extern "C"

@@ -11,8 +11,9 @@ from .indexer import index_topk
 from .a8 import A8, gated_a8, linear_a8, norm_quant8
 from . import cache, compressor
 from .ffn import GatedFeedForward
+from .kv4 import PagedKV4, sattn4, sparse_attn4
 
 __all__ = ["fake_quant", "fake_quant_fp4", "fake_quant_fp8", "rmsnorm", "rope_", "rope_dev_", "sparse_attn_decode",
            "sparse_attn_decode2", "sparse_attn_decode_split", "kv_write", "sattn2", "index_score", "topk_indices",
            "sparse_attn", "index_topk", "cache", "compressor", "A8", "norm_quant8", "linear_a8", "gated_a8",
-           "GatedFeedForward"]
+           "GatedFeedForward", "PagedKV4", "sattn4", "sparse_attn4"]
