@@ -13,72 +13,9 @@
 // operand type, and the output once, after the rotation.
 #include <type_traits>
 
-#include "kv4_core.h"
+#include "kv4_attn_core.h"
 
 namespace {
-
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-
-struct Kv4AttnArgs {
-  const uint16_t* q;  // [R, H, DQK]
-  long q_rstride;
-  int R, H;
-  const uint16_t* win;  // window rows: slot stride, rows a slot
-  long win_sstride;
-  int win_rows, win_slots;
-  const int* widx;      // [R, wt] rows of win, or null: the ring by positions
-  int wt;
-  const uint8_t* pool;
-  Kv4Table map;
-  const int* idx;       // [R, t]
-  int t;
-  int rows_per_slot;    // query row r belongs to batch row r / rows_per_slot
-  const long* seq;      // per batch row: its sequence (null: itself)
-  const long* pos;      // ring: per row
-  const long* pmax;
-  const long* plim;
-  float scale;          // softmax scale times log2(e)
-  const float* sink;
-  const float* cos_t;
-  const float* sin_t;
-  long n_pos;           // rows of the tables
-  int rd;
-  uint16_t* out;        // [R, H, 512]
-  int wtiles, tiles, chunk, nsplit, groups;
-  float* part;          // splits: [R, H, nsplit, 2] maximum and sum, then [R, H, nsplit, 512]
-};
-
-__device__ __align__(16) uint8_t g_kv4_none[1152];  // what a key that is not there reads
-
-DSV41_DEV f32x4_t mfma_f16_16x16x32(uint4 a, uint4 b, f32x4_t c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8_t, a), __builtin_bit_cast(h16x8_t, b), c, 0, 0, 0);
-}
-
-typedef __bf16 b16x2_t __attribute__((ext_vector_type(2)));
-DSV41_DEV uint32_t pack_bf16(float a, float b) { return __builtin_bit_cast(uint32_t, b16x2_t{(__bf16)a, (__bf16)b}); }
-DSV41_DEV uint32_t pack_f16(float a, float b) { return __builtin_bit_cast(uint32_t, h16x2_t{(_Float16)a, (_Float16)b}); }
-
-// LDS transpose read: within 16 lanes, lane i receives element i % 4 of the 8 bytes of lanes i/4, i/4+4, i/4+8, i/4+12.
-DSV41_DEV uint2 lds_read_tr(uint32_t addr) {
-  typedef __attribute__((ext_vector_type(4))) short s4;
-  const s4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)addr);
-  return __builtin_bit_cast(uint2, v);
-}
-
-// The values in LDS: row `key` of 1024 bytes, its 16-byte unit u at u ^ swizzle(key), so that neither the writes (16 keys,
-// one unit each) nor the transpose reads (4 keys by 16 columns a group of lanes) meet in a bank.
-DSV41_DEV uint32_t v_swizzle(int key) { return ((key & 7) << 1) | ((key >> 3) & 1); }
-
-// Output of one (row, head, 4 columns from c on): the inverse rotation, one rounding.
-DSV41_DEV uint2 finish4(const Kv4AttnArgs& a, long pos, int c, float4 o) {
-  if (a.rd > 0 && c >= 512 - a.rd) {
-    if (pos < 0 || pos >= a.n_pos) return make_uint2(0x7fc07fc0u, 0x7fc07fc0u);  // (no angle: NaN)
-    const long j = pos * (a.rd / 2) + ((c - (512 - a.rd)) >> 1);
-    const float c0 = a.cos_t[j], s0 = a.sin_t[j], c1 = a.cos_t[j + 1], s1 = a.sin_t[j + 1];
-    o = make_float4(o.x * c0 + o.y * s0, o.y * c0 - o.x * s0, o.z * c1 + o.w * s1, o.w * c1 - o.z * s1);
-  }
-  return make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
-}
 
 template <int HB, int DQK>
 __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const Kv4AttnArgs a) {
@@ -374,39 +311,71 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const Kv4AttnArgs a) {
 }
 
 struct Plan {
-  int hb, nsplit, chunk;
+  bool many;  // the cache's rows decoded once, the 64-head kernel (window and cache in one list)
+  int wtiles, tiles, nsplit, chunk, groups;
+  long list, rows, part;  // bytes of the workspace
 };
 
-// Heads a workgroup, and splits of the tiles until the card's CUs have work.
-Plan plan_of(int R, int H, int tiles) {
-  Plan p{16, 1, tiles};
-  const long units = (long)R * ((H + p.hb - 1) / p.hb);
-  long ns = units >= 512 ? 1 : (512 + units - 1) / units;
-  if (ns > tiles) ns = tiles;
-  p.chunk = (int)((tiles + ns - 1) / ns);
-  p.nsplit = (tiles + p.chunk - 1) / p.chunk;
-  return p;
+// Splits of the tiles until the card's CUs have work: `want` workgroups.
+void split(Plan& p, long units, long want) {
+  if (p.tiles == 0) p.tiles = 1;  // (no key at all: zeros)
+  long ns = units >= want ? 1 : (want + units - 1) / units;
+  if (ns > p.tiles) ns = p.tiles;
+  p.chunk = (int)((p.tiles + ns - 1) / ns);
+  p.nsplit = (p.tiles + p.chunk - 1) / p.chunk;
 }
 
-long part_bytes(int R, int H, int nsplit) { return nsplit > 1 ? 4L * R * H * nsplit * 514 : 0; }
+Plan plan_of(int R, int H, int wt, int t, int dim, long rows) {
+  Plan p{};
+  p.groups = (H + 63) / 64;
+  p.many = rows > 0 && H > 32 && (long)R * p.groups >= 128 && (long)R * t >= 8 * rows;
+  if (p.many) {
+    p.tiles = (wt + t + 31) / 32;
+    split(p, (long)R * p.groups, 256);
+    p.list = ((long)R * (wt + t) * 4 + 255) & ~255L;
+    p.rows = (rows * dim * 2 + 255) & ~255L;
+  } else {
+    p.groups = (H + 15) / 16;
+    p.wtiles = (wt + 63) / 64;
+    p.tiles = p.wtiles + (t + 63) / 64;
+    split(p, (long)R * p.groups, 512);
+  }
+  p.part = p.nsplit > 1 ? 4L * R * H * p.nsplit * 514 : 0;
+  return p;
+}
 
 template <int HB, int DQK>
 void launch(const Kv4AttnArgs& a, hipStream_t st) {
   kv4_attn_kernel<HB, DQK><<<(unsigned)((long)a.R * a.groups * a.nsplit), 256, 0, st>>>(a);
 }
 
-int run(Kv4AttnArgs& a, int dqk, void* ws, long ws_bytes, hipStream_t st) {
-  a.wtiles = a.widx ? (a.wt + 63) / 64 : (a.win_rows + 63) / 64;
-  a.tiles = a.wtiles + (a.t + 63) / 64;
-  if (a.tiles == 0) a.tiles = 1;  // (no key at all: zeros)
-  const Plan p = plan_of(a.R, a.H, a.tiles);
+int run(Kv4AttnArgs& a, int dqk, int b, void* ws, long ws_bytes, hipStream_t st) {
+  const long rows = b > 0 ? (long)b * a.map.cols << a.map.shift : 0;
+  const Plan p = plan_of(a.R, a.H, a.pos ? a.win_rows : a.wt, a.t, dqk, rows);
+  a.wtiles = p.wtiles;
+  a.tiles = p.tiles;
   a.nsplit = p.nsplit;
   a.chunk = p.chunk;
-  a.groups = (a.H + p.hb - 1) / p.hb;
+  a.groups = p.groups;
   if ((long)a.R * a.groups * a.nsplit >= (1L << 31) || (long)a.R * a.H >= (1L << 31)) return (int)hipErrorInvalidValue;
-  if (ws_bytes < part_bytes(a.R, a.H, a.nsplit) || (a.nsplit > 1 && (!ws || ((uintptr_t)ws & 15)))) return (int)hipErrorInvalidValue;
-  a.part = (float*)ws;
-  dqk == 512 ? launch<16, 512>(a, st) : launch<16, 576>(a, st);
+  const long need = p.list + p.rows + p.part;
+  if (need > 0 && (!ws || ((uintptr_t)ws & 15) || ws_bytes < need)) return (int)hipErrorInvalidValue;
+  a.part = (float*)((char*)ws + p.list + p.rows);
+  if (p.many) {
+    if ((long)a.wt + a.t + a.win_rows + (rows / b) >= (1L << 31) || rows / (1 << a.map.shift) + a.R >= (1L << 31))
+      return (int)hipErrorInvalidValue;
+    int* const list = (int*)ws;
+    uint16_t* const decoded = (uint16_t*)((char*)ws + p.list);
+    kv4_unpack_launch(a, dqk, b, decoded, list, st);
+    DSV41_CHECK_LAUNCH();
+    a.n2 = (int)(rows / b);
+    a.pool = (const uint8_t*)decoded;
+    a.idx = list;
+    a.t += a.wt;
+    kv4_attn64_launch(a, dqk, st);
+  } else {
+    dqk == 512 ? launch<16, 512>(a, st) : launch<16, 576>(a, st);
+  }
   DSV41_CHECK_LAUNCH();
   if (a.nsplit > 1) {
     kv4_combine_kernel<<<a.R * a.H, 128, 0, st>>>(a);
@@ -418,17 +387,17 @@ int run(Kv4AttnArgs& a, int dqk, void* ws, long ws_bytes, hipStream_t st) {
 bool attn_ok(const Kv4AttnArgs& a, int dim, const void* table, int slots, int cols, int pages, int page) {
   return (dim == 512 || dim == 576) && a.q && a.H > 0 && a.sink && a.out && a.t >= 0 && (a.t == 0 || (a.idx && a.pool)) &&
          (((uintptr_t)a.q | (uintptr_t)a.win | (uintptr_t)a.pool) & 15) == 0 && ((uintptr_t)a.out & 7) == 0 &&
-         a.win_sstride % 8 == 0 && kv4_map_ok(table, slots, cols, pages, page);
+         a.win_sstride % 8 == 0 && kv4_map_ok(table, slots, cols, pages, page) && (long)pages * page < (1L << 31);
 }
 
 }  // namespace
 
 extern "C" {
 
-long dsv41_kv4_attn_workspace_bytes(int R, int H, int wt, int t) {
+long dsv41_kv4_attn_workspace_bytes(int R, int H, int wt, int t, int dim, long rows) {
   if (R <= 0 || H <= 0 || wt < 0 || t < 0) return 0;
-  const int tiles = (wt + 63) / 64 + (t + 63) / 64;
-  return part_bytes(R, H, plan_of(R, H, tiles > 0 ? tiles : 1).nsplit);
+  const Plan p = plan_of(R, H, wt, t, dim, rows);
+  return p.list + p.rows + p.part;
 }
 
 int dsv41_sattn4(const void* q, const void* kv_win, long win_sstride, int win_slots, int win, const void* pool, int pages, int page,
@@ -464,7 +433,7 @@ int dsv41_sattn4(const void* q, const void* kv_win, long win_sstride, int win_sl
       rd > 512 || rd % 4 || (rd > 0 && (!cos_t || !sin_t)))
     return (int)hipErrorInvalidValue;
   a.map = kv4_map(table, slots, cols, pages, page);
-  return run(a, dim, ws, ws_bytes, (hipStream_t)stream);
+  return run(a, dim, 0, ws, ws_bytes, (hipStream_t)stream);
 }
 
 int dsv41_sparse_attn4(const void* q, const void* kv, long kv_bstride, int n_kv, const int* widx, int wt,
@@ -494,7 +463,7 @@ int dsv41_sparse_attn4(const void* q, const void* kv, long kv_bstride, int n_kv,
   if (!attn_ok(a, dim, table, slots, cols, pages, page) || wt < 0 || n_kv < 0 || (wt > 0 && (!kv || !widx)))
     return (int)hipErrorInvalidValue;
   a.map = kv4_map(table, slots, cols, pages, page);
-  return run(a, dim, ws, ws_bytes, (hipStream_t)stream);
+  return run(a, dim, b, ws, ws_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

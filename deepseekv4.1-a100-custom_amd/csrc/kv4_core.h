@@ -8,6 +8,12 @@
 #pragma once
 #include "common.h"
 
+struct Kv4Table {
+  const int* table;  // [slots, cols]: the page of rows j << shift .. of a sequence, -1 none
+  int slots, cols, pages;
+  int shift;         // page = 1 << shift rows
+};
+
 namespace {
 
 typedef _Float16 h16x2_t __attribute__((ext_vector_type(2)));
@@ -19,12 +25,6 @@ constexpr int kv4_row_bytes(int dim) { return dim == 512 ? 288 : 336; }
 constexpr int kKv4NoPages = 1;   // reserve found too few free pages
 constexpr int kKv4Ignored = 2;   // an entry was left out: an index out of range, or one named twice
 constexpr int kKv4Dropped = 4;   // an appended row had no page of its own, or no rope angle
-
-struct Kv4Table {
-  const int* table;  // [slots, cols]: the page of rows j << shift .. of a sequence, -1 none
-  int slots, cols, pages;
-  int shift;         // page = 1 << shift rows
-};
 
 // The page of row `row` of sequence `seq`, -1 where there is none.
 DSV41_DEV int kv4_page(const Kv4Table& m, long seq, long row) {
@@ -51,6 +51,19 @@ DSV41_DEV uint4 kv4_values(uint32_t codes, _Float16 scale) {
                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 1) * s),
                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 2) * s),
                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 3) * s));
+}
+
+// Eight codes and their scale as bf16 (the values' fp32 bits end above bf16's last one).
+DSV41_DEV uint4 kv4_bf16(uint32_t codes, uint32_t scale) {
+  const uint4 h = kv4_values(codes, kv4_scales<false>(scale)[0]);
+  const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const h16x2_t p = __builtin_bit_cast(h16x2_t, w[i]);
+    o[i] = (__float_as_uint((float)p[0]) >> 16) | (__float_as_uint((float)p[1]) & 0xffff0000u);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 // log2 of a page's rows, -1 where it is no power of two from 16 to 256.

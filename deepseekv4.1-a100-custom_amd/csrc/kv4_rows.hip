@@ -106,19 +106,6 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const RowsArgs a) {
   }
 }
 
-// Eight codes and their scale as bf16 (the values' fp32 bits end above bf16's last one).
-DSV41_DEV uint4 kv4_bf16(uint32_t codes, uint32_t scale) {
-  const uint4 h = kv4_values(codes, kv4_scales<false>(scale)[0]);
-  const uint32_t w[4] = {h.x, h.y, h.z, h.w};
-  uint32_t o[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const h16x2_t p = __builtin_bit_cast(h16x2_t, w[i]);
-    o[i] = (__float_as_uint((float)p[0]) >> 16) | (__float_as_uint((float)p[1]) & 0xffff0000u);
-  }
-  return make_uint4(o[0], o[1], o[2], o[3]);
-}
-
 template <int DIM>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const RowsArgs a) {
   const long r = blockIdx.x * 4L + (threadIdx.x >> 6);

@@ -73,7 +73,7 @@ SIGNATURES = {
     "dsv41_kv4_compact": [_P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _L, _P],
     "dsv41_kv4_copy_workspace_bytes": [_I, _I],
     "dsv41_kv4_copy": [_P, _I, _P, _I, _I, _I, _P, _P, _I, _P, _P, _L, _P],
-    "dsv41_kv4_attn_workspace_bytes": [_I, _I, _I, _I],
+    "dsv41_kv4_attn_workspace_bytes": [_I, _I, _I, _I, _I, _L],
     "dsv41_sattn4": [_P, _P, _L, _I, _I, _P, _I, _I, _I, _P, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _L, _I, _F, _P,
                      _I, _I, _P, _L, _P],
     "dsv41_sparse_attn4": [_P, _P, _L, _I, _P, _I, _P, _I, _I, _I, _P, _I, _I, _P, _I, _P, _P, _F, _P, _I, _I, _I, _P, _L,

@@ -234,8 +234,8 @@ def _indices(name: str, idx, shape: tuple, index: int):
     return (idx, idx.shape[-1]) if idx.shape[-1] else (None, 0)
 
 
-def _workspace(rows: int, h: int, wt: int, t: int, dev):
-    n = lib().dsv41_kv4_attn_workspace_bytes(rows, h, wt, t)
+def _workspace(rows: int, h: int, wt: int, t: int, dim: int, held: int, dev):
+    n = lib().dsv41_kv4_attn_workspace_bytes(rows, h, wt, t, dim, held)
     return (torch.empty(n // 4, dtype=torch.float32, device=dev) if n else None), n
 
 
@@ -266,7 +266,7 @@ def sattn4(q, kv_win, cache: PagedKV4, idx, pos, attn_sink, cos, sin, rd: int, s
     _, (pos, seq, pmax, plim) = cache._i64("sattn4", b, pos, seq, pmax, plim)
     out = torch.empty(b, 1, h, 512, dtype=torch.bfloat16, device=q.device)
     win = kv_win.shape[1]
-    ws, size = _workspace(b, h, win, t, q.device)
+    ws, size = _workspace(b, h, win, t, d, 0, q.device)
     _launch("dsv41_sattn4", index, q.data_ptr(), kv_win.data_ptr(), kv_win.stride(0), kv_win.shape[0], win,
             cache.pool.data_ptr(), cache.pages, cache.page, d, cache.table.data_ptr(), cache.slots, cache.cols, ptr(idx), t,
             pos.data_ptr(), seq.data_ptr(), pmax.data_ptr(), ptr(plim), sink.data_ptr(), ptr(cos), ptr(sin),
@@ -296,7 +296,7 @@ def sparse_attn4(q, kv, cache: PagedKV4, attn_sink, win_idxs, topk_idxs, softmax
         raise RuntimeError(f"sparse_attn4: {b} batch rows over {cache.slots} sequences")
     _, (seq,) = cache._i64("sparse_attn4", b, seq)
     out = torch.empty(b, s, h, 512, dtype=torch.bfloat16, device=q.device)
-    ws, size = _workspace(b * s, h, w, t, q.device)
+    ws, size = _workspace(b * s, h, w, t, d, b * cache.cols * cache.page, q.device)
     _launch("dsv41_sparse_attn4", index, q.data_ptr(), ptr(kv), kv.stride(0) if kv is not None else 0,
             kv.shape[1] if kv is not None else 0, ptr(win_idxs), w, cache.pool.data_ptr(), cache.pages, cache.page, d,
             cache.table.data_ptr(), cache.slots, cache.cols, ptr(idx), t, ptr(seq), sink.data_ptr(), softmax_scale,

@@ -411,9 +411,9 @@ long dsv41_kv4_copy_workspace_bytes(int n, int dst_pages);
 int dsv41_kv4_copy(const void* src_pool, int src_pages, void* dst_pool, int dst_pages, int page, int dim, const long* src,
                    const long* dst, int n, int* err, void* ws, long ws_bytes, void* stream);
 
-/* Workspace of the two attention calls: R query rows, H heads, wt window (or ring) rows and t cache rows a query.  Needs
- * no zeroing and no life beyond the call; 16-byte aligned. */
-long dsv41_kv4_attn_workspace_bytes(int R, int H, int wt, int t);
+/* Workspace of the two attention calls: R query rows, H heads, wt window (or ring) rows and t cache rows a query; rows = b *
+ * cols * page of dsv41_sparse_attn4, 0 for dsv41_sattn4.  Needs no zeroing and no life beyond the call; 16-byte aligned. */
+long dsv41_kv4_attn_workspace_bytes(int R, int H, int wt, int t, int dim, long rows);
 
 /* dsv41_sattn2 over a 4-bit cache: query row b at position pos[b] of sequence seq[b] over the ring kv_win[seq] (bf16
  * [win_slots, win, dim], slot stride win_sstride) and the cache rows idx[b, :] (-1, or without a page: none).  o = sum_j

@@ -118,7 +118,7 @@ def test_entry_points_refuse():
     # a workspace too small for the splits of one row over many keys
     bad = list(args)
     bad[13] = 4096
-    assert L.dsv41_kv4_attn_workspace_bytes(1, 16, 128, 4096) > 0 and L.dsv41_sattn4(*bad) == inv
+    assert L.dsv41_kv4_attn_workspace_bytes(1, 16, 128, 4096, 512, 0) > 0 and L.dsv41_sattn4(*bad) == inv
     args = [P, P, 128 * 512, 128, P, 128, P, 4, 16, 512, P, 2, 3, P, 10, None, P, 1.0, P, 1, 1, 16, None, 0, None]
     for at, v in [(0, None), (1, None), (4, None), (5, -1), (3, -1), (6, None), (13, None), (14, -1), (16, None), (18, None),
                   (21, 0)]:
