@@ -384,37 +384,34 @@ int run(Kv4AttnArgs& a, int dqk, int b, void* ws, long ws_bytes, hipStream_t st)
   return 0;
 }
 
-bool attn_ok(const Kv4AttnArgs& a, int dim, const void* table, int slots, int cols, int pages, int page) {
-  return (dim == 512 || dim == 576) && a.q && a.H > 0 && a.sink && a.out && a.t >= 0 && (a.t == 0 || (a.idx && a.pool)) &&
-         (((uintptr_t)a.q | (uintptr_t)a.win | (uintptr_t)a.pool) & 15) == 0 && ((uintptr_t)a.out & 7) == 0 &&
-         a.win_sstride % 8 == 0 && kv4_map_ok(table, slots, cols, pages, page) && (long)pages * page < (1L << 31);
+bool attn_ok(const Kv4AttnArgs& a, const dsv41_kv4* c) {
+  return kv4_ok(c) && a.q && a.H > 0 && a.sink && a.out && a.t >= 0 && (a.t == 0 || a.idx) &&
+         (((uintptr_t)a.q | (uintptr_t)a.win) & 15) == 0 && ((uintptr_t)a.out & 7) == 0 && a.win_sstride % 8 == 0;
 }
 
 }  // namespace
 
 extern "C" {
 
-long dsv41_kv4_attn_workspace_bytes(int R, int H, int wt, int t, int dim, long rows) {
+long dsv41_kv4_attn_workspace_bytes(const dsv41_kv4* c, int R, int H, int wt, int t, int b) {
   if (R <= 0 || H <= 0 || wt < 0 || t < 0) return 0;
-  const Plan p = plan_of(R, H, wt, t, dim, rows);
+  const Plan p = plan_of(R, H, wt, t, c->dim, (long)b * c->cols * c->page);
   return p.list + p.rows + p.part;
 }
 
-int dsv41_sattn4(const void* q, const void* kv_win, long win_sstride, int win_slots, int win, const void* pool, int pages, int page,
-                 int dim, const int* table, int slots, int cols, const int* idx, int t, const long* pos, const long* seq,
-                 const long* pmax, const long* plim, const float* sink, const float* cos_t, const float* sin_t,
-                 long n_pos, int rd, float scale, void* out, int B, int h, void* ws, long ws_bytes, void* stream) {
+int dsv41_sattn4(const dsv41_kv4* c, const void* q, const void* kv_win, long win_sstride, int win_slots, int win,
+                 const int* idx, int t, const long* pos, const long* seq, const long* pmax, const long* plim,
+                 const float* sink, const float* cos_t, const float* sin_t, long n_pos, int rd, float scale, void* out,
+                 int B, int h, void* ws, long ws_bytes, void* stream) {
   if (B <= 0) return B < 0 ? (int)hipErrorInvalidValue : 0;
   Kv4AttnArgs a{};
   a.q = (const uint16_t*)q;
-  a.q_rstride = (long)h * dim;
   a.R = B;
   a.H = h;
   a.win = (const uint16_t*)kv_win;
   a.win_sstride = win_sstride;
   a.win_rows = win;
   a.win_slots = win_slots;
-  a.pool = (const uint8_t*)pool;
   a.idx = idx;
   a.t = t;
   a.rows_per_slot = 1;
@@ -429,22 +426,22 @@ int dsv41_sattn4(const void* q, const void* kv_win, long win_sstride, int win_sl
   a.n_pos = n_pos;
   a.rd = rd;
   a.out = (uint16_t*)out;
-  if (!attn_ok(a, dim, table, slots, cols, pages, page) || !kv_win || win <= 0 || !pos || !seq || !pmax || rd < 0 ||
-      rd > 512 || rd % 4 || (rd > 0 && (!cos_t || !sin_t)))
+  if (!attn_ok(a, c) || !kv_win || win <= 0 || !pos || !seq || !pmax || rd < 0 || rd > 512 || rd % 4 ||
+      (rd > 0 && (!cos_t || !sin_t)))
     return (int)hipErrorInvalidValue;
-  a.map = kv4_map(table, slots, cols, pages, page);
-  return run(a, dim, 0, ws, ws_bytes, (hipStream_t)stream);
+  a.q_rstride = (long)h * c->dim;
+  a.pool = (const uint8_t*)c->pool;
+  a.map = kv4_map(*c);
+  return run(a, c->dim, 0, ws, ws_bytes, (hipStream_t)stream);
 }
 
-int dsv41_sparse_attn4(const void* q, const void* kv, long kv_bstride, int n_kv, const int* widx, int wt,
-                       const void* pool, int pages, int page, int dim, const int* table, int slots, int cols,
-                       const int* idx, int t, const long* seq, const float* sink, float scale, void* out, int b, int s,
-                       int h, void* ws, long ws_bytes, void* stream) {
+int dsv41_sparse_attn4(const dsv41_kv4* c, const void* q, const void* kv, long kv_bstride, int n_kv, const int* widx,
+                       int wt, const int* idx, int t, const long* seq, const float* sink, float scale, void* out, int b,
+                       int s, int h, void* ws, long ws_bytes, void* stream) {
   if (b <= 0 || s <= 0) return b < 0 || s < 0 ? (int)hipErrorInvalidValue : 0;
   if ((long)b * s >= (1L << 31)) return (int)hipErrorInvalidValue;
   Kv4AttnArgs a{};
   a.q = (const uint16_t*)q;
-  a.q_rstride = (long)h * dim;
   a.R = b * s;
   a.H = h;
   a.win = (const uint16_t*)kv;
@@ -452,7 +449,6 @@ int dsv41_sparse_attn4(const void* q, const void* kv, long kv_bstride, int n_kv,
   a.win_rows = n_kv;
   a.widx = widx;
   a.wt = wt;
-  a.pool = (const uint8_t*)pool;
   a.idx = idx;
   a.t = t;
   a.rows_per_slot = s;
@@ -460,10 +456,11 @@ int dsv41_sparse_attn4(const void* q, const void* kv, long kv_bstride, int n_kv,
   a.scale = scale * kLog2e;
   a.sink = sink;
   a.out = (uint16_t*)out;
-  if (!attn_ok(a, dim, table, slots, cols, pages, page) || wt < 0 || n_kv < 0 || (wt > 0 && (!kv || !widx)))
-    return (int)hipErrorInvalidValue;
-  a.map = kv4_map(table, slots, cols, pages, page);
-  return run(a, dim, b, ws, ws_bytes, (hipStream_t)stream);
+  if (!attn_ok(a, c) || wt < 0 || n_kv < 0 || (wt > 0 && (!kv || !widx))) return (int)hipErrorInvalidValue;
+  a.q_rstride = (long)h * c->dim;
+  a.pool = (const uint8_t*)c->pool;
+  a.map = kv4_map(*c);
+  return run(a, c->dim, b, ws, ws_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

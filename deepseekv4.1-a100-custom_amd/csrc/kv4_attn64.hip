@@ -47,7 +47,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn64_kernel(const Kv4AttnAr
   const int h0 = hg * 64;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, g = lane >> 4;
-  // this wave's group of heads, its keys and head block (2 group + own) in the scores, its 128 columns in the product
+  // this wave's group of heads, its keys and head block (2 group + own) in the scores, its eight blocks of 16
+  // columns (every fourth) in the product
   const int group = wave >> 2, kb = wave & 1, own = (wave >> 1) & 1, hb = 2 * group + own, cols = wave & 3;
   const int slot = r / a.rows_per_slot;
   const int t0 = sp * a.chunk, t1 = min(t0 + a.chunk, a.tiles), T = t1 - t0;
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn64_kernel(const Kv4AttnAr
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       v_get[i][e] = base + kVAt + (kr + 4 * e) * 1024 +
-                    (((uint32_t)(cols * 16 + 2 * i + ((l16 & 3) >> 1)) ^ swizzle(kr + 4 * e)) << 4) + (l16 & 1) * 8;
+                    (((uint32_t)(8 * i + 2 * cols + ((l16 & 3) >> 1)) ^ swizzle(kr + 4 * e)) << 4) + (l16 & 1) * 8;
   const uint32_t t_get = base + kTAt + key * 128 + ((g ^ ((key >> 1) & 7)) << 4);  // (unit 4 + g: bit 2 the other way)
   // (probabilities: a head's four units likewise, by the head)
   const uint32_t p_get = base + kPAt + (32 * group + l16) * 64 + ((g ^ (l16 >> 2)) << 4);
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn64_kernel(const Kv4AttnAr
         const int i = k & 1, c = k >> 1;
         o[i][c] = mfma_bf16_16x16x32(__builtin_bit_cast(uint4, vf[c]), __builtin_bit_cast(uint4, pb[i]), o[i][c]);
         if (i == 1) {  // (this column block is done: its values of tile u - 1)
-          const uint2 lo = lds_read_tr((v_get[c & 1][0] + old) ^ (c >> 1 << 6)), hi = lds_read_tr((v_get[c & 1][1] + old) ^ (c >> 1 << 6));
+          const uint2 lo = lds_read_tr(v_get[c & 1][0] + old + (c >> 1) * 256), hi = lds_read_tr(v_get[c & 1][1] + old + (c >> 1) * 256);
           vf[c] = u32x4{lo.x, lo.y, hi.x, hi.y};
         }
       }
@@ -231,20 +232,20 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_attn64_kernel(const Kv4AttnAr
     const float sum = w[0] + w[1];
     const int h = h0 + 16 * (2 * group + i) + l16;
     if (h >= a.H) continue;
-    const int col = cols * 128 + 4 * g;
+    const int col = 16 * cols + 4 * g;
     if (a.nsplit > 1) {
       const long at = ((long)r * a.H + h) * a.nsplit + sp;
       if (cols == 0 && g == 0) *(float2*)(a.part + 2 * at) = make_float2(m[i], sum);
       float* dst = a.part + 2L * a.R * a.H * a.nsplit + at * 512 + col;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) *(float4*)(dst + 16 * c) = make_float4(o[i][c][0], o[i][c][1], o[i][c][2], o[i][c][3]);
+      for (int c = 0; c < 8; ++c) *(float4*)(dst + 64 * c) = make_float4(o[i][c][0], o[i][c][1], o[i][c][2], o[i][c][3]);
     } else {
       const float den = sum + exp2f(a.sink[h] * kLog2e - m[i]);
       const float inv = m[i] == -__builtin_inff() ? 0.0f : 1.0f / den;  // (no key: zeros)
       uint16_t* dst = a.out + ((long)r * a.H + h) * 512 + col;
 #pragma unroll
       for (int c = 0; c < 8; ++c)
-        *(uint2*)(dst + 16 * c) = make_uint2(pack_bf16(o[i][c][0] * inv, o[i][c][1] * inv), pack_bf16(o[i][c][2] * inv, o[i][c][3] * inv));
+        *(uint2*)(dst + 64 * c) = make_uint2(pack_bf16(o[i][c][0] * inv, o[i][c][1] * inv), pack_bf16(o[i][c][2] * inv, o[i][c][3] * inv));
     }
   }
 }

@@ -73,12 +73,12 @@ inline int kv4_shift(int page) {
   return -1;
 }
 
-inline bool kv4_map_ok(const void* table, int slots, int cols, int pages, int page) {
-  return table && slots > 0 && cols > 0 && (long)slots * cols < (1L << 31) && pages > 0 && kv4_shift(page) >= 0;
+inline bool kv4_ok(const dsv41_kv4* c) {
+  return c && c->pool && ((uintptr_t)c->pool & 15) == 0 && c->table && c->refs && c->err && c->slots > 0 && c->cols > 0 &&
+         (long)c->slots * c->cols < (1L << 31) && c->pages > 0 && kv4_shift(c->page) >= 0 &&
+         (long)c->pages * c->page < (1L << 31) && (c->dim == 512 || c->dim == 576);
 }
 
-inline Kv4Table kv4_map(const int* table, int slots, int cols, int pages, int page) {
-  return Kv4Table{table, slots, cols, pages, kv4_shift(page)};
-}
+inline Kv4Table kv4_map(const dsv41_kv4& c) { return Kv4Table{c.table, c.slots, c.cols, c.pages, kv4_shift(c.page)}; }
 
 }  // namespace

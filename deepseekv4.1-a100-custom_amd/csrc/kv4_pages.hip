@@ -321,74 +321,69 @@ __global__ void __launch_bounds__(256) copy_kernel(const CopyArgs a) {
 
 constexpr int kFewCopies = 1024;
 
-bool pages_args(PagesArgs& a, int* table, int slots, int cols, int* refs, int pages, int page, int* err) {
-  if (!kv4_map_ok(table, slots, cols, pages, page) || !refs) return false;
-  a = PagesArgs{};
-  a.table = table;
-  a.slots = slots;
-  a.cols = cols;
-  a.refs = refs;
-  a.pages = pages;
-  a.shift = kv4_shift(page);
-  a.err = err;
-  return true;
+PagesArgs pages_args(const dsv41_kv4& c) {
+  PagesArgs a{};
+  a.table = c.table;
+  a.slots = c.slots;
+  a.cols = c.cols;
+  a.refs = c.refs;
+  a.pages = c.pages;
+  a.shift = kv4_shift(c.page);
+  a.err = c.err;
+  a.pool = (uint8_t*)c.pool;
+  a.page_bytes = (long)kv4_row_bytes(c.dim) * c.page;
+  return a;
 }
+
+// A grid of a workgroup per entry and 256 columns.
+bool grid_ok(const dsv41_kv4* c) { return kv4_ok(c) && c->cols <= 256 * 65535; }
 
 }  // namespace
 
 extern "C" {
 
-int dsv41_kv4_fork(const long* src, const long* dst, const long* rows, int n, int* table, int slots, int cols, int* refs,
-                   int pages, int page, int* err, void* stream) {
-  PagesArgs a;
-  if (n < 0 || !pages_args(a, table, slots, cols, refs, pages, page, err) || !err || cols > 256 * 65535)
-    return (int)hipErrorInvalidValue;
+int dsv41_kv4_fork(const dsv41_kv4* c, const long* src, const long* dst, const long* rows, int n, void* stream) {
+  if (!grid_ok(c) || n < 0) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
   if (!src || !dst) return (int)hipErrorInvalidValue;
+  PagesArgs a = pages_args(*c);
   a.src = src;
   a.seq = dst;
   a.begin = rows;
   a.n = n;
-  fork_kernel<<<dim3(n, (cols + 255) / 256), 256, 0, (hipStream_t)stream>>>(a);
+  fork_kernel<<<dim3(n, (c->cols + 255) / 256), 256, 0, (hipStream_t)stream>>>(a);
   DSV41_CHECK_LAUNCH();
   return 0;
 }
 
-int dsv41_kv4_release(const long* seq, const long* rows, int n, int* table, int slots, int cols, int* refs, int pages,
-                      int page, int* err, void* stream) {
-  PagesArgs a;
-  if (n < 0 || !pages_args(a, table, slots, cols, refs, pages, page, err) || !err || cols > 256 * 65535)
-    return (int)hipErrorInvalidValue;
+int dsv41_kv4_release(const dsv41_kv4* c, const long* seq, const long* rows, int n, void* stream) {
+  if (!grid_ok(c) || n < 0) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
   if (!seq) return (int)hipErrorInvalidValue;
+  PagesArgs a = pages_args(*c);
   a.seq = seq;
   a.begin = rows;
   a.n = n;
-  release_kernel<<<dim3(n, (cols + 255) / 256), 256, 0, (hipStream_t)stream>>>(a);
+  release_kernel<<<dim3(n, (c->cols + 255) / 256), 256, 0, (hipStream_t)stream>>>(a);
   DSV41_CHECK_LAUNCH();
   return 0;
 }
 
-long dsv41_kv4_reserve_workspace_bytes(int n, int slots, int pages) {
-  return 4 * ((long)slots + 3L * pages + 2L * n);
+long dsv41_kv4_reserve_workspace_bytes(const dsv41_kv4* c, int n) {
+  return 4 * ((long)c->slots + 3L * c->pages + 2L * n);
 }
 
-int dsv41_kv4_reserve(const long* seq, const long* begin, const long* end, int n, void* pool, int dim, int* table,
-                      int slots, int cols, int* refs, int pages, int page, int* err, void* ws, long ws_bytes,
-                      void* stream) {
-  PagesArgs a;
-  if (n < 0 || n > kMostEntries || !pages_args(a, table, slots, cols, refs, pages, page, err) || !err || !pool ||
-      ((uintptr_t)pool & 15) || (dim != 512 && dim != 576))
-    return (int)hipErrorInvalidValue;
+int dsv41_kv4_reserve(const dsv41_kv4* c, const long* seq, const long* begin, const long* end, int n, void* ws,
+                      long ws_bytes, void* stream) {
+  if (!kv4_ok(c) || n < 0 || n > kMostEntries) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
-  if (!seq || !begin || !end || !ws || ws_bytes < dsv41_kv4_reserve_workspace_bytes(n, slots, pages))
+  if (!seq || !begin || !end || !ws || ((uintptr_t)ws & 3) || ws_bytes < dsv41_kv4_reserve_workspace_bytes(c, n))
     return (int)hipErrorInvalidValue;
+  PagesArgs a = pages_args(*c);
   a.seq = seq;
   a.begin = begin;
   a.end = end;
   a.n = n;
-  a.pool = (uint8_t*)pool;
-  a.page_bytes = (long)kv4_row_bytes(dim) * page;
   a.ws = (int*)ws;
   reserve_plan_kernel<<<1, kPlanThreads, 0, (hipStream_t)stream>>>(a);
   DSV41_CHECK_LAUNCH();
@@ -397,39 +392,33 @@ int dsv41_kv4_reserve(const long* seq, const long* begin, const long* end, int n
   return 0;
 }
 
-long dsv41_kv4_compact_workspace_bytes(int pages) { return 4 * (2 + 3L * pages); }
+long dsv41_kv4_compact_workspace_bytes(const dsv41_kv4* c) { return 4 * (2 + 3L * c->pages); }
 
-int dsv41_kv4_compact(void* pool, int dim, int* table, int slots, int cols, int* refs, int pages, int page, int* live,
-                      void* ws, long ws_bytes, void* stream) {
-  PagesArgs a;
-  if (!pages_args(a, table, slots, cols, refs, pages, page, nullptr) || !pool || ((uintptr_t)pool & 15) ||
-      (dim != 512 && dim != 576) || !live || !ws || ws_bytes < dsv41_kv4_compact_workspace_bytes(pages))
+int dsv41_kv4_compact(const dsv41_kv4* c, int* live, void* ws, long ws_bytes, void* stream) {
+  if (!kv4_ok(c) || !live || !ws || ((uintptr_t)ws & 3) || ws_bytes < dsv41_kv4_compact_workspace_bytes(c))
     return (int)hipErrorInvalidValue;
-  a.pool = (uint8_t*)pool;
-  a.page_bytes = (long)kv4_row_bytes(dim) * page;
+  PagesArgs a = pages_args(*c);
   a.ws = (int*)ws;
   a.live = live;
   compact_plan_kernel<<<1, kPlanThreads, 0, (hipStream_t)stream>>>(a);
   DSV41_CHECK_LAUNCH();
-  compact_move_kernel<<<pages < 2048 ? pages : 2048, 256, 0, (hipStream_t)stream>>>(a);
+  compact_move_kernel<<<c->pages < 2048 ? c->pages : 2048, 256, 0, (hipStream_t)stream>>>(a);
   DSV41_CHECK_LAUNCH();
   return 0;
 }
 
-long dsv41_kv4_copy_workspace_bytes(int n, int dst_pages) { return n > kFewCopies ? 4L * dst_pages : 0; }
+long dsv41_kv4_copy_workspace_bytes(const dsv41_kv4* c, int n) { return n > kFewCopies ? 4L * c->pages : 0; }
 
-int dsv41_kv4_copy(const void* src_pool, int src_pages, void* dst_pool, int dst_pages, int page, int dim, const long* src,
-                   const long* dst, int n, int* err, void* ws, long ws_bytes, void* stream) {
-  if (n < 0 || kv4_shift(page) < 0 || (dim != 512 && dim != 576) || src_pages <= 0 || dst_pages <= 0)
-    return (int)hipErrorInvalidValue;
+int dsv41_kv4_copy(const dsv41_kv4* c, const dsv41_kv4* other, const long* src, const long* dst, int n, void* ws,
+                   long ws_bytes, void* stream) {
+  if (!kv4_ok(c) || !kv4_ok(other) || c->dim != other->dim || c->page != other->page || n < 0) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
-  if (!src_pool || !dst_pool || (((uintptr_t)src_pool | (uintptr_t)dst_pool) & 15) || !src || !dst || !err ||
-      (n > kFewCopies && (!ws || ws_bytes < dsv41_kv4_copy_workspace_bytes(n, dst_pages))))
+  if (!src || !dst || (n > kFewCopies && (!ws || ((uintptr_t)ws & 3) || ws_bytes < dsv41_kv4_copy_workspace_bytes(c, n))))
     return (int)hipErrorInvalidValue;
-  const long pb = (long)kv4_row_bytes(dim) * page;
-  const char *s0 = (const char*)src_pool, *d0 = (const char*)dst_pool;
-  if (s0 < d0 + dst_pages * pb && d0 < s0 + src_pages * pb) return (int)hipErrorInvalidValue;  // (one memory)
-  CopyArgs a{(const uint8_t*)src_pool, (uint8_t*)dst_pool, src_pages, dst_pages, n, pb, src, dst, err,
+  const long pb = (long)kv4_row_bytes(c->dim) * c->page;
+  const char *s0 = (const char*)other->pool, *d0 = (const char*)c->pool;
+  if (s0 < d0 + c->pages * pb && d0 < s0 + other->pages * pb) return (int)hipErrorInvalidValue;  // (one memory)
+  CopyArgs a{(const uint8_t*)other->pool, (uint8_t*)c->pool, other->pages, c->pages, n, pb, src, dst, c->err,
              n > kFewCopies ? (int*)ws : nullptr};
   if (a.last) {
     copy_last_kernel<<<1, kPlanThreads, 0, (hipStream_t)stream>>>(a);

@@ -124,39 +124,39 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const RowsArgs a) {
   if (DIM == 576 && lane < 8) *(uint4*)(out + 512 + 8 * lane) = tail;
 }
 
-bool rows_ok(const RowsArgs& a, int pages, int page, int dim, const int* table, int slots, int cols) {
-  return (dim == 512 || dim == 576) && a.seq && a.row && a.pool && ((uintptr_t)a.pool & 15) == 0 && a.n < (1L << 32) &&
-         kv4_map_ok(table, slots, cols, pages, page);
+void rows_args(RowsArgs& a, const dsv41_kv4& c, const long* seq, const long* row, long n) {
+  a = RowsArgs{};
+  a.seq = seq;
+  a.row = row;
+  a.n = n;
+  a.pool = (uint8_t*)c.pool;
+  a.map = kv4_map(c);
+  a.refs = c.refs;
+  a.err = c.err;
 }
 
 }  // namespace
 
 extern "C" {
 
-int dsv41_kv4_append(const void* x, long x_rstride, const long* seq, const long* row, long n, int ratio,
-                     const float* cos_t, const float* sin_t, long n_pos, int rd, void* pool, int pages, int page,
-                     int dim, const int* table, int slots, int cols, const int* refs, int* err, void* stream) {
-  if (n <= 0) return n < 0 ? (int)hipErrorInvalidValue : 0;
-  RowsArgs a{};
+int dsv41_kv4_append(const dsv41_kv4* c, const void* x, long x_rstride, const long* seq, const long* row, long n,
+                     int ratio, const float* cos_t, const float* sin_t, long n_pos, int rd, void* stream) {
+  if (!kv4_ok(c) || n < 0 || n >= (1L << 32)) return (int)hipErrorInvalidValue;
+  if (n == 0) return 0;
+  if (!seq || !row || !x || ((uintptr_t)x & 15) || x_rstride < c->dim || x_rstride % 8 || ratio < 1 || rd < 0 ||
+      rd > c->dim || (rd & 1) || (rd > 0 && (!cos_t || !sin_t)))
+    return (int)hipErrorInvalidValue;
+  RowsArgs a;
+  rows_args(a, *c, seq, row, n);
   a.x = (const uint16_t*)x;
   a.x_rstride = x_rstride;
-  a.seq = seq;
-  a.row = row;
-  a.n = n;
   a.ratio = ratio;
   a.cos_t = cos_t;
   a.sin_t = sin_t;
   a.n_pos = n_pos;
   a.rd = rd;
-  a.pool = (uint8_t*)pool;
-  a.refs = refs;
-  a.err = err;
-  if (!rows_ok(a, pages, page, dim, table, slots, cols) || !x || ((uintptr_t)x & 15) || x_rstride < dim ||
-      x_rstride % 8 || ratio < 1 || !refs || !err || rd < 0 || rd > dim || (rd & 1) || (rd > 0 && (!cos_t || !sin_t)))
-    return (int)hipErrorInvalidValue;
-  a.map = kv4_map(table, slots, cols, pages, page);
   const unsigned grid = (unsigned)((n + 3) / 4);
-  if (dim == 512)
+  if (c->dim == 512)
     kv4_append_kernel<512><<<grid, 256, 0, (hipStream_t)stream>>>(a);
   else
     kv4_append_kernel<576><<<grid, 256, 0, (hipStream_t)stream>>>(a);
@@ -164,19 +164,15 @@ int dsv41_kv4_append(const void* x, long x_rstride, const long* seq, const long*
   return 0;
 }
 
-int dsv41_kv4_read(const void* pool, int pages, int page, int dim, const int* table, int slots, int cols,
-                   const long* seq, const long* row, long n, void* out, void* stream) {
-  if (n <= 0) return n < 0 ? (int)hipErrorInvalidValue : 0;
-  RowsArgs a{};
-  a.seq = seq;
-  a.row = row;
-  a.n = n;
-  a.pool = (uint8_t*)pool;
+int dsv41_kv4_read(const dsv41_kv4* c, const long* seq, const long* row, long n, void* out, void* stream) {
+  if (!kv4_ok(c) || n < 0 || n >= (1L << 32)) return (int)hipErrorInvalidValue;
+  if (n == 0) return 0;
+  if (!seq || !row || !out || ((uintptr_t)out & 15)) return (int)hipErrorInvalidValue;
+  RowsArgs a;
+  rows_args(a, *c, seq, row, n);
   a.out = (uint16_t*)out;
-  if (!rows_ok(a, pages, page, dim, table, slots, cols) || !out || ((uintptr_t)out & 15)) return (int)hipErrorInvalidValue;
-  a.map = kv4_map(table, slots, cols, pages, page);
   const unsigned grid = (unsigned)((n + 3) / 4);
-  if (dim == 512)
+  if (c->dim == 512)
     kv4_read_kernel<512><<<grid, 256, 0, (hipStream_t)stream>>>(a);
   else
     kv4_read_kernel<576><<<grid, 256, 0, (hipStream_t)stream>>>(a);

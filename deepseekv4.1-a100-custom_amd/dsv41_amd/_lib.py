@@ -63,21 +63,19 @@ SIGNATURES = {
     "dsv41_f32_proj2": [_P, _L, _P, _P, _I, _I, _I, _P, _P, _P],
     "dsv41_compress_pool_decode": [_P, _P, _L, _P, _P, _L, _I, _P, _P, _I, _I, _I, _P, _F, _P, _L, _P, _P],
     "dsv41_compress_pool_prefill": [_P, _P, _L, _P, _P, _I, _L, _I, _I, _I, _P, _F, _P, _L, _I, _P],
-    "dsv41_kv4_append": [_P, _L, _P, _P, _L, _I, _P, _P, _L, _I, _P, _I, _I, _I, _P, _I, _I, _P, _P, _P],
-    "dsv41_kv4_read": [_P, _I, _I, _I, _P, _I, _I, _P, _P, _L, _P, _P],
-    "dsv41_kv4_fork": [_P, _P, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P],
-    "dsv41_kv4_release": [_P, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P],
-    "dsv41_kv4_reserve_workspace_bytes": [_I, _I, _I],
-    "dsv41_kv4_reserve": [_P, _P, _P, _I, _P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _L, _P],
-    "dsv41_kv4_compact_workspace_bytes": [_I],
-    "dsv41_kv4_compact": [_P, _I, _P, _I, _I, _P, _I, _I, _P, _P, _L, _P],
-    "dsv41_kv4_copy_workspace_bytes": [_I, _I],
-    "dsv41_kv4_copy": [_P, _I, _P, _I, _I, _I, _P, _P, _I, _P, _P, _L, _P],
-    "dsv41_kv4_attn_workspace_bytes": [_I, _I, _I, _I, _I, _L],
-    "dsv41_sattn4": [_P, _P, _L, _I, _I, _P, _I, _I, _I, _P, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _L, _I, _F, _P,
-                     _I, _I, _P, _L, _P],
-    "dsv41_sparse_attn4": [_P, _P, _L, _I, _P, _I, _P, _I, _I, _I, _P, _I, _I, _P, _I, _P, _P, _F, _P, _I, _I, _I, _P, _L,
-                           _P],
+    "dsv41_kv4_append": [_P, _P, _L, _P, _P, _L, _I, _P, _P, _L, _I, _P],
+    "dsv41_kv4_read": [_P, _P, _P, _L, _P, _P],
+    "dsv41_kv4_fork": [_P, _P, _P, _P, _I, _P],
+    "dsv41_kv4_release": [_P, _P, _P, _I, _P],
+    "dsv41_kv4_reserve_workspace_bytes": [_P, _I],
+    "dsv41_kv4_reserve": [_P, _P, _P, _P, _I, _P, _L, _P],
+    "dsv41_kv4_compact_workspace_bytes": [_P],
+    "dsv41_kv4_compact": [_P, _P, _P, _L, _P],
+    "dsv41_kv4_copy_workspace_bytes": [_P, _I],
+    "dsv41_kv4_copy": [_P, _P, _P, _P, _I, _P, _L, _P],
+    "dsv41_kv4_attn_workspace_bytes": [_P, _I, _I, _I, _I, _I],
+    "dsv41_sattn4": [_P, _P, _P, _L, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _L, _I, _F, _P, _I, _I, _P, _L, _P],
+    "dsv41_sparse_attn4": [_P, _P, _P, _L, _I, _P, _I, _P, _I, _P, _P, _F, _P, _I, _I, _I, _P, _L, _P],
 }
 _RESTYPE = {"dsv41_attn_workspace_bytes": _L, "dsv41_select_workspace_bytes": _L,
             "dsv41_index_select_workspace_bytes": _L, "dsv41_candidate_blocks_workspace_bytes": _L,

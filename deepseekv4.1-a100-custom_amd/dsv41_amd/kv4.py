@@ -21,10 +21,12 @@ it leaves out and notes in the cache's error word, which check() raises for (eve
 Forward only, as everything here."""
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
-from ._lib import as_f32, as_i64, lib, ptr
+from ._lib import as_f32, lib, ptr
 from .a8 import _aligned, _index, _launch, _no_grad
 
 ROW_BYTES = {512: 288, 576: 336}
@@ -33,6 +35,13 @@ _E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -
 _ERRORS = ((1, "too few free pages"), (2, "an entry was left out (an index out of range, or one named twice)"),
            (4, "a row was dropped (no page of the sequence's own there, or no rope angle)"))
 _MOST_ENTRIES = 4096
+_I64, _I32, _BF16 = torch.int64, torch.int32, torch.bfloat16
+
+
+class _Cache(ctypes.Structure):
+    """dsv41_kv4 of include/dsv41_hip.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("pool", "table", "refs", "err")] +
+                [(n, ctypes.c_int) for n in ("pages", "page", "slots", "cols", "dim")])
 
 
 class PagedKV4:
@@ -50,15 +59,20 @@ class PagedKV4:
         if table.dtype != torch.int32 or table.dim() != 2 or refs.dtype != torch.int32 or refs.shape != pool.shape[:1]:
             raise ValueError(f"PagedKV4: table {tuple(table.shape)} {table.dtype}, refs {tuple(refs.shape)} {refs.dtype} "
                              f"(int32 [slots, columns] and [{pool.shape[0]}])")
-        if 0 in pool.shape or 0 in table.shape or table.numel() >= 1 << 31 or pool.shape[0] >= 1 << 31:
+        if 0 in pool.shape or 0 in table.shape or table.numel() >= 1 << 31 or pool.shape[0] * pool.shape[1] >= 1 << 31:
             raise ValueError(f"PagedKV4: pool {tuple(pool.shape)}, table {tuple(table.shape)}")
         if not (pool.is_contiguous() and table.is_contiguous() and refs.is_contiguous()) or pool.data_ptr() % 16:
             raise ValueError("PagedKV4: contiguous tensors, the pool 16-byte aligned")
-        self.device = torch.device("cuda", _index(pool, table, refs))
+        self.index = _index(pool, table, refs)
+        self.device = torch.device("cuda", self.index)
         self.pool, self.table, self.refs, self.dim = pool, table, refs, dim
         self.pages, self.page = pool.shape[:2]
         self.slots, self.cols = table.shape
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._c = _Cache(pool.data_ptr(), table.data_ptr(), refs.data_ptr(), self.err.data_ptr(), self.pages, self.page,
+                         self.slots, self.cols, dim)
+        self._at = ctypes.addressof(self._c)
+        self._sizes = {}
 
     @classmethod
     def empty(cls, pages: int, slots: int, cap: int, dim: int = 576, page: int = 64, device="cuda") -> "PagedKV4":
@@ -69,20 +83,25 @@ class PagedKV4:
                    torch.full((slots, -(-cap // page)), -1, dtype=torch.int32, device=device),
                    torch.zeros(pages, dtype=torch.int32, device=device), dim)
 
-    def _map(self):
-        return self.table.data_ptr(), self.slots, self.cols, self.refs.data_ptr(), self.pages, self.page
+    def _i64(self, name: str, t, n: int) -> torch.Tensor:
+        """n index entries as contiguous int64 on the cache's GPU (from a tensor or a list)."""
+        if not isinstance(t, torch.Tensor):
+            t = torch.as_tensor(t, dtype=_I64)
+        if t.numel() != n:
+            raise RuntimeError(f"{name}: {t.numel()} entries beside {n}")
+        if t.dtype is not _I64 or t.get_device() != self.index or not t.is_contiguous():
+            t = t.to(device=self.device, dtype=_I64, non_blocking=True).contiguous()
+        return t
 
-    def _i64(self, name: str, n: int | None, *ts):
-        """Index tensors (or lists) as int64 on the cache's GPU, n each."""
-        out = []
-        for t in ts:
-            if t is not None:
-                t = as_i64(t if isinstance(t, torch.Tensor) else torch.as_tensor(t, dtype=torch.int64), self.device)
-                n = t.numel() if n is None else n
-                if t.numel() != n:
-                    raise RuntimeError(f"{name}: {t.numel()} entries beside {n}")
-            out.append(t)
-        return n, out
+    def _size(self, rows: int, h: int, wt: int, t: int, b: int) -> int:
+        """Workspace bytes of an attention call."""
+        key = (rows, h, wt, t, b)
+        n = self._sizes.get(key)
+        if n is None:
+            if len(self._sizes) > 1024:
+                self._sizes.clear()
+            n = self._sizes[key] = lib().dsv41_kv4_attn_workspace_bytes(self._at, *key)
+        return n
 
     def _done(self) -> None:
         if _lib.CHECK_ERRORS:
@@ -108,24 +127,25 @@ class PagedKV4:
             raise RuntimeError(f"kv4.append: ratio {ratio}, {rd} rotated columns")
         _no_grad("kv4.append", latent)
         index = _index(self.pool, latent)
-        x = latent.reshape(-1, dim)
-        if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < dim or x.data_ptr() % 16:
-            x = x.contiguous()
-            x = _aligned(x)
-        n, (seq, row) = self._i64("kv4.append", x.shape[0], seq, row)
+        x = latent if latent.dim() == 2 else latent.reshape(-1, dim)
+        n, stride = x.shape[0], x.stride(0)
+        if n == 1:
+            stride = dim
+        if x.stride(1) != 1 or stride % 8 or stride < dim or x.data_ptr() % 16:
+            x, stride = _aligned(x.contiguous()), dim
+        seq, row = self._i64("kv4.append", seq, n), self._i64("kv4.append", row, n)
         cos, sin = _angles("kv4.append", cos, sin, rd, index)
-        _launch("dsv41_kv4_append", index, x.data_ptr(), x.stride(0) if n > 1 else dim, seq.data_ptr(), row.data_ptr(), n,
-                ratio, ptr(cos), ptr(sin), cos.shape[0] if rd else 0, rd, self.pool.data_ptr(), self.pages, self.page, dim,
-                self.table.data_ptr(), self.slots, self.cols, self.refs.data_ptr(), self.err.data_ptr())
+        _launch("dsv41_kv4_append", index, self._at, x.data_ptr(), stride, seq.data_ptr(), row.data_ptr(), n, ratio, ptr(cos),
+                ptr(sin), cos.shape[0] if rd else 0, rd)
         self._done()
 
     def read(self, seq, row) -> torch.Tensor:
         """Rows row[i] of sequences seq[i] as bf16 [..., dim] (the shape of row; exact), zeros where there is none."""
         shape = row.shape if isinstance(row, torch.Tensor) else (len(row),)
-        n, (seq, row) = self._i64("kv4.read", None, seq, row)
-        out = torch.empty(*shape, self.dim, dtype=torch.bfloat16, device=self.device)
-        _launch("dsv41_kv4_read", self.device.index, self.pool.data_ptr(), self.pages, self.page, self.dim,
-                self.table.data_ptr(), self.slots, self.cols, seq.data_ptr(), row.data_ptr(), n, out.data_ptr())
+        out = torch.empty(*shape, self.dim, dtype=_BF16, device=self.device)
+        n = out.numel() // self.dim
+        seq, row = self._i64("kv4.read", seq, n), self._i64("kv4.read", row, n)
+        _launch("dsv41_kv4_read", self.index, self._at, seq.data_ptr(), row.data_ptr(), n, out.data_ptr())
         return out
 
     # ---- pages
@@ -133,40 +153,41 @@ class PagedKV4:
         """Rows begin[i] .. end[i] - 1 of sequence seq[i] made writable: a page of its own wherever it has none or shares
         one, the lowest free pages in the order of the arguments; where a shared page is replaced, its rows before
         begin[i] are copied.  Distinct sequences, 4096 at most."""
-        n, (seq, begin, end) = self._i64("kv4.reserve", None, seq, begin, end)
+        n = len(seq)
         if n > _MOST_ENTRIES:
             raise RuntimeError(f"kv4.reserve: {n} sequences (at most {_MOST_ENTRIES})")
-        size = lib().dsv41_kv4_reserve_workspace_bytes(n, self.slots, self.pages)
-        ws = torch.empty(size // 4, dtype=torch.int32, device=self.device)
-        table, slots, cols, refs, pages, page = self._map()
-        _launch("dsv41_kv4_reserve", self.device.index, seq.data_ptr(), begin.data_ptr(), end.data_ptr(), n,
-                self.pool.data_ptr(), self.dim, table, slots, cols, refs, pages, page, self.err.data_ptr(), ws.data_ptr(), size)
+        seq, begin, end = (self._i64("kv4.reserve", t, n) for t in (seq, begin, end))
+        size = 4 * (self.slots + 3 * self.pages + 2 * n)
+        ws = torch.empty(size // 4, dtype=_I32, device=self.device)
+        _launch("dsv41_kv4_reserve", self.index, self._at, seq.data_ptr(), begin.data_ptr(), end.data_ptr(), n,
+                ws.data_ptr(), size)
         self._done()
 
     def fork(self, src, dst, rows=None) -> None:
         """Sequence dst[i] gets the first rows[i] rows (None: all) of src[i] in place of its own, by naming their pages:
         nothing is copied before reserve makes a shared page writable.  A destination may be named once and may not be a
         source of the same call."""
-        n, (src, dst, rows) = self._i64("kv4.fork", None, src, dst, rows)
-        _launch("dsv41_kv4_fork", self.device.index, src.data_ptr(), dst.data_ptr(), ptr(rows), n, *self._map(),
-                self.err.data_ptr())
+        n = len(src)
+        src, dst = self._i64("kv4.fork", src, n), self._i64("kv4.fork", dst, n)
+        rows = None if rows is None else self._i64("kv4.fork", rows, n)
+        _launch("dsv41_kv4_fork", self.index, self._at, src.data_ptr(), dst.data_ptr(), ptr(rows), n)
         self._done()
 
     def release(self, seq, rows=None) -> None:
         """The pages behind the first rows[i] rows (None: 0, all of them) of sequence seq[i] are given up."""
-        n, (seq, rows) = self._i64("kv4.release", None, seq, rows)
-        _launch("dsv41_kv4_release", self.device.index, seq.data_ptr(), ptr(rows), n, *self._map(), self.err.data_ptr())
+        n = len(seq)
+        seq = self._i64("kv4.release", seq, n)
+        rows = None if rows is None else self._i64("kv4.release", rows, n)
+        _launch("dsv41_kv4_release", self.index, self._at, seq.data_ptr(), ptr(rows), n)
         self._done()
 
     def compact(self) -> torch.Tensor:
         """The live pages moved to the front of the pool (those that stand there stay); table and refs follow.  Returns how
         many they are, int32 [1] on the GPU: the pool's pages behind them are free."""
-        size = lib().dsv41_kv4_compact_workspace_bytes(self.pages)
-        ws = torch.empty(size // 4, dtype=torch.int32, device=self.device)
-        live = torch.empty(1, dtype=torch.int32, device=self.device)
-        table, slots, cols, refs, pages, page = self._map()
-        _launch("dsv41_kv4_compact", self.device.index, self.pool.data_ptr(), self.dim, table, slots, cols, refs, pages, page,
-                live.data_ptr(), ws.data_ptr(), size)
+        size = 4 * (2 + 3 * self.pages)
+        ws = torch.empty(size // 4, dtype=_I32, device=self.device)
+        live = torch.empty(1, dtype=_I32, device=self.device)
+        _launch("dsv41_kv4_compact", self.index, self._at, live.data_ptr(), ws.data_ptr(), size)
         return live
 
     def copy_pages(self, other: "PagedKV4", src, dst) -> None:
@@ -175,17 +196,18 @@ class PagedKV4:
         it."""
         if other.dim != self.dim or other.page != self.page:
             raise RuntimeError(f"kv4.copy_pages: pages of {other.page} rows of {other.dim} into {self.page} of {self.dim}")
-        index = _index(self.pool, other.pool)
-        a, b = self.pool.data_ptr(), other.pool.data_ptr()
-        if a < b + other.pool.numel() and b < a + self.pool.numel():
+        if other.index != self.index:
+            raise RuntimeError(f"kv4.copy_pages: pools on {other.device}, {self.device}")
+        a, b = self._c.pool, other._c.pool
+        if a < b + other.pages * other.pool.stride(0) and b < a + self.pages * self.pool.stride(0):
             raise RuntimeError("kv4.copy_pages: the pools are one memory (fork and reserve share and copy within a pool)")
-        n, (src, dst) = self._i64("kv4.copy_pages", None, src, dst)
+        n = len(src)
         if n >= 1 << 31:
             raise RuntimeError(f"kv4.copy_pages: {n} pages")
-        size = lib().dsv41_kv4_copy_workspace_bytes(n, self.pages)
-        ws = torch.empty(size // 4, dtype=torch.int32, device=self.device) if size else None
-        _launch("dsv41_kv4_copy", index, b, other.pages, a, self.pages, self.page, self.dim, src.data_ptr(), dst.data_ptr(), n,
-                self.err.data_ptr(), ptr(ws), size)
+        src, dst = self._i64("kv4.copy_pages", src, n), self._i64("kv4.copy_pages", dst, n)
+        size = lib().dsv41_kv4_copy_workspace_bytes(self._at, n)
+        ws = torch.empty(size // 4, dtype=_I32, device=self.device) if size else None
+        _launch("dsv41_kv4_copy", self.index, self._at, other._at, src.data_ptr(), dst.data_ptr(), n, ptr(ws), size)
         self._done()
 
 
@@ -234,11 +256,6 @@ def _indices(name: str, idx, shape: tuple, index: int):
     return (idx, idx.shape[-1]) if idx.shape[-1] else (None, 0)
 
 
-def _workspace(rows: int, h: int, wt: int, t: int, dim: int, held: int, dev):
-    n = lib().dsv41_kv4_attn_workspace_bytes(rows, h, wt, t, dim, held)
-    return (torch.empty(n // 4, dtype=torch.float32, device=dev) if n else None), n
-
-
 def _values_of(name: str, d_v: int | None) -> None:
     if d_v not in (None, 512):
         raise RuntimeError(f"{name}: values of {d_v} columns (512)")
@@ -263,12 +280,13 @@ def sattn4(q, kv_win, cache: PagedKV4, idx, pos, attn_sink, cos, sin, rd: int, s
     cos, sin = _angles("sattn4", cos, sin, rd, index)
     kv_win = _window("sattn4", kv_win, d)
     idx, t = _indices("sattn4", idx, (b, 1), index)
-    _, (pos, seq, pmax, plim) = cache._i64("sattn4", b, pos, seq, pmax, plim)
-    out = torch.empty(b, 1, h, 512, dtype=torch.bfloat16, device=q.device)
-    win = kv_win.shape[1]
-    ws, size = _workspace(b, h, win, t, d, 0, q.device)
-    _launch("dsv41_sattn4", index, q.data_ptr(), kv_win.data_ptr(), kv_win.stride(0), kv_win.shape[0], win,
-            cache.pool.data_ptr(), cache.pages, cache.page, d, cache.table.data_ptr(), cache.slots, cache.cols, ptr(idx), t,
+    pos, seq, pmax = (cache._i64("sattn4", x, b) for x in (pos, seq, pmax))
+    plim = None if plim is None else cache._i64("sattn4", plim, b)
+    out = torch.empty(b, 1, h, 512, dtype=_BF16, device=cache.device)
+    slots, win = kv_win.shape[:2]
+    size = cache._size(b, h, win, t, 0)
+    ws = torch.empty(size // 4, dtype=torch.float32, device=cache.device) if size else None
+    _launch("dsv41_sattn4", index, cache._at, q.data_ptr(), kv_win.data_ptr(), kv_win.stride(0), slots, win, ptr(idx), t,
             pos.data_ptr(), seq.data_ptr(), pmax.data_ptr(), ptr(plim), sink.data_ptr(), ptr(cos), ptr(sin),
             cos.shape[0] if rd else 0, rd, softmax_scale, out.data_ptr(), b, h, ptr(ws), size)
     return out
@@ -294,11 +312,11 @@ def sparse_attn4(q, kv, cache: PagedKV4, attn_sink, win_idxs, topk_idxs, softmax
     idx, t = _indices("sparse_attn4", topk_idxs, (b, s), index)
     if seq is None and b > cache.slots:
         raise RuntimeError(f"sparse_attn4: {b} batch rows over {cache.slots} sequences")
-    _, (seq,) = cache._i64("sparse_attn4", b, seq)
-    out = torch.empty(b, s, h, 512, dtype=torch.bfloat16, device=q.device)
-    ws, size = _workspace(b * s, h, w, t, d, b * cache.cols * cache.page, q.device)
-    _launch("dsv41_sparse_attn4", index, q.data_ptr(), ptr(kv), kv.stride(0) if kv is not None else 0,
-            kv.shape[1] if kv is not None else 0, ptr(win_idxs), w, cache.pool.data_ptr(), cache.pages, cache.page, d,
-            cache.table.data_ptr(), cache.slots, cache.cols, ptr(idx), t, ptr(seq), sink.data_ptr(), softmax_scale,
+    seq = None if seq is None else cache._i64("sparse_attn4", seq, b)
+    out = torch.empty(b, s, h, 512, dtype=_BF16, device=cache.device)
+    size = cache._size(b * s, h, w, t, b)
+    ws = torch.empty(size // 4, dtype=torch.float32, device=cache.device) if size else None
+    _launch("dsv41_sparse_attn4", index, cache._at, q.data_ptr(), ptr(kv), kv.stride(0) if kv is not None else 0,
+            kv.shape[1] if kv is not None else 0, ptr(win_idxs), w, ptr(idx), t, ptr(seq), sink.data_ptr(), softmax_scale,
             out.data_ptr(), b, s, h, ptr(ws), size)
     return out

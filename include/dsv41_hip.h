@@ -362,76 +362,75 @@ int dsv41_gated_a8(const void* a8, const void* s8, const void* wg8, const void* 
 /* Compressed rows held as the codes of their grid (qmode 2 of dsv41_append_rows), in pages.  A row of `dim` values (512, or
  * 576 with the values in its first 512): 256 bytes of E2M1 codes, two a byte with the lower value in the lower four bits,
  * and 32 e4m3 scales, one per 16 values; for 576 then 32 bytes of codes and 4 of scales of the last 64 values and 12 zeros:
- * 288 (336) bytes.  pool: [pages, page, row bytes], 16-byte aligned, page a power of two from 16 to 256.  table int32
- * [slots, cols]: the page of rows j * page .. of a sequence, -1 none (entries outside the pool count as none).  refs int32
- * [pages]: the table's entries that name a page; 0: free.  err: one int32, whose bits the calls set and the caller polls
- * and clears: 1 too few free pages, 2 an entry was left out (an index out of range, or one named twice), 4 an appended
- * row was dropped (no page of the sequence's own there, or no rope angle).  Calls on one cache must be stream-ordered. */
+ * 288 (336) bytes.  Calls on one cache must be stream-ordered. */
+typedef struct {
+  void* pool;  /* [pages, page, row bytes], 16-byte aligned; pages * page < 2^31 */
+  int* table;  /* [slots, cols]: the page of rows j * page .. of a sequence, -1 none (entries outside the pool: none) */
+  int* refs;   /* [pages]: the table's entries that name a page; 0: free */
+  int* err;    /* one word whose bits the calls set and the caller polls and clears: 1 too few free pages, 2 an entry was
+                * left out (an index out of range, or one named twice), 4 an appended row was dropped (no page of the
+                * sequence's own there, or no rope angle) */
+  int pages, page; /* rows a page: a power of two from 16 to 256 */
+  int slots, cols;
+  int dim;
+} dsv41_kv4;
 
 /* Rows into the cache: y = x with its last rd columns rotated by the angle of position row * ratio (products exact, one
  * rounding to bf16: the compressed row of cache.append_compressed_decode / write_compress_kv, dsv41/decode.py:157-164),
  * then per 16 values s = e4m3(max(amax, 6 * 2^-9) / 6), codes E2M1(clamp(y / s, -6, 6)) into row row[r] of sequence
  * seq[r] (row < 0: none).  A group with an infinity or a NaN reads back as NaN.  x bf16, rows x_rstride apart, 16-byte
  * aligned, x_rstride % 8 == 0; cos_t / sin_t [n_pos, rd / 2].  Rows of one call must differ. */
-int dsv41_kv4_append(const void* x, long x_rstride, const long* seq, const long* row, long n, int ratio,
-                     const float* cos_t, const float* sin_t, long n_pos, int rd, void* pool, int pages, int page,
-                     int dim, const int* table, int slots, int cols, const int* refs, int* err, void* stream);
+int dsv41_kv4_append(const dsv41_kv4* c, const void* x, long x_rstride, const long* seq, const long* row, long n,
+                     int ratio, const float* cos_t, const float* sin_t, long n_pos, int rd, void* stream);
 
 /* The values of rows as bf16 [n, dim] (exact), zeros where there is no row. */
-int dsv41_kv4_read(const void* pool, int pages, int page, int dim, const int* table, int slots, int cols,
-                   const long* seq, const long* row, long n, void* out, void* stream);
+int dsv41_kv4_read(const dsv41_kv4* c, const long* seq, const long* row, long n, void* out, void* stream);
 
 /* Sequence dst[i] names the pages of the first rows[i] rows (null: all) of src[i] instead of its own, which are given up.
  * Pages are shared until dsv41_kv4_reserve makes one writable.  A pair whose dst is any pair's src or an earlier pair's
  * dst is left out. */
-int dsv41_kv4_fork(const long* src, const long* dst, const long* rows, int n, int* table, int slots, int cols, int* refs,
-                   int pages, int page, int* err, void* stream);
+int dsv41_kv4_fork(const dsv41_kv4* c, const long* src, const long* dst, const long* rows, int n, void* stream);
 
 /* The pages behind the first rows[i] rows (null: 0) of sequence seq[i] are given up. */
-int dsv41_kv4_release(const long* seq, const long* rows, int n, int* table, int slots, int cols, int* refs, int pages,
-                      int page, int* err, void* stream);
+int dsv41_kv4_release(const dsv41_kv4* c, const long* seq, const long* rows, int n, void* stream);
 
 /* Rows begin[i] .. end[i] - 1 of sequence seq[i] made writable: a page of its own wherever it has none or shares one (by
  * the counts at the call), the lowest free pages in the order of the arguments; what a replaced first page held before
  * begin[i] is copied.  Up to 4096 entries a call, distinct sequences (a repeated one is left out). */
-long dsv41_kv4_reserve_workspace_bytes(int n, int slots, int pages);
-int dsv41_kv4_reserve(const long* seq, const long* begin, const long* end, int n, void* pool, int dim, int* table,
-                      int slots, int cols, int* refs, int pages, int page, int* err, void* ws, long ws_bytes,
-                      void* stream);
+long dsv41_kv4_reserve_workspace_bytes(const dsv41_kv4* c, int n);
+int dsv41_kv4_reserve(const dsv41_kv4* c, const long* seq, const long* begin, const long* end, int n, void* ws,
+                      long ws_bytes, void* stream);
 
 /* The live pages (refs > 0), L of them, moved to the front: those from L on go, in order, to the free ones before L; table
  * and refs follow.  live[0] = L. */
-long dsv41_kv4_compact_workspace_bytes(int pages);
-int dsv41_kv4_compact(void* pool, int dim, int* table, int slots, int cols, int* refs, int pages, int page, int* live,
-                      void* ws, long ws_bytes, void* stream);
+long dsv41_kv4_compact_workspace_bytes(const dsv41_kv4* c);
+int dsv41_kv4_compact(const dsv41_kv4* c, int* live, void* ws, long ws_bytes, void* stream);
 
-/* Page dst[i] of dst_pool := page src[i] of src_pool (another pool; -1: none).  Where a destination is named twice the
- * last pair has it. */
-long dsv41_kv4_copy_workspace_bytes(int n, int dst_pages);
-int dsv41_kv4_copy(const void* src_pool, int src_pages, void* dst_pool, int dst_pages, int page, int dim, const long* src,
-                   const long* dst, int n, int* err, void* ws, long ws_bytes, void* stream);
+/* Page dst[i] of c's pool := page src[i] of other's (another pool, pages of one size; -1: none).  Where a destination is
+ * named twice the last pair has it.  No table and no count changes. */
+long dsv41_kv4_copy_workspace_bytes(const dsv41_kv4* c, int n);
+int dsv41_kv4_copy(const dsv41_kv4* c, const dsv41_kv4* other, const long* src, const long* dst, int n, void* ws,
+                   long ws_bytes, void* stream);
 
-/* Workspace of the two attention calls: R query rows, H heads, wt window (or ring) rows and t cache rows a query; rows = b *
- * cols * page of dsv41_sparse_attn4, 0 for dsv41_sattn4.  Needs no zeroing and no life beyond the call; 16-byte aligned. */
-long dsv41_kv4_attn_workspace_bytes(int R, int H, int wt, int t, int dim, long rows);
+/* Workspace of the two attention calls: R query rows, H heads, wt window (or ring) rows and t cache rows a query, b batch
+ * rows of dsv41_sparse_attn4 (0 for dsv41_sattn4).  Needs no zeroing and no life beyond the call; 16-byte aligned. */
+long dsv41_kv4_attn_workspace_bytes(const dsv41_kv4* c, int R, int H, int wt, int t, int b);
 
 /* dsv41_sattn2 over a 4-bit cache: query row b at position pos[b] of sequence seq[b] over the ring kv_win[seq] (bf16
  * [win_slots, win, dim], slot stride win_sstride) and the cache rows idx[b, :] (-1, or without a page: none).  o = sum_j
  * p_j v_j / (sum_j p_j + exp(sink)), the values the rows' first 512 columns; fp32 sums, the inverse rope on the last rd
  * (a multiple of 4) output columns, one rounding.  A row that sees no key is zeros.  out bf16 [B, h, 512]. */
-int dsv41_sattn4(const void* q, const void* kv_win, long win_sstride, int win_slots, int win, const void* pool, int pages,
-                 int page, int dim, const int* table, int slots, int cols, const int* idx, int t, const long* pos,
-                 const long* seq, const long* pmax, const long* plim, const float* sink, const float* cos_t,
-                 const float* sin_t, long n_pos, int rd, float scale, void* out, int B, int h, void* ws, long ws_bytes,
-                 void* stream);
+int dsv41_sattn4(const dsv41_kv4* c, const void* q, const void* kv_win, long win_sstride, int win_slots, int win,
+                 const int* idx, int t, const long* pos, const long* seq, const long* pmax, const long* plim,
+                 const float* sink, const float* cos_t, const float* sin_t, long n_pos, int rd, float scale, void* out,
+                 int B, int h, void* ws, long ws_bytes, void* stream);
 
 /* dsv41_sparse_attn_kv2 over a 4-bit cache: q bf16 [b, s, h, dim]; window rows kv bf16 [b, n_kv, dim] (batch stride
  * kv_bstride) by widx [b, s, wt] and cache rows of sequence seq[b] (null: b) by idx [b, s, t], -1 none; out bf16
  * [b, s, h, 512], without a rotation. */
-int dsv41_sparse_attn4(const void* q, const void* kv, long kv_bstride, int n_kv, const int* widx, int wt,
-                       const void* pool, int pages, int page, int dim, const int* table, int slots, int cols,
-                       const int* idx, int t, const long* seq, const float* sink, float scale, void* out, int b, int s,
-                       int h, void* ws, long ws_bytes, void* stream);
+int dsv41_sparse_attn4(const dsv41_kv4* c, const void* q, const void* kv, long kv_bstride, int n_kv, const int* widx,
+                       int wt, const int* idx, int t, const long* seq, const float* sink, float scale, void* out, int b,
+                       int s, int h, void* ws, long ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------ numerics */
 

@@ -1,4 +1,6 @@
 """The paged 4-bit cache on the CPU: what its calls refuse, workspace sizes, and the tests' own 64-bit forms."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -35,7 +37,7 @@ def _cache(dim=576):
     """A cache's handle without a GPU behind it, to reach the checks of arguments (no call below gets past them)."""
     c = kv4.PagedKV4.__new__(kv4.PagedKV4)
     c.pool, c.table, c.refs = _tensors(dim=dim)
-    c.dim, c.pages, c.page, c.slots, c.cols, c.device = dim, 4, 16, 2, 3, torch.device("cpu")
+    c.dim, c.pages, c.page, c.slots, c.cols, c.device, c.index = dim, 4, 16, 2, 3, torch.device("cpu"), -1
     return c
 
 
@@ -48,7 +50,7 @@ def test_calls_refuse():
         with pytest.raises(RuntimeError):
             c.append(*bad)
     with pytest.raises(RuntimeError, match="beside"):
-        c._i64("x", 2, i, torch.zeros(3))
+        c._i64("x", torch.zeros(3), 2)
     with pytest.raises(RuntimeError, match="at most"):
         c.reserve(torch.zeros(4097), torch.zeros(4097), torch.zeros(4097))
     with pytest.raises(RuntimeError, match="pages of"):
@@ -79,49 +81,70 @@ def test_indices_and_windows_refuse():
         kv4._angles("x", torch.zeros(4, 31), torch.zeros(4, 31), 64, -1)
 
 
+def _struct(**k):
+    P = 1 << 20
+    return kv4._Cache(**{**dict(pool=P, table=P, refs=P, err=P, pages=4, page=16, slots=2, cols=3, dim=512), **k})
+
+
+BAD_CACHES = [dict(pool=None), dict(pool=(1 << 20) + 8), dict(table=None), dict(refs=None), dict(err=None), dict(slots=0),
+              dict(cols=0), dict(pages=0), dict(page=48), dict(page=8), dict(page=512), dict(dim=128), dict(dim=640),
+              dict(slots=1 << 20, cols=1 << 12), dict(pages=1 << 27)]
+
+
 def test_entry_points_refuse():
     """Arguments that the C entry points turn away before any launch (addresses are never followed there)."""
     L, P, inv = _lib.lib(), 1 << 20, 1
-    ok = dict(table=P, slots=2, cols=3, refs=P, pages=4, page=16, err=P)
-
-    def pages(**k):
-        d = {**ok, **k}
-        return d["table"], d["slots"], d["cols"], d["refs"], d["pages"], d["page"], d["err"]
-    for k in (dict(table=None), dict(slots=0), dict(cols=0), dict(refs=None), dict(pages=0), dict(page=48), dict(page=8),
-              dict(page=512), dict(err=None), dict(slots=1 << 20, cols=1 << 12), dict(cols=256 * 65535 + 1, slots=1)):
-        assert L.dsv41_kv4_fork(P, P, None, 1, *pages(**k), None) == inv, k
-        assert L.dsv41_kv4_release(P, None, 1, *pages(**k), None) == inv, k
-    assert L.dsv41_kv4_fork(None, P, None, 1, *pages(), None) == inv
-    assert L.dsv41_kv4_fork(P, P, None, -1, *pages(), None) == inv
-    assert L.dsv41_kv4_fork(None, None, None, 0, *pages(), None) == 0
-    assert L.dsv41_kv4_release(None, None, 1, *pages(), None) == inv
-    need = L.dsv41_kv4_reserve_workspace_bytes(5, 2, 4)
+    c = ctypes.byref(_struct())
+    big = 1 << 40
+    for k in BAD_CACHES:
+        x = ctypes.byref(_struct(**k))
+        assert L.dsv41_kv4_fork(x, P, P, None, 1, None) == inv, k
+        assert L.dsv41_kv4_release(x, P, None, 1, None) == inv, k
+        assert L.dsv41_kv4_reserve(x, P, P, P, 1, P, big, None) == inv, k
+        assert L.dsv41_kv4_compact(x, P, P, big, None) == inv, k
+        assert L.dsv41_kv4_copy(x, ctypes.byref(_struct(pool=1 << 40)), P, P, 1, None, 0, None) == inv, k
+        assert L.dsv41_kv4_copy(ctypes.byref(_struct(pool=1 << 40)), x, P, P, 1, None, 0, None) == inv, k
+        assert L.dsv41_kv4_append(x, P, 1024, P, P, 1, 4, P, P, 9, 64, None) == inv, k
+        assert L.dsv41_kv4_read(x, P, P, 1, P, None) == inv, k
+        assert L.dsv41_sattn4(x, P, P, 128 * 512, 2, 128, P, 10, P, P, P, None, P, P, P, 100, 64, 1.0, P, 1, 16, None, 0, None) == inv
+        assert L.dsv41_sparse_attn4(x, P, P, 128 * 512, 128, P, 128, P, 10, None, P, 1.0, P, 1, 1, 16, None, 0, None) == inv
+    assert L.dsv41_kv4_fork(None, P, P, None, 1, None) == inv
+    wide = ctypes.byref(_struct(slots=1, cols=256 * 65535 + 1))
+    assert L.dsv41_kv4_fork(wide, P, P, None, 1, None) == inv and L.dsv41_kv4_release(wide, P, None, 1, None) == inv
+    assert L.dsv41_kv4_fork(c, None, P, None, 1, None) == inv and L.dsv41_kv4_fork(c, P, None, None, 1, None) == inv
+    assert L.dsv41_kv4_fork(c, P, P, None, -1, None) == inv and L.dsv41_kv4_fork(c, None, None, None, 0, None) == 0
+    assert L.dsv41_kv4_release(c, None, None, 1, None) == inv
+    need = L.dsv41_kv4_reserve_workspace_bytes(c, 5)
     assert need == 4 * (2 + 12 + 10)
-    for n, pool, dim, ws, size in [(4097, P, 512, P, 1 << 30), (1, None, 512, P, need), (1, P + 8, 512, P, need),
-                                   (1, P, 128, P, need), (5, P, 512, None, need), (5, P, 512, P, need - 1)]:
-        assert L.dsv41_kv4_reserve(P, P, P, n, pool, dim, *pages(), ws, size, None) == inv
-    assert L.dsv41_kv4_compact(P, 512, P, 2, 3, P, 4, 16, None, P, 1 << 20, None) == inv
-    assert L.dsv41_kv4_compact(P, 512, P, 2, 3, P, 4, 16, P, P, L.dsv41_kv4_compact_workspace_bytes(4) - 1, None) == inv
-    assert L.dsv41_kv4_copy_workspace_bytes(10, 100) == 0 and L.dsv41_kv4_copy_workspace_bytes(5000, 100) == 400
-    assert L.dsv41_kv4_copy(P, 4, P + 512, 4, 16, 512, P, P, 1, P, None, 0, None) == inv  # (one memory)
-    assert L.dsv41_kv4_copy(P, 4, 1 << 30, 4, 16, 512, P, P, 5000, P, None, 0, None) == inv
-    for x, stride, ratio, rd, dim in [(None, 512, 4, 64, 512), (P + 2, 512, 4, 64, 512), (P, 500, 4, 64, 512),
-                                      (P, 516, 4, 64, 512), (P, 512, 0, 64, 512), (P, 512, 4, 65, 512), (P, 640, 4, 64, 640)]:
-        assert L.dsv41_kv4_append(x, stride, P, P, 1, ratio, P, P, 9, rd, P, 4, 16, dim, P, 2, 3, P, P, None) == inv
-    assert L.dsv41_kv4_read(P, 4, 16, 512, P, 2, 3, P, P, 1, P + 2, None) == inv
-    args = [P, P, 128 * 512, 2, 128, P, 4, 16, 512, P, 2, 3, P, 10, P, P, P, None, P, P, P, 100, 64, 1.0, P, 1, 16, None, 0, None]
-    for at, v in [(0, None), (0, P + 2), (1, None), (4, 0), (5, None), (8, 256), (7, 20), (14, None), (15, None), (16, None),
-                  (18, None), (19, None), (22, 62), (22, 516), (24, None), (26, 0), (13, -1), (2, 12)]:
+    for n, ws, size in [(4097, P, big), (-1, P, big), (5, None, need), (5, P + 2, need), (5, P, need - 1)]:
+        assert L.dsv41_kv4_reserve(c, P, P, P, n, ws, size, None) == inv
+    need = L.dsv41_kv4_compact_workspace_bytes(c)
+    assert need == 4 * 14
+    assert L.dsv41_kv4_compact(c, None, P, big, None) == inv and L.dsv41_kv4_compact(c, P, P, need - 1, None) == inv
+    assert L.dsv41_kv4_copy_workspace_bytes(c, 10) == 0 and L.dsv41_kv4_copy_workspace_bytes(c, 5000) == 16
+    assert L.dsv41_kv4_copy(c, ctypes.byref(_struct(pool=P + 512)), P, P, 1, None, 0, None) == inv  # (one memory)
+    far = dict(pool=1 << 40)
+    assert L.dsv41_kv4_copy(c, ctypes.byref(_struct(**far)), P, P, 5000, None, 0, None) == inv
+    assert L.dsv41_kv4_copy(c, ctypes.byref(_struct(**far, page=32)), P, P, 1, None, 0, None) == inv
+    assert L.dsv41_kv4_copy(c, ctypes.byref(_struct(**far, dim=576)), P, P, 1, None, 0, None) == inv
+    for x, stride, ratio, rd in [(None, 512, 4, 64), (P + 2, 512, 4, 64), (P, 500, 4, 64), (P, 516, 4, 64), (P, 512, 0, 64),
+                                 (P, 512, 4, 65), (P, 512, 4, 514), (P, 512, 4, -2)]:
+        assert L.dsv41_kv4_append(c, x, stride, P, P, 1, ratio, P, P, 9, rd, None) == inv
+    assert L.dsv41_kv4_append(c, P, 512, P, P, 1, 4, None, P, 9, 64, None) == inv
+    assert L.dsv41_kv4_read(c, P, P, 1, P + 2, None) == inv
+    args = [c, P, P, 128 * 512, 2, 128, P, 10, P, P, P, None, P, P, P, 100, 64, 1.0, P, 1, 16, None, 0, None]
+    for at, v in [(1, None), (1, P + 2), (2, None), (3, 12), (5, 0), (6, None), (7, -1), (8, None), (9, None), (10, None),
+                  (12, None), (13, None), (16, 62), (16, 516), (16, -4), (18, None), (19, -1), (20, 0)]:
         bad = list(args)
         bad[at] = v
         assert L.dsv41_sattn4(*bad) == inv, (at, v)
     # a workspace too small for the splits of one row over many keys
     bad = list(args)
-    bad[13] = 4096
-    assert L.dsv41_kv4_attn_workspace_bytes(1, 16, 128, 4096, 512, 0) > 0 and L.dsv41_sattn4(*bad) == inv
-    args = [P, P, 128 * 512, 128, P, 128, P, 4, 16, 512, P, 2, 3, P, 10, None, P, 1.0, P, 1, 1, 16, None, 0, None]
-    for at, v in [(0, None), (1, None), (4, None), (5, -1), (3, -1), (6, None), (13, None), (14, -1), (16, None), (18, None),
-                  (21, 0)]:
+    bad[7] = 4096
+    assert L.dsv41_kv4_attn_workspace_bytes(c, 1, 16, 128, 4096, 0) > 0 and L.dsv41_sattn4(*bad) == inv
+    args = [c, P, P, 128 * 512, 128, P, 128, P, 10, None, P, 1.0, P, 1, 1, 16, None, 0, None]
+    for at, v in [(1, None), (2, None), (4, -1), (5, None), (6, -1), (7, None), (8, -1), (10, None), (12, None), (13, -1),
+                  (14, -1), (15, 0)]:
         bad = list(args)
         bad[at] = v
         assert L.dsv41_sparse_attn4(*bad) == inv, (at, v)
