@@ -24,9 +24,12 @@ struct RowsArgs {
   uint16_t* out;
 };
 
-// The grid's scale of 16 values and the codes of this lane's eight.  Quotients are correctly rounded: bf16 values over
-// a 4-bit significand often lie on a border of the grid, which then goes to the even code.  The scale saturates at 448,
-// the codes at 6; a group with an infinity or a NaN reads back as NaN (scale 0x7f).
+// The grid's scale of 16 values and the codes of this lane's eight.  bf16 values over a 4-bit significand often lie on a
+// border of the grid, where the even code is right, so a quotient may not be off there.  Quotients are products with a
+// reciprocal (two fp32 roundings) rounded to bf16: one that is a border comes out as the border, which has 3 bits (the
+// scale's 5); any other is at least 2^-8 of itself away from one -- two integers of at most 8 bits that differ -- and bf16
+// moves it by 2^-9.  The conversions round to even and saturate: the scale at 448, the codes at 6.  A group with an
+// infinity or a NaN reads back as NaN (scale 0x7f).
 DSV41_DEV uint32_t kv4_encode(const float* v, uint8_t* scale) {
   float a = 0.0f;
   bool bad = false;
@@ -35,22 +38,23 @@ DSV41_DEV uint32_t kv4_encode(const float* v, uint8_t* scale) {
     a = fmaxf(a, fabsf(v[i]));
     bad |= !(fabsf(v[i]) < __builtin_inff());
   }
-  a = fmaxf(a, bad ? __builtin_inff() : 0.0f);
-  a = group_max(a, 2);
-  if (!(a < __builtin_inff())) {
-    *scale = 0x7f;
-    return 0;
-  }
-  const float s = round_e4m3(fminf(__fdiv_rn(fmaxf(a, 6.0f * 0.001953125f), 6.0f), 448.0f));
-  *scale = (uint8_t)e4m3_bits(s);
+  a = group_max(bad ? __builtin_inff() : a, 2);
+  const float t = round_bf16(fminf(fmaxf(a, 6.0f * 0.001953125f) * (1.0f / 6.0f), 448.0f));
+  const int byte = __builtin_amdgcn_cvt_pk_fp8_f32(t, t, 0, false);
+  const float inv = __builtin_amdgcn_rcpf(__builtin_amdgcn_cvt_f32_fp8(byte, 0));
+  const bool nan = !(a < __builtin_inff());
+  *scale = nan ? 0x7f : (uint8_t)byte;
+  typedef __bf16 b16x2_t __attribute__((ext_vector_type(2)));
   uint32_t codes = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float w = fminf(__fdiv_rn(fabsf(v[i]), s), 6.0f);  // E2M1 by magnitude: 0 .5 1 1.5 | 2 3 | 4 6
-    const float c = w < 2.0f ? rintf(w * 2.0f) : (w < 4.0f ? rintf(w) + 2.0f : rintf(w * 0.5f) + 4.0f);
-    codes |= ((uint32_t)c | (v[i] < 0.0f ? 8u : 0u)) << (4 * i);
-  }
-  return codes;
+#define DSV41_PAIR(i)                                                                                                  \
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(                                                                   \
+      codes, b16x2_t{(__bf16)fmaf(v[2 * i], inv, 0.0f), (__bf16)fmaf(v[2 * i + 1], inv, 0.0f)}, 1.0f, i)
+  DSV41_PAIR(0);  // (plus zero: -0 has the code of 0)
+  DSV41_PAIR(1);
+  DSV41_PAIR(2);
+  DSV41_PAIR(3);
+#undef DSV41_PAIR
+  return nan ? 0 : codes;
 }
 
 // Eight values of a row from element e on: bf16, the last rd columns rotated.  The rotation's products are exact in 64
