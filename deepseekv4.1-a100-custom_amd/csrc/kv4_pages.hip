@@ -9,7 +9,8 @@
 namespace {
 
 constexpr int kPlanThreads = 1024;
-constexpr int kPer = 8;              // counts a thread looks at in one round
+constexpr int kPer = 8;              // counts a thread looks at in one round of reserve
+constexpr int kPlanPages = 16;       // and of compact
 constexpr int kMostEntries = 4096;   // sequences of one reserve call
 
 struct PagesArgs {
@@ -209,47 +210,52 @@ __global__ void __launch_bounds__(256) reserve_copy_kernel(const PagesArgs a) {
 // One workgroup: L live pages; the live ones of L and above go, in order, to the free ones below L.  Sources and
 // destinations do not meet, so the moves need no order.
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagesArgs a) {
-  __shared__ int tmp[kPlanThreads / 64];
+  __shared__ int2 tmp[2][kPlanThreads / 64];
   const int t = threadIdx.x;
   int* const from = a.ws + 2;
   int* const to = from + a.pages;
   int* const where = to + a.pages;
-  int live = 0;
-  for (int p0 = 0; p0 < a.pages; p0 += kPlanThreads * kPer) {
+  // which of the kPlanPages pages of a round from p on are live, a bit each (refs is read 16 bytes at a time where it may)
+  const bool wide = ((uintptr_t)a.refs & 15) == 0;
+  auto bits = [&](int p) {
+    unsigned m = 0;
+    if (wide && p + kPlanPages <= a.pages) {
 #pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-      const int p = p0 + u * kPlanThreads + t;
-      live += p < a.pages && a.refs[p] > 0;
-    }
-  }
-  block_scan_dpp<kPlanThreads>(live, tmp, &live);
-  int ns = 0, nd = 0;
-  for (int p0 = 0; p0 < a.pages; p0 += kPlanThreads * kPer) {
-    const int p = p0 + t * kPer;
-    unsigned src = 0, dst = 0;
-#pragma unroll
-    for (int u = 0; u < kPer; ++u)
-      if (p + u < a.pages) {
-        const bool l = a.refs[p + u] > 0;
-        src |= l && p + u >= live ? 1u << u : 0u;
-        dst |= !l && p + u < live ? 1u << u : 0u;
+      for (int u = 0; u < kPlanPages; u += 4) {
+        const int4 r = *(const int4*)(a.refs + p + u);
+        m |= ((r.x > 0 ? 1u : 0u) | (r.y > 0 ? 2u : 0u) | (r.z > 0 ? 4u : 0u) | (r.w > 0 ? 8u : 0u)) << u;
       }
-    int ss, sd;
-    int rs = ns + block_scan_dpp<kPlanThreads>(__popc(src), tmp, &ss);
-    int rd = nd + block_scan_dpp<kPlanThreads>(__popc(dst), tmp, &sd);
-#pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-      if (src >> u & 1) from[rs++] = p + u;
-      if (dst >> u & 1) to[rd++] = p + u;
+    } else {
+      for (int u = 0; u < kPlanPages; ++u) m |= p + u < a.pages && a.refs[p + u] > 0 ? 1u << u : 0u;
     }
-    ns += ss;
-    nd += sd;
+    return m;
+  };
+  const int step = kPlanThreads * kPlanPages;
+  const unsigned first = bits(t * kPlanPages);
+  int count = __popc(first);
+  for (int p0 = step; p0 < a.pages; p0 += step) count += __popc(bits(p0 + t * kPlanPages));
+  int2 total;
+  block_scan2_dpp<kPlanThreads>(count, 0, tmp[0], &total);
+  const int live = total.x;
+  int2 base = make_int2(0, 0);
+  for (int p0 = 0; p0 < a.pages; p0 += step) {
+    const int p = p0 + t * kPlanPages;
+    const unsigned l = p0 == 0 ? first : bits(p);
+    const int n = min(max(live - p, 0), kPlanPages);  // pages of p .. that stay in front
+    const unsigned front = n == 32 ? ~0u : (1u << n) - 1, held = a.pages - p >= kPlanPages ? ~0u : p < a.pages ? (1u << (a.pages - p)) - 1 : 0u;
+    unsigned src = l & ~front, dst = ~l & front & held;
+    const int which = (p0 / step + 1) & 1;
+    const int2 r = block_scan2_dpp<kPlanThreads>(__popc(src), __popc(dst), tmp[which], &total);
+    for (int i = base.x + r.x; src; src &= src - 1) from[i++] = p + __ffs(src) - 1;
+    for (int i = base.y + r.y; dst; dst &= dst - 1) to[i++] = p + __ffs(dst) - 1;
+    base.x += total.x;
+    base.y += total.y;
   }
   __syncthreads();
-  for (int r = t; r < ns; r += kPlanThreads) where[from[r]] = to[r];
+  for (int r = t; r < base.x; r += kPlanThreads) where[from[r]] = to[r];
   if (t == 0) {
     a.ws[0] = live;
-    a.ws[1] = ns;
+    a.ws[1] = base.x;
     *a.live = live;
   }
 }
@@ -286,17 +292,17 @@ struct CopyArgs {
   int* last;  // [dst_pages] or null
 };
 
-// The last pair that names a page as its destination (of many pairs, by one workgroup; of few every workgroup looks).
-__global__ void __launch_bounds__(kPlanThreads) copy_last_kernel(const CopyArgs a) {
-  for (int i = threadIdx.x; i < a.n; i += kPlanThreads) {
-    const long d = a.to[i];
-    if (d >= 0 && d < a.dst_pages) __hip_atomic_store(a.last + d, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.n; i += kPlanThreads) {
-    const long d = a.to[i], s = a.from[i];
-    if (d >= 0 && d < a.dst_pages && s >= 0 && s < a.src_pages) atomicMax(a.last + d, i);
-  }
+// The last pair that names a page as its destination (of many pairs; of few every workgroup looks itself).
+__global__ void __launch_bounds__(256) copy_clear_kernel(const CopyArgs a) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < a.dst_pages) a.last[i] = -1;
+}
+
+__global__ void __launch_bounds__(256) copy_last_kernel(const CopyArgs a) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.n) return;
+  const long d = a.to[i], s = a.from[i];
+  if (d >= 0 && d < a.dst_pages && s >= 0 && s < a.src_pages) atomicMax(a.last + d, i);
 }
 
 __global__ void __launch_bounds__(256) copy_kernel(const CopyArgs a) {
@@ -421,7 +427,9 @@ int dsv41_kv4_copy(const dsv41_kv4* c, const dsv41_kv4* other, const long* src, 
   CopyArgs a{(const uint8_t*)other->pool, (uint8_t*)c->pool, other->pages, c->pages, n, pb, src, dst, c->err,
              n > kFewCopies ? (int*)ws : nullptr};
   if (a.last) {
-    copy_last_kernel<<<1, kPlanThreads, 0, (hipStream_t)stream>>>(a);
+    copy_clear_kernel<<<(c->pages + 255) / 256, 256, 0, (hipStream_t)stream>>>(a);
+    DSV41_CHECK_LAUNCH();
+    copy_last_kernel<<<(n + 255) / 256, 256, 0, (hipStream_t)stream>>>(a);
     DSV41_CHECK_LAUNCH();
   }
   copy_kernel<<<n, 256, 0, (hipStream_t)stream>>>(a);
