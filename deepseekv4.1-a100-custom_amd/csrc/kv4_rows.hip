@@ -6,6 +6,8 @@
 
 namespace {
 
+constexpr int kRows = 2;  // rows a wave
+
 struct RowsArgs {
   const uint16_t* x;
   long x_rstride;
@@ -31,15 +33,11 @@ struct RowsArgs {
 // moves it by 2^-9.  The conversions round to even and saturate: the scale at 448, the codes at 6.  A group with an
 // infinity or a NaN reads back as NaN (scale 0x7f).
 DSV41_DEV uint32_t kv4_encode(const float* v, uint8_t* scale) {
-  float a = 0.0f;
-  bool bad = false;
+  uint32_t top = 0;  // the largest magnitude's bits: a NaN's are above an infinity's
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    a = fmaxf(a, fabsf(v[i]));
-    bad |= !(fabsf(v[i]) < __builtin_inff());
-  }
-  a = group_max(bad ? __builtin_inff() : a, 2);
-  const float t = round_bf16(fminf(fmaxf(a, 6.0f * 0.001953125f) * (1.0f / 6.0f), 448.0f));
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  const float a = group_max(__uint_as_float(min(top, 0x7f800000u)), 2);
+  const float t = (float)(__bf16)fminf(fmaxf(a, 6.0f * 0.001953125f) * (1.0f / 6.0f), 448.0f);
   const int byte = __builtin_amdgcn_cvt_pk_fp8_f32(t, t, 0, false);
   const float inv = __builtin_amdgcn_rcpf(__builtin_amdgcn_cvt_f32_fp8(byte, 0));
   const bool nan = !(a < __builtin_inff());
@@ -65,67 +63,116 @@ DSV41_DEV void kv4_load(const uint4 raw, int e, int dim, const RowsArgs& a, long
   for (int i = 0; i < 4; ++i) {
     v[2 * i] = __uint_as_float(w[i] << 16);
     v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    const int at = e + 2 * i - (dim - a.rd);
-    if (at >= 0) {
-      const long j = pos * (a.rd / 2) + (at >> 1);
-      const double c = a.cos_t[j], s = a.sin_t[j], p = v[2 * i], q = v[2 * i + 1];
-      v[2 * i] = round_bf16((float)(p * c - q * s));
-      v[2 * i + 1] = round_bf16((float)(p * s + q * c));
-    }
+  }
+  const int from = dim - a.rd;
+  if (e + 8 <= from) return;
+  const float* const ct = a.cos_t + pos * (a.rd / 2);
+  const float* const st = a.sin_t + pos * (a.rd / 2);
+  float co[4], si[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = max(e + 2 * i - from, 0) >> 1;
+    co[i] = ct[j];
+    si[i] = st[j];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const double c = co[i], s = si[i], p = v[2 * i], q = v[2 * i + 1];
+    const float y = (float)(p * c - q * s), z = (float)(p * s + q * c);
+    uint32_t w2;
+    asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(w2) : "v"(y), "v"(z));
+    const uint32_t y2 = e + 2 * i < from ? w[i] : w2;
+    v[2 * i] = __uint_as_float(y2 << 16);
+    v[2 * i + 1] = __uint_as_float(y2 & 0xffff0000u);
   }
 }
 
 template <int DIM>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const RowsArgs a) {
-  const long r = blockIdx.x * 4L + (threadIdx.x >> 6);
-  if (r >= a.n) return;
   const int lane = threadIdx.x & 63;
-  const long seq = a.seq[r], row = a.row[r];
-  if (row < 0) return;
-  const uint16_t* x = a.x + r * a.x_rstride;
-  const uint4 raw = *(const uint4*)(x + 8 * lane);
-  const uint4 raw2 = DIM == 576 ? *(const uint4*)(x + 512 + 8 * (lane & 7)) : make_uint4(0, 0, 0, 0);
-  const int p = kv4_page(a.map, seq, row);
-  const long pos = row * a.ratio;
-  if (p < 0 || a.refs[p] > 1 || (a.rd > 0 && pos >= a.n_pos)) {
-    if (lane == 0) atomicOr(a.err, seq < 0 || seq >= a.map.slots ? kKv4Ignored : kKv4Dropped);
-    return;
+  const long r0 = (blockIdx.x * 4L + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kRows;
+  const uint16_t* const x = a.x + r0 * a.x_rstride;
+  const int n = (int)min((long)kRows, a.n - r0);
+  if (n <= 0) return;
+  uint4 raw[kRows], tail;
+  long pos[kRows];
+  uint8_t* dst[kRows];
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) raw[u] = *(const uint4*)(x + min(u, n - 1) * a.x_rstride + 8 * lane);
+  if (DIM == 576) tail = *(const uint4*)(x + min((lane >> 3) % kRows, n - 1) * a.x_rstride + 512 + 8 * (lane & 7));
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const long seq = a.seq[r0 + min(u, n - 1)], row = a.row[r0 + min(u, n - 1)];
+    const int p = kv4_page(a.map, seq, row);
+    pos[u] = row * a.ratio;
+    dst[u] = nullptr;
+    if (u >= n || row < 0) continue;
+    if (p < 0 || a.refs[p] > 1 || (a.rd > 0 && pos[u] >= a.n_pos)) {
+      if (lane == 0) atomicOr(a.err, seq < 0 || seq >= a.map.slots ? kKv4Ignored : kKv4Dropped);
+    } else {
+      dst[u] = a.pool + kv4_offset(a.map, p, row, kv4_row_bytes(DIM));
+    }
   }
-  uint8_t* dst = a.pool + kv4_offset(a.map, p, row, kv4_row_bytes(DIM));
   float v[8];
   uint8_t scale;
-  kv4_load(raw, 8 * lane, DIM, a, pos, v);
-  const uint32_t codes = kv4_encode(v, &scale);
-  ((uint32_t*)dst)[lane] = codes;
-  if ((lane & 1) == 0) dst[256 + (lane >> 1)] = scale;
-  if (DIM == 576) {
-    kv4_load(raw2, 512 + 8 * (lane & 7), DIM, a, pos, v);
-    const uint32_t tail = kv4_encode(v, &scale);
-    if (lane < 8) {
-      ((uint32_t*)dst)[72 + lane] = tail;
-      if ((lane & 1) == 0) dst[320 + (lane >> 1)] = scale;
-    } else if (lane < 11) {
-      ((uint32_t*)dst)[73 + lane] = 0;
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    if (!dst[u]) continue;
+    kv4_load(raw[u], 8 * lane, DIM, a, pos[u], v);
+    ((uint32_t*)dst[u])[lane] = kv4_encode(v, &scale);
+    if ((lane & 1) == 0) dst[u][256 + (lane >> 1)] = scale;
+  }
+  if (DIM == 576) {  // the last columns of all the rows at once, eight lanes each
+    long at = pos[0];
+    uint8_t* to = dst[0];
+#pragma unroll
+    for (int u = 1; u < kRows; ++u) {
+      at = (lane >> 3) == u ? pos[u] : at;
+      to = (lane >> 3) == u ? dst[u] : to;
     }
+    if (lane >= 8 * kRows || !to) return;
+    const int l = lane & 7;
+    kv4_load(tail, 512 + 8 * l, DIM, a, at, v);
+    ((uint32_t*)to)[72 + l] = kv4_encode(v, &scale);
+    if ((l & 1) == 0) to[320 + (l >> 1)] = scale;
+    if (l < 3) ((uint32_t*)to)[81 + l] = 0;
   }
 }
 
 template <int DIM>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const RowsArgs a) {
-  const long r = blockIdx.x * 4L + (threadIdx.x >> 6);
-  if (r >= a.n) return;
   const int lane = threadIdx.x & 63;
-  const long row = a.row[r];
-  const int p = kv4_page(a.map, a.seq[r], row);
-  uint16_t* out = a.out + r * DIM;
-  uint4 v = make_uint4(0, 0, 0, 0), tail = v;
-  if (p >= 0) {
-    const uint8_t* src = a.pool + kv4_offset(a.map, p, row, kv4_row_bytes(DIM));
-    v = kv4_bf16(((const uint32_t*)src)[lane], src[256 + (lane >> 1)]);
-    if (DIM == 576) tail = kv4_bf16(((const uint32_t*)src)[72 + (lane & 7)], src[320 + ((lane & 7) >> 1)]);
+  const long r0 = (blockIdx.x * 4L + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kRows;
+  const int n = (int)min((long)kRows, a.n - r0);
+  if (n <= 0) return;
+  const uint8_t* src[kRows];
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const long row = a.row[r0 + min(u, n - 1)];
+    const int p = kv4_page(a.map, a.seq[r0 + min(u, n - 1)], row);
+    src[u] = p >= 0 ? a.pool + kv4_offset(a.map, p, row, kv4_row_bytes(DIM)) : nullptr;
   }
-  *(uint4*)(out + 8 * lane) = v;
-  if (DIM == 576 && lane < 8) *(uint4*)(out + 512 + 8 * lane) = tail;
+  uint32_t code[kRows], sc[kRows], ct = 0, st = 0;
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    code[u] = src[u] ? ((const uint32_t*)src[u])[lane] : 0;
+    sc[u] = src[u] ? src[u][256 + (lane >> 1)] : 0;
+  }
+  const int l = lane & 7;
+  if (DIM == 576) {
+    const uint8_t* from = src[0];
+#pragma unroll
+    for (int u = 1; u < kRows; ++u) from = (lane >> 3) == u ? src[u] : from;
+    if (from) {
+      ct = ((const uint32_t*)from)[72 + l];
+      st = from[320 + (l >> 1)];
+    }
+  }
+  uint16_t* const out = a.out + r0 * DIM;
+#pragma unroll
+  for (int u = 0; u < kRows; ++u)
+    if (u < n) *(uint4*)(out + u * DIM + 8 * lane) = kv4_bf16(code[u], sc[u]);
+  if (DIM == 576 && (lane >> 3) < n) *(uint4*)(out + (lane >> 3) * DIM + 512 + 8 * l) = kv4_bf16(ct, st);
 }
 
 void rows_args(RowsArgs& a, const dsv41_kv4& c, const long* seq, const long* row, long n) {
@@ -159,7 +206,7 @@ int dsv41_kv4_append(const dsv41_kv4* c, const void* x, long x_rstride, const lo
   a.sin_t = sin_t;
   a.n_pos = n_pos;
   a.rd = rd;
-  const unsigned grid = (unsigned)((n + 3) / 4);
+  const unsigned grid = (unsigned)((n + 4 * kRows - 1) / (4 * kRows));
   if (c->dim == 512)
     kv4_append_kernel<512><<<grid, 256, 0, (hipStream_t)stream>>>(a);
   else
@@ -175,7 +222,7 @@ int dsv41_kv4_read(const dsv41_kv4* c, const long* seq, const long* row, long n,
   RowsArgs a;
   rows_args(a, *c, seq, row, n);
   a.out = (uint16_t*)out;
-  const unsigned grid = (unsigned)((n + 3) / 4);
+  const unsigned grid = (unsigned)((n + 4 * kRows - 1) / (4 * kRows));
   if (c->dim == 512)
     kv4_read_kernel<512><<<grid, 256, 0, (hipStream_t)stream>>>(a);
   else
