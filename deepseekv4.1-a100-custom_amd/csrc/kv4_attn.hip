@@ -22,13 +22,16 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
   constexpr int NB = HB / 16;              // head blocks
   constexpr int TS = DQK == 576 ? 2 : 0;   // k steps of the last 64 columns
   constexpr int RB = kv4_row_bytes(DQK);
-  __shared__ __align__(16) uint8_t s_v[64 * 1024];
+  __shared__ __align__(1024) uint8_t s_v[64 * 1024];
   __shared__ __align__(16) uint8_t s_p[HB * 128];
   __shared__ __align__(16) float s_m[HB * 4];
 
-  const int b = blockIdx.x;
-  const int sp = b % a.nsplit, rh = b / a.nsplit;
-  const int hg = rh % a.groups, r = rh / a.groups;
+  // The head groups of a (row, split) read the same rows of the cache: eight workgroups apart they share an XCD's L2.
+  const int b = blockIdx.x, units = a.R * a.nsplit, full = units & ~7;
+  const int n8 = b < full * a.groups ? 8 : units - full;
+  const int in = b < full * a.groups ? b % (8 * a.groups) : b - full * a.groups;
+  const int u0 = (b < full * a.groups ? b / (8 * a.groups) * 8 : full) + in % n8;
+  const int hg = in / n8, sp = u0 % a.nsplit, r = u0 / a.nsplit;
   const int h0 = hg * HB;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l16 = lane & 15, g = lane >> 4;
@@ -36,6 +39,47 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
   const long seq = a.seq ? a.seq[slot] : slot;
   const long pos = a.pos ? a.pos[r] : 0;
   const int t0 = sp * a.chunk, t1 = min(t0 + a.chunk, a.tiles);
+
+  const int key = wave * 16 + l16;  // this lane's key of a tile
+
+  // the row of the window that this lane's key of tile u is, nullptr: none
+  auto window = [&](int u) -> const uint16_t* {
+    const int j = u * 64 + key;
+    long row = -1;
+    if (a.widx) {
+      if (j < a.wt) row = a.widx[(long)r * a.wt + j];
+      if (row >= a.win_rows) row = -1;
+    } else if (j < a.win_rows) {  // slot j of the ring holds the newest position of its residue
+      const long pmax = a.pmax[r], plim = a.plim ? a.plim[r] : pos;
+      int d = (int)(pmax - j) % a.win_rows;  // (positions fit in 31 bits)
+      if (d < 0) d += a.win_rows;
+      const long held = pmax - d;
+      if (held >= 0 && held <= plim && pos - held < a.win_rows && seq >= 0 && seq < a.win_slots) row = j;
+    }
+    return row >= 0 ? a.win + (a.widx ? (long)slot : seq) * a.win_sstride + row * DQK : nullptr;
+  };
+  // the cache's rows
+  const int* const ids = a.idx + (long)r * a.t;
+  const long rows = (long)a.map.cols << a.map.shift;
+  const bool known = seq >= 0 && seq < a.map.slots;
+  const int* const pages = a.map.table + (known ? seq : 0) * a.map.cols;
+  // the index of this lane's key of tile u, -1: none
+  auto index = [&](int u) {
+    const int j = (u - a.wtiles) * 64 + key;
+    return j < a.t && u < t1 ? ids[j] : -1;
+  };
+  auto there = [&](int i) { return known && i >= 0 && i < rows; };
+  auto source = [&](int i, int p) -> const uint8_t* {
+    return there(i) && (unsigned)p < (unsigned)a.map.pages ? a.pool + kv4_offset(a.map, p, i, RB) : nullptr;
+  };
+  // The way to the first tile's rows, two loads deep, is gone before Q is asked for.
+  int t = t0;
+  const uint16_t* wrow = t < min(t1, a.wtiles) ? window(t) : nullptr;
+  int i0 = -1, p0 = -1;
+  if (t0 >= a.wtiles && t0 < t1) {
+    i0 = index(t0);
+    p0 = pages[there(i0) ? i0 >> a.map.shift : 0];
+  }
 
   // Q: head l % 16 of each block, quarter l / 16 of the 512 columns, in k steps of 8
   uint4 q[NB][16 + TS];
@@ -60,8 +104,11 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
   }
 
   const uint32_t v_base = lds_addr_of(s_v), p_base = lds_addr_of(s_p), m_base = lds_addr_of(s_m);
-  const int key = wave * 16 + l16;  // this lane's key of a tile
-  const uint32_t v_row = v_base + key * 1024, v_sw = v_swizzle(key);
+  // this lane's unit 0 of its key's row, and its place in the transpose reads of key g * 8 + l16 / 4; the other units, and
+  // the keys 4 further, are an XOR away
+  const uint32_t v_put = v_base + key * 1024 + 256 * g + (v_swizzle(key) << 4);
+  const uint32_t v_get = v_base + (g * 8 + (l16 >> 2)) * 1024 + wave * 256 +
+                         (((((l16 & 3) >> 1) ^ (g & 1)) | (l16 >> 2) << 1) << 4) + (l16 & 1) * 8;
 
   // the softmax of a tile's scores and the product with its values in LDS
   auto attend = [&](f32x4_t (&s)[NB], bool valid, auto f16) {
@@ -110,6 +157,8 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
           (uint64_t)pk.y << 32 | pk.x;
     }
     lds_barrier();
+    uint32_t va = v_get;
+    asm volatile("" : "+v"(va));  // (eight addresses computed anew: as the loops' invariants they would fill the registers)
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       uint4 pb[NB];
@@ -121,11 +170,8 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
       for (int c = 0; c < 8; ++c) {
         uint2 v[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int kr = kk * 32 + g * 8 + u * 4 + (l16 >> 2);
-          const int unit = (wave * 8 + c) * 2 + ((l16 & 3) >> 1);
-          v[u] = lds_read_tr(v_base + kr * 1024 + ((unit ^ v_swizzle(kr)) << 4) + (l16 & 1) * 8);
-        }
+        for (int u = 0; u < 2; ++u)
+          v[u] = lds_read_tr((va ^ ((2 * c ^ 8 * u) << 4)) + u * 4096 + kk * 32768);
         const uint4 av = make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
 #pragma unroll
         for (int n = 0; n < NB; ++n)
@@ -133,85 +179,36 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
       }
     }
   };
-  auto put_v = [&](int k, uint4 x) {
-    *(__attribute__((address_space(3))) u32x4*)(v_row + (((uint32_t)(16 * g + k) ^ v_sw) << 4)) = __builtin_bit_cast(u32x4, x);
+  auto put_v = [&](uint32_t to, int k, uint4 x) {
+    *(__attribute__((address_space(3))) u32x4*)(to ^ k << 4) = __builtin_bit_cast(u32x4, x);
   };
 
   // ---- window rows
 #pragma unroll 1
-  for (int t = t0; t < min(t1, a.wtiles); ++t) {
-    const int j = t * 64 + key;
-    long row = -1;
-    if (a.widx) {
-      if (j < a.wt) row = a.widx[(long)r * a.wt + j];
-      if (row >= a.win_rows) row = -1;
-    } else if (j < a.win_rows) {  // slot j of the ring holds the newest position of its residue
-      const long pmax = a.pmax[r], plim = a.plim ? a.plim[r] : pos;
-      int d = (int)(pmax - j) % a.win_rows;  // (positions fit in 31 bits)
-      if (d < 0) d += a.win_rows;
-      const long held = pmax - d;
-      if (held >= 0 && held <= plim && pos - held < a.win_rows && seq >= 0 && seq < a.win_slots) row = j;
-    }
-    const bool valid = row >= 0;
-    const uint16_t* src = valid ? a.win + (a.widx ? (long)slot : seq) * a.win_sstride + row * DQK : (const uint16_t*)g_kv4_none;
+  for (; t < min(t1, a.wtiles); ++t) {
+    const bool valid = wrow != nullptr;
+    const uint16_t* src = valid ? wrow : (const uint16_t*)g_kv4_none;
+    uint4 x[16 + TS];
+#pragma unroll
+    for (int k = 0; k < 16 + TS; ++k) x[k] = *(const uint4*)(src + (k < 16 ? 128 * g + 8 * k : 512 + 16 * g + 8 * (k - 16)));
+    if (t + 1 < min(t1, a.wtiles)) wrow = window(t + 1);
     f32x4_t s[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) s[n] = f32x4_t{0, 0, 0, 0};
     lds_barrier();  // (the last tile's values have been read)
+    uint32_t to = v_put;
+    asm volatile("" : "+v"(to));
 #pragma unroll
     for (int k = 0; k < 16 + TS; ++k) {
-      const uint4 x = *(const uint4*)(src + (k < 16 ? 128 * g + 8 * k : 512 + 16 * g + 8 * (k - 16)));
-      if (k < 16) put_v(k, x);
+      if (k < 16) put_v(to, k, x[k]);
 #pragma unroll
-      for (int n = 0; n < NB; ++n) s[n] = mfma_bf16_16x16x32(x, q[n][k], s[n]);
+      for (int n = 0; n < NB; ++n) s[n] = mfma_bf16_16x16x32(x[k], q[n][k], s[n]);
     }
     attend(s, valid, std::false_type{});
   }
 
   // ---- rows of the cache
-  int t = max(t0, a.wtiles);
   if (t < t1) {
-    // Q to fp16; a head that reaches 2^16 scaled to under 2^15, which its scores are multiplied by again
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      float top = 0.0f;
-#pragma unroll
-      for (int k = 0; k < 16 + TS; ++k) {
-        const uint32_t w[4] = {q[n][k].x, q[n][k].y, q[n][k].z, q[n][k].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          top = fmaxf(fmaxf(top, fabsf(__uint_as_float(w[i] << 16))), fabsf(__uint_as_float(w[i] & 0xffff0000u)));
-      }
-      top = row_max4(top);
-      float down = 1.0f;
-      if (top >= 65536.0f) {  // (an infinity leaves zeros and infinities: its head's result is NaN)
-        const int e = min(((__float_as_int(top) >> 23) & 255) - 127, 127) - 14;
-        down = pow2i(-e);
-        cq[n] *= pow2i(e);
-      }
-#pragma unroll
-      for (int k = 0; k < 16 + TS; ++k) {
-        const uint32_t w[4] = {q[n][k].x, q[n][k].y, q[n][k].z, q[n][k].w};
-        uint32_t f[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          f[i] = pack_f16(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down);
-        q[n][k] = make_uint4(f[0], f[1], f[2], f[3]);
-      }
-    }
-    const int* ids = a.idx + (long)r * a.t;
-    const long rows = (long)a.map.cols << a.map.shift;
-    const bool known = seq >= 0 && seq < a.map.slots;
-    const int* const pages = a.map.table + (known ? seq : 0) * a.map.cols;
-    // the index of this lane's key of tile u, -1: none
-    auto index = [&](int u) {
-      const int j = (u - a.wtiles) * 64 + key;
-      return j < a.t && u < t1 ? ids[j] : -1;
-    };
-    auto there = [&](int i) { return known && i >= 0 && i < rows; };
-    auto source = [&](int i, int p) -> const uint8_t* {
-      return there(i) && (unsigned)p < (unsigned)a.map.pages ? a.pool + kv4_offset(a.map, p, i, RB) : nullptr;
-    };
     uint4 code[4];
     uint2 sc, tail;
     uint32_t tsc = 0;
@@ -225,9 +222,41 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
         tsc = p[320 + g];
       }
     };
-    int i0 = index(t), i1 = index(t + 1);
-    const uint8_t* row = source(i0, pages[there(i0) ? i0 >> a.map.shift : 0]);
+    if (t > t0) {
+      i0 = index(t);
+      p0 = pages[there(i0) ? i0 >> a.map.shift : 0];
+    }
+    int i1 = index(t + 1);
+    const uint8_t* row = source(i0, p0);
     load(row);
+    // Q to fp16; a head that reaches 2^16 scaled to under 2^15, which its scores are multiplied by again
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+      u16x2_t top2{0, 0};
+#pragma unroll
+      for (int k = 0; k < 16 + TS; ++k) {
+        const uint32_t w[4] = {q[n][k].x, q[n][k].y, q[n][k].z, q[n][k].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(u16x2_t, w[i] & 0x7fff7fffu));
+      }
+      const uint32_t most = max((int)top2[0], (int)top2[1]);  // (a NaN's bits are above an infinity's; both are scaled)
+      const float top = row_max4(__uint_as_float(min(most, 0x7f80u) << 16));
+      // (an infinity leaves zeros and infinities: its head's result is NaN)
+      const int e = top >= 65536.0f ? min(((__float_as_int(top) >> 23) & 255) - 127, 127) - 14 : 0;
+      const float down = pow2i(-e);
+      cq[n] *= pow2i(e);
+#pragma unroll
+      for (int k = 0; k < 16 + TS; ++k) {
+        const uint32_t w[4] = {q[n][k].x, q[n][k].y, q[n][k].z, q[n][k].w};
+        uint32_t f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          f[i] = pack_f16(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down);
+        q[n][k] = make_uint4(f[0], f[1], f[2], f[3]);
+      }
+    }
 #pragma unroll 1
     for (; t < t1; ++t) {
       const int p1 = pages[there(i1) ? i1 >> a.map.shift : 0];  // (the next tile's, and the index of the one behind it)
@@ -239,11 +268,13 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
 #pragma unroll
       for (int n = 0; n < NB; ++n) s[n] = f32x4_t{0, 0, 0, 0};
       lds_barrier();
+      uint32_t to = v_put;
+      asm volatile("" : "+v"(to));
 #pragma unroll
       for (int k = 0; k < 16 + TS; ++k) {
         const uint32_t w[4] = {code[(k / 4) % 4].x, code[(k / 4) % 4].y, code[(k / 4) % 4].z, code[(k / 4) % 4].w};
         const uint4 x = kv4_values(k < 16 ? w[k % 4] : (k == 16 ? tail.x : tail.y), sv[k / 2]);
-        if (k < 16) put_v(k, x);
+        if (k < 16) put_v(to, k, x);
 #pragma unroll
         for (int n = 0; n < NB; ++n) s[n] = mfma_f16_16x16x32(x, q[n][k], s[n]);
       }
@@ -351,7 +382,7 @@ Plan plan_of(int R, int H, int wt, int t, int dim, long rows) {
     p.groups = (H + 15) / 16;
     p.wtiles = (wt + 63) / 64;
     p.tiles = p.wtiles + (t + 63) / 64;
-    split(p, (long)R * p.groups, 512);
+    split(p, (long)R * p.groups, 256);
   }
   p.part = p.nsplit > 1 ? 4L * R * H * p.nsplit * 514 : 0;
   return p;
