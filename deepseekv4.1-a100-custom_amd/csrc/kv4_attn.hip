@@ -360,8 +360,10 @@ struct Plan {
   long list, rows, part;  // bytes of the workspace
 };
 
-// Splits of the tiles until the card's CUs have work: `want` workgroups.
-void split(Plan& p, long units, long want) {
+// Splits of the tiles until each of the card's CUs has a workgroup: two on a CU cost more in partial results than they
+// hide (4 sequences of 64 heads and 2048 rows: 20.3 us with 256, 24.4 with 512, 37.3 with 1024, 26.0 with 128).
+void split(Plan& p, long units) {
+  const long want = 256;
   if (p.tiles == 0) p.tiles = 1;  // (no key at all: zeros)
   long ns = units >= want ? 1 : (want + units - 1) / units;
   if (ns > p.tiles) ns = p.tiles;
@@ -372,17 +374,20 @@ void split(Plan& p, long units, long want) {
 Plan plan_of(int R, int H, int wt, int t, int dim, long rows) {
   Plan p{};
   p.groups = (H + 63) / 64;
-  p.many = rows > 0 && H > 32 && (long)R * p.groups >= 128 && (long)R * t >= 8 * rows;
+  // Decoding first pays with more than half a group of 64 heads (512 rows of 2048 keys: 64 heads 203 us for 357, 32 heads
+  // 198 for 186), when the lists name 2^17 rows (2048 each: 64 query rows 56 us for 67, 32 of them 47 for 45; 512 each:
+  // 602 rows 109 for 157, 150 of them 65 for 53) and each row of the cache eight times.
+  p.many = rows > 0 && H > 32 && (long)R * t >= 1L << 17 && (long)R * t >= 8 * rows;
   if (p.many) {
     p.tiles = (wt + t + 31) / 32;
-    split(p, (long)R * p.groups, 256);
+    split(p, (long)R * p.groups);
     p.list = ((long)R * (wt + t) * 4 + 255) & ~255L;
     p.rows = (rows * dim * 2 + 255) & ~255L;
   } else {
     p.groups = (H + 15) / 16;
     p.wtiles = (wt + 63) / 64;
     p.tiles = p.wtiles + (t + 63) / 64;
-    split(p, (long)R * p.groups, 256);
+    split(p, (long)R * p.groups);
   }
   p.part = p.nsplit > 1 ? 4L * R * H * p.nsplit * 514 : 0;
   return p;

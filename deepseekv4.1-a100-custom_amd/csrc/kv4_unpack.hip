@@ -59,9 +59,16 @@ __global__ void __launch_bounds__(256) kv4_unpack_kernel(const UnpackArgs a) {
     const int w = a.widx[r * a.wt + i];
     out[i] = w < a.win_rows ? w : -1;
   }
-  for (int i = threadIdx.x; i < a.t; i += 256) {
-    const int c = a.idx[r * a.t + i];
-    out[a.wt + i] = kv4_page(a.map, seq, c) >= 0 ? a.win_rows + c : -1;
+  const int* const in = a.idx + r * a.t;
+  for (int i0 = threadIdx.x; i0 < a.t; i0 += 8 * 256) {  // eight entries a lane in flight
+    int c[8], p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = in[min(i0 + 256 * j, a.t - 1)];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = kv4_page(a.map, seq, c[j]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + 256 * j < a.t) out[a.wt + i0 + 256 * j] = p[j] >= 0 ? a.win_rows + c[j] : -1;
   }
 }
 
