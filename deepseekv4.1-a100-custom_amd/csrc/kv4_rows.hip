@@ -14,7 +14,7 @@ struct RowsArgs {
   const long* seq;
   const long* row;
   long n;
-  int ratio;
+  int ratio, by_pos;
   const float* cos_t;
   const float* sin_t;
   long n_pos;
@@ -102,7 +102,12 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const RowsArgs a) {
   if (DIM == 576) tail = *(const uint4*)(x + min((lane >> 3) % kRows, n - 1) * a.x_rstride + 512 + 8 * (lane & 7));
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
-    const long seq = a.seq[r0 + min(u, n - 1)], row = a.row[r0 + min(u, n - 1)];
+    const long seq = a.seq[r0 + min(u, n - 1)];
+    long row = a.row[r0 + min(u, n - 1)];
+    if (a.by_pos) {
+      const uint32_t next = (uint32_t)row + 1, ratio = (uint32_t)a.ratio;
+      row = row >= 0 && row < (1L << 31) && next % ratio == 0 ? (long)(next / ratio) - 1 : -1;
+    }
     const int p = kv4_page(a.map, seq, row);
     pos[u] = row * a.ratio;
     dst[u] = nullptr;
@@ -191,7 +196,7 @@ void rows_args(RowsArgs& a, const dsv41_kv4& c, const long* seq, const long* row
 extern "C" {
 
 int dsv41_kv4_append(const dsv41_kv4* c, const void* x, long x_rstride, const long* seq, const long* row, long n,
-                     int ratio, const float* cos_t, const float* sin_t, long n_pos, int rd, void* stream) {
+                     int ratio, int by_pos, const float* cos_t, const float* sin_t, long n_pos, int rd, void* stream) {
   if (!kv4_ok(c) || n < 0 || n >= (1L << 32)) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
   if (!seq || !row || !x || ((uintptr_t)x & 15) || x_rstride < c->dim || x_rstride % 8 || ratio < 1 || rd < 0 ||
@@ -202,6 +207,7 @@ int dsv41_kv4_append(const dsv41_kv4* c, const void* x, long x_rstride, const lo
   a.x = (const uint16_t*)x;
   a.x_rstride = x_rstride;
   a.ratio = ratio;
+  a.by_pos = by_pos;
   a.cos_t = cos_t;
   a.sin_t = sin_t;
   a.n_pos = n_pos;

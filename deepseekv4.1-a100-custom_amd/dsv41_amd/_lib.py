@@ -63,7 +63,7 @@ SIGNATURES = {
     "dsv41_f32_proj2": [_P, _L, _P, _P, _I, _I, _I, _P, _P, _P],
     "dsv41_compress_pool_decode": [_P, _P, _L, _P, _P, _L, _I, _P, _P, _I, _I, _I, _P, _F, _P, _L, _P, _P],
     "dsv41_compress_pool_prefill": [_P, _P, _L, _P, _P, _I, _L, _I, _I, _I, _P, _F, _P, _L, _I, _P],
-    "dsv41_kv4_append": [_P, _P, _L, _P, _P, _L, _I, _P, _P, _L, _I, _P],
+    "dsv41_kv4_append": [_P, _P, _L, _P, _P, _L, _I, _I, _P, _P, _L, _I, _P],
     "dsv41_kv4_read": [_P, _P, _P, _L, _P, _P],
     "dsv41_kv4_fork": [_P, _P, _P, _P, _I, _P],
     "dsv41_kv4_release": [_P, _P, _P, _I, _P],

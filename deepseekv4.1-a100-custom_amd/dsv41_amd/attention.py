@@ -25,6 +25,7 @@ from .compressor import compress_pool, new_rings
 from .fused import fake_quant_fp4, fake_quant_fp8, norm_quant, rmsnorm, rope_, rope_dev_
 from .indexer import index_topk
 from .kernels import sparse_attn
+from .kv4 import PagedKV4, sparse_attn4
 from .w8 import W8, fp8_gemm_tc
 
 
@@ -93,11 +94,14 @@ class SparseAttention:
     indexer's i_wq_b, i_weights_proj [HI, dim], i_wk [128, D], i_k_norm_w; wo_a / wo_b (optional) for the
     o-projection.  Caches for `slots` sequences (batch row i is sequence i): ring [slots, window, D], compressed rows
     [slots, cap, D], index keys [slots, cap, 128] (bf16, the reference storage; with e4m3=True also an e4m3 copy +
-    per-row scales, which the selection then reads), compressor rings [slots, 8, D]."""
+    per-row scales, which the selection then reads), compressor rings [slots, 8, D].  With kv4, a kv4.PagedKV4 of rows of
+    head_dim (512), the compressed rows are held there in 4 bits instead: a call takes the pages that its rows need, and a
+    sequence's pages may be forked, released and compacted between calls.  The rows' values are the same."""
 
     def __init__(self, weights: dict, *, n_heads: int, head_dim: int, rope_head_dim: int, window: int, ratio: int,
                  index_n_heads: int, index_topk_k: int, cos: torch.Tensor, sin: torch.Tensor, slots: int, cap: int,
-                 eps: float = 1e-6, e4m3: bool = True, n_groups: int = 0, o_lora_rank: int = 0):
+                 eps: float = 1e-6, e4m3: bool = True, n_groups: int = 0, o_lora_rank: int = 0,
+                 kv4: PagedKV4 | None = None):
         self.w = weights
         self.H, self.D, self.rd, self.W, self.ratio = n_heads, head_dim, rope_head_dim, window, ratio
         self.HI, self.topk, self.eps = index_n_heads, index_topk_k, eps
@@ -108,7 +112,14 @@ class SparseAttention:
         self.sink = weights["attn_sink"].float().contiguous()
         self.ring = torch.zeros(slots, window, head_dim, dtype=torch.bfloat16, device=dev)
         if ratio:
-            self.ckv = torch.zeros(slots, cap, head_dim, dtype=torch.bfloat16, device=dev)
+            self.cap = cap
+            if kv4 is None:
+                self.ckv = torch.zeros(slots, cap, head_dim, dtype=torch.bfloat16, device=dev)
+            elif kv4.dim != head_dim or head_dim != 512 or kv4.slots < slots or kv4.cols * kv4.page < cap:
+                raise ValueError(f"SparseAttention: {slots} sequences of {cap} rows of {head_dim} in a cache of {kv4.slots} "
+                                 f"of {kv4.cols * kv4.page} of {kv4.dim} (rows of 512)")
+            else:
+                self.ckv = kv4
             self.index_k = torch.zeros(slots, cap, 128, dtype=torch.bfloat16, device=dev)
             self.k8 = torch.zeros(slots, cap, 128, dtype=torch.uint8, device=dev) if e4m3 else None
             self.ks = torch.zeros(slots, cap, dtype=torch.float32, device=dev) if e4m3 else None
@@ -143,16 +154,18 @@ class SparseAttention:
             ratio = self.ratio
             end = start_pos + s
             clen = end // ratio
-            if clen > self.ckv.shape[1]:
-                raise RuntimeError(f"SparseAttention: {clen} compressed rows exceed the cache capacity {self.ckv.shape[1]}")
+            if clen > self.cap:
+                raise RuntimeError(f"SparseAttention: {clen} compressed rows exceed the cache capacity {self.cap}")
             ckv, cscore = compressor_proj(x, w["c_wkv"], w["c_wgate"])
             latent = compress_pool(ckv, cscore, start_pos, ratio, self.ring_kv[:b], self.ring_score[:b],
                                    w["c_norm_w"], eps)
             new = latent is not None and latent.shape[1] > 0
-            ww = widx.shape[-1]
+            paged = isinstance(self.ckv, PagedKV4)  # (its attention takes the two index lists apart)
+            ww = 0 if paged else widx.shape[-1]
             kk = min(self.topk, clen)
             idx = torch.empty(b, s, ww + kk, dtype=torch.int32, device=x.device)
-            idx[:, :, :ww].copy_(widx)
+            if not paged:
+                idx[:, :, :ww].copy_(widx)
             if kk:
                 if new:  # the indexer's key append precedes its selection (dsv41/model.py:696-732)
                     C.write_index_k(self.index_k, F.linear(latent, w["i_wk"]), w["i_k_norm_w"], eps, start_pos,
@@ -160,13 +173,28 @@ class SparseAttention:
                 qi, wi = _indexer_query(x, qrq, w["i_wq_b"], w["i_weights_proj"], self.cos, self.sin, rd, start_pos,
                                         self.HI)
                 keys, ks = self._keys(b)
-                index_topk(qi, wi, keys, start_pos, ratio, self.topk, win_kv.shape[1], k_scale=ks,
+                index_topk(qi, wi, keys, start_pos, ratio, self.topk, 0 if paged else win_kv.shape[1], k_scale=ks,
                            out=idx[:, :, ww:])
+            if paged:
+                if new:
+                    self._append4(latent, start_pos // ratio)
+                o = sparse_attn4(q, win_kv, self.ckv, self.sink, widx, idx, self.scale)
+                rope_(o, rd, self.cos, self.sin, start_pos, inverse=True)
+                return o
             if new:
                 C.write_compress_kv(self.ckv, latent, start_pos, ratio, self.cos, self.sin, rd)
             o = sparse_attn(q, win_kv, self.sink, idx, self.scale, kv2=self.ckv[:b, :clen] if clen else None)
         rope_(o, rd, self.cos, self.sin, start_pos, inverse=True)
         return o
+
+    def _append4(self, latent: torch.Tensor, first: int) -> None:
+        """Rows first .. of sequences 0 .. of the 4-bit cache, on pages of their own."""
+        b, n, _ = latent.shape
+        seq = torch.arange(b, device=latent.device)
+        begin = torch.full_like(seq, first)
+        self.ckv.reserve(seq, begin, begin + n)
+        row = first + torch.arange(n, device=latent.device)
+        self.ckv.append(latent, seq.repeat_interleave(n), row.repeat(b), self.ratio, self.cos, self.sin, self.rd)
 
     def __call__(self, x: torch.Tensor, start_pos: int) -> torch.Tensor:
         """Attention.__call__ (dsv41/model.py:1350-1576): attend() then, with wo_a / wo_b given, the block-diagonal

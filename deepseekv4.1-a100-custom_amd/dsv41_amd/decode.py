@@ -12,6 +12,7 @@ import torch
 from . import cache as C
 from .fused2 import sattn2
 from .fused3 import DecodeSelector
+from .kv4 import PagedKV4, sattn4
 
 
 class DecodeLayer:
@@ -20,7 +21,8 @@ class DecodeLayer:
     None): the row a step that closes no compression group writes, per sequence -- the reference's per-slot table
     under DSV41_SLOT_CAPS (the last row of the slot's own capacity, dsv41/decode.py:62-68, :176-181), needed when
     the tables are as_strided views of per-slot capacities (dsv41/slots.py:1-11); None: the tables' spare last
-    row."""
+    row.  ckv may be a kv4.PagedKV4 instead of a table: the compressed rows in 4 bits and pages.  Its pages are the
+    caller's: before a step closes a group its row must be reserved (many steps' rows at once, or in the same graph)."""
 
     def __init__(self, ring, ckv, k8, ks, sink, cos, sin, ratio: int, topk: int, rd: int = 64, dv: int = 512,
                  eps: float = 1e-6, kbf16=None, nw_tab=None):
@@ -29,7 +31,10 @@ class DecodeLayer:
         self.ratio, self.topk, self.rd, self.dv, self.eps = ratio, topk, rd, dv, eps
         self.kbf16 = kbf16
         self.nw_tab = None if nw_tab is None else nw_tab.to(device=ring.device, dtype=torch.int64).contiguous()
-        self.scale = ckv.shape[-1] ** -0.5
+        self.paged = isinstance(ckv, PagedKV4)
+        if self.paged and (dv != 512 or ring.shape[-1] != ckv.dim):
+            raise ValueError(f"DecodeLayer: values of {dv} in rows of {ring.shape[-1]} beside a cache of {ckv.dim}")
+        self.scale = (ckv.dim if self.paged else ckv.shape[-1]) ** -0.5
         self._selectors = {}
         self._qbufs = {}
         self._attn_ws = {}
@@ -48,10 +53,19 @@ class DecodeLayer:
         q8 = wf = None
         if q_idx is not None:
             q8, wf = self._qbuf(q_idx.shape[0], q_idx.device)
-        C.decode_appends(kv_raw, kv_norm, self.ring, latent, self.ckv, k_raw, k_norm, self.kbf16, self.k8, self.ks,
+        latent, ckv = self._append4(latent, pos, seq)
+        C.decode_appends(kv_raw, kv_norm, self.ring, latent, ckv, k_raw, k_norm, self.kbf16, self.k8, self.ks,
                          pos, seq, self.ratio, self.cos, self.sin, self.rd, self.eps, q_idx, w_idx, q8, wf,
                          nw_tab=self.nw_tab)
         self._prepared = (q8, wf) if q_idx is not None else None
+
+    def _append4(self, latent, pos, seq):
+        """The compressed rows into a 4-bit cache, which then are no part of the other appends' launch; a table's are."""
+        if not self.paged:
+            return latent, self.ckv
+        if latent is not None:
+            self.ckv.append_decode(latent, seq, pos, self.ratio, self.cos, self.sin, self.rd)
+        return None, None
 
     def appends_select(self, kv_raw, kv_norm, latent, k_raw, k_norm, pos, seq, q_idx, w_idx, cl=None, cand=None):
         """appends() followed by select(), the appends inside the indexer's first launch (dsv41_decode_select when
@@ -66,7 +80,8 @@ class DecodeLayer:
         if self.k8 is None or k_raw is None:
             self.appends(kv_raw, kv_norm, latent, k_raw, k_norm, pos, seq, q_idx, w_idx)
             return self.select(q_idx, w_idx, pos, seq, cl)
-        app = dict(kv_raw=kv_raw, kv_norm=kv_norm, ring=self.ring, latent=latent, ckv=self.ckv, k_raw=k_raw,
+        latent, ckv = self._append4(latent, pos, seq)
+        app = dict(kv_raw=kv_raw, kv_norm=kv_norm, ring=self.ring, latent=latent, ckv=ckv, k_raw=k_raw,
                    k_norm=k_norm, kbf=self.kbf16, k8=self.k8, k_scale=self.ks, ratio=self.ratio, cos=self.cos,
                    sin=self.sin, rd=self.rd, eps=self.eps, q_idx=q_idx, w_idx=w_idx, nw_tab=self.nw_tab)
         self._prepared = None
@@ -101,16 +116,21 @@ class DecodeLayer:
 
     def check(self) -> None:
         """Raise RuntimeError when a launch of this layer reported an error through a workspace error word (the
-        indexer's row barriers, the attention's in-launch split merge); clears the words.  Synchronises."""
+        indexer's row barriers, the attention's in-launch split merge, a 4-bit cache); clears the words.  Synchronises."""
         from ._lib import attn_error_word, check_error_word
         for sel in self._selectors.values():
             sel.check()
+        if self.paged:
+            self.ckv.check()
         for (B, h), ws in self._attn_ws.items():
             w = attn_error_word(ws, B, h, ws.numel() * 4)
             if w is not None:
                 check_error_word("attention", w)
 
     def attend(self, q, idx, pos, seq, pmax, plim=None):
+        if self.paged:
+            return sattn4(q, self.ring, self.ckv, idx, pos, self.sink, self.cos, self.sin,
+                          0 if self.dv < q.shape[-1] else self.rd, self.scale, seq, pmax, plim)
         ws = self.attn_workspace(q.shape[0], q.shape[2], self.ring.shape[1] + idx.shape[-1], q.device)
         return sattn2(q, self.ring, self.ckv, idx, pos, self.sink, self.cos, self.sin, 0 if self.dv < q.shape[-1]
                       else self.rd, self.scale, seq, pmax, plim=plim, d_v=self.dv, ws=ws)

@@ -6,7 +6,7 @@ values and 336 a row of 576 instead of 1024 and 1152, in pages that sequences sh
 
   c = PagedKV4.empty(pages, slots, cap, dim)
   c.reserve(seq, begin, end)             pages of their own for rows begin .. end - 1 (copied where they are shared)
-  c.append(latent, seq, row, ratio, cos, sin, rd)
+  c.append(latent, seq, row, ratio, cos, sin, rd)      (append_decode: the rows by the tokens' positions)
   o = sattn4(q, ring, c, idx, ...)       decode: fused2.sattn2 with the cache in the place of kv_c
   o = sparse_attn4(q, kv, c, sink, win_idxs, topk_idxs, scale)     prefill: kernels.sparse_attn with kv2 in 4 bits
   c.fork(src, dst, rows)                 dst goes on from src's first rows (a prefix, samples of one prompt, drafts)
@@ -120,6 +120,15 @@ class PagedKV4:
         step that closes no group): its last rd columns rotated by the angle of position row * ratio, rounded to bf16 and
         put on the 4-bit grid, as the bf16 tables' appends do.  The rows' pages must be the sequences' own (reserve); the
         rows of one call must differ."""
+        self._append(latent, seq, row, ratio, 0, cos, sin, rd)
+
+    def append_decode(self, latent: torch.Tensor, seq, pos, ratio: int, cos: torch.Tensor, sin: torch.Tensor,
+                      rd: int) -> None:
+        """append of a decode step (dsv41/decode.py:157-164): latent[i] to the row of the group that position pos[i] closes,
+        row (pos[i] + 1) / ratio - 1; positions that close none leave the cache alone (no spare row)."""
+        self._append(latent, seq, pos, ratio, 1, cos, sin, rd)
+
+    def _append(self, latent, seq, row, ratio: int, by_pos: int, cos, sin, rd: int) -> None:
         dim = self.dim
         if latent.shape[-1] != dim or latent.dtype != torch.bfloat16:
             raise RuntimeError(f"kv4.append: latent {tuple(latent.shape)} {latent.dtype} (bf16 rows of {dim})")
@@ -135,8 +144,8 @@ class PagedKV4:
             x, stride = _aligned(x.contiguous()), dim
         seq, row = self._i64("kv4.append", seq, n), self._i64("kv4.append", row, n)
         cos, sin = _angles("kv4.append", cos, sin, rd, index)
-        _launch("dsv41_kv4_append", index, self._at, x.data_ptr(), stride, seq.data_ptr(), row.data_ptr(), n, ratio, ptr(cos),
-                ptr(sin), cos.shape[0] if rd else 0, rd)
+        _launch("dsv41_kv4_append", index, self._at, x.data_ptr(), stride, seq.data_ptr(), row.data_ptr(), n, ratio, by_pos,
+                ptr(cos), ptr(sin), cos.shape[0] if rd else 0, rd)
         self._done()
 
     def read(self, seq, row) -> torch.Tensor:

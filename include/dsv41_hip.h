@@ -378,10 +378,12 @@ typedef struct {
 /* Rows into the cache: y = x with its last rd columns rotated by the angle of position row * ratio (products exact, one
  * rounding to bf16: the compressed row of cache.append_compressed_decode / write_compress_kv, dsv41/decode.py:157-164),
  * then per 16 values s = e4m3(max(amax, 6 * 2^-9) / 6), codes E2M1(clamp(y / s, -6, 6)) into row row[r] of sequence
- * seq[r] (row < 0: none).  A group with an infinity or a NaN reads back as NaN.  x bf16, rows x_rstride apart, 16-byte
- * aligned, x_rstride % 8 == 0; cos_t / sin_t [n_pos, rd / 2].  Rows of one call must differ. */
+ * seq[r] (row < 0: none).  With by_pos row[r] is a token's position instead, which closes the group of row (row[r] + 1) /
+ * ratio - 1 or none (a decode step, dsv41/decode.py:157-164).  A group of 16 with an infinity or a NaN reads back as NaN.
+ * x bf16, rows x_rstride apart, 16-byte aligned, x_rstride % 8 == 0; cos_t / sin_t [n_pos, rd / 2].  Rows of one call must
+ * differ. */
 int dsv41_kv4_append(const dsv41_kv4* c, const void* x, long x_rstride, const long* seq, const long* row, long n,
-                     int ratio, const float* cos_t, const float* sin_t, long n_pos, int rd, void* stream);
+                     int ratio, int by_pos, const float* cos_t, const float* sin_t, long n_pos, int rd, void* stream);
 
 /* The values of rows as bf16 [n, dim] (exact), zeros where there is no row. */
 int dsv41_kv4_read(const dsv41_kv4* c, const long* seq, const long* row, long n, void* out, void* stream);

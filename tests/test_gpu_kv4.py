@@ -154,6 +154,25 @@ def test_append_drops_and_notes():
     assert not c.read([9, 0, 0, -1], [0, 63, 1 << 40, 3]).any()
 
 
+@pytest.mark.parametrize("ratio", [1, 2, 4, 128])
+def test_append_decode(ratio):
+    """The rows by the tokens' positions: those that close a group, the first and the last of a page among them."""
+    from dsv41_amd.kv4 import PagedKV4
+    g = _gen(ratio)
+    pos = torch.tensor([0, ratio - 1, 17 * ratio - 1, 17 * ratio, 16 * ratio - 1, 32 * ratio - 2, 32 * ratio - 1, -1, 1 << 40])
+    seq = torch.arange(9)
+    x = _rows(g, 9, 576).to(DEV)
+    cos, sin = (t.to(DEV) for t in _angles(33 * ratio))
+    a, b = (PagedKV4.empty(30, 9, 40, 576, 16, DEV) for _ in range(2))
+    for c in (a, b):
+        c.reserve(seq, [0] * 9, [40] * 9)
+    a.append_decode(x, seq, pos, ratio, cos, sin, 64)
+    row = [int(p + 1) // ratio - 1 if p >= 0 and p < 1 << 31 and (p + 1) % ratio == 0 else -1 for p in pos]
+    b.append(x, seq, row, ratio, cos, sin, 64)
+    a.check()
+    assert torch.equal(a.pool, b.pool) and sum(r >= 0 for r in row) >= 4
+
+
 def test_append_strided_rows_and_far_offsets():
     """Rows cut out of wider ones; and a page whose bytes stand past 2^32 of the pool."""
     from dsv41_amd.kv4 import PagedKV4
@@ -341,6 +360,98 @@ def test_prefill_many_rows():
     for heads in (16, 32, 48, 64, 80, 128):
         _prefill(576, heads, 1, 530, 400, 100, seed=heads)
     _prefill(512, 64, 1, 530, 400, 200)
+
+
+@pytest.mark.parametrize("dim,heads,b,s,prior,t,w,page,seq", [
+    (576, 33, 1, 530, 400, 256, 100, 16, None),    # one split, half of the second group's heads
+    (576, 64, 1, 530, 400, 256, 1, 32, None),
+    (512, 80, 1, 530, 400, 250, 37, 64, None),     # two groups of 64 heads, lists that end inside a tile
+    (512, 64, 3, 177, 2500, 257, 128, 16, [4, 0, 2]),
+    (576, 64, 2, 65, 4300, 1025, 128, 256, [1, 1]),  # two splits; one sequence twice
+    (512, 128, 1, 68, 8200, 2000, 64, 128, None)])
+def test_prefill_cache_decoded_first(dim, heads, b, s, prior, t, w, page, seq):
+    """2^17 listed rows and more, eight times the cache's: its rows are decoded once and attended to as bf16."""
+    assert b * s * t >= 1 << 17
+    _prefill(dim, heads, b, s, prior, t, w, page, seed=heads, seq=seq, strided=t % 2 == 1)
+
+
+def _many(g, dim=576, heads=40, s=520, t=260, n=200, page=16):
+    """A call whose cache is decoded first: q, the cache with a hole, its rows, lists with rows of the hole and none."""
+    c, rows = _filled(g, [n, n], dim, page)
+    c.table[1, 3] = -1
+    q = torch.randn(1, s, heads, dim, generator=g).to(BF)
+    idx = torch.randint(0, n + 30, (1, s, t), generator=g, dtype=torch.int32)
+    idx[0, :, ::5] = -1
+    idx[0, 7] = -1
+    idx[0, 8, :] = 3 * page + 2  # (the hole alone)
+    idx[0, 9, 3:] = 2 ** 31 - 1
+    held = -(-n // page) * page  # (rows behind the last one of a page are there, as zeros)
+    there = lambda i: (i >= 0) & (i < held) & (i // page != 3)  # noqa: E731
+    return c, torch.cat((rows[1], torch.zeros(held - n, dim, dtype=torch.float64))), q, idx, there
+
+
+def test_decoded_first_without_a_window():
+    """No window; pages that are not there, indices past the table, rows without a key; a sequence out of range."""
+    from dsv41_amd.kv4 import sparse_attn4
+    g = _gen(21)
+    c, rows, q, idx, there = _many(g)
+    sink = torch.randn(40, generator=g)
+    sink[3], sink[4] = -float("inf"), float("inf")
+    args = (q.to(DEV), None, c, sink.to(DEV), None, idx.to(DEV), 0.04)
+    o = sparse_attn4(*args, seq=torch.tensor([1], device=DEV))
+    ref = torch.zeros(1, q.shape[1], 40, 512, dtype=torch.float64)
+    for i in range(q.shape[1]):
+        k = idx[0, i][there(idx[0, i])].long()
+        ref[0, i] = R.attend(q[0, i].double(), rows[k], sink.double().clamp(-1e300, 1e300), 0.04)
+    assert not ref[0, 7].any() and not ref[0, 8].any() and ref[0, 9].any()
+    _close(o, ref, rows.abs().max().item())
+    for bad in (-1, 2, 1 << 40):
+        assert not sparse_attn4(*args, seq=torch.tensor([bad], device=DEV)).any()
+
+
+def test_decoded_first_nan_stays_in_its_rows():
+    """A query of NaN, a cache row of NaN and one of an infinity in the window: the queries that name them and no other."""
+    from dsv41_amd.kv4 import sparse_attn4
+    g = _gen(22)
+    c, rows, q, idx, there = _many(g)
+    c.table[1, 3] = c.table[0, 3]
+    idx[idx == 5] = 6
+    idx[0, 11, 4] = 5
+    q[0, 12, 39, 3] = float("nan")
+    x = torch.full((1, 576), float("nan"), dtype=BF, device=DEV)
+    c.append(x, [1], [5], 1, None, None, 0)
+    kv = torch.randn(1, 9, 576, generator=g).to(BF)
+    kv[0, 8, 575] = float("inf")
+    win = torch.randint(-1, 8, (1, q.shape[1], 6), generator=g, dtype=torch.int32)
+    win[0, 13, 2] = 8
+    o = sparse_attn4(q.to(DEV), kv.to(DEV), c, torch.zeros(40, device=DEV), win.to(DEV), idx.to(DEV), 0.04,
+                     seq=torch.tensor([1], device=DEV)).cpu()
+    nan = torch.isnan(o[0]).any(-1)
+    # (a key column of infinity: a score of -inf is no key, one of +inf leaves inf - inf)
+    assert nan[11].all() and nan[12, 39] and not nan[12, :39].any() and torch.equal(nan[13], q[0, 13, :, 575] > 0)
+    nan[11:14] = False
+    assert not nan.any()
+
+
+def test_decoded_first_from_a_graph():
+    """Captured with the lists and rows that it decodes; replayed on others, against the eager call."""
+    from dsv41_amd.kv4 import sparse_attn4
+    g = _gen(23)
+    c, rows, q, idx, there = _many(g)
+    q, idx, sink = q.to(DEV), idx.to(DEV), torch.zeros(40, device=DEV)
+    seq = torch.tensor([1], device=DEV)
+    run = lambda: sparse_attn4(q, None, c, sink, None, idx, 0.04, seq=seq)  # noqa: E731
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for i in range(4):
+        q.copy_(torch.randn(q.shape, generator=g).to(BF))
+        idx.copy_(torch.randint(-1, 220, idx.shape, generator=g, dtype=torch.int32))
+        seq.fill_(i % 2)
+        c.append(_rows(g, 3, 576).to(DEV), [0, 1, 1], [i, i, 40 + i], 1, None, None, 0)
+        graph.replay()
+        assert torch.equal(out, run()), i
 
 
 def test_prefill_sequences_and_strides():
@@ -621,3 +732,119 @@ def test_captured_step():
             assert torch.equal(a.table, b.table) and torch.equal(a.refs, b.refs) and torch.equal(a.pool, b.pool)
     for a, b, *_ in made:
         a.check()
+
+
+# ------------------------------------------------------------------------------------------------ in the layers
+def _layer_weights(g, dim, q_rank, H, D, HI):
+    n = lambda *s: torch.randn(*s, generator=g) * s[-1] ** -0.5  # noqa: E731
+    w = dict(wq_a=n(q_rank, dim), q_norm_w=1 + 0.1 * n(q_rank), wq_b=n(H * D, q_rank), wkv=n(D, dim), kv_norm_w=1 + 0.1 * n(D),
+             c_norm_w=1 + 0.1 * n(D), i_wq_b=n(HI * 128, q_rank), i_weights_proj=n(HI, dim), i_wk=n(128, D),
+             i_k_norm_w=1 + 0.1 * n(128))
+    w = {k: v.to(BF).to(DEV) for k, v in w.items()}
+    w.update(c_wkv=n(D, dim).to(DEV), c_wgate=n(D, dim).to(DEV), attn_sink=torch.randn(H, generator=g).to(DEV))
+    return w
+
+
+def _alike(a, b, most):
+    """Two outputs that are each off by 2^-8 (|o| + V), V the largest value (see _close), then rotated -- sqrt 2 of it at
+    most -- and rounded again: 7 2^-8 V apart; as a whole by twice 2^-8 of the norm and two roundings."""
+    a, b = a.double(), b.double()
+    assert torch.isfinite(a).all() and (a - b).abs().max() <= 7 * 2.0 ** -8 * most
+    assert (a - b).norm() <= 3 * 2.0 ** -8 * b.norm()
+
+
+@pytest.mark.parametrize("b", [1, 2])
+def test_attention_layer_over_a_4_bit_cache(b):
+    """SparseAttention with its compressed rows in a PagedKV4 beside one with the bf16 table, over a prompt, a
+    continuation that selects, steps that close a group and steps that do not, and a second prompt in the same slots."""
+    from dsv41_amd.attention import SparseAttention
+    from dsv41_amd.kv4 import PagedKV4
+    g = _gen(40 + b)
+    dim, q_rank, H, D, HI, ratio, cap = 256, 128, 20, 512, 16, 2, 400
+    w = _layer_weights(g, dim, q_rank, H, D, HI)
+    cos, sin = (t.to(DEV) for t in _angles(2 * cap))
+    kw = dict(n_heads=H, head_dim=D, rope_head_dim=64, window=32, ratio=ratio, index_n_heads=HI, index_topk_k=100, cos=cos,
+              sin=sin, slots=b, cap=cap)
+    c = PagedKV4.empty(b * -(-cap // 32), b, cap, D, 32, DEV)
+    one, two = SparseAttention(w, **kw), SparseAttention(w, kv4=c, **kw)
+    x = torch.randn(b, 700, dim, generator=g).to(BF).to(DEV)
+    for lo, hi in ((0, 1), (1, 2), (0, 333), (333, 601), (601, 602), (602, 603), (603, 604), (0, 90)):
+        o, p = one.attend(x[:, lo:hi], lo), two.attend(x[:, lo:hi], lo)
+        n = hi // ratio
+        rows = torch.arange(n, device=DEV).repeat(b)
+        got = c.read(torch.arange(b, device=DEV).repeat_interleave(n), rows).view(b, n, D)
+        assert (got != one.ckv[:, :n]).any(-1).sum().item() <= 2 * b  # (rotated in fp32 there, in 64 bits here)
+        assert torch.equal(one.ring, two.ring)
+        _alike(p, o, max(one.ckv.abs().max().item(), one.ring.abs().max().item(), 1.0))
+    c.check()
+    with pytest.raises(RuntimeError, match="capacity"):
+        two.attend(x[:, :1], 2 * cap + 1)
+    for bad in (PagedKV4.empty(9, b, cap, 576, 32, DEV), PagedKV4.empty(9, b, cap - 40, D, 32, DEV)):
+        with pytest.raises(ValueError, match="SparseAttention"):
+            SparseAttention(w, kv4=bad, **kw)
+
+
+def test_decode_layer_over_a_4_bit_cache():
+    """DecodeLayer with a PagedKV4 in the place of the bf16 table: appends, selection and attention of steps that close a
+    group and steps that do not, by both ways of the appends; then the step from a graph."""
+    from dsv41_amd.decode import DecodeLayer
+    from dsv41_amd.kv4 import PagedKV4
+    from dsv41_amd.workloads import DecodeConfig, make_decode_inputs
+    cfg = DecodeConfig("T", [8300, 900, 40], topk=512, spare=20)
+    (l0,), st = make_decode_inputs(cfg, DEV, seed=9)
+    B, cap = 3, l0["ckv"].shape[1]
+    cos, sin = (t.to(DEV) for t in _angles(8400))
+    c = PagedKV4.empty(B * -(-cap // 64), B, cap, 576, 64, DEV)
+    rows = torch.arange(cap, device=DEV).repeat(B)
+    seqs = torch.arange(B, device=DEV).repeat_interleave(cap)
+    c.reserve([0, 1, 2], [0, 0, 0], [cap] * 3)
+    c.append(l0["ckv"], seqs, rows, 1, None, None, 0)
+    l0["ckv"] = c.read(seqs, rows).view(B, cap, 576)
+    mk = lambda ckv: DecodeLayer(l0["ring"].clone(), ckv, l0["k8"].clone(), l0["ks"].clone(), st["sink"], cos, sin,  # noqa: E731
+                                 cfg.ratio, cfg.topk)
+    one, two = mk(l0["ckv"].clone()), mk(c)
+    g = _gen(10)
+    kv_raw, latent, k_raw, pos = st["kv_raw"].clone(), st["latent"].clone(), st["k_raw"].clone(), st["pos"].clone()
+
+    def step(lay, fused):
+        a = (kv_raw, st["kv_norm"], latent, k_raw, st["k_norm"], pos, st["seq"], st["q_idx"], st["w_idx"])
+        if fused:
+            idx = lay.appends_select(*a)
+        else:
+            lay.appends(*a)
+            idx = lay.select(st["q_idx"], st["w_idx"], pos, st["seq"])
+        return idx.clone(), lay.attend(st["q"], idx, pos, st["seq"], pos)
+
+    def same(a, b, i):
+        assert torch.equal(a[0], b[0]), i
+        top = max(l0["ckv"].abs().max().item(), one.ring.abs().max().item(), one.ckv.abs().max().item())
+        _alike(b[1], a[1], top)
+        cl = ((pos + 1) // cfg.ratio - 1).tolist()
+        got = c.read([0, 1, 2], cl)
+        want = torch.stack([one.ckv[s, r] for s, r in enumerate(cl)])
+        assert (got != want).sum().item() <= 2, i
+
+    def fresh(i):
+        kv_raw.copy_(torch.randn(kv_raw.shape, generator=g))
+        latent.copy_(torch.randn(latent.shape, generator=g))
+        k_raw.copy_(torch.randn(k_raw.shape, generator=g))
+        pos.add_(1 if i else 0)
+
+    for i in range(6):
+        fresh(i)
+        same(step(one, i % 2 == 0), step(two, i % 2 == 0), i)
+        one.check(), two.check()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(two, True)
+    for i in range(1, 6):
+        fresh(i)
+        graph.replay()
+        same(step(one, True), out, i)
+    two.check()
+    c.release([1])
+    two.appends(kv_raw, st["kv_norm"], latent, k_raw, st["k_norm"], torch.full_like(pos, 903), st["seq"])
+    with pytest.raises(RuntimeError, match="dropped"):
+        two.check()
+    with pytest.raises(ValueError, match="DecodeLayer"):
+        DecodeLayer(l0["ring"], PagedKV4.empty(1, 1, 1, 512, 64, DEV), l0["k8"], l0["ks"], st["sink"], cos, sin, 4, 512)

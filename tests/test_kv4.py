@@ -104,7 +104,7 @@ def test_entry_points_refuse():
         assert L.dsv41_kv4_compact(x, P, P, big, None) == inv, k
         assert L.dsv41_kv4_copy(x, ctypes.byref(_struct(pool=1 << 40)), P, P, 1, None, 0, None) == inv, k
         assert L.dsv41_kv4_copy(ctypes.byref(_struct(pool=1 << 40)), x, P, P, 1, None, 0, None) == inv, k
-        assert L.dsv41_kv4_append(x, P, 1024, P, P, 1, 4, P, P, 9, 64, None) == inv, k
+        assert L.dsv41_kv4_append(x, P, 1024, P, P, 1, 4, 0, P, P, 9, 64, None) == inv, k
         assert L.dsv41_kv4_read(x, P, P, 1, P, None) == inv, k
         assert L.dsv41_sattn4(x, P, P, 128 * 512, 2, 128, P, 10, P, P, P, None, P, P, P, 100, 64, 1.0, P, 1, 16, None, 0, None) == inv
         assert L.dsv41_sparse_attn4(x, P, P, 128 * 512, 128, P, 128, P, 10, None, P, 1.0, P, 1, 1, 16, None, 0, None) == inv
@@ -129,8 +129,8 @@ def test_entry_points_refuse():
     assert L.dsv41_kv4_copy(c, ctypes.byref(_struct(**far, dim=576)), P, P, 1, None, 0, None) == inv
     for x, stride, ratio, rd in [(None, 512, 4, 64), (P + 2, 512, 4, 64), (P, 500, 4, 64), (P, 516, 4, 64), (P, 512, 0, 64),
                                  (P, 512, 4, 65), (P, 512, 4, 514), (P, 512, 4, -2)]:
-        assert L.dsv41_kv4_append(c, x, stride, P, P, 1, ratio, P, P, 9, rd, None) == inv
-    assert L.dsv41_kv4_append(c, P, 512, P, P, 1, 4, None, P, 9, 64, None) == inv
+        assert L.dsv41_kv4_append(c, x, stride, P, P, 1, ratio, 0, P, P, 9, rd, None) == inv
+    assert L.dsv41_kv4_append(c, P, 512, P, P, 1, 4, 1, None, P, 9, 64, None) == inv
     assert L.dsv41_kv4_read(c, P, P, 1, P + 2, None) == inv
     args = [c, P, P, 128 * 512, 2, 128, P, 10, P, P, P, None, P, P, P, 100, 64, 1.0, P, 1, 16, None, 0, None]
     for at, v in [(1, None), (1, P + 2), (2, None), (3, 12), (5, 0), (6, None), (7, -1), (8, None), (9, None), (10, None),
