@@ -1,6 +1,6 @@
 // Sparse attention over window rows (bf16) and selected rows of the paged 4-bit cache.
 //
-// One workgroup of four waves: one query row, HB heads, a run of 64-key tiles (first the window's, then the cache's).
+// One workgroup of four waves: one query row, 16 heads, a run of 64-key tiles (first the window's, then the cache's).
 // Each wave scores 16 of a tile's keys: S^T = K Q^T by 16x16x32 MFMAs, the keys' fragments straight from memory into
 // registers -- lane (key l % 16, quarter l / 16) holds 128 consecutive values of its key, 64 bytes of codes, which are
 // the operands of 16 k steps if Q is held in the same order.  The decoded rows go to LDS once, as the values; then each
@@ -9,22 +9,28 @@
 // Decoding is exact in fp16 (E2M1 times e4m3 has 6 significand bits), two packed instructions for two values; Q in fp16
 // is exact too, but for numbers under 2^-14 (off by 2^-25 at most, a logit by less than fp32's own rounding of the sum)
 // and for heads that reach 2^16, which are scaled by a power of two.  Window rows have bf16's range, so they stay in bf16.
-// Sums, the softmax's maximum and sum and O are fp32; the probabilities are rounded to fp16 (bf16 for window rows), the
-// operand type, and the output once, after the rotation.
+// Sums, the softmax's maximum and sum and O are fp32; the reference maximum moves only for a score 2^8 above it; the
+// probabilities are rounded to fp16 (bf16 for window rows), the operand type, and the output once, after the rotation.
+//
+// What bounds it.  A step of single tokens: latency.  Four sequences of 2048 selected rows and 64 heads of 576 read 4 MB
+// and take 16.7 us, of them 8 us for a workgroup's one or two tiles -- index, page and row, three dependent loads, then
+// 1700 cycles of decoding and scores and 1750 of softmax and product -- and joining the splits 4.2 us; one sequence of 300
+// rows of 512 8.8 and 4.3 us.  Prompts of few heads: decoding, 350 instructions a wave and tile beside 34 MFMAs (602 query
+// rows of 512 + 128 keys, 20 heads of 512: 83 us).  32 heads a workgroup halve that but leave one workgroup a CU (97 us, and
+// 16.8 us for 12.8 of one token); the rows in bf16 first cost as much with 32 heads as with 64 (94 us).
 #include <type_traits>
 
 #include "kv4_attn_core.h"
 
 namespace {
 
-template <int HB, int DQK>
-__global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const Kv4AttnArgs a) {
-  constexpr int NB = HB / 16;              // head blocks
+template <int DQK>
+__global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
   constexpr int TS = DQK == 576 ? 2 : 0;   // k steps of the last 64 columns
   constexpr int RB = kv4_row_bytes(DQK);
   __shared__ __align__(1024) uint8_t s_v[64 * 1024];
-  __shared__ __align__(16) uint8_t s_p[HB * 128];
-  __shared__ __align__(16) float s_m[HB * 4];
+  __shared__ __align__(16) uint8_t s_p[16 * 128];
+  __shared__ __align__(16) float s_m[16 * 4];
 
   // The head groups of a (row, split) read the same rows of the cache: eight workgroups apart they share an XCD's L2.
   const int b = blockIdx.x, units = a.R * a.nsplit, full = units & ~7;
@@ -32,7 +38,7 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
   const int in = b < full * a.groups ? b % (8 * a.groups) : b - full * a.groups;
   const int u0 = (b < full * a.groups ? b / (8 * a.groups) * 8 : full) + in % n8;
   const int hg = in / n8, sp = u0 % a.nsplit, r = u0 / a.nsplit;
-  const int h0 = hg * HB;
+  const int h0 = hg * 16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l16 = lane & 15, g = lane >> 4;
   const int slot = r / a.rows_per_slot;
@@ -81,27 +87,18 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
     p0 = pages[there(i0) ? i0 >> a.map.shift : 0];
   }
 
-  // Q: head l % 16 of each block, quarter l / 16 of the 512 columns, in k steps of 8
-  uint4 q[NB][16 + TS];
+  // Q: head l % 16, quarter l / 16 of the 512 columns, in k steps of 8
+  uint4 q[16 + TS];
+  const int h = h0 + l16;
+  const uint16_t* const qrow = a.q + r * a.q_rstride + (long)(h < a.H ? h : a.H - 1) * DQK;
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const int h = h0 + 16 * n + l16;
-    const uint16_t* src = a.q + r * a.q_rstride + (long)(h < a.H ? h : a.H - 1) * DQK;
+  for (int k = 0; k < 16; ++k) q[k] = *(const uint4*)(qrow + 128 * g + 8 * k);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) q[n][k] = *(const uint4*)(src + 128 * g + 8 * k);
+  for (int k = 0; k < TS; ++k) q[16 + k] = *(const uint4*)(qrow + 512 + 16 * g + 8 * k);
+  f32x4_t o[8];
+  float m = -__builtin_inff(), l = 0.0f, cq = a.scale;
 #pragma unroll
-    for (int k = 0; k < TS; ++k) q[n][16 + k] = *(const uint4*)(src + 512 + 16 * g + 8 * k);
-  }
-  f32x4_t o[NB][8];
-  float m[NB], l[NB], cq[NB];
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    m[n] = -__builtin_inff();
-    l[n] = 0.0f;
-    cq[n] = a.scale;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) o[n][c] = f32x4_t{0, 0, 0, 0};
-  }
+  for (int c = 0; c < 8; ++c) o[c] = f32x4_t{0, 0, 0, 0};
 
   const uint32_t v_base = lds_addr_of(s_v), p_base = lds_addr_of(s_p), m_base = lds_addr_of(s_m);
   // this lane's unit 0 of its key's row, and its place in the transpose reads of key g * 8 + l16 / 4; the other units, and
@@ -111,61 +108,43 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
                          (((((l16 & 3) >> 1) ^ (g & 1)) | (l16 >> 2) << 1) << 4) + (l16 & 1) * 8;
 
   // the softmax of a tile's scores and the product with its values in LDS
-  auto attend = [&](f32x4_t (&s)[NB], bool valid, auto f16) {
+  auto attend = [&](f32x4_t& s, bool valid, auto f16) {
     constexpr bool F16 = decltype(f16)::value;
     const uint32_t mask = (uint32_t)(__ballot(valid) & 0xffffu) >> (4 * g);
-    float mx[NB];
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[n][i] = (mask >> i & 1) ? s[n][i] * cq[n] : -__builtin_inff();
-      mx[n] = row_max4(fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3])));
-      if (g == 0) *(__attribute__((address_space(3))) float*)(m_base + ((16 * n + l16) * 4 + wave) * 4) = mx[n];
-    }
+    for (int i = 0; i < 4; ++i) s[i] = (mask >> i & 1) ? s[i] * cq : -__builtin_inff();
+    float mx = row_max4(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+    if (g == 0) *(__attribute__((address_space(3))) float*)(m_base + (l16 * 4 + wave) * 4) = mx;
     lds_barrier();
-    bool up = false;
+    const f32x4_t w = *(__attribute__((address_space(3))) f32x4_t*)(m_base + l16 * 16);
+    mx = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+    if (__any(mx > m + 8.0f)) {  // (alike in every wave: all have the same maxima)
+      const float to = fmaxf(m, mx);
+      const float f = to > m ? exp2f(m - to) : 1.0f;
+      m = to;
+      l *= f;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const f32x4_t w = *(__attribute__((address_space(3))) f32x4_t*)(m_base + (16 * n + l16) * 16);
-      mx[n] = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
-      up |= mx[n] > m[n] + 8.0f;
+      for (int c = 0; c < 8; ++c) o[c] *= f;
     }
-    if (__any(up)) {  // (alike in every wave: all have the same maxima)
+    const float ref = m == -__builtin_inff() ? 0.0f : m;
+    float p[4];
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const float to = fmaxf(m[n], mx[n]);
-        const float f = to > m[n] ? exp2f(m[n] - to) : 1.0f;
-        m[n] = to;
-        l[n] *= f;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) o[n][c] *= f;
-      }
+    for (int i = 0; i < 4; ++i) {
+      p[i] = exp2f(s[i] - ref);
+      l += p[i];
     }
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const float ref = m[n] == -__builtin_inff() ? 0.0f : m[n];
-      float p[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[i] = exp2f(s[n][i] - ref);
-        l[n] += p[i];
-      }
-      const uint2 pk = F16 ? make_uint2(pack_f16(p[0], p[1]), pack_f16(p[2], p[3]))
-                           : make_uint2(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]));
-      *(__attribute__((address_space(3))) uint64_t*)(p_base + (16 * n + l16) * 128 +
-                                                     (((wave * 2 + (g >> 1)) ^ (l16 & 7)) << 4) + (g & 1) * 8) =
-          (uint64_t)pk.y << 32 | pk.x;
-    }
+    const uint2 pk = F16 ? make_uint2(pack_f16(p[0], p[1]), pack_f16(p[2], p[3]))
+                         : make_uint2(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]));
+    *(__attribute__((address_space(3))) uint64_t*)(p_base + l16 * 128 +
+                                                   (((wave * 2 + (g >> 1)) ^ (l16 & 7)) << 4) + (g & 1) * 8) =
+        (uint64_t)pk.y << 32 | pk.x;
     lds_barrier();
     uint32_t va = v_get;
     asm volatile("" : "+v"(va));  // (eight addresses computed anew: as the loops' invariants they would fill the registers)
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
-      uint4 pb[NB];
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-        pb[n] = __builtin_bit_cast(uint4, *(__attribute__((address_space(3))) u32x4*)(p_base + (16 * n + l16) * 128 +
-                                                                                      (((kk * 4 + g) ^ (l16 & 7)) << 4)));
+      const uint4 pb = __builtin_bit_cast(
+          uint4, *(__attribute__((address_space(3))) u32x4*)(p_base + l16 * 128 + (((kk * 4 + g) ^ (l16 & 7)) << 4)));
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         uint2 v[2];
@@ -173,9 +152,7 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
         for (int u = 0; u < 2; ++u)
           v[u] = lds_read_tr((va ^ ((2 * c ^ 8 * u) << 4)) + u * 4096 + kk * 32768);
         const uint4 av = make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-          o[n][c] = F16 ? mfma_f16_16x16x32(av, pb[n], o[n][c]) : mfma_bf16_16x16x32(av, pb[n], o[n][c]);
+        o[c] = F16 ? mfma_f16_16x16x32(av, pb, o[c]) : mfma_bf16_16x16x32(av, pb, o[c]);
       }
     }
   };
@@ -192,17 +169,14 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
 #pragma unroll
     for (int k = 0; k < 16 + TS; ++k) x[k] = *(const uint4*)(src + (k < 16 ? 128 * g + 8 * k : 512 + 16 * g + 8 * (k - 16)));
     if (t + 1 < min(t1, a.wtiles)) wrow = window(t + 1);
-    f32x4_t s[NB];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) s[n] = f32x4_t{0, 0, 0, 0};
+    f32x4_t s = {0, 0, 0, 0};
     lds_barrier();  // (the last tile's values have been read)
     uint32_t to = v_put;
     asm volatile("" : "+v"(to));
 #pragma unroll
     for (int k = 0; k < 16 + TS; ++k) {
       if (k < 16) put_v(to, k, x[k]);
-#pragma unroll
-      for (int n = 0; n < NB; ++n) s[n] = mfma_bf16_16x16x32(x[k], q[n][k], s[n]);
+      s = mfma_bf16_16x16x32(x[k], q[k], s);
     }
     attend(s, valid, std::false_type{});
   }
@@ -230,32 +204,29 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
     const uint8_t* row = source(i0, p0);
     load(row);
     // Q to fp16; a head that reaches 2^16 scaled to under 2^15, which its scores are multiplied by again
+    typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+    u16x2_t top2{0, 0};
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
-      u16x2_t top2{0, 0};
+    for (int k = 0; k < 16 + TS; ++k) {
+      const uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
 #pragma unroll
-      for (int k = 0; k < 16 + TS; ++k) {
-        const uint32_t w[4] = {q[n][k].x, q[n][k].y, q[n][k].z, q[n][k].w};
+      for (int i = 0; i < 4; ++i)
+        top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(u16x2_t, w[i] & 0x7fff7fffu));
+    }
+    const uint32_t most = max((int)top2[0], (int)top2[1]);  // (a NaN's bits are above an infinity's; both are scaled)
+    const float top = row_max4(__uint_as_float(min(most, 0x7f80u) << 16));
+    // (an infinity leaves zeros and infinities: its head's result is NaN)
+    const int e = top >= 65536.0f ? min(((__float_as_int(top) >> 23) & 255) - 127, 127) - 14 : 0;
+    const float down = pow2i(-e);
+    cq *= pow2i(e);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(u16x2_t, w[i] & 0x7fff7fffu));
-      }
-      const uint32_t most = max((int)top2[0], (int)top2[1]);  // (a NaN's bits are above an infinity's; both are scaled)
-      const float top = row_max4(__uint_as_float(min(most, 0x7f80u) << 16));
-      // (an infinity leaves zeros and infinities: its head's result is NaN)
-      const int e = top >= 65536.0f ? min(((__float_as_int(top) >> 23) & 255) - 127, 127) - 14 : 0;
-      const float down = pow2i(-e);
-      cq[n] *= pow2i(e);
+    for (int k = 0; k < 16 + TS; ++k) {
+      const uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
+      uint32_t f[4];
 #pragma unroll
-      for (int k = 0; k < 16 + TS; ++k) {
-        const uint32_t w[4] = {q[n][k].x, q[n][k].y, q[n][k].z, q[n][k].w};
-        uint32_t f[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          f[i] = pack_f16(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down);
-        q[n][k] = make_uint4(f[0], f[1], f[2], f[3]);
-      }
+      for (int i = 0; i < 4; ++i)
+        f[i] = pack_f16(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down);
+      q[k] = make_uint4(f[0], f[1], f[2], f[3]);
     }
 #pragma unroll 1
     for (; t < t1; ++t) {
@@ -264,9 +235,7 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
       const h16x2_t s01 = kv4_scales<false>(sc.x), s23 = kv4_scales<true>(sc.x);
       const h16x2_t s45 = kv4_scales<false>(sc.y), s67 = kv4_scales<true>(sc.y);
       const _Float16 sv[9] = {s01[0], s01[1], s23[0], s23[1], s45[0], s45[1], s67[0], s67[1], kv4_scales<false>(tsc)[0]};
-      f32x4_t s[NB];
-#pragma unroll
-      for (int n = 0; n < NB; ++n) s[n] = f32x4_t{0, 0, 0, 0};
+      f32x4_t s = {0, 0, 0, 0};
       lds_barrier();
       uint32_t to = v_put;
       asm volatile("" : "+v"(to));
@@ -275,8 +244,7 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
         const uint32_t w[4] = {code[(k / 4) % 4].x, code[(k / 4) % 4].y, code[(k / 4) % 4].z, code[(k / 4) % 4].w};
         const uint4 x = kv4_values(k < 16 ? w[k % 4] : (k == 16 ? tail.x : tail.y), sv[k / 2]);
         if (k < 16) put_v(to, k, x);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) s[n] = mfma_f16_16x16x32(x, q[n][k], s[n]);
+        s = mfma_f16_16x16x32(x, q[k], s);
       }
       const bool valid = row != nullptr;
       row = source(i1, p1);
@@ -288,33 +256,26 @@ __global__ void __launch_bounds__(256, HB <= 32 ? 2 : 1) kv4_attn_kernel(const K
 
   // ---- sums of the waves' keys, output
   lds_barrier();
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    l[n] = row_sum4(l[n]);
-    if (g == 0) *(__attribute__((address_space(3))) float*)(m_base + ((16 * n + l16) * 4 + wave) * 4) = l[n];
-  }
+  l = row_sum4(l);
+  if (g == 0) *(__attribute__((address_space(3))) float*)(m_base + (l16 * 4 + wave) * 4) = l;
   lds_barrier();
+  const f32x4_t w = *(__attribute__((address_space(3))) f32x4_t*)(m_base + l16 * 16);
+  l = (w[0] + w[1]) + (w[2] + w[3]);
+  if (h >= a.H) return;
+  if (a.nsplit > 1) {
+    const long at = ((long)r * a.H + h) * a.nsplit + sp;
+    if (wave == 0 && g == 0) *(float2*)(a.part + 2 * at) = make_float2(m, l);
+    float* dst = a.part + 2L * a.R * a.H * a.nsplit + at * 512 + wave * 128 + 4 * g;
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const f32x4_t w = *(__attribute__((address_space(3))) f32x4_t*)(m_base + (16 * n + l16) * 16);
-    l[n] = (w[0] + w[1]) + (w[2] + w[3]);
-    const int h = h0 + 16 * n + l16;
-    if (h >= a.H) continue;
-    if (a.nsplit > 1) {
-      const long at = ((long)r * a.H + h) * a.nsplit + sp;
-      if (wave == 0 && g == 0) *(float2*)(a.part + 2 * at) = make_float2(m[n], l[n]);
-      float* dst = a.part + 2L * a.R * a.H * a.nsplit + at * 512 + wave * 128 + 4 * g;
+    for (int c = 0; c < 8; ++c) *(float4*)(dst + 16 * c) = make_float4(o[c][0], o[c][1], o[c][2], o[c][3]);
+  } else {
+    const float den = l + exp2f(a.sink[h] * kLog2e - m);
+    const float inv = m == -__builtin_inff() ? 0.0f : 1.0f / den;  // (no key: zeros)
+    uint16_t* dst = a.out + ((long)r * a.H + h) * 512 + wave * 128 + 4 * g;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) *(float4*)(dst + 16 * c) = make_float4(o[n][c][0], o[n][c][1], o[n][c][2], o[n][c][3]);
-    } else {
-      const float den = l[n] + exp2f(a.sink[h] * kLog2e - m[n]);
-      const float inv = m[n] == -__builtin_inff() ? 0.0f : 1.0f / den;  // (no key: zeros)
-      uint16_t* dst = a.out + ((long)r * a.H + h) * 512 + wave * 128 + 4 * g;
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        *(uint2*)(dst + 16 * c) = finish4(a, pos, wave * 128 + 16 * c + 4 * g,
-                                          make_float4(o[n][c][0] * inv, o[n][c][1] * inv, o[n][c][2] * inv, o[n][c][3] * inv));
-    }
+    for (int c = 0; c < 8; ++c)
+      *(uint2*)(dst + 16 * c) = finish4(a, pos, wave * 128 + 16 * c + 4 * g,
+                                        make_float4(o[c][0] * inv, o[c][1] * inv, o[c][2] * inv, o[c][3] * inv));
   }
 }
 
@@ -355,76 +316,71 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const Kv4AttnArgs a) {
 }
 
 struct Plan {
-  bool many;  // the cache's rows decoded once, the 64-head kernel (window and cache in one list)
+  bool many;  // the cache's rows decoded first
   int wtiles, tiles, nsplit, chunk, groups;
   long list, rows, part;  // bytes of the workspace
 };
 
-// Splits of the tiles until each of the card's CUs has a workgroup: two on a CU cost more in partial results than they
-// hide (4 sequences of 64 heads and 2048 rows: 20.3 us with 256, 24.4 with 512, 37.3 with 1024, 26.0 with 128).
-void split(Plan& p, long units) {
-  const long want = 256;
-  if (p.tiles == 0) p.tiles = 1;  // (no key at all: zeros)
-  long ns = units >= want ? 1 : (want + units - 1) / units;
-  if (ns > p.tiles) ns = p.tiles;
-  p.chunk = (int)((p.tiles + ns - 1) / ns);
-  p.nsplit = (p.tiles + p.chunk - 1) / p.chunk;
-}
-
 Plan plan_of(int R, int H, int wt, int t, int dim, long rows) {
   Plan p{};
-  p.groups = (H + 63) / 64;
-  // Decoding first pays with more than half a group of 64 heads (512 rows of 2048 keys: 64 heads 203 us for 357, 32 heads
-  // 198 for 186), when the lists name 2^17 rows (2048 each: 64 query rows 56 us for 67, 32 of them 47 for 45; 512 each:
-  // 602 rows 109 for 157, 150 of them 65 for 53) and each row of the cache eight times.
-  p.many = rows > 0 && H > 32 && (long)R * t >= 1L << 17 && (long)R * t >= 8 * rows;
+  // Decoding first, then the bf16 kernel of 64 heads a workgroup, pays with more than half of them (512 query rows of 2048
+  // keys: 64 heads 185 us for 360, 32 heads 180 for 187, 16 heads 178 for 99), from 32 query rows (40 of 512 keys 30.3 us for
+  // 31.5, 80 34.7 for 36.7, 150 37.2 for 53.2) and with each row of the cache listed four times (2048 keys of 16384 rows: 32
+  // query rows 39.7 us for 45.6, 16 36.6 for 30.9).  The bf16 kernel's grid ends at 65535 query rows.
+  p.many = rows > 0 && H > 32 && R >= 32 && R <= 65528 && (long)R * t >= 4 * rows;
   if (p.many) {
-    p.tiles = (wt + t + 31) / 32;
-    split(p, (long)R * p.groups);
     p.list = ((long)R * (wt + t) * 4 + 255) & ~255L;
     p.rows = (rows * dim * 2 + 255) & ~255L;
-  } else {
-    p.groups = (H + 15) / 16;
-    p.wtiles = (wt + 63) / 64;
-    p.tiles = p.wtiles + (t + 63) / 64;
-    split(p, (long)R * p.groups);
+    p.part = dsv41_attn_workspace_bytes(R, H, wt + t, 512, 0);
+    return p;
   }
+  p.groups = (H + 15) / 16;
+  p.wtiles = (wt + 63) / 64;
+  p.tiles = p.wtiles + (t + 63) / 64;
+  if (p.tiles == 0) p.tiles = 1;  // (no key at all: zeros)
+  // Splits of the tiles until each of the card's CUs has a workgroup: two on a CU cost more in partial results than they
+  // hide (4 sequences of 64 heads and 2048 rows: 20.3 us with 256, 24.4 with 512, 37.3 with 1024, 26.0 with 128).
+  const long units = (long)R * p.groups, want = (256 + units - 1) / units;
+  const long ns = want < p.tiles ? want : p.tiles;
+  p.chunk = (int)((p.tiles + ns - 1) / ns);
+  p.nsplit = (p.tiles + p.chunk - 1) / p.chunk;
   p.part = p.nsplit > 1 ? 4L * R * H * p.nsplit * 514 : 0;
   return p;
 }
 
-template <int HB, int DQK>
-void launch(const Kv4AttnArgs& a, hipStream_t st) {
-  kv4_attn_kernel<HB, DQK><<<(unsigned)((long)a.R * a.groups * a.nsplit), 256, 0, st>>>(a);
-}
-
-int run(Kv4AttnArgs& a, int dqk, int b, void* ws, long ws_bytes, hipStream_t st) {
+// Batch rows b of a prompt, 0: single tokens.
+int run(Kv4AttnArgs& a, int dqk, int b, float scale, void* ws, long ws_bytes, hipStream_t st) {
   const long rows = b > 0 ? (long)b * a.map.cols << a.map.shift : 0;
   const Plan p = plan_of(a.R, a.H, a.pos ? a.win_rows : a.wt, a.t, dqk, rows);
+  const long need = p.list + p.rows + p.part;
+  if (need > 0 && (!ws || ((uintptr_t)ws & 15) || ws_bytes < need)) return (int)hipErrorInvalidValue;
+  void* const part = (char*)ws + p.list + p.rows;
+  if (p.many) {
+    const long l = (long)a.wt + a.t, n = rows / b, pages = rows >> a.map.shift;
+    if (l >= (1L << 31) || a.win_rows + n >= (1L << 31) || pages + a.R >= (1L << 31)) return (int)hipErrorInvalidValue;
+    int* const list = (int*)ws;
+    void* const table = (char*)ws + p.list;
+    kv4_unpack_launch(a, dqk, b, table, list, st);
+    DSV41_CHECK_LAUNCH();
+    if (a.win_rows > 0)
+      return dsv41_sparse_attn_kv2(a.q, a.win, table, a.sink, list, a.out, b, a.rows_per_slot, a.H, dqk, 512, a.win_rows,
+                                   a.win_sstride, (int)n, n * dqk, (int)l, l, scale, 0, part, p.part, st);
+    return dsv41_sparse_attn(a.q, table, a.sink, list, a.out, b, a.rows_per_slot, a.H, dqk, 512, (int)n, n * dqk, (int)l,
+                             scale, 0, part, p.part, st);
+  }
+  a.scale = scale * kLog2e;
   a.wtiles = p.wtiles;
   a.tiles = p.tiles;
   a.nsplit = p.nsplit;
   a.chunk = p.chunk;
   a.groups = p.groups;
+  a.part = (float*)part;
   if ((long)a.R * a.groups * a.nsplit >= (1L << 31) || (long)a.R * a.H >= (1L << 31)) return (int)hipErrorInvalidValue;
-  const long need = p.list + p.rows + p.part;
-  if (need > 0 && (!ws || ((uintptr_t)ws & 15) || ws_bytes < need)) return (int)hipErrorInvalidValue;
-  a.part = (float*)((char*)ws + p.list + p.rows);
-  if (p.many) {
-    if ((long)a.wt + a.t + a.win_rows + (rows / b) >= (1L << 31) || rows / (1 << a.map.shift) + a.R >= (1L << 31))
-      return (int)hipErrorInvalidValue;
-    int* const list = (int*)ws;
-    uint16_t* const decoded = (uint16_t*)((char*)ws + p.list);
-    kv4_unpack_launch(a, dqk, b, decoded, list, st);
-    DSV41_CHECK_LAUNCH();
-    a.n2 = (int)(rows / b);
-    a.pool = (const uint8_t*)decoded;
-    a.idx = list;
-    a.t += a.wt;
-    kv4_attn64_launch(a, dqk, st);
-  } else {
-    dqk == 512 ? launch<16, 512>(a, st) : launch<16, 576>(a, st);
-  }
+  const unsigned grid = (unsigned)((long)a.R * a.groups * a.nsplit);
+  if (dqk == 512)
+    kv4_attn_kernel<512><<<grid, 256, 0, st>>>(a);
+  else
+    kv4_attn_kernel<576><<<grid, 256, 0, st>>>(a);
   DSV41_CHECK_LAUNCH();
   if (a.nsplit > 1) {
     kv4_combine_kernel<<<a.R * a.H, 128, 0, st>>>(a);
@@ -435,7 +391,7 @@ int run(Kv4AttnArgs& a, int dqk, int b, void* ws, long ws_bytes, hipStream_t st)
 
 bool attn_ok(const Kv4AttnArgs& a, const dsv41_kv4* c) {
   return kv4_ok(c) && a.q && a.H > 0 && a.sink && a.out && a.t >= 0 && (a.t == 0 || a.idx) &&
-         (((uintptr_t)a.q | (uintptr_t)a.win) & 15) == 0 && ((uintptr_t)a.out & 7) == 0 && a.win_sstride % 8 == 0;
+         (((uintptr_t)a.q | (uintptr_t)a.win | (uintptr_t)a.out) & 15) == 0 && a.win_sstride % 8 == 0;
 }
 
 }  // namespace
@@ -468,7 +424,6 @@ int dsv41_sattn4(const dsv41_kv4* c, const void* q, const void* kv_win, long win
   a.pos = pos;
   a.pmax = pmax;
   a.plim = plim;
-  a.scale = scale * kLog2e;
   a.sink = sink;
   a.cos_t = cos_t;
   a.sin_t = sin_t;
@@ -481,7 +436,7 @@ int dsv41_sattn4(const dsv41_kv4* c, const void* q, const void* kv_win, long win
   a.q_rstride = (long)h * c->dim;
   a.pool = (const uint8_t*)c->pool;
   a.map = kv4_map(*c);
-  return run(a, c->dim, 0, ws, ws_bytes, (hipStream_t)stream);
+  return run(a, c->dim, 0, scale, ws, ws_bytes, (hipStream_t)stream);
 }
 
 int dsv41_sparse_attn4(const dsv41_kv4* c, const void* q, const void* kv, long kv_bstride, int n_kv, const int* widx,
@@ -502,14 +457,13 @@ int dsv41_sparse_attn4(const dsv41_kv4* c, const void* q, const void* kv, long k
   a.t = t;
   a.rows_per_slot = s;
   a.seq = seq;
-  a.scale = scale * kLog2e;
   a.sink = sink;
   a.out = (uint16_t*)out;
   if (!attn_ok(a, c) || wt < 0 || n_kv < 0 || (wt > 0 && (!kv || !widx))) return (int)hipErrorInvalidValue;
   a.q_rstride = (long)h * c->dim;
   a.pool = (const uint8_t*)c->pool;
   a.map = kv4_map(*c);
-  return run(a, c->dim, b, ws, ws_bytes, (hipStream_t)stream);
+  return run(a, c->dim, b, scale, ws, ws_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -16,7 +16,6 @@ struct Kv4AttnArgs {
   Kv4Table map;
   const int* idx;       // [R, t]
   int t;
-  int n2;               // many rows: the decoded rows of a slot
   int rows_per_slot;    // query row r belongs to batch row r / rows_per_slot
   const long* seq;      // per batch row: its sequence (null: itself)
   const long* pos;      // ring: per row
@@ -71,6 +70,5 @@ DSV41_DEV uint2 finish4(const Kv4AttnArgs& a, long pos, int c, float4 o) {
 
 }  // namespace
 
-// Many query rows: rows and lists made ready (kv4_unpack.hip), the 64-head kernel (kv4_attn64.hip).
+// Many query rows: the cache's rows in bf16, [b, slots' rows, dim], and one list of window and cache rows [R, wt + t].
 void kv4_unpack_launch(const Kv4AttnArgs& a, int dim, int b, void* rows, int* list, hipStream_t st);
-void kv4_attn64_launch(const Kv4AttnArgs& a, int dqk, hipStream_t st);
