@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
   // the keys 4 further, are an XOR away
   const uint32_t v_put = v_base + key * 1024 + 256 * g + (v_swizzle(key) << 4);
   const uint32_t v_get = v_base + (g * 8 + (l16 >> 2)) * 1024 + wave * 256 +
-                         (((((l16 & 3) >> 1) ^ (g & 1)) | (l16 >> 2) << 1) << 4) + (l16 & 1) * 8;
+                         ((((l16 & 3) >> 1) | ((l16 >> 2) << 1 ^ (g & 1) << 3)) << 4) + (l16 & 1) * 8;
 
   // the softmax of a tile's scores and the product with its values in LDS
   auto attend = [&](f32x4_t& s, bool valid, auto f16) {
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
         (uint64_t)pk.y << 32 | pk.x;
     lds_barrier();
     uint32_t va = v_get;
-    asm volatile("" : "+v"(va));  // (eight addresses computed anew: as the loops' invariants they would fill the registers)
+    asm volatile("" : "+v"(va));  // (addresses computed anew: as the loops' invariants they would fill the registers)
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       const uint4 pb = __builtin_bit_cast(
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
         uint2 v[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-          v[u] = lds_read_tr((va ^ ((2 * c ^ 8 * u) << 4)) + u * 4096 + kk * 32768);
+          v[u] = lds_read_tr((va ^ ((2 * c + u) << 4)) + u * 4096 + kk * 32768);
         const uint4 av = make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
         o[c] = F16 ? mfma_f16_16x16x32(av, pb, o[c]) : mfma_bf16_16x16x32(av, pb, o[c]);
       }

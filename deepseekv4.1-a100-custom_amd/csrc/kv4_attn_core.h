@@ -54,8 +54,8 @@ DSV41_DEV uint2 lds_read_tr(uint32_t addr) {
 }
 
 // The values in LDS: row `key` of 1024 bytes, its 16-byte unit u at u ^ swizzle(key), so that neither the writes (16 keys,
-// one unit each) nor the transpose reads (4 keys by 16 columns a group of lanes) meet in a bank.
-DSV41_DEV uint32_t v_swizzle(int key) { return ((key & 7) << 1) | ((key >> 3) & 1); }
+// one unit each) nor the transpose reads (eight keys at a time, four and the four eight on, 32 bytes each) meet in a bank.
+DSV41_DEV uint32_t v_swizzle(int key) { return ((key & 3) << 1) | (key & 8) | ((key >> 2) & 1); }
 
 // Output of one (row, head, 4 columns from c on): the inverse rotation, one rounding.
 DSV41_DEV uint2 finish4(const Kv4AttnArgs& a, long pos, int c, float4 o) {
