@@ -96,7 +96,8 @@ class SparseAttention:
     [slots, cap, D], index keys [slots, cap, 128] (bf16, the reference storage; with e4m3=True also an e4m3 copy +
     per-row scales, which the selection then reads), compressor rings [slots, 8, D].  With kv4, a kv4.PagedKV4 of rows of
     head_dim (512), the compressed rows are held there in 4 bits instead: a call takes the pages that its rows need, and a
-    sequence's pages may be forked, released and compacted between calls.  The rows' values are the same."""
+    sequence's pages may be forked, released and compacted between calls; kv4.check() tells of a pool that ran out.  The
+    rows' values are the same."""
 
     def __init__(self, weights: dict, *, n_heads: int, head_dim: int, rope_head_dim: int, window: int, ratio: int,
                  index_n_heads: int, index_topk_k: int, cos: torch.Tensor, sin: torch.Tensor, slots: int, cap: int,
@@ -111,6 +112,8 @@ class SparseAttention:
         dev = cos.device
         self.sink = weights["attn_sink"].float().contiguous()
         self.ring = torch.zeros(slots, window, head_dim, dtype=torch.bfloat16, device=dev)
+        if kv4 is not None and not ratio:
+            raise ValueError("SparseAttention: a layer without compressed rows has none for a 4-bit cache")
         if ratio:
             self.cap = cap
             if kv4 is None:
@@ -154,13 +157,14 @@ class SparseAttention:
             ratio = self.ratio
             end = start_pos + s
             clen = end // ratio
-            if clen > self.cap:
-                raise RuntimeError(f"SparseAttention: {clen} compressed rows exceed the cache capacity {self.cap}")
+            paged = isinstance(self.ckv, PagedKV4)  # (its attention takes the two index lists apart)
+            cap = self.cap if paged else self.ckv.shape[1]
+            if clen > cap:
+                raise RuntimeError(f"SparseAttention: {clen} compressed rows exceed the cache capacity {cap}")
             ckv, cscore = compressor_proj(x, w["c_wkv"], w["c_wgate"])
             latent = compress_pool(ckv, cscore, start_pos, ratio, self.ring_kv[:b], self.ring_score[:b],
                                    w["c_norm_w"], eps)
             new = latent is not None and latent.shape[1] > 0
-            paged = isinstance(self.ckv, PagedKV4)  # (its attention takes the two index lists apart)
             ww = 0 if paged else widx.shape[-1]
             kk = min(self.topk, clen)
             idx = torch.empty(b, s, ww + kk, dtype=torch.int32, device=x.device)

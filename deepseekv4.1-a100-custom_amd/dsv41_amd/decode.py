@@ -31,7 +31,6 @@ class DecodeLayer:
         self.ratio, self.topk, self.rd, self.dv, self.eps = ratio, topk, rd, dv, eps
         self.kbf16 = kbf16
         self.nw_tab = None if nw_tab is None else nw_tab.to(device=ring.device, dtype=torch.int64).contiguous()
-        self.paged = isinstance(ckv, PagedKV4)
         if self.paged and (dv != 512 or ring.shape[-1] != ckv.dim):
             raise ValueError(f"DecodeLayer: values of {dv} in rows of {ring.shape[-1]} beside a cache of {ckv.dim}")
         self.scale = (ckv.dim if self.paged else ckv.shape[-1]) ** -0.5
@@ -39,6 +38,10 @@ class DecodeLayer:
         self._qbufs = {}
         self._attn_ws = {}
         self._prepared = None
+
+    @property
+    def paged(self) -> bool:
+        return isinstance(self.ckv, PagedKV4)
 
     def _qbuf(self, B, dev):
         buf = self._qbufs.get(B)

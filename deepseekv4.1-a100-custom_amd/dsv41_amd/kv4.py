@@ -15,7 +15,7 @@ values and 336 a row of 576 instead of 1024 and 1152, in pages that sequences sh
   c.copy_pages(other, src, dst)          pages out of another pool
 
 Every call is asynchronous on the current stream, synchronises with nothing and may be captured; calls on one cache must
-be stream-ordered.  What a call cannot do on the device -- too few free pages, an index out of range, a row without a page --
+be stream-ordered.  Index arguments are tensors or lists (captured calls: tensors on the GPU).  What a call cannot do on the device -- too few free pages, an index out of range, a row without a page --
 it leaves out and notes in the cache's error word, which check() raises for (every call does with DSV41_CHECK_ERRORS=1).
 
 Forward only, as everything here."""
@@ -36,6 +36,7 @@ _ERRORS = ((1, "too few free pages"), (2, "an entry was left out (an index out o
            (4, "a row was dropped (no page of the sequence's own there, or no rope angle)"))
 _MOST_ENTRIES = 4096
 _I64, _I32, _BF16 = torch.int64, torch.int32, torch.bfloat16
+_INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 
 class _Cache(ctypes.Structure):
@@ -65,7 +66,7 @@ class PagedKV4:
             raise ValueError("PagedKV4: contiguous tensors, the pool 16-byte aligned")
         self.index = _index(pool, table, refs)
         self.device = torch.device("cuda", self.index)
-        self.pool, self.table, self.refs, self.dim = pool, table, refs, dim
+        self._pool, self._table, self._refs, self.dim = pool, table, refs, dim
         self.pages, self.page = pool.shape[:2]
         self.slots, self.cols = table.shape
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -83,13 +84,23 @@ class PagedKV4:
                    torch.full((slots, -(-cap // page)), -1, dtype=torch.int32, device=device),
                    torch.zeros(pages, dtype=torch.int32, device=device), dim)
 
+    # (what the calls work on is fixed: the tensors' contents change, the tensors do not)
+    pool = property(lambda self: self._pool)
+    table = property(lambda self: self._table)
+    refs = property(lambda self: self._refs)
+
     def _i64(self, name: str, t, n: int) -> torch.Tensor:
         """n index entries as contiguous int64 on the cache's GPU (from a tensor or a list)."""
         if not isinstance(t, torch.Tensor):
-            t = torch.as_tensor(t, dtype=_I64)
+            t = torch.as_tensor(t)
+            t = t.to(_I64) if t.numel() == 0 else t
         if t.numel() != n:
             raise RuntimeError(f"{name}: {t.numel()} entries beside {n}")
         if t.dtype is not _I64 or t.get_device() != self.index or not t.is_contiguous():
+            if t.dtype not in _INTEGERS:
+                raise RuntimeError(f"{name}: entries of {t.dtype} (integers)")
+            if not t.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"{name}: entries in host memory in a captured call (a replay would read them again)")
             t = t.to(device=self.device, dtype=_I64, non_blocking=True).contiguous()
         return t
 
@@ -125,7 +136,8 @@ class PagedKV4:
     def append_decode(self, latent: torch.Tensor, seq, pos, ratio: int, cos: torch.Tensor, sin: torch.Tensor,
                       rd: int) -> None:
         """append of a decode step (dsv41/decode.py:157-164): latent[i] to the row of the group that position pos[i] closes,
-        row (pos[i] + 1) / ratio - 1; positions that close none leave the cache alone (no spare row)."""
+        row (pos[i] + 1) / ratio - 1; positions that close none, or are not in 0 .. 2^31 - 1, leave the cache alone (no spare
+        row)."""
         self._append(latent, seq, pos, ratio, 1, cos, sin, rd)
 
     def _append(self, latent, seq, row, ratio: int, by_pos: int, cos, sin, rd: int) -> None:
@@ -259,6 +271,8 @@ def _indices(name: str, idx, shape: tuple, index: int):
         return None, 0
     if idx.shape[:-1] != shape or idx.get_device() != index:
         raise RuntimeError(f"{name}: indices {tuple(idx.shape)} on {idx.device} for {shape}")
+    if idx.dtype not in _INTEGERS:
+        raise RuntimeError(f"{name}: indices of {idx.dtype} (integers)")
     if idx.dtype != torch.int32:
         idx = idx.clamp(-1, 2 ** 31 - 1).to(torch.int32)
     idx = idx.contiguous()

@@ -173,6 +173,32 @@ def test_append_decode(ratio):
     assert torch.equal(a.pool, b.pool) and sum(r >= 0 for r in row) >= 4
 
 
+def test_index_arguments(monkeypatch):
+    """Lists and tensors of any integer type are the same; others, and host memory in a capture, are refused; the tensors of
+    a cache stay."""
+    from dsv41_amd.kv4 import PagedKV4, sparse_attn4
+    c = PagedKV4.empty(4, 2, 40, 512, 16, DEV)
+    c.reserve([0, 1], torch.tensor([0, 0], dtype=torch.int32), torch.tensor([20, 3], dtype=torch.int16, device=DEV))
+    c.append(torch.full((2, 512), 6.0, dtype=BF, device=DEV), torch.tensor([0, 9, 1, 9], device=DEV)[::2], [19, 2], 4, None, None, 0)
+    c.check()
+    assert c.read([0, 1], torch.tensor([19, 2], dtype=torch.uint8)).eq(6).all() and c.read([], []).shape == (0, 512)
+    q, sink = torch.zeros(1, 1, 16, 512, dtype=BF, device=DEV), torch.zeros(16, device=DEV)
+    for bad in (torch.tensor([0.0, 1.0]), [0.5, 1.0], torch.tensor([True, False], device=DEV)):
+        with pytest.raises(RuntimeError, match="integers"):
+            c.release(bad)
+    with pytest.raises(RuntimeError, match="integers"):
+        sparse_attn4(q, None, c, sink, None, torch.zeros(1, 1, 4, device=DEV), 1.0)
+    for name in ("pool", "table", "refs"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name).clone())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    on = torch.tensor([0, 1], device=DEV)
+    c.reserve(on, on, on.to(torch.int32))
+    for bad in ([0, 1], torch.tensor([0, 1])):
+        with pytest.raises(RuntimeError, match="host memory"):
+            c.release(bad)
+
+
 def test_append_strided_rows_and_far_offsets():
     """Rows cut out of wider ones; and a page whose bytes stand past 2^32 of the pool."""
     from dsv41_amd.kv4 import PagedKV4
@@ -778,6 +804,8 @@ def test_attention_layer_over_a_4_bit_cache(b):
         assert torch.equal(one.ring, two.ring)
         _alike(p, o, max(one.ckv.abs().max().item(), one.ring.abs().max().item(), 1.0))
     c.check()
+    with pytest.raises(ValueError, match="without compressed rows"):
+        SparseAttention(w, kv4=c, **dict(kw, ratio=0))
     with pytest.raises(RuntimeError, match="capacity"):
         two.attend(x[:, :1], 2 * cap + 1)
     for bad in (PagedKV4.empty(9, b, cap, 576, 32, DEV), PagedKV4.empty(9, b, cap - 40, D, 32, DEV)):

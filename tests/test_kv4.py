@@ -36,7 +36,7 @@ def test_cache_refuses():
 def _cache(dim=576):
     """A cache's handle without a GPU behind it, to reach the checks of arguments (no call below gets past them)."""
     c = kv4.PagedKV4.__new__(kv4.PagedKV4)
-    c.pool, c.table, c.refs = _tensors(dim=dim)
+    c._pool, c._table, c._refs = _tensors(dim=dim)
     c.dim, c.pages, c.page, c.slots, c.cols, c.device, c.index = dim, 4, 16, 2, 3, torch.device("cpu"), -1
     return c
 
