@@ -107,6 +107,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
   const uint32_t v_get = v_base + (g * 8 + (l16 >> 2)) * 1024 + wave * 256 +
                          ((((l16 & 3) >> 1) | ((l16 >> 2) << 1 ^ (g & 1) << 3)) << 4) + (l16 & 1) * 8;
 
+  const uint32_t p_put = p_base + l16 * 128 + (((wave * 2 + (g >> 1)) ^ (l16 & 7)) << 4) + (g & 1) * 8;
+
   // the softmax of a tile's scores and the product with its values in LDS
   auto attend = [&](f32x4_t& s, bool valid, auto f16) {
     constexpr bool F16 = decltype(f16)::value;
@@ -115,30 +117,31 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     for (int i = 0; i < 4; ++i) s[i] = (mask >> i & 1) ? s[i] * cq : -__builtin_inff();
     float mx = row_max4(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
     if (g == 0) *(__attribute__((address_space(3))) float*)(m_base + (l16 * 4 + wave) * 4) = mx;
+    // the probabilities by the reference as it stands; where the tile then turns out to move it, once more
+    float p[4];
+    auto probabilities = [&]() {
+      const float ref = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+      const uint2 pk = F16 ? make_uint2(pack_f16(p[0], p[1]), pack_f16(p[2], p[3]))
+                           : make_uint2(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]));
+      *(__attribute__((address_space(3))) uint64_t*)p_put = (uint64_t)pk.y << 32 | pk.x;
+    };
+    probabilities();
     lds_barrier();
     const f32x4_t w = *(__attribute__((address_space(3))) f32x4_t*)(m_base + l16 * 16);
     mx = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
     if (__any(mx > m + 8.0f)) {  // (alike in every wave: all have the same maxima)
       const float to = fmaxf(m, mx);
-      const float f = to > m ? exp2f(m - to) : 1.0f;
+      const float f = to > m ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
       m = to;
       l *= f;
 #pragma unroll
       for (int c = 0; c < 8; ++c) o[c] *= f;
+      probabilities();
+      lds_barrier();
     }
-    const float ref = m == -__builtin_inff() ? 0.0f : m;
-    float p[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      p[i] = exp2f(s[i] - ref);
-      l += p[i];
-    }
-    const uint2 pk = F16 ? make_uint2(pack_f16(p[0], p[1]), pack_f16(p[2], p[3]))
-                         : make_uint2(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]));
-    *(__attribute__((address_space(3))) uint64_t*)(p_base + l16 * 128 +
-                                                   (((wave * 2 + (g >> 1)) ^ (l16 & 7)) << 4) + (g & 1) * 8) =
-        (uint64_t)pk.y << 32 | pk.x;
-    lds_barrier();
+    l += (p[0] + p[1]) + (p[2] + p[3]);
     uint32_t va = v_get;
     asm volatile("" : "+v"(va));  // (addresses computed anew: as the loops' invariants they would fill the registers)
 #pragma unroll
