@@ -48,8 +48,15 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
 
   const int key = wave * 16 + l16;  // this lane's key of a tile
 
+  typedef const __attribute__((address_space(1))) uint8_t* row_t;
+  row_t none = (row_t)g_kv4_none;  // (its address read once)
+  asm volatile("" : "+s"(none));
+
+  auto get16 = [](row_t p) { return __builtin_bit_cast(uint4, *(const __attribute__((address_space(1))) u32x4*)p); };
+  auto get8 = [](row_t p) { return __builtin_bit_cast(uint2, *(const __attribute__((address_space(1))) u32x2*)p); };
+
   // the row of the window that this lane's key of tile u is, nullptr: none
-  auto window = [&](int u) -> const uint16_t* {
+  auto window = [&](int u) -> row_t {
     const int j = u * 64 + key;
     long row = -1;
     if (a.widx) {
@@ -62,29 +69,28 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
       const long held = pmax - d;
       if (held >= 0 && held <= plim && pos - held < a.win_rows && seq >= 0 && seq < a.win_slots) row = j;
     }
-    return row >= 0 ? a.win + (a.widx ? (long)slot : seq) * a.win_sstride + row * DQK : nullptr;
+    return row >= 0 ? (row_t)(a.win + (a.widx ? (long)slot : seq) * a.win_sstride + row * DQK) : nullptr;
   };
   // the cache's rows
   const int* const ids = a.idx + (long)r * a.t;
   const long rows = (long)a.map.cols << a.map.shift;
   const bool known = seq >= 0 && seq < a.map.slots;
   const int* const pages = a.map.table + (known ? seq : 0) * a.map.cols;
-  // the index of this lane's key of tile u, -1: none
-  auto index = [&](int u) {
-    const int j = (u - a.wtiles) * 64 + key;
-    return j < a.t && u < t1 ? ids[j] : -1;
-  };
-  auto there = [&](int i) { return known && i >= 0 && i < rows; };
-  auto source = [&](int i, int p) -> const uint8_t* {
-    return there(i) && (unsigned)p < (unsigned)a.map.pages ? a.pool + kv4_offset(a.map, p, i, RB) : nullptr;
+  // the way to this lane's key of tile u (where the list ends, the last entry's, which source() then leaves out)
+  auto index = [&](int u) { return ids[min((u - a.wtiles) * 64 + key, a.t - 1)]; };
+  auto page = [&](int i) { return pages[i >= 0 && i < rows ? i >> a.map.shift : 0]; };
+  auto source = [&](int u, int i, int p) -> row_t {
+    const bool there = known && u < t1 && (u - a.wtiles) * 64 + key < a.t && i >= 0 && i < rows;
+    return there && (unsigned)p < (unsigned)a.map.pages ? (row_t)(a.pool + kv4_offset(a.map, p, i, RB)) : nullptr;
   };
   // The way to the first tile's rows, two loads deep, is gone before Q is asked for.
   int t = t0;
-  const uint16_t* wrow = t < min(t1, a.wtiles) ? window(t) : nullptr;
-  int i0 = -1, p0 = -1;
-  if (t0 >= a.wtiles && t0 < t1) {
+  row_t wrow = t < min(t1, a.wtiles) ? window(t) : nullptr;
+  int i0 = -1, i1 = -1, p0 = -1;
+  if (t0 >= a.wtiles && t0 < t1 && a.t > 0) {
     i0 = index(t0);
-    p0 = pages[there(i0) ? i0 >> a.map.shift : 0];
+    i1 = index(t0 + 1);
+    p0 = page(i0);
   }
 
   // Q: head l % 16, quarter l / 16 of the 512 columns, in k steps of 8
@@ -144,19 +150,26 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     l += (p[0] + p[1]) + (p[2] + p[3]);
     uint32_t va = v_get;
     asm volatile("" : "+v"(va));  // (addresses computed anew: as the loops' invariants they would fill the registers)
+    auto values = [&](int i) {  // of column block i % 8, keys 32 (i / 8) ..
+      const int c = i % 8, at = i / 8 * 32768;
+      const uint2 lo = lds_read_tr((va ^ ((2 * c) << 4)) + at), hi = lds_read_tr((va ^ ((2 * c + 1) << 4)) + 4096 + at);
+      return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    };
+    // (reads five products ahead, pinned: the compiler kept one or two in flight, and more than 15 wait for one another)
+    constexpr int kAhead = 4;
+    uint4 pb[2], v[16];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      const uint4 pb = __builtin_bit_cast(
+    for (int kk = 0; kk < 2; ++kk)
+      pb[kk] = __builtin_bit_cast(
           uint4, *(__attribute__((address_space(3))) u32x4*)(p_base + l16 * 128 + (((kk * 4 + g) ^ (l16 & 7)) << 4)));
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint2 v[2];
+    for (int i = 0; i < kAhead; ++i) v[i] = values(i);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          v[u] = lds_read_tr((va ^ ((2 * c + u) << 4)) + u * 4096 + kk * 32768);
-        const uint4 av = make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
-        o[c] = F16 ? mfma_f16_16x16x32(av, pb, o[c]) : mfma_bf16_16x16x32(av, pb, o[c]);
-      }
+    for (int i = 0; i < 16; ++i) {
+      if (i + kAhead < 16) v[i + kAhead] = values(i + kAhead);
+      o[i % 8] = F16 ? mfma_f16_16x16x32(v[i], pb[i / 8], o[i % 8]) : mfma_bf16_16x16x32(v[i], pb[i / 8], o[i % 8]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   auto put_v = [&](uint32_t to, int k, uint4 x) {
@@ -167,10 +180,10 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
 #pragma unroll 1
   for (; t < min(t1, a.wtiles); ++t) {
     const bool valid = wrow != nullptr;
-    const uint16_t* src = valid ? wrow : (const uint16_t*)g_kv4_none;
+    row_t src = valid ? wrow : none;
     uint4 x[16 + TS];
 #pragma unroll
-    for (int k = 0; k < 16 + TS; ++k) x[k] = *(const uint4*)(src + (k < 16 ? 128 * g + 8 * k : 512 + 16 * g + 8 * (k - 16)));
+    for (int k = 0; k < 16 + TS; ++k) x[k] = get16(src + 2 * (k < 16 ? 128 * g + 8 * k : 512 + 16 * g + 8 * (k - 16)));
     if (t + 1 < min(t1, a.wtiles)) wrow = window(t + 1);
     f32x4_t s = {0, 0, 0, 0};
     lds_barrier();  // (the last tile's values have been read)
@@ -185,27 +198,29 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
   }
 
   // ---- rows of the cache
-  if (t < t1) {
+  if (t < t1 && a.t > 0) {
     uint4 code[4];
     uint2 sc, tail;
     uint32_t tsc = 0;
-    auto load = [&](const uint8_t* row) {
-      const uint8_t* p = row ? row : g_kv4_none;
+    auto load = [&](row_t row) {
+      row_t p = row ? row : none;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) code[k] = *(const uint4*)(p + 64 * g + 16 * k);
-      sc = *(const uint2*)(p + 256 + 8 * g);
+      for (int k = 0; k < 4; ++k) code[k] = get16(p + 64 * g + 16 * k);
+      sc = get8(p + 256 + 8 * g);
       if (TS) {
-        tail = *(const uint2*)(p + 288 + 8 * g);
+        tail = get8(p + 288 + 8 * g);
         tsc = p[320 + g];
       }
     };
     if (t > t0) {
       i0 = index(t);
-      p0 = pages[there(i0) ? i0 >> a.map.shift : 0];
+      i1 = index(t + 1);
+      p0 = page(i0);
     }
-    int i1 = index(t + 1);
-    const uint8_t* row = source(i0, p0);
+    row_t row = source(t, i0, p0);
     load(row);
+    // (a tile ahead of its rows the page, two ahead the index, asked for behind the rows' loads: nothing waits for them)
+    int p1 = page(i1), i2 = index(t + 2);
     // Q to fp16; a head that reaches 2^16 scaled to under 2^15, which its scores are multiplied by again
     typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
     u16x2_t top2{0, 0};
@@ -233,8 +248,6 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     }
 #pragma unroll 1
     for (; t < t1; ++t) {
-      const int p1 = pages[there(i1) ? i1 >> a.map.shift : 0];  // (the next tile's, and the index of the one behind it)
-      const int i2 = index(t + 2);
       const h16x2_t s01 = kv4_scales<false>(sc.x), s23 = kv4_scales<true>(sc.x);
       const h16x2_t s45 = kv4_scales<false>(sc.y), s67 = kv4_scales<true>(sc.y);
       const _Float16 sv[9] = {s01[0], s01[1], s23[0], s23[1], s45[0], s45[1], s67[0], s67[1], kv4_scales<false>(tsc)[0]};
@@ -250,9 +263,12 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
         s = mfma_f16_16x16x32(x, q[k], s);
       }
       const bool valid = row != nullptr;
-      row = source(i1, p1);
+      row = source(t + 1, i1, p1);
       load(row);
-      i1 = i2;
+      // (moved here: the compiler's move at the loop's end, of the value then on its way, would wait for it)
+      asm volatile("v_mov_b32 %0, %1" : "=&v"(i1) : "v"(i2));
+      p1 = page(i1);
+      i2 = index(t + 3);
       attend(s, valid, std::true_type{});
     }
   }

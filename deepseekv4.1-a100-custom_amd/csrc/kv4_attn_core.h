@@ -35,6 +35,7 @@ struct Kv4AttnArgs {
 namespace {
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 __device__ __align__(16) uint8_t g_kv4_none[1152];  // what a key that is not there reads
 
