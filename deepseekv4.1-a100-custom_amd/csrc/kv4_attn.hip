@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
   const int u0 = (b < full * a.groups ? b / (8 * a.groups) * 8 : full) + in % n8;
   const int hg = in / n8, sp = u0 % a.nsplit, r = u0 / a.nsplit;
   const int h0 = hg * 16;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, g = lane >> 4;
   const int slot = r / a.rows_per_slot;
   const long seq = a.seq ? a.seq[slot] : slot;
@@ -83,35 +83,68 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     const bool there = known && u < t1 && (u - a.wtiles) * 64 + key < a.t && i >= 0 && i < rows;
     return there && (unsigned)p < (unsigned)a.map.pages ? (row_t)(a.pool + kv4_offset(a.map, p, i, RB)) : nullptr;
   };
-  // The way to the first tile's rows, two loads deep, is gone before Q is asked for.
-  int t = t0;
-  row_t wrow = t < min(t1, a.wtiles) ? window(t) : nullptr;
-  int i0 = -1, i1 = -1, p0 = -1;
-  if (t0 >= a.wtiles && t0 < t1 && a.t > 0) {
-    i0 = index(t0);
-    i1 = index(t0 + 1);
-    p0 = page(i0);
-  }
-
-  // Q: head l % 16, quarter l / 16 of the 512 columns, in k steps of 8
-  uint4 q[16 + TS];
-  const int h = h0 + l16;
-  const uint16_t* const qrow = a.q + r * a.q_rstride + (long)(h < a.H ? h : a.H - 1) * DQK;
-#pragma unroll
-  for (int k = 0; k < 16; ++k) q[k] = *(const uint4*)(qrow + 128 * g + 8 * k);
-#pragma unroll
-  for (int k = 0; k < TS; ++k) q[16 + k] = *(const uint4*)(qrow + 512 + 16 * g + 8 * k);
-  f32x4_t o[8];
-  float m = -__builtin_inff(), l = 0.0f, cq = a.scale;
-#pragma unroll
-  for (int c = 0; c < 8; ++c) o[c] = f32x4_t{0, 0, 0, 0};
-
   const uint32_t v_base = lds_addr_of(s_v), p_base = lds_addr_of(s_p), m_base = lds_addr_of(s_m);
   // this lane's unit 0 of its key's row, and its place in the transpose reads of key g * 8 + l16 / 4; the other units, and
   // the keys 4 further, are an XOR away
   const uint32_t v_put = v_base + key * 1024 + 256 * g + (v_swizzle(key) << 4);
   const uint32_t v_get = v_base + (g * 8 + (l16 >> 2)) * 1024 + wave * 256 +
                          ((((l16 & 3) >> 1) | ((l16 >> 2) << 1 ^ (g & 1) << 3)) << 4) + (l16 & 1) * 8;
+
+  // The way to the first rows, two loads deep, is gone before Q is asked for.
+  int t = t0;
+  const int first = max(t0, a.wtiles);
+  const bool cached = first < t1 && a.t > 0;
+  int i0 = -1, i1 = -1;
+  if (cached) {
+    i0 = index(first);
+    i1 = index(first + 1);
+  }
+
+  // Q: head l % 16, quarter l / 16 of the 512 columns, in k steps of 8.  A lane's own 16 bytes of 16 rows would be 64
+  // requests a load, so whole rows (of bf16, Q's and the window's) go to LDS by direct loads, in the values' places.
+  const int h = h0 + l16;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int head = wave * 4 + j;
+    lds_dma16_off(a.q + r * a.q_rstride + (long)min(h0 + head, a.H - 1) * DQK, (lane ^ v_swizzle(head)) << 4, v_base + head * 1024);
+  }
+  uint4 q[16 + TS];
+  const uint16_t* const qrow = a.q + r * a.q_rstride + (long)min(h, a.H - 1) * DQK;
+#pragma unroll
+  for (int k = 0; k < TS; ++k) q[16 + k] = *(const uint4*)(qrow + 512 + 16 * g + 8 * k);
+  uint4 code[4];
+  uint2 sc, tail;
+  uint32_t tsc = 0;
+  auto load = [&](row_t row) {
+    row_t p = row ? row : none;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) code[k] = get16(p + 64 * g + 16 * k);
+    sc = get8(p + 256 + 8 * g);
+    if (TS) {
+      tail = get8(p + 288 + 8 * g);
+      tsc = p[320 + g];
+    }
+  };
+  row_t wrow = t < min(t1, a.wtiles) ? window(t) : nullptr;
+  row_t row = nullptr;
+  int p1 = -1, i2 = -1;
+  if (cached) {
+    row = source(first, i0, page(i0));
+    load(row);
+    // (a tile ahead of its rows the page, two ahead the index, asked for behind the rows' loads: nothing waits for them)
+    p1 = page(i1);
+    i2 = index(first + 2);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  lds_barrier();
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
+    q[k] = __builtin_bit_cast(uint4, *(__attribute__((address_space(3))) u32x4*)(
+                                         (v_base + l16 * 1024 + 256 * g + (v_swizzle(l16) << 4)) ^ k << 4));
+  f32x4_t o[8];
+  float m = -__builtin_inff(), l = 0.0f, cq = a.scale;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) o[c] = f32x4_t{0, 0, 0, 0};
 
   const uint32_t p_put = p_base + l16 * 128 + (((wave * 2 + (g >> 1)) ^ (l16 & 7)) << 4) + (g & 1) * 8;
 
@@ -180,47 +213,30 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
 #pragma unroll 1
   for (; t < min(t1, a.wtiles); ++t) {
     const bool valid = wrow != nullptr;
-    row_t src = valid ? wrow : none;
-    uint4 x[16 + TS];
+    const uint64_t src = (uint64_t)(valid ? wrow : none);
+    lds_barrier();  // (the last tile's values have been read)
 #pragma unroll
-    for (int k = 0; k < 16 + TS; ++k) x[k] = get16(src + 2 * (k < 16 ? 128 * g + 8 * k : 512 + 16 * g + 8 * (k - 16)));
+    for (int j = 0; j < 16; ++j) {
+      const uint64_t p = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(src >> 32), j) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)src, j);
+      lds_dma16_off((const void*)p, (lane ^ v_swizzle(j)) << 4, v_base + (wave * 16 + j) * 1024);
+    }
+    uint4 x[TS + 1];
+#pragma unroll
+    for (int k = 0; k < TS; ++k) x[k] = get16((row_t)src + 1024 + 32 * g + 16 * k);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a wave reads its own keys' rows)
     if (t + 1 < min(t1, a.wtiles)) wrow = window(t + 1);
     f32x4_t s = {0, 0, 0, 0};
-    lds_barrier();  // (the last tile's values have been read)
-    uint32_t to = v_put;
-    asm volatile("" : "+v"(to));
 #pragma unroll
     for (int k = 0; k < 16 + TS; ++k) {
-      if (k < 16) put_v(to, k, x[k]);
-      s = mfma_bf16_16x16x32(x[k], q[k], s);
+      const uint4 y = k < 16 ? __builtin_bit_cast(uint4, *(__attribute__((address_space(3))) u32x4*)(v_put ^ k << 4)) : x[k - 16];
+      s = mfma_bf16_16x16x32(y, q[k], s);
     }
     attend(s, valid, std::false_type{});
   }
 
   // ---- rows of the cache
-  if (t < t1 && a.t > 0) {
-    uint4 code[4];
-    uint2 sc, tail;
-    uint32_t tsc = 0;
-    auto load = [&](row_t row) {
-      row_t p = row ? row : none;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) code[k] = get16(p + 64 * g + 16 * k);
-      sc = get8(p + 256 + 8 * g);
-      if (TS) {
-        tail = get8(p + 288 + 8 * g);
-        tsc = p[320 + g];
-      }
-    };
-    if (t > t0) {
-      i0 = index(t);
-      i1 = index(t + 1);
-      p0 = page(i0);
-    }
-    row_t row = source(t, i0, p0);
-    load(row);
-    // (a tile ahead of its rows the page, two ahead the index, asked for behind the rows' loads: nothing waits for them)
-    int p1 = page(i1), i2 = index(t + 2);
+  if (cached) {
     // Q to fp16; a head that reaches 2^16 scaled to under 2^15, which its scores are multiplied by again
     typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
     u16x2_t top2{0, 0};
