@@ -55,21 +55,23 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
   auto get16 = [](row_t p) { return __builtin_bit_cast(uint4, *(const __attribute__((address_space(1))) u32x4*)p); };
   auto get8 = [](row_t p) { return __builtin_bit_cast(uint2, *(const __attribute__((address_space(1))) u32x2*)p); };
 
-  // the row of the window that this lane's key of tile u is, nullptr: none
-  auto window = [&](int u) -> row_t {
+  // the row of the window that this lane's key of tile u is, nullptr: none; by its index where there is a list
+  const bool ring = !a.widx;
+  const long pmax = ring && a.pmax ? a.pmax[r] : 0, plim = ring && a.plim ? a.plim[r] : pos;
+  auto listed = [&](int u) { return ring || a.wt == 0 ? -1 : a.widx[(long)r * a.wt + min(u * 64 + key, a.wt - 1)]; };
+  auto window = [&](int u, int i) -> row_t {
     const int j = u * 64 + key;
-    long row = -1;
-    if (a.widx) {
-      if (j < a.wt) row = a.widx[(long)r * a.wt + j];
-      if (row >= a.win_rows) row = -1;
-    } else if (j < a.win_rows) {  // slot j of the ring holds the newest position of its residue
-      const long pmax = a.pmax[r], plim = a.plim ? a.plim[r] : pos;
+    bool there;
+    if (ring) {  // slot j of the ring holds the newest position of its residue
+      i = j;
       int d = (int)(pmax - j) % a.win_rows;  // (positions fit in 31 bits)
       if (d < 0) d += a.win_rows;
       const long held = pmax - d;
-      if (held >= 0 && held <= plim && pos - held < a.win_rows && seq >= 0 && seq < a.win_slots) row = j;
+      there = j < a.win_rows && held >= 0 && held <= plim && pos - held < a.win_rows && seq >= 0 && seq < a.win_slots;
+    } else {
+      there = j < a.wt && i >= 0 && i < a.win_rows;
     }
-    return row >= 0 ? (row_t)(a.win + (a.widx ? (long)slot : seq) * a.win_sstride + row * DQK) : nullptr;
+    return there ? (row_t)(a.win + (ring ? seq : (long)slot) * a.win_sstride + (long)i * DQK) : nullptr;
   };
   // the cache's rows
   const int* const ids = a.idx + (long)r * a.t;
@@ -94,7 +96,12 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
   int t = t0;
   const int first = max(t0, a.wtiles);
   const bool cached = first < t1 && a.t > 0;
-  int i0 = -1, i1 = -1;
+  const int wend = min(t1, a.wtiles);
+  int w0 = -1, w1 = -1, i0 = -1, i1 = -1;
+  if (t < wend) {
+    w0 = listed(t);
+    w1 = listed(t + 1);
+  }
   if (cached) {
     i0 = index(first);
     i1 = index(first + 1);
@@ -125,7 +132,6 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
       tsc = p[320 + g];
     }
   };
-  row_t wrow = t < min(t1, a.wtiles) ? window(t) : nullptr;
   row_t row = nullptr;
   int p1 = -1, i2 = -1;
   if (cached) {
@@ -211,7 +217,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
 
   // ---- window rows
 #pragma unroll 1
-  for (; t < min(t1, a.wtiles); ++t) {
+  for (; t < wend; ++t) {
+    const row_t wrow = window(t, w0);
     const bool valid = wrow != nullptr;
     const uint64_t src = (uint64_t)(valid ? wrow : none);
     lds_barrier();  // (the last tile's values have been read)
@@ -221,17 +228,28 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
                          (uint32_t)__builtin_amdgcn_readlane((int)src, j);
       lds_dma16_off((const void*)p, (lane ^ v_swizzle(j)) << 4, v_base + (wave * 16 + j) * 1024);
     }
-    uint4 x[TS + 1];
+    uint4 x[16 + TS];
 #pragma unroll
-    for (int k = 0; k < TS; ++k) x[k] = get16((row_t)src + 1024 + 32 * g + 16 * k);
+    for (int k = 0; k < TS; ++k) x[16 + k] = get16((row_t)src + 1024 + 32 * g + 16 * k);
+    w0 = w1;
+    w1 = listed(t + 2);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a wave reads its own keys' rows)
-    if (t + 1 < min(t1, a.wtiles)) wrow = window(t + 1);
-    f32x4_t s = {0, 0, 0, 0};
+    auto part = [&](int k) { x[k] = __builtin_bit_cast(uint4, *(__attribute__((address_space(3))) u32x4*)(v_put ^ k << 4)); };
+    f32x4_t s = {0, 0, 0, 0}, s2 = s;
+    constexpr int kAhead = 6;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) part(k);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int k = 0; k < 16 + TS; ++k) {
-      const uint4 y = k < 16 ? __builtin_bit_cast(uint4, *(__attribute__((address_space(3))) u32x4*)(v_put ^ k << 4)) : x[k - 16];
-      s = mfma_bf16_16x16x32(y, q[k], s);
+      if (k + kAhead < 16) part(k + kAhead);
+      if (k & 1)
+        s2 = mfma_bf16_16x16x32(x[k], q[k], s2);
+      else
+        s = mfma_bf16_16x16x32(x[k], q[k], s);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    s += s2;
     attend(s, valid, std::false_type{});
   }
 
