@@ -12,12 +12,15 @@
 // Sums, the softmax's maximum and sum and O are fp32; the reference maximum moves only for a score 2^8 above it; the
 // probabilities are rounded to fp16 (bf16 for window rows), the operand type, and the output once, after the rotation.
 //
+// Whole rows go to LDS by direct loads, a row a wave and load: a lane's own 16 bytes of 16 rows are 64 requests a load (Q and
+// window rows so: a prompt of 2 x 301 queries 77.7 us for 62.7).  Codes come that way all the same, 4 loads a tile: the
+// LDS has no room for them beside the values of two workgroups, and an exchange of lanes costs what it saves.
+//
 // What bounds it.  A step of single tokens: latency.  Four sequences of 2048 selected rows and 64 heads of 576 read 4 MB
-// and take 16.7 us, of them 8 us for a workgroup's one or two tiles -- index, page and row, three dependent loads, then
-// 1700 cycles of decoding and scores and 1750 of softmax and product -- and joining the splits 4.2 us; one sequence of 300
-// rows of 512 8.8 and 4.3 us.  Prompts of few heads: decoding, 350 instructions a wave and tile beside 34 MFMAs (602 query
-// rows of 512 + 128 keys, 20 heads of 512: 83 us).  32 heads a workgroup halve that but leave one workgroup a CU (97 us, and
-// 16.8 us for 12.8 of one token); the rows in bf16 first cost as much with 32 heads as with 64 (94 us).
+// and take 18.4 us in a graph, of them 4.2 us for joining the splits; one sequence of 300 rows of 512 11.7 us.  Prompts
+// of few heads: the writes of the decoded rows to LDS (13 cycles a wave's kilobyte, 840 a tile and workgroup) and the
+// chain of a tile's phases, 4300 cycles beside another workgroup (602 query rows of 512 + 128 keys, 20 heads of 512:
+// 62.7 us).  32 heads a workgroup halve the decoding but leave one workgroup a CU (97 us when 16 heads took 83).
 #include <type_traits>
 
 #include "kv4_attn_core.h"
@@ -377,24 +380,28 @@ struct Plan {
 Plan plan_of(int R, int H, int wt, int t, int dim, long rows) {
   Plan p{};
   // Decoding first, then the bf16 kernel of 64 heads a workgroup, pays with more than half of them (512 query rows of 2048
-  // keys: 64 heads 185 us for 360, 32 heads 180 for 187, 16 heads 178 for 99), from 32 query rows (40 of 512 keys 30.3 us for
-  // 31.5, 80 34.7 for 36.7, 150 37.2 for 53.2) and with each row of the cache listed four times (2048 keys of 16384 rows: 32
-  // query rows 39.7 us for 45.6, 16 36.6 for 30.9).  The bf16 kernel's grid ends at 65535 query rows.
-  p.many = rows > 0 && H > 32 && R >= 32 && R <= 65528 && (long)R * t >= 4 * rows;
+  // keys: 64 heads 183 us for 303, 33 heads 180 for 229, 32 heads 180 for 158), from 2^18 keys of 16 heads each on (602
+  // query rows of 512 keys: 64 heads 99 us for 118, 48 and 33 heads 96 for 94; 150 rows, 64 heads 37.3 for 41.6, 33 heads 35.7
+  // for 27.8; 32 rows of 2048 39.6 for 40.6, 16 of them 36.7 for 27.5) and with each row of the cache listed four times.
+  // (From 16 query rows on the bf16 kernel joins its splits by a kernel of its own; its grid ends at 65535.)
+  p.groups = (H + 15) / 16;
+  p.many = rows > 0 && H > 32 && R >= 16 && R <= 65528 && (long)R * t * p.groups >= 1L << 18 && (long)R * t >= 4 * rows;
   if (p.many) {
     p.list = ((long)R * (wt + t) * 4 + 255) & ~255L;
     p.rows = (rows * dim * 2 + 255) & ~255L;
     p.part = dsv41_attn_workspace_bytes(R, H, wt + t, 512, 0);
     return p;
   }
-  p.groups = (H + 15) / 16;
   p.wtiles = (wt + 63) / 64;
   p.tiles = p.wtiles + (t + 63) / 64;
   if (p.tiles == 0) p.tiles = 1;  // (no key at all: zeros)
-  // Splits of the tiles until each of the card's CUs has a workgroup: two on a CU cost more in partial results than they
-  // hide (4 sequences of 64 heads and 2048 rows: 20.3 us with 256, 24.4 with 512, 37.3 with 1024, 26.0 with 128).
-  const long units = (long)R * p.groups, want = (256 + units - 1) / units;
-  const long ns = want < p.tiles ? want : p.tiles;
+  // Splits until each of the card's CUs has a workgroup, two where one would have more than 12 tiles: before, two cost more
+  // in partial results than they hide (64 heads, 34 tiles: 4 sequences 18.4 us and 20.6, 16 27.9 and 29.9, 32 42.1 and 37.7).
+  // Of more than 16 tiles no split has a single one (1 sequence 15.3 us for 17.8; 10 tiles 12.3 for 11.7).
+  const long units = (long)R * p.groups, most = p.tiles > 16 ? (p.tiles + 1) / 2 : p.tiles;
+  long ns = (256 + units - 1) / units;
+  if (p.tiles > 12 * ns) ns = (512 + units - 1) / units;
+  if (ns > most) ns = most;
   p.chunk = (int)((p.tiles + ns - 1) / ns);
   p.nsplit = (p.tiles + p.chunk - 1) / p.chunk;
   p.part = p.nsplit > 1 ? 4L * R * H * p.nsplit * 514 : 0;
