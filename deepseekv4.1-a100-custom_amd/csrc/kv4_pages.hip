@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const PagesA
 __global__ void __launch_bounds__(256) reserve_copy_kernel(const PagesArgs a) { carry(a, blockIdx.x, threadIdx.x); }
 
 // ---- compact
-// Workspace (int32): live, moves, from [pages], to [pages], where [pages] (of a moved page).
+// Workspace (int32): live, moves, from [pages], to [pages], where [pages] (the move of a page).
 // One workgroup: L live pages; the live ones of L and above go, in order, to the free ones below L.  Sources and
 // destinations do not meet, so the moves need no order.
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagesArgs a) {
@@ -258,13 +258,15 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagesA
     unsigned src = l & ~front, dst = ~l & front & held;
     const int which = (p0 / step + 1) & 1;
     const int2 r = block_scan2_dpp<kPlanThreads>(__popc(src), __popc(dst), tmp[which], &total);
-    for (int i = base.x + r.x; src; src &= src - 1) from[i++] = p + __ffs(src) - 1;
+    for (int i = base.x + r.x; src; src &= src - 1, ++i) {
+      const int s = p + __ffs(src) - 1;
+      from[i] = s;
+      where[s] = i;
+    }
     for (int i = base.y + r.y; dst; dst &= dst - 1) to[i++] = p + __ffs(dst) - 1;
     base.x += total.x;
     base.y += total.y;
   }
-  __syncthreads();
-  for (int r = t; r < base.x; r += kPlanThreads) where[from[r]] = to[r];
   if (t == 0) {
     a.ws[0] = live;
     a.ws[1] = base.x;
@@ -280,7 +282,10 @@ __global__ void __launch_bounds__(256) compact_move_kernel(const PagesArgs a) {
   const int entries = a.slots * a.cols;
   for (int i = blockIdx.x * 256 + threadIdx.x; i < entries; i += gridDim.x * 256) {
     const int p = a.table[i];
-    if (p >= live && p < a.pages) a.table[i] = where[p];
+    if (p >= live && p < a.pages) {
+      const int k = where[p];
+      a.table[i] = (unsigned)k < (unsigned)moves ? to[k] : -1;  // (no such move: a page whose count says that it is free)
+    }
   }
   for (int r = blockIdx.x; r < moves; r += gridDim.x) {
     const int s = from[r], d = to[r];
