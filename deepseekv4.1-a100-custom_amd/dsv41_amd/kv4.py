@@ -35,6 +35,7 @@ _E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -
 _ERRORS = ((1, "too few free pages"), (2, "an entry was left out (an index out of range, or one named twice)"),
            (4, "a row was dropped (no page of the sequence's own there, or no rope angle)"))
 _MOST_ENTRIES = 4096
+_FEW_COPIES = 4096  # pairs up to which a copy needs no workspace
 _I64, _I32, _BF16 = torch.int64, torch.int32, torch.bfloat16
 _INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
@@ -73,6 +74,7 @@ class PagedKV4:
         self._c = _Cache(pool.data_ptr(), table.data_ptr(), refs.data_ptr(), self.err.data_ptr(), self.pages, self.page,
                          self.slots, self.cols, dim)
         self._at = ctypes.addressof(self._c)
+        self._span = pool.data_ptr(), pool.data_ptr() + pool.numel()
         self._sizes = {}
 
     @classmethod
@@ -174,7 +176,7 @@ class PagedKV4:
         """Rows begin[i] .. end[i] - 1 of sequence seq[i] made writable: a page of its own wherever it has none or shares
         one, the lowest free pages in the order of the arguments; where a shared page is replaced, its rows before
         begin[i] are copied.  Distinct sequences, 4096 at most."""
-        n = len(seq)
+        n = _count(seq)
         if n > _MOST_ENTRIES:
             raise RuntimeError(f"kv4.reserve: {n} sequences (at most {_MOST_ENTRIES})")
         seq, begin, end = (self._i64("kv4.reserve", t, n) for t in (seq, begin, end))
@@ -188,7 +190,7 @@ class PagedKV4:
         """Sequence dst[i] gets the first rows[i] rows (None: all) of src[i] in place of its own, by naming their pages:
         nothing is copied before reserve makes a shared page writable.  A destination may be named once and may not be a
         source of the same call."""
-        n = len(src)
+        n = _count(src)
         src, dst = self._i64("kv4.fork", src, n), self._i64("kv4.fork", dst, n)
         rows = None if rows is None else self._i64("kv4.fork", rows, n)
         _launch("dsv41_kv4_fork", self.index, self._at, src.data_ptr(), dst.data_ptr(), ptr(rows), n)
@@ -196,7 +198,7 @@ class PagedKV4:
 
     def release(self, seq, rows=None) -> None:
         """The pages behind the first rows[i] rows (None: 0, all of them) of sequence seq[i] are given up."""
-        n = len(seq)
+        n = _count(seq)
         seq = self._i64("kv4.release", seq, n)
         rows = None if rows is None else self._i64("kv4.release", rows, n)
         _launch("dsv41_kv4_release", self.index, self._at, seq.data_ptr(), ptr(rows), n)
@@ -219,17 +221,20 @@ class PagedKV4:
             raise RuntimeError(f"kv4.copy_pages: pages of {other.page} rows of {other.dim} into {self.page} of {self.dim}")
         if other.index != self.index:
             raise RuntimeError(f"kv4.copy_pages: pools on {other.device}, {self.device}")
-        a, b = self._c.pool, other._c.pool
-        if a < b + other.pages * other.pool.stride(0) and b < a + self.pages * self.pool.stride(0):
+        if self._span[0] < other._span[1] and other._span[0] < self._span[1]:
             raise RuntimeError("kv4.copy_pages: the pools are one memory (fork and reserve share and copy within a pool)")
-        n = len(src)
+        n = _count(src)
         if n >= 1 << 31:
             raise RuntimeError(f"kv4.copy_pages: {n} pages")
         src, dst = self._i64("kv4.copy_pages", src, n), self._i64("kv4.copy_pages", dst, n)
-        size = lib().dsv41_kv4_copy_workspace_bytes(self._at, n)
+        size = 4 * self.pages if n > _FEW_COPIES else 0  # (dsv41_kv4_copy_workspace_bytes)
         ws = torch.empty(size // 4, dtype=_I32, device=self.device) if size else None
         _launch("dsv41_kv4_copy", self.index, self._at, other._at, src.data_ptr(), dst.data_ptr(), n, ptr(ws), size)
         self._done()
+
+
+def _count(t) -> int:
+    return t.numel() if isinstance(t, torch.Tensor) else len(t)
 
 
 def _angles(name: str, cos, sin, rd: int, index: int):

@@ -173,3 +173,16 @@ def test_model_of_pages():
     m.release([0], [0])
     assert m.compact() == 3 and m.table[2].tolist() == [0, 1, -1, -1] and m.table[1, 0] == 2
     assert not m.reserve([0], [0], [64])
+
+
+def test_workspace_sizes_agree():
+    """The sizes that the Python calls allocate are those that the library asks for."""
+    from dsv41_amd import kv4
+    L = _lib.lib()
+    s = _struct(pages=700, slots=9, cols=11)
+    c = ctypes.byref(s)
+    for n in (1, 4, 5, kv4._MOST_ENTRIES):
+        assert L.dsv41_kv4_reserve_workspace_bytes(c, n) == 4 * (9 + 3 * 700 + 2 * n)
+    assert L.dsv41_kv4_compact_workspace_bytes(c) == 4 * (2 + 3 * 700)
+    assert L.dsv41_kv4_copy_workspace_bytes(c, kv4._FEW_COPIES) == 0
+    assert L.dsv41_kv4_copy_workspace_bytes(c, kv4._FEW_COPIES + 1) == 4 * 700
