@@ -272,6 +272,12 @@ def test_decode(dim, heads, counts, drafts, t):
     _decode(dim, heads, counts, drafts, t)
 
 
+@pytest.mark.parametrize("dim,counts,drafts,t", [(576, [2100, 2100], 20, 2048), (512, [1200], 1, 1100), (576, [1000] * 8, 16, 900)])
+def test_decode_long_lists(dim, counts, drafts, t):
+    """Two workgroups a CU of splits, splits of two tiles, and one split of many."""
+    _decode(dim, 64, counts, drafts, t)
+
+
 @pytest.mark.parametrize("dim", [512, 576])
 def test_decode_masks(dim):
     """Entries out of the sequence's pages, holes, a list of nothing, rings that hold nothing yet."""
