@@ -13,7 +13,7 @@
 // probabilities are rounded to fp16 (bf16 for window rows), the operand type, and the output once, after the rotation.
 //
 // Whole rows go to LDS by direct loads, a row a wave and load: a lane's own 16 bytes of 16 rows are 64 requests a load (Q and
-// window rows so: a prompt of 2 x 301 queries 77.7 us for 62.7).  Codes come that way all the same, 4 loads a tile: the
+// window rows so, with their reads ahead: a prompt of 2 x 301 queries 62.7 us for 77.7).  Codes come that way all the same, 4 loads a tile: the
 // LDS has no room for them beside the values of two workgroups, and an exchange of lanes costs what it saves.
 //
 // What bounds it.  A step of single tokens: latency.  Four sequences of 2048 selected rows and 64 heads of 576 read 4 MB
@@ -378,6 +378,8 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const Kv4AttnArgs a) {
       finish4(a, a.pos ? a.pos[r] : 0, 4 * threadIdx.x, o);
 }
 
+constexpr int kMost = 0x7fffffff - 4096;  // entries of a list, which are counted on past its end in 32 bits
+
 struct Plan {
   bool many;  // the cache's rows decoded first
   int wtiles, tiles, nsplit, chunk, groups;
@@ -392,7 +394,8 @@ Plan plan_of(int R, int H, int wt, int t, int dim, long rows) {
   // for 27.8; 32 rows of 2048 39.6 for 40.6, 16 of them 36.7 for 27.5) and with each row of the cache listed four times.
   // (From 16 query rows on the bf16 kernel joins its splits by a kernel of its own; its grid ends at 65535.)
   p.groups = (H + 15) / 16;
-  p.many = rows > 0 && H > 32 && R >= 16 && R <= 65528 && (long)R * t * p.groups >= 1L << 18 && (long)R * t >= 4 * rows;
+  p.many = rows > 0 && H > 32 && R >= 16 && R <= 65528 && (long)R * t * p.groups >= 1L << 18 && (long)R * t >= 4 * rows &&
+           (long)wt + t <= kMost;
   if (p.many) {
     p.list = ((long)R * (wt + t) * 4 + 255) & ~255L;
     p.rows = (rows * dim * 2 + 255) & ~255L;
@@ -424,7 +427,7 @@ int run(Kv4AttnArgs& a, int dqk, int b, float scale, void* ws, long ws_bytes, hi
   void* const part = (char*)ws + p.list + p.rows;
   if (p.many) {
     const long l = (long)a.wt + a.t, n = rows / b, pages = rows >> a.map.shift;
-    if (l >= (1L << 31) || a.win_rows + n >= (1L << 31) || pages + a.R >= (1L << 31)) return (int)hipErrorInvalidValue;
+    if (a.win_rows + n >= (1L << 31) || pages + a.R >= (1L << 31)) return (int)hipErrorInvalidValue;
     int* const list = (int*)ws;
     void* const table = (char*)ws + p.list;
     kv4_unpack_launch(a, dqk, b, table, list, st);
@@ -457,7 +460,8 @@ int run(Kv4AttnArgs& a, int dqk, int b, float scale, void* ws, long ws_bytes, hi
 }
 
 bool attn_ok(const Kv4AttnArgs& a, const dsv41_kv4* c) {
-  return kv4_ok(c) && a.q && a.H > 0 && a.sink && a.out && a.t >= 0 && (a.t == 0 || a.idx) &&
+  return kv4_ok(c) && a.q && a.H > 0 && a.sink && a.out && a.t >= 0 && a.t <= kMost && a.wt <= kMost && a.win_rows <= kMost &&
+         (a.t == 0 || a.idx) &&
          (((uintptr_t)a.q | (uintptr_t)a.win | (uintptr_t)a.out) & 15) == 0 && a.win_sstride % 8 == 0;
 }
 
@@ -466,7 +470,7 @@ bool attn_ok(const Kv4AttnArgs& a, const dsv41_kv4* c) {
 extern "C" {
 
 long dsv41_kv4_attn_workspace_bytes(const dsv41_kv4* c, int R, int H, int wt, int t, int b) {
-  if (R <= 0 || H <= 0 || wt < 0 || t < 0) return 0;
+  if (R <= 0 || H <= 0 || wt < 0 || t < 0 || wt > kMost || t > kMost) return 0;
   const Plan p = plan_of(R, H, wt, t, c->dim, (long)b * c->cols * c->page);
   return p.list + p.rows + p.part;
 }

@@ -134,7 +134,8 @@ def test_entry_points_refuse():
     assert L.dsv41_kv4_read(c, P, P, 1, P + 2, None) == inv
     args = [c, P, P, 128 * 512, 2, 128, P, 10, P, P, P, None, P, P, P, 100, 64, 1.0, P, 1, 16, None, 0, None]
     for at, v in [(1, None), (1, P + 2), (2, None), (3, 12), (5, 0), (6, None), (7, -1), (8, None), (9, None), (10, None),
-                  (12, None), (13, None), (16, 62), (16, 516), (16, -4), (18, None), (19, -1), (20, 0)]:
+                  (12, None), (13, None), (16, 62), (16, 516), (16, -4), (18, None), (18, P + 8), (19, -1), (20, 0), (5, 0x7fffffff),
+                  (7, 0x7fffffff)]:
         bad = list(args)
         bad[at] = v
         assert L.dsv41_sattn4(*bad) == inv, (at, v)
@@ -144,7 +145,7 @@ def test_entry_points_refuse():
     assert L.dsv41_kv4_attn_workspace_bytes(c, 1, 16, 128, 4096, 0) > 0 and L.dsv41_sattn4(*bad) == inv
     args = [c, P, P, 128 * 512, 128, P, 128, P, 10, None, P, 1.0, P, 1, 1, 16, None, 0, None]
     for at, v in [(1, None), (2, None), (4, -1), (5, None), (6, -1), (7, None), (8, -1), (10, None), (12, None), (13, -1),
-                  (14, -1), (15, 0)]:
+                  (14, -1), (15, 0), (4, 0x7fffffff), (6, 0x7fffffff), (8, 0x7fffffff), (12, P + 8)]:
         bad = list(args)
         bad[at] = v
         assert L.dsv41_sparse_attn4(*bad) == inv, (at, v)
