@@ -75,7 +75,7 @@ inline int kv4_shift(int page) {
 
 inline bool kv4_ok(const dsv41_kv4* c) {
   return c && c->pool && ((uintptr_t)c->pool & 15) == 0 && c->table && c->refs && c->err && c->slots > 0 && c->cols > 0 &&
-         (long)c->slots * c->cols < (1L << 31) && c->pages > 0 && kv4_shift(c->page) >= 0 &&
+         (long)c->slots * c->cols <= (1L << 31) - (1L << 20) && c->pages > 0 && kv4_shift(c->page) >= 0 &&
          (long)c->pages * c->page < (1L << 31) && (c->dim == 512 || c->dim == 576);
 }
 

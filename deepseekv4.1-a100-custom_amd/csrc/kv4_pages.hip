@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(256) compact_move_kernel(const PagesArgs a) {
   const int* const to = from + a.pages;
   const int* const where = to + a.pages;
   const int entries = a.slots * a.cols;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < entries; i += gridDim.x * 256) {
+  for (long i = blockIdx.x * 256 + threadIdx.x; i < entries; i += gridDim.x * 256L) {
     const int p = a.table[i];
     if (p >= live && p < a.pages) {
       const int k = where[p];

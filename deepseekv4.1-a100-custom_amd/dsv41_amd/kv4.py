@@ -61,7 +61,7 @@ class PagedKV4:
         if table.dtype != torch.int32 or table.dim() != 2 or refs.dtype != torch.int32 or refs.shape != pool.shape[:1]:
             raise ValueError(f"PagedKV4: table {tuple(table.shape)} {table.dtype}, refs {tuple(refs.shape)} {refs.dtype} "
                              f"(int32 [slots, columns] and [{pool.shape[0]}])")
-        if 0 in pool.shape or 0 in table.shape or table.numel() >= 1 << 31 or pool.shape[0] * pool.shape[1] >= 1 << 31:
+        if 0 in pool.shape or 0 in table.shape or table.numel() > (1 << 31) - (1 << 20) or pool.shape[0] * pool.shape[1] >= 1 << 31:
             raise ValueError(f"PagedKV4: pool {tuple(pool.shape)}, table {tuple(table.shape)}")
         if not (pool.is_contiguous() and table.is_contiguous() and refs.is_contiguous()) or pool.data_ptr() % 16:
             raise ValueError("PagedKV4: contiguous tensors, the pool 16-byte aligned")
