@@ -348,29 +348,36 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const Kv4AttnArgs a) {
   const long at = ((long)r * a.H + h) * a.nsplit;
   const float* ml = a.part + 2 * at;
   const float* src = a.part + 2L * a.R * a.H * a.nsplit + at * 512 + 4 * threadIdx.x;
-  float m = -__builtin_inff();
-#pragma unroll 8
-  for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, ml[2 * s]);
-  const float ref = m == -__builtin_inff() ? 0.0f : m;  // (no key: zeros, but a NaN stays one)
-  float den = exp2f(a.sink[h] * kLog2e - ref);
-  float4 o = make_float4(0, 0, 0, 0);
-  for (int s0 = 0; s0 < a.nsplit; s0 += 8) {  // (eight splits' loads in flight; the sums go in order)
-    float4 v[8];
-    float2 st[8];
+  float4 v[8];  // (eight splits' loads in flight, the first before their maxima are known; the sums go in order)
+  float2 st[8];
+  auto load = [&](int s0) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int s = min(s0 + i, a.nsplit - 1);
-      v[i] = *(const float4*)(src + 512L * s);
       st[i] = *(const float2*)(ml + 2 * s);
+      v[i] = *(const float4*)(src + 512L * s);
     }
+  };
+  load(0);
+  float m = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, st[i].x);
+#pragma unroll 8
+  for (int s = 8; s < a.nsplit; ++s) m = fmaxf(m, ml[2 * s]);
+  const float ref = m == -__builtin_inff() ? 0.0f : m;  // (no key: zeros, but a NaN stays one)
+  float den = exp2f(a.sink[h] * kLog2e - ref);
+  float4 o = make_float4(0, 0, 0, 0);
+  for (int s0 = 0;;) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float w = s0 + i < a.nsplit ? exp2f(st[i].x - ref) : 0.0f;
       if (s0 + i < a.nsplit) {
+        const float w = exp2f(st[i].x - ref);
         den += w * st[i].y;
         o = make_float4(o.x + w * v[i].x, o.y + w * v[i].y, o.z + w * v[i].z, o.w + w * v[i].w);
       }
     }
+    if ((s0 += 8) >= a.nsplit) break;
+    load(s0);
   }
   const float inv = m == -__builtin_inff() ? 0.0f : 1.0f / den;
   o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
