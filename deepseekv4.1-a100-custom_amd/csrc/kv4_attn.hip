@@ -17,7 +17,7 @@
 // LDS has no room for them beside the values of two workgroups, and an exchange of lanes costs what it saves.
 //
 // What bounds it.  A step of single tokens: latency.  Four sequences of 2048 selected rows and 64 heads of 576 read 4 MB
-// and take 18.4 us in a graph, of them 4.2 us for joining the splits; one sequence of 300 rows of 512 11.7 us.  Prompts
+// and take 17.3 us in a graph, of them 4.0 us for joining the splits; one sequence of 300 rows of 512 10.8 us.  Prompts
 // of few heads: the writes of the decoded rows to LDS (13 cycles a wave's kilobyte, 840 a tile and workgroup) and the
 // chain of a tile's phases, 4300 cycles beside another workgroup (602 query rows of 512 + 128 keys, 20 heads of 512:
 // 62.7 us).  32 heads a workgroup halve the decoding but leave one workgroup a CU (97 us when 16 heads took 83).
@@ -348,11 +348,11 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const Kv4AttnArgs a) {
   const long at = ((long)r * a.H + h) * a.nsplit;
   const float* ml = a.part + 2 * at;
   const float* src = a.part + 2L * a.R * a.H * a.nsplit + at * 512 + 4 * threadIdx.x;
-  float4 v[8];  // (eight splits' loads in flight, the first before their maxima are known; the sums go in order)
-  float2 st[8];
+  float4 v[12];  // (twelve splits' loads in flight, the first before their maxima are known; the sums go in order)
+  float2 st[12];
   auto load = [&](int s0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 12; ++i) {
       const int s = min(s0 + i, a.nsplit - 1);
       st[i] = *(const float2*)(ml + 2 * s);
       v[i] = *(const float4*)(src + 512L * s);
@@ -361,22 +361,22 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const Kv4AttnArgs a) {
   load(0);
   float m = -__builtin_inff();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, st[i].x);
+  for (int i = 0; i < 12; ++i) m = fmaxf(m, st[i].x);
 #pragma unroll 8
-  for (int s = 8; s < a.nsplit; ++s) m = fmaxf(m, ml[2 * s]);
+  for (int s = 12; s < a.nsplit; ++s) m = fmaxf(m, ml[2 * s]);
   const float ref = m == -__builtin_inff() ? 0.0f : m;  // (no key: zeros, but a NaN stays one)
   float den = exp2f(a.sink[h] * kLog2e - ref);
   float4 o = make_float4(0, 0, 0, 0);
   for (int s0 = 0;;) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 12; ++i) {
       if (s0 + i < a.nsplit) {
         const float w = exp2f(st[i].x - ref);
         den += w * st[i].y;
         o = make_float4(o.x + w * v[i].x, o.y + w * v[i].y, o.z + w * v[i].z, o.w + w * v[i].w);
       }
     }
-    if ((s0 += 8) >= a.nsplit) break;
+    if ((s0 += 12) >= a.nsplit) break;
     load(s0);
   }
   const float inv = m == -__builtin_inff() ? 0.0f : 1.0f / den;
