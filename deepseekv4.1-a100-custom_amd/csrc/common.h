@@ -240,6 +240,12 @@ DSV41_DEV void lds_dma16_off(const void* base, uint32_t off, uint32_t lds_addr) 
   const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
   asm volatile(DSV41_LOAD_LDS("global_load_lds_dwordx4 %1, %2") ::"s"(m), "v"(off), "s"(base) : "memory", "m0");
 }
+// The same of a base that a vector instruction has made (a lane's pointer, by v_readlane): a load may read such a scalar
+// register five wait states later, which the compiler does not see to here either.
+DSV41_DEV void lds_dma16_lane(const void* base, uint32_t off, uint32_t lds_addr) {
+  const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
+  asm volatile("s_nop 3\n\t" DSV41_LOAD_LDS("global_load_lds_dwordx4 %1, %2") ::"s"(m), "v"(off), "s"(base) : "memory", "m0");
+}
 DSV41_DEV void lds_dma4_off(const void* base, uint32_t off, uint32_t lds_addr) {
   const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
   asm volatile(DSV41_LOAD_LDS("global_load_lds_dword %1, %2") ::"s"(m), "v"(off), "s"(base) : "memory", "m0");

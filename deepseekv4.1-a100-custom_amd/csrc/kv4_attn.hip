@@ -27,13 +27,6 @@
 
 namespace {
 
-// As lds_dma16_off, of a base that a vector instruction may have made (a lane's pointer): a load may read such a scalar
-// register five wait states later, which the compiler does not see to for inline assembly.
-DSV41_DEV void row_to_lds(const void* base, uint32_t off, uint32_t lds_addr) {
-  const uint32_t m = __builtin_amdgcn_readfirstlane(lds_addr);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m), "v"(off), "s"(base) : "memory", "m0");
-}
-
 template <int DQK>
 __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
   constexpr int TS = DQK == 576 ? 2 : 0;   // k steps of the last 64 columns
@@ -123,7 +116,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int head = wave * 4 + j;
-    row_to_lds(a.q + r * a.q_rstride + (long)min(h0 + head, a.H - 1) * DQK, (lane ^ v_swizzle(head)) << 4, v_base + head * 1024);
+    lds_dma16_off(a.q + r * a.q_rstride + (long)min(h0 + head, a.H - 1) * DQK, (lane ^ v_swizzle(head)) << 4, v_base + head * 1024);
   }
   uint4 q[16 + TS];
   const uint16_t* const qrow = a.q + r * a.q_rstride + (long)min(h, a.H - 1) * DQK;
@@ -236,7 +229,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     for (int j = 0; j < 16; ++j) {
       const uint64_t p = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(src >> 32), j) << 32 |
                          (uint32_t)__builtin_amdgcn_readlane((int)src, j);
-      row_to_lds((const void*)p, (lane ^ v_swizzle(j)) << 4, v_base + (wave * 16 + j) * 1024);
+      lds_dma16_lane((const void*)p, (lane ^ v_swizzle(j)) << 4, v_base + (wave * 16 + j) * 1024);
     }
     uint4 x[16 + TS];
 #pragma unroll
