@@ -8,7 +8,7 @@
 // Release, fork and small calls are launches and little else (3 to 5 us).  A plan is one workgroup of 1024 lanes over the
 // counts: reserve reads them from the front until it has found enough (8.2 us, of 63 sequences as of 4), compact all
 // of them twice, 16 a lane (13.6 k pages 7.0 us; 8 a lane, one at a time, 14.1).  Moves and copies run at the memory's rate:
-// compact 2400 pages of 21.5 kB, 104 MB, in 17.5 us, copy 6001 of them, 258 MB, in 40.8 us.
+// compact 2400 pages of 21.5 kB, 104 MB, in 17.5 us, copy 6001 of them, 258 MB, in 46.7 us.
 #include "kv4_core.h"
 
 namespace {
@@ -322,29 +322,52 @@ __global__ void __launch_bounds__(256) copy_last_kernel(const CopyArgs a) {
   if (d >= 0 && d < a.dst_pages && s >= 0 && s < a.src_pages) atomicMax(a.last + d, i);
 }
 
+// A workgroup has P pairs: it looks through those behind its own once.
+template <int P>
 __global__ void __launch_bounds__(256) copy_kernel(const CopyArgs a) {
-  const int i = blockIdx.x;
-  const long s = a.from[i], d = a.to[i];
-  if (s == -1 || d == -1) return;
-  if (s < 0 || s >= a.src_pages || d < 0 || d >= a.dst_pages) {
-    if (threadIdx.x == 0) atomicOr(a.err, kKv4Ignored);
-    return;
+  __shared__ int s_later;
+  const int i0 = blockIdx.x * P, t = threadIdx.x;
+  long s[P], d[P];
+  int mine = 0, later = 0;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    s[p] = i0 + p < a.n ? a.from[i0 + p] : -1;
+    d[p] = i0 + p < a.n ? a.to[i0 + p] : -1;
+    if (s[p] == -1 || d[p] == -1) continue;
+    if (s[p] >= 0 && s[p] < a.src_pages && d[p] >= 0 && d[p] < a.dst_pages)
+      mine |= 1 << p;
+    else if (t == 0)
+      atomicOr(a.err, kKv4Ignored);
   }
-  bool later = false;
-  if (a.last)
-    later = a.last[d] != i;
-  else
-    for (int k = i + 1 + threadIdx.x; k < a.n; k += 256) later |= a.to[k] == d && a.from[k] >= 0 && a.from[k] < a.src_pages;
-  if (__syncthreads_or(later)) {
-    if (threadIdx.x == 0) atomicOr(a.err, kKv4Ignored);
-    return;
+  if (mine == 0) return;
+  if (t == 0) s_later = 0;
+  if (a.last) {
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      if (mine >> p & 1) later |= a.last[d[p]] != i0 + p ? 1 << p : 0;
+  } else {
+    for (int k = i0 + 1 + t; k < a.n; k += 256) {
+      const long to = a.to[k];
+      int hit = 0;
+#pragma unroll
+      for (int p = 0; p < P; ++p) hit |= to == d[p] && k > i0 + p ? 1 << p : 0;
+      if (hit && a.from[k] >= 0 && a.from[k] < a.src_pages) later |= hit;
+    }
   }
-  copy_bytes(a.dst + d * a.page_bytes, a.src + s * a.page_bytes, a.page_bytes);
+  __syncthreads();
+  if (later & mine) atomicOr(&s_later, later);
+  __syncthreads();
+  later = s_later & mine;
+  if (later && t == 0) atomicOr(a.err, kKv4Ignored);
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+    if ((mine & ~later) >> p & 1) copy_bytes(a.dst + d[p] * a.page_bytes, a.src + s[p] * a.page_bytes, a.page_bytes);
 }
 
-// Pairs up to which every workgroup looks through those behind its own (in a graph, 129 pairs 4.5 us, with the two launches
-// of claims 7.7; 1000 9.0 and 13.6, 2048 16.9 and 21.4, 4001 32.4 and 34.5, 6001 53.3 and 48.7).
-constexpr int kFewCopies = 4096;
+// Pairs up to which every workgroup looks through those behind its own: a pair each up to kLone, beyond that four (in a
+// graph, a pair and four: 129 pairs 4.6 and 6.3 us, 2048 15.8 and 18.0, 4001 31.2 and 32.5, 6001 52.3 and 49.9, 14000 of 5 kB
+// 67.4 and 38.0; claims by two launches before the copy 7.7, 21.4, 34.5, 48.7, but 61 for 51 call by call).
+constexpr int kLone = 4096, kFewCopies = 16384;
 
 PagesArgs pages_args(const dsv41_kv4& c) {
   PagesArgs a{};
@@ -453,7 +476,10 @@ int dsv41_kv4_copy(const dsv41_kv4* c, const dsv41_kv4* other, const long* src, 
     copy_last_kernel<<<(n + 255) / 256, 256, 0, (hipStream_t)stream>>>(a);
     DSV41_CHECK_LAUNCH();
   }
-  copy_kernel<<<n, 256, 0, (hipStream_t)stream>>>(a);
+  if (a.last || n <= kLone)
+    copy_kernel<1><<<n, 256, 0, (hipStream_t)stream>>>(a);
+  else
+    copy_kernel<4><<<(n + 3) / 4, 256, 0, (hipStream_t)stream>>>(a);
   DSV41_CHECK_LAUNCH();
   return 0;
 }

@@ -35,7 +35,7 @@ _E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -
 _ERRORS = ((1, "too few free pages"), (2, "an entry was left out (an index out of range, or one named twice)"),
            (4, "a row was dropped (no page of the sequence's own there, or no rope angle)"))
 _MOST_ENTRIES = 4096
-_FEW_COPIES = 4096  # pairs up to which a copy needs no workspace
+_FEW_COPIES = 16384  # pairs up to which a copy needs no workspace
 _I64, _I32, _BF16 = torch.int64, torch.int32, torch.bfloat16
 _INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 

@@ -628,7 +628,7 @@ def test_copy_on_write_keeps_the_parent():
 
 
 @pytest.mark.parametrize("n,pages", [(1, 3), (50, 64), (1024, 1500), (1025, 1500), (3000, 5000), (4096, 5000),
-                                     (4097, 5000)])
+                                     (4097, 5000), (16385, 17000)])
 def test_copy_pages(n, pages):
     from dsv41_amd.kv4 import PagedKV4
     g = _gen(n)

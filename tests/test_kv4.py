@@ -121,10 +121,10 @@ def test_entry_points_refuse():
     need = L.dsv41_kv4_compact_workspace_bytes(c)
     assert need == 4 * 14
     assert L.dsv41_kv4_compact(c, None, P, big, None) == inv and L.dsv41_kv4_compact(c, P, P, need - 1, None) == inv
-    assert L.dsv41_kv4_copy_workspace_bytes(c, 10) == 0 and L.dsv41_kv4_copy_workspace_bytes(c, 5000) == 16
+    assert L.dsv41_kv4_copy_workspace_bytes(c, 10) == 0 and L.dsv41_kv4_copy_workspace_bytes(c, 50000) == 16
     assert L.dsv41_kv4_copy(c, ctypes.byref(_struct(pool=P + 512)), P, P, 1, None, 0, None) == inv  # (one memory)
     far = dict(pool=1 << 40)
-    assert L.dsv41_kv4_copy(c, ctypes.byref(_struct(**far)), P, P, 5000, None, 0, None) == inv
+    assert L.dsv41_kv4_copy(c, ctypes.byref(_struct(**far)), P, P, 50000, None, 0, None) == inv
     assert L.dsv41_kv4_copy(c, ctypes.byref(_struct(**far, page=32)), P, P, 1, None, 0, None) == inv
     assert L.dsv41_kv4_copy(c, ctypes.byref(_struct(**far, dim=576)), P, P, 1, None, 0, None) == inv
     for x, stride, ratio, rd in [(None, 512, 4, 64), (P + 2, 512, 4, 64), (P, 500, 4, 64), (P, 516, 4, 64), (P, 512, 0, 64),
