@@ -177,8 +177,17 @@ def as_i64(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
     if t.dim() != 1:
         t = t.reshape(-1)
     if t.device != dev or t.dtype != torch.int64 or not t.is_contiguous():
-        t = t.to(device=dev, dtype=torch.int64, non_blocking=True).contiguous()
+        t = to_i64(t, dev)
     return t
+
+
+def to_i64(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """t as contiguous int64 on GPU dev, asynchronously.  A copy out of pinned memory is still to come when the call
+    returns, and its owner may fill it for the next step by then: its entries go by way of other host memory, which the
+    runtime has read when a copy returns.  (A captured copy reads the pinned memory at every replay, as it is meant to.)"""
+    if not t.is_cuda and t.is_pinned() and not torch.cuda.is_current_stream_capturing():
+        t = t.clone()
+    return t.to(device=dev, dtype=torch.int64, non_blocking=True).contiguous()
 
 
 def as_bf16(t: torch.Tensor) -> torch.Tensor:

@@ -15,7 +15,8 @@ values and 336 a row of 576 instead of 1024 and 1152, in pages that sequences sh
   c.copy_pages(other, src, dst)          pages out of another pool
 
 Every call is asynchronous on the current stream, synchronises with nothing and may be captured; calls on one cache must
-be stream-ordered.  Index arguments are tensors or lists (captured calls: tensors on the GPU).  What a call cannot do on the device -- too few free pages, an index out of range, a row without a page --
+be stream-ordered.  Index arguments are tensors or lists (captured calls: tensors on the GPU); host memory may be filled
+anew when a call returns.  What a call cannot do on the device -- too few free pages, an index out of range, a row without a page --
 it leaves out and notes in the cache's error word, which check() raises for (every call does with DSV41_CHECK_ERRORS=1).
 
 Forward only, as everything here."""
@@ -26,7 +27,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import as_f32, lib, ptr
+from ._lib import as_f32, lib, ptr, to_i64
 from .a8 import _aligned, _index, _launch, _no_grad
 
 ROW_BYTES = {512: 288, 576: 336}
@@ -103,7 +104,7 @@ class PagedKV4:
                 raise RuntimeError(f"{name}: entries of {t.dtype} (integers)")
             if not t.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError(f"{name}: entries in host memory in a captured call (a replay would read them again)")
-            t = t.to(device=self.device, dtype=_I64, non_blocking=True).contiguous()
+            t = to_i64(t, self.device)
         return t
 
     def _size(self, rows: int, h: int, wt: int, t: int, b: int) -> int:
