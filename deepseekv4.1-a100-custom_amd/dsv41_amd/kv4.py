@@ -279,9 +279,9 @@ def _indices(name: str, idx, shape: tuple, index: int):
         raise RuntimeError(f"{name}: indices {tuple(idx.shape)} on {idx.device} for {shape}")
     if idx.dtype not in _INTEGERS:
         raise RuntimeError(f"{name}: indices of {idx.dtype} (integers)")
-    if idx.dtype != torch.int32:
-        idx = idx.clamp(-1, 2 ** 31 - 1).to(torch.int32)
-    idx = idx.contiguous()
+    if idx.dtype == _I64:  # (the narrower types have no such values, nor room for the bounds)
+        idx = idx.clamp(-1, 2 ** 31 - 1)
+    idx = idx.to(torch.int32).contiguous()
     return (idx, idx.shape[-1]) if idx.shape[-1] else (None, 0)
 
 

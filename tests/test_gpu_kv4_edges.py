@@ -41,3 +41,18 @@ def test_rows_go_where_a_pinned_index_said():
     c.append(x, seq, row, 1, None, None, 0)
     row.copy_(torch.tensor([40, 41]))
     assert c.read([0, 0, 0, 0], [3, 20, 40, 41]).eq(6).all(1).tolist() == [True, True, False, False]
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int16, torch.int8, torch.uint8])
+def test_attention_takes_any_integer_list(dtype):
+    from dsv41_amd.kv4 import sparse_attn4
+    g = _gen(31)
+    c, _ = _filled(g, [100], 576, 16)
+    q = torch.randn(1, 2, 16, 576, generator=g).to(BF).to(DEV)
+    kv = torch.randn(1, 9, 576, generator=g).to(BF).to(DEV)
+    sink = torch.zeros(16, device=DEV)
+    idx, win = torch.randint(0, 100, (1, 2, 40), generator=g), torch.randint(0, 9, (1, 2, 5), generator=g)
+    if dtype != torch.uint8:
+        idx[0, 1, ::3], win[0, 0, 1] = -1, -1
+    run = lambda t: sparse_attn4(q, kv, c, sink, win.to(t).to(DEV), idx.to(t).to(DEV), 0.04)  # noqa: E731
+    assert torch.equal(run(dtype), run(torch.int32))
