@@ -6,9 +6,10 @@
 // the operands of 16 k steps if Q is held in the same order.  The decoded rows go to LDS once, as the values; then each
 // wave multiplies the tile's probabilities by 128 of the 512 value columns, O^T += V^T P^T.
 //
-// Decoding is exact in fp16 (E2M1 times e4m3 has 6 significand bits), two packed instructions for two values; Q in fp16
-// is exact too, but for numbers under 2^-14 (off by 2^-25 at most, a logit by less than fp32's own rounding of the sum)
-// and for heads that reach 2^16, which are scaled by a power of two.  Window rows have bf16's range, so they stay in bf16.
+// Decoding is exact in fp16 (E2M1 times e4m3 has 6 significand bits), two packed instructions for two values; Q in fp16,
+// each head scaled by a power of two, is exact too, but for values under 2^-28 of their head's largest (off by 2^-39 of it
+// at most, a logit by less than fp32's own rounding of a sum with that one).  Window rows have bf16's range, so they stay
+// in bf16.
 // Sums, the softmax's maximum and sum and O are fp32; the reference maximum moves only for a score 2^8 above it; the
 // probabilities are rounded to fp16 (bf16 for window rows), the operand type, and the output once, after the rotation.
 //
@@ -258,7 +259,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
 
   // ---- rows of the cache
   if (cached) {
-    // Q to fp16; a head that reaches 2^16 scaled to under 2^15, which its scores are multiplied by again
+    // Q to fp16: each head scaled by the power of two that brings its largest value to 2^14 or more, so that heads far under
+    // fp16's normal numbers keep their bits; the scores are multiplied by its inverse
     typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
     u16x2_t top2{0, 0};
 #pragma unroll
@@ -270,8 +272,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     }
     const uint32_t most = max((int)top2[0], (int)top2[1]);  // (a NaN's bits are above an infinity's; both are scaled)
     const float top = row_max4(__uint_as_float(min(most, 0x7f80u) << 16));
-    // (an infinity leaves zeros and infinities: its head's result is NaN)
-    const int e = top >= 65536.0f ? min(((__float_as_int(top) >> 23) & 255) - 127, 127) - 14 : 0;
+    // (an infinity leaves zeros and infinities: its head's result is NaN; 2^126 at most: subnormal bf16 is then exact)
+    const int e = max(min(((__float_as_int(top) >> 23) & 255) - 127, 127) - 14, -126);
     const float down = pow2i(-e);
     cq *= pow2i(e);
 #pragma unroll

@@ -56,3 +56,13 @@ def test_attention_takes_any_integer_list(dtype):
         idx[0, 1, ::3], win[0, 0, 1] = -1, -1
     run = lambda t: sparse_attn4(q, kv, c, sink, win.to(t).to(DEV), idx.to(t).to(DEV), 0.04)  # noqa: E731
     assert torch.equal(run(dtype), run(torch.int32))
+
+
+# ------------------------------------------------------------------------------------------------ numbers
+@pytest.mark.parametrize("qmul,scale", [(1e-6, 5e4), (1e-9, 3e8), (1e-36, 1e36), (2.0 ** -130, 2.0 ** 127)])
+def test_decode_queries_below_fp16(qmul, scale):
+    """Queries below fp16's smallest numbers under a scale that makes their logits ordinary ones; the ring is empty."""
+    def no_ring(idx, pos, pmax):
+        pmax[:] = -1
+    _decode(512, 20, [700, 300], 1, 400, qmul=qmul, scale=scale * 0.05, mask=no_ring, rd=0)
+    _decode(576, 16, [200], 3, 90, qmul=qmul, scale=scale * 0.05, mask=no_ring, rd=0)
