@@ -12,6 +12,9 @@
 // in bf16.
 // Sums, the softmax's maximum and sum and O are fp32; the reference maximum moves only for a score 2^8 above it; the
 // probabilities are rounded to fp16 (bf16 for window rows), the operand type, and the output once, after the rotation.
+// Of a cache's rows the reference is 2^7 under the maximum, so that the largest probability is 2^7 to 2^15 and fp16's last
+// bit, 2^-24, is 2^-31 of it or less: n keys of a long flat rest are off by n 2^-32 of the peak's weight together (with the
+// maximum as the reference weights under 2^-25 were lost, 2^18 of them 0.5 % of the numerator).
 //
 // Whole rows go to LDS by direct loads, a row a wave and load: a lane's own 16 bytes of 16 rows are 64 requests a load (Q and
 // window rows so, with their reads ahead: a prompt of 2 x 301 queries 62.7 us for 77.7).  Codes come that way all the same, 4 loads a tile: the
@@ -27,6 +30,8 @@
 #include "kv4_attn_core.h"
 
 namespace {
+
+constexpr float kLow = 7.0f;  // the reference of fp16 probabilities under the maximum, in powers of two
 
 template <int DQK>
 __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
@@ -161,6 +166,7 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
   // the softmax of a tile's scores and the product with its values in LDS
   auto attend = [&](f32x4_t& s, bool valid, auto f16) {
     constexpr bool F16 = decltype(f16)::value;
+    constexpr float kUnder = F16 ? kLow : 0.0f;  // what the reference is under the maximum that it was taken from
     const uint32_t mask = (uint32_t)(__ballot(valid) & 0xffffu) >> (4 * g);
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[i] = (mask >> i & 1) ? s[i] * cq : -__builtin_inff();
@@ -180,8 +186,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     lds_barrier();
     const f32x4_t w = *(__attribute__((address_space(3))) f32x4_t*)(m_base + l16 * 16);
     mx = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
-    if (__any(mx > m + 8.0f)) {  // (alike in every wave: all have the same maxima)
-      const float to = fmaxf(m, mx);
+    if (__any(mx > m + (8.0f + kUnder))) {  // (alike in every wave: all have the same maxima)
+      const float to = fmaxf(m, mx - kUnder);
       const float f = to > m ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
       m = to;
       l *= f;
@@ -276,6 +282,10 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
     const int e = max(min(((__float_as_int(top) >> 23) & 255) - 127, 127) - 14, -126);
     const float down = pow2i(-e);
     cq *= pow2i(e);
+    m -= kLow;  // (the window's reference is its maximum)
+    l *= pow2i((int)kLow);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) o[c] *= pow2i((int)kLow);
 #pragma unroll
     for (int k = 0; k < 16 + TS; ++k) {
       const uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};

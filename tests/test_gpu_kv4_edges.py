@@ -66,3 +66,34 @@ def test_decode_queries_below_fp16(qmul, scale):
         pmax[:] = -1
     _decode(512, 20, [700, 300], 1, 400, qmul=qmul, scale=scale * 0.05, mask=no_ring, rd=0)
     _decode(576, 16, [200], 3, 90, qmul=qmul, scale=scale * 0.05, mask=no_ring, rd=0)
+
+
+@pytest.mark.parametrize("window", [False, True])
+def test_long_list_behind_a_peak(window):
+    """One key (of the cache, or of the window) of weight 1, then 2^18 of 2^-25.5 each, 0.55 % of the weight together, over
+    one split.  Scores come from column 512, which is no value.  The output is off by its rounding (2^-8 of it), the peak's
+    probability's (2^-8 of its value 1.5) and each small one's: 2^-25 where the peak has 2^7 or more, so n 2^-32."""
+    from dsv41_amd.kv4 import PagedKV4, sparse_attn4
+    n, s = 1 << 18, 520
+    rows = torch.zeros(2, 576)
+    rows[0, :512], rows[0, 512] = 1.5, 6.0  # (the grid's: 6 times a power of two)
+    rows[1, :512] = 6.0
+    c = PagedKV4.empty(1, 1, 16, 576, 16, DEV)
+    c.reserve([0], [0], [2])
+    c.append(rows.to(BF).to(DEV), [0, 0], [0, 1], 1, None, None, 0)
+    q = torch.zeros(1, s, 16, 576, dtype=BF, device=DEV)
+    q[..., 512] = 1.0
+    scale = 25.5 * torch.log(torch.tensor(2.0, dtype=torch.float64)).item() / 6
+    idx = torch.ones(1, s, n + 64, dtype=torch.int32, device=DEV)
+    idx[:, :, :64] = -1
+    kv = win = None
+    if window:
+        kv, win = rows[:1].to(BF).to(DEV).view(1, 1, 576), torch.zeros(1, s, 1, dtype=torch.int32, device=DEV)
+    else:
+        idx[:, :, 0] = 0
+    o = sparse_attn4(q, kv, c, torch.full((16,), -1e30, device=DEV), win, idx, scale)
+    w = n * 2.0 ** -25.5
+    want = (1.5 + 6 * w) / (1 + w)
+    bound = 2.0 ** -8 * want + 2.0 ** -8 * 1.5 + 6 * n * 2.0 ** -32
+    assert (o.double() - want).abs().max().item() <= bound
+    assert bound < 0.5 * 6 * w  # (what it leaves out would show)
