@@ -332,8 +332,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
   if (h >= a.H) return;
   if (a.nsplit > 1) {
     const long at = ((long)r * a.H + h) * a.nsplit + sp;
-    if (wave == 0 && g == 0) *(float2*)(a.part + 2 * at) = make_float2(m, l);
-    float* dst = a.part + 2L * a.R * a.H * a.nsplit + at * 512 + wave * 128 + 4 * g;
+    if (wave == 0 && g == 0) *(float2*)(a.part + 512L * a.R * a.H * a.nsplit + 2 * at) = make_float2(m, l);
+    float* dst = a.part + at * 512 + wave * 128 + 4 * g;
 #pragma unroll
     for (int c = 0; c < 8; ++c) *(float4*)(dst + 16 * c) = make_float4(o[c][0], o[c][1], o[c][2], o[c][3]);
   } else {
@@ -351,8 +351,8 @@ __global__ void __launch_bounds__(256, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
 __global__ void __launch_bounds__(128) kv4_combine_kernel(const Kv4AttnArgs a) {
   const int r = blockIdx.x / a.H, h = blockIdx.x % a.H;
   const long at = ((long)r * a.H + h) * a.nsplit;
-  const float* ml = a.part + 2 * at;
-  const float* src = a.part + 2L * a.R * a.H * a.nsplit + at * 512 + 4 * threadIdx.x;
+  const float* ml = a.part + 512L * a.R * a.H * a.nsplit + 2 * at;
+  const float* src = a.part + at * 512 + 4 * threadIdx.x;
   float4 v[12];  // (twelve splits' loads in flight, the first before their maxima are known; the sums go in order)
   float2 st[12];
   auto load = [&](int s0) {

@@ -29,7 +29,7 @@ struct Kv4AttnArgs {
   int rd;
   uint16_t* out;        // [R, H, 512]
   int wtiles, tiles, chunk, nsplit, groups;
-  float* part;          // splits: [R, H, nsplit, 2] maximum and sum, then [R, H, nsplit, 512]
+  float* part;          // splits: [R, H, nsplit, 512] (16-byte aligned), then [R, H, nsplit, 2] reference and sum
 };
 
 namespace {

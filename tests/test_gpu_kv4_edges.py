@@ -97,3 +97,32 @@ def test_long_list_behind_a_peak(window):
     bound = 2.0 ** -8 * want + 2.0 ** -8 * 1.5 + 6 * n * 2.0 ** -32
     assert (o.double() - want).abs().max().item() <= bound
     assert bound < 0.5 * 6 * w  # (what it leaves out would show)
+
+
+@pytest.mark.parametrize("H,t", [(1, 63), (3, 200), (16, 63)])
+def test_partial_results_stand_aligned(H, t):
+    """The splits' partial results: rows of 512 at the workspace's start, 16-byte aligned, whatever the number of rows, heads
+    and splits, then their references (in powers of two) and sums; joined here they are the output."""
+    from dsv41_amd._lib import lib
+    g = _gen(t + H)
+    c, _ = _filled(g, [300], 576, 16)
+    D = lambda x: x.to(DEV)  # noqa: E731
+    q, ring, sink = (D(torch.randn(*s, generator=g)) for s in ((1, H, 576), (1, 128, 576), (H,)))
+    q, ring = q.to(BF), ring.to(BF)
+    idx = D(torch.randperm(300, generator=g)[:t].to(torch.int32))
+    pos, seq = D(torch.tensor([700])), D(torch.tensor([0]))
+    size = lib().dsv41_kv4_attn_workspace_bytes(c._at, 1, H, 128, t, 0)
+    n = 2 + -(-t // 64)
+    assert size == 4 * H * n * 514
+    ws, out = torch.zeros(size // 4, device=DEV), torch.zeros(H, 512, dtype=BF, device=DEV)
+    rc = lib().dsv41_sattn4(c._at, q.data_ptr(), ring.data_ptr(), 128 * 576, 1, 128, idx.data_ptr(), t, pos.data_ptr(),
+                            seq.data_ptr(), pos.data_ptr(), None, sink.data_ptr(), None, None, 0, 0, 0.04, out.data_ptr(), 1, H,
+                            ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    o, ml = ws[:H * n * 512].view(H, n, 512).double(), ws[H * n * 512:].view(H, n, 2).double()
+    top = ml[..., 0].amax(1)
+    w = torch.exp2(ml[..., 0] - top[:, None])
+    den = (w * ml[..., 1]).sum(1) + torch.exp2(sink.double() / torch.log(torch.tensor(2.0, dtype=torch.float64)) - top)
+    want = (w[..., None] * o).sum(1) / den[:, None]
+    # (one rounding to bf16; the powers of two and the sums are off by 2^-20 of their terms)
+    assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -18 * ring.double().abs().max()).all()
