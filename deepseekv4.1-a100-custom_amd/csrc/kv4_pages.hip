@@ -283,8 +283,10 @@ __global__ void __launch_bounds__(256) compact_move_kernel(const PagesArgs a) {
   for (long i = blockIdx.x * 256 + threadIdx.x; i < entries; i += gridDim.x * 256L) {
     const int p = a.table[i];
     if (p >= live && p < a.pages) {
-      const int k = where[p];
-      a.table[i] = (unsigned)k < (unsigned)moves ? to[k] : -1;  // (no such move: a page whose count says that it is free)
+      const int k = where[p];  // (what the workspace held where the page's count says that it is free: no move then)
+      const bool moved = (unsigned)k < (unsigned)moves && from[k] == p;
+      a.table[i] = moved ? to[k] : -1;
+      if (!moved) atomicOr(a.err, kKv4Ignored);
     }
   }
   for (int r = blockIdx.x; r < moves; r += gridDim.x) {

@@ -207,11 +207,13 @@ class PagedKV4:
 
     def compact(self) -> torch.Tensor:
         """The live pages moved to the front of the pool (those that stand there stay); table and refs follow.  Returns how
-        many they are, int32 [1] on the GPU: the pool's pages behind them are free."""
+        many they are, int32 [1] on the GPU: the pool's pages behind them are free.  The counts have to be the table's: an
+        entry behind the live pages whose page has none is taken out and noted."""
         size = 4 * (2 + 3 * self.pages)
         ws = torch.empty(size // 4, dtype=_I32, device=self.device)
         live = torch.empty(1, dtype=_I32, device=self.device)
         _launch("dsv41_kv4_compact", self.index, self._at, live.data_ptr(), ws.data_ptr(), size)
+        self._done()
         return live
 
     def copy_pages(self, other: "PagedKV4", src, dst) -> None:

@@ -404,7 +404,7 @@ int dsv41_kv4_reserve(const dsv41_kv4* c, const long* seq, const long* begin, co
                       long ws_bytes, void* stream);
 
 /* The live pages (refs > 0), L of them, moved to the front: those from L on go, in order, to the free ones before L; table
- * and refs follow.  live[0] = L. */
+ * and refs follow.  live[0] = L.  An entry behind L whose page has no count becomes -1 and is noted (bit 2). */
 long dsv41_kv4_compact_workspace_bytes(const dsv41_kv4* c);
 int dsv41_kv4_compact(const dsv41_kv4* c, int* live, void* ws, long ws_bytes, void* stream);
 

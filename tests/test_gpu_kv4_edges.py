@@ -126,3 +126,23 @@ def test_partial_results_stand_aligned(H, t):
     want = (w[..., None] * o).sum(1) / den[:, None]
     # (one rounding to bf16; the powers of two and the sums are off by 2^-20 of their terms)
     assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -18 * ring.double().abs().max()).all()
+
+
+# ------------------------------------------------------------------------------------------------ pages
+def test_compact_of_a_page_without_a_count():
+    """A table's entry whose page has no count names no page of another sequence afterwards, whatever the workspace held,
+    and is noted."""
+    from dsv41_amd._lib import lib
+    from dsv41_amd.kv4 import PagedKV4
+    pool = torch.randint(0, 256, (9, 16, 288), generator=_gen(1), dtype=torch.uint8).to(DEV)
+    table = torch.tensor([[6, 5, -1], [7, -1, 8]], dtype=torch.int32, device=DEV)
+    refs = torch.tensor([0, 0, 0, 0, 0, 1, 1, 0, 1], dtype=torch.int32, device=DEV)  # (page 7 is named, but not counted)
+    c = PagedKV4(pool.clone(), table.clone(), refs.clone(), dim=512)
+    size = lib().dsv41_kv4_compact_workspace_bytes(c._at)
+    ws = torch.ones(size // 4, dtype=torch.int32, device=DEV)
+    live = torch.zeros(1, dtype=torch.int32, device=DEV)
+    assert lib().dsv41_kv4_compact(c._at, live.data_ptr(), ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream) == 0
+    assert live.item() == 3 and c.table.tolist() == [[1, 0, -1], [-1, -1, 2]] and c.refs.tolist() == [1] * 3 + [0] * 6
+    assert torch.equal(c.pool[:3], pool[[5, 6, 8]])
+    with pytest.raises(RuntimeError, match="left out"):
+        c.check()
