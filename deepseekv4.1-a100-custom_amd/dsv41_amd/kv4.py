@@ -270,6 +270,8 @@ def _window(name: str, kv: torch.Tensor, dim: int) -> torch.Tensor:
         raise RuntimeError(f"{name}: window rows {tuple(kv.shape)} {kv.dtype} (bf16 [., ., {dim}])")
     if kv.stride(2) != 1 or kv.stride(1) != dim or kv.stride(0) % 8 or kv.data_ptr() % 16:
         kv = _aligned(kv.contiguous())
+        if kv.stride(0) % 8:  # (a batch of one has any stride)
+            kv = kv.view(-1).view(kv.shape)
     return kv
 
 
@@ -340,6 +342,8 @@ def sparse_attn4(q, kv, cache: PagedKV4, attn_sink, win_idxs, topk_idxs, softmax
     win_idxs, w = _indices("sparse_attn4", win_idxs, (b, s), index)
     if w and kv is None:
         raise RuntimeError("sparse_attn4: window indices without rows")
+    if kv is not None and kv.shape[1] == 0:  # (every index is past the end)
+        kv, win_idxs, w = None, None, 0
     idx, t = _indices("sparse_attn4", topk_idxs, (b, s), index)
     if seq is None and b > cache.slots:
         raise RuntimeError(f"sparse_attn4: {b} batch rows over {cache.slots} sequences")

@@ -146,3 +146,27 @@ def test_compact_of_a_page_without_a_count():
     assert torch.equal(c.pool[:3], pool[[5, 6, 8]])
     with pytest.raises(RuntimeError, match="left out"):
         c.check()
+
+
+# ------------------------------------------------------------------------------------------------ views
+def test_windows_of_one_batch_row_and_of_none():
+    """Window rows of one batch row (or ring) cut out of a wider buffer, whose batch stride is then any number; and a window
+    without rows beside a list."""
+    from dsv41_amd.kv4 import sattn4, sparse_attn4
+    g = _gen(13)
+    c, _ = _filled(g, [60], 576, 16)
+    q = torch.randn(1, 3, 16, 576, generator=g).to(BF).to(DEV)
+    sink = torch.zeros(16, device=DEV)
+    wide = torch.randn(128 * 576 + 4, generator=g).to(BF).to(DEV)
+    odd = wide.as_strided((1, 128, 576), (128 * 576 + 4, 576, 1))
+    assert odd.stride(0) % 8 and odd.is_contiguous()
+    idx = torch.randint(0, 60, (1, 3, 20), generator=g, dtype=torch.int32).to(DEV)
+    win = torch.randint(0, 128, (1, 3, 9), generator=g, dtype=torch.int32).to(DEV)
+    assert torch.equal(sparse_attn4(q, odd, c, sink, win, idx, 0.04), sparse_attn4(q, odd.clone(), c, sink, win, idx, 0.04))
+    one = torch.tensor([500], device=DEV)
+    step = lambda r: sattn4(q[:, :1], r, c, idx[:, :1], one, sink, None, None, 0, 0.04, one * 0, one)  # noqa: E731
+    assert torch.equal(step(odd), step(odd.clone()))
+    none = torch.zeros(1, 0, 576, dtype=BF, device=DEV)
+    want = sparse_attn4(q, None, c, sink, None, idx, 0.04)
+    assert torch.equal(sparse_attn4(q, none, c, sink, win, idx, 0.04), want) and want.any()
+    assert not sparse_attn4(q, none, c, sink, win, None, 0.04).any()
