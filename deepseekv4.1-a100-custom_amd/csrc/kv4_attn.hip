@@ -439,7 +439,7 @@ int run(Kv4AttnArgs& a, int dqk, int b, float scale, void* ws, long ws_bytes, hi
   void* const part = (char*)ws + p.list + p.rows;
   if (p.many) {
     const long l = (long)a.wt + a.t, n = rows / b, pages = rows >> a.map.shift;
-    if (a.win_rows + n >= (1L << 31) || pages + a.R >= (1L << 31)) return (int)hipErrorInvalidValue;
+    if (a.win_rows + n >= (1L << 31) || !kv4_grid_ok(pages + a.R)) return (int)hipErrorInvalidValue;
     int* const list = (int*)ws;
     void* const table = (char*)ws + p.list;
     kv4_unpack_launch(a, dqk, b, table, list, st);
@@ -457,7 +457,7 @@ int run(Kv4AttnArgs& a, int dqk, int b, float scale, void* ws, long ws_bytes, hi
   a.chunk = p.chunk;
   a.groups = p.groups;
   a.part = (float*)part;
-  if ((long)a.R * a.groups * a.nsplit >= (1L << 31) || (long)a.R * a.H >= (1L << 31)) return (int)hipErrorInvalidValue;
+  if (!kv4_grid_ok((long)a.R * a.groups * a.nsplit) || (p.nsplit > 1 && !kv4_grid_ok((long)a.R * a.H))) return (int)hipErrorInvalidValue;
   const unsigned grid = (unsigned)((long)a.R * a.groups * a.nsplit);
   if (dqk == 512)
     kv4_attn_kernel<512><<<grid, 256, 0, st>>>(a);

@@ -79,6 +79,9 @@ inline bool kv4_ok(const dsv41_kv4* c) {
          (long)c->pages * c->page < (1L << 31) && (c->dim == 512 || c->dim == 576);
 }
 
+// Whether a launch of so many workgroups of 256 stays under 2^32 lanes, the runtime's bound.
+inline bool kv4_grid_ok(long blocks) { return blocks < 1L << 24; }
+
 inline Kv4Table kv4_map(const dsv41_kv4& c) { return Kv4Table{c.table, c.slots, c.cols, c.pages, kv4_shift(c.page)}; }
 
 }  // namespace

@@ -386,14 +386,14 @@ PagesArgs pages_args(const dsv41_kv4& c) {
 }
 
 // A grid of a workgroup per entry and 256 columns.
-bool grid_ok(const dsv41_kv4* c) { return kv4_ok(c) && c->cols <= 256 * 65535; }
+bool grid_ok(const dsv41_kv4* c, int n) { return kv4_ok(c) && c->cols <= 256 * 65535 && n >= 0 && kv4_grid_ok(n); }
 
 }  // namespace
 
 extern "C" {
 
 int dsv41_kv4_fork(const dsv41_kv4* c, const long* src, const long* dst, const long* rows, int n, void* stream) {
-  if (!grid_ok(c) || n < 0) return (int)hipErrorInvalidValue;
+  if (!grid_ok(c, n)) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
   if (!src || !dst) return (int)hipErrorInvalidValue;
   PagesArgs a = pages_args(*c);
@@ -407,7 +407,7 @@ int dsv41_kv4_fork(const dsv41_kv4* c, const long* src, const long* dst, const l
 }
 
 int dsv41_kv4_release(const dsv41_kv4* c, const long* seq, const long* rows, int n, void* stream) {
-  if (!grid_ok(c) || n < 0) return (int)hipErrorInvalidValue;
+  if (!grid_ok(c, n)) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
   if (!seq) return (int)hipErrorInvalidValue;
   PagesArgs a = pages_args(*c);
@@ -463,7 +463,8 @@ long dsv41_kv4_copy_workspace_bytes(const dsv41_kv4* c, int n) { return n > kFew
 
 int dsv41_kv4_copy(const dsv41_kv4* c, const dsv41_kv4* other, const long* src, const long* dst, int n, void* ws,
                    long ws_bytes, void* stream) {
-  if (!kv4_ok(c) || !kv4_ok(other) || c->dim != other->dim || c->page != other->page || n < 0) return (int)hipErrorInvalidValue;
+  if (!kv4_ok(c) || !kv4_ok(other) || c->dim != other->dim || c->page != other->page || n < 0 || !kv4_grid_ok(n))
+    return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
   if (!src || !dst || (n > kFewCopies && (!ws || ((uintptr_t)ws & 3) || ws_bytes < dsv41_kv4_copy_workspace_bytes(c, n))))
     return (int)hipErrorInvalidValue;

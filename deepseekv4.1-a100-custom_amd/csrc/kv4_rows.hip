@@ -185,6 +185,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const RowsArgs a) {
   if (DIM == 576 && (lane >> 3) < n) *(uint4*)(out + (lane >> 3) * DIM + 512 + 8 * l) = kv4_bf16(ct, st);
 }
 
+long rows_blocks(long n) { return n / (4 * kRows) + (n % (4 * kRows) != 0); }
+
 void rows_args(RowsArgs& a, const dsv41_kv4& c, const long* seq, const long* row, long n) {
   a = RowsArgs{};
   a.seq = seq;
@@ -202,7 +204,7 @@ extern "C" {
 
 int dsv41_kv4_append(const dsv41_kv4* c, const void* x, long x_rstride, const long* seq, const long* row, long n,
                      int ratio, int by_pos, const float* cos_t, const float* sin_t, long n_pos, int rd, void* stream) {
-  if (!kv4_ok(c) || n < 0 || n >= (1L << 32)) return (int)hipErrorInvalidValue;
+  if (!kv4_ok(c) || n < 0 || !kv4_grid_ok(rows_blocks(n))) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
   if (!seq || !row || !x || ((uintptr_t)x & 15) || x_rstride < c->dim || x_rstride % 8 || ratio < 1 || rd < 0 ||
       rd > c->dim || (rd & 1) || (rd > 0 && (!cos_t || !sin_t)))
@@ -217,7 +219,7 @@ int dsv41_kv4_append(const dsv41_kv4* c, const void* x, long x_rstride, const lo
   a.sin_t = sin_t;
   a.n_pos = n_pos;
   a.rd = rd;
-  const unsigned grid = (unsigned)((n + 4 * kRows - 1) / (4 * kRows));
+  const unsigned grid = (unsigned)rows_blocks(n);
   if (c->dim == 512)
     kv4_append_kernel<512><<<grid, 256, 0, (hipStream_t)stream>>>(a);
   else
@@ -227,13 +229,13 @@ int dsv41_kv4_append(const dsv41_kv4* c, const void* x, long x_rstride, const lo
 }
 
 int dsv41_kv4_read(const dsv41_kv4* c, const long* seq, const long* row, long n, void* out, void* stream) {
-  if (!kv4_ok(c) || n < 0 || n >= (1L << 32)) return (int)hipErrorInvalidValue;
+  if (!kv4_ok(c) || n < 0 || !kv4_grid_ok(rows_blocks(n))) return (int)hipErrorInvalidValue;
   if (n == 0) return 0;
   if (!seq || !row || !out || ((uintptr_t)out & 15)) return (int)hipErrorInvalidValue;
   RowsArgs a;
   rows_args(a, *c, seq, row, n);
   a.out = (uint16_t*)out;
-  const unsigned grid = (unsigned)((n + 4 * kRows - 1) / (4 * kRows));
+  const unsigned grid = (unsigned)rows_blocks(n);
   if (c->dim == 512)
     kv4_read_kernel<512><<<grid, 256, 0, (hipStream_t)stream>>>(a);
   else

@@ -192,6 +192,7 @@ class PagedKV4:
         nothing is copied before reserve makes a shared page writable.  A destination may be named once and may not be a
         source of the same call."""
         n = _count(src)
+        _launchable("kv4.fork", n)
         src, dst = self._i64("kv4.fork", src, n), self._i64("kv4.fork", dst, n)
         rows = None if rows is None else self._i64("kv4.fork", rows, n)
         _launch("dsv41_kv4_fork", self.index, self._at, src.data_ptr(), dst.data_ptr(), ptr(rows), n)
@@ -200,6 +201,7 @@ class PagedKV4:
     def release(self, seq, rows=None) -> None:
         """The pages behind the first rows[i] rows (None: 0, all of them) of sequence seq[i] are given up."""
         n = _count(seq)
+        _launchable("kv4.release", n)
         seq = self._i64("kv4.release", seq, n)
         rows = None if rows is None else self._i64("kv4.release", rows, n)
         _launch("dsv41_kv4_release", self.index, self._at, seq.data_ptr(), ptr(rows), n)
@@ -227,8 +229,7 @@ class PagedKV4:
         if self._span[0] < other._span[1] and other._span[0] < self._span[1]:
             raise RuntimeError("kv4.copy_pages: the pools are one memory (fork and reserve share and copy within a pool)")
         n = _count(src)
-        if n >= 1 << 31:
-            raise RuntimeError(f"kv4.copy_pages: {n} pages")
+        _launchable("kv4.copy_pages", n)
         src, dst = self._i64("kv4.copy_pages", src, n), self._i64("kv4.copy_pages", dst, n)
         size = 4 * self.pages if n > _FEW_COPIES else 0  # (dsv41_kv4_copy_workspace_bytes)
         ws = torch.empty(size // 4, dtype=_I32, device=self.device) if size else None
@@ -238,6 +239,11 @@ class PagedKV4:
 
 def _count(t) -> int:
     return t.numel() if isinstance(t, torch.Tensor) else len(t)
+
+
+def _launchable(name: str, n: int) -> None:
+    if n >= 1 << 24:  # (a workgroup of 256 each: 2^32 lanes)
+        raise RuntimeError(f"{name}: {n} entries (at most {(1 << 24) - 1})")
 
 
 def _angles(name: str, cos, sin, rd: int, index: int):

@@ -362,7 +362,8 @@ int dsv41_gated_a8(const void* a8, const void* s8, const void* wg8, const void* 
 /* Compressed rows held as the codes of their grid (qmode 2 of dsv41_append_rows), in pages.  A row of `dim` values (512, or
  * 576 with the values in its first 512): 256 bytes of E2M1 codes, two a byte with the lower value in the lower four bits,
  * and 32 e4m3 scales, one per 16 values; for 576 then 32 bytes of codes and 4 of scales of the last 64 values and 12 zeros:
- * 288 (336) bytes.  Calls on one cache must be stream-ordered. */
+ * 288 (336) bytes.  Calls on one cache must be stream-ordered.  A call takes what one launch of under 2^32 lanes does: fork, release
+ * and copy 2^24 - 1 entries, append and read 2^27 - 8 rows, the attentions 2^24 - 1 workgroups of a query row and 16 heads. */
 typedef struct {
   void* pool;  /* [pages, page, row bytes], 16-byte aligned; pages * page < 2^31 */
   int* table;  /* [slots, cols]: the page of rows j * page .. of a sequence, -1 none (entries outside the pool: none) */
