@@ -95,9 +95,11 @@ class SparseAttention:
     o-projection.  Caches for `slots` sequences (batch row i is sequence i): ring [slots, window, D], compressed rows
     [slots, cap, D], index keys [slots, cap, 128] (bf16, the reference storage; with e4m3=True also an e4m3 copy +
     per-row scales, which the selection then reads), compressor rings [slots, 8, D].  With kv4, a kv4.PagedKV4 of rows of
-    head_dim (512), the compressed rows are held there in 4 bits instead: a call takes the pages that its rows need, and a
-    sequence's pages may be forked, released and compacted between calls; kv4.check() tells of a pool that ran out.  The
-    rows' values are the same."""
+    head_dim (512), the compressed rows are held there in 4 bits instead: a call takes the pages that its rows need, and
+    between calls the pool may be compacted and the pages of a sequence that is over released; kv4.check() tells of a pool
+    that ran out.  The rows' values are the same.  The other tables stay [slots, ...]: kv4.fork gives sequence dst the
+    compressed rows of src alone, so a fork of the whole sequence also copies row src of ring, index_k, k8, ks, ring_kv and
+    ring_score (those that there are) to row dst; both then go on from the same position."""
 
     def __init__(self, weights: dict, *, n_heads: int, head_dim: int, rope_head_dim: int, window: int, ratio: int,
                  index_n_heads: int, index_topk_k: int, cos: torch.Tensor, sin: torch.Tensor, slots: int, cap: int,

@@ -170,3 +170,34 @@ def test_windows_of_one_batch_row_and_of_none():
     want = sparse_attn4(q, None, c, sink, None, idx, 0.04)
     assert torch.equal(sparse_attn4(q, none, c, sink, win, idx, 0.04), want) and want.any()
     assert not sparse_attn4(q, none, c, sink, win, None, 0.04).any()
+
+
+# ------------------------------------------------------------------------------------------------ in the layer
+def test_attention_layer_forks_a_sequence():
+    """A sequence of the layer forked as its documentation says -- the pages by fork, the other tables' rows copied -- and
+    both go on apart, beside a layer over a bf16 table whose rows were all copied."""
+    from dsv41_amd.attention import SparseAttention
+    from dsv41_amd.kv4 import PagedKV4
+    g = _gen(91)
+    dim, q_rank, H, D, HI, cap = 256, 128, 20, 512, 16, 300
+    w = _layer_weights(g, dim, q_rank, H, D, HI)
+    cos, sin = (t.to(DEV) for t in _angles(2 * cap))
+    kw = dict(n_heads=H, head_dim=D, rope_head_dim=64, window=32, ratio=2, index_n_heads=HI, index_topk_k=60, cos=cos, sin=sin,
+              slots=2, cap=cap)
+    c = PagedKV4.empty(24, 2, cap, D, 32, DEV)
+    one, two = SparseAttention(w, **kw), SparseAttention(w, kv4=c, **kw)
+    x = torch.randn(2, 420, dim, generator=g).to(BF).to(DEV)
+    most = lambda: max(one.ckv.abs().max().item(), one.ring.abs().max().item(), 1.0)  # noqa: E731
+    _alike(two.attend(x[:, :301], 0), one.attend(x[:, :301], 0), most())
+    for lay in (one, two):
+        for t in (lay.ring, lay.index_k, lay.k8, lay.ks, lay.ring_kv, lay.ring_score):
+            t[1] = t[0]
+    one.ckv[1] = one.ckv[0]
+    c.fork([0], [1])
+    for lo, hi in ((301, 302), (302, 303), (303, 350), (350, 420)):
+        _alike(two.attend(x[:, lo:hi], lo), one.attend(x[:, lo:hi], lo), most())
+    c.check()
+    assert (c.refs > 1).any()  # (whole pages of the prefix are still shared)
+    n = 420 // 2
+    got = c.read(torch.arange(2, device=DEV).repeat_interleave(n), torch.arange(n, device=DEV).repeat(2)).view(2, n, D)
+    assert (got != one.ckv[:, :n]).any(-1).sum().item() <= 4  # (rotated in fp32 there, in 64 bits here)
