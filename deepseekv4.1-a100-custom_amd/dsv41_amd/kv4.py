@@ -5,7 +5,7 @@ E2M1 times an e4m3 scale per 16 -- stored in bf16.  PagedKV4 holds them as the g
 values and 336 a row of 576 instead of 1024 and 1152, in pages that sequences share:
 
   c = PagedKV4.empty(pages, slots, cap, dim)
-  c.reserve(seq, begin, end)             pages of their own for rows begin .. end - 1 (copied where they are shared)
+  c.reserve(seq, begin, end)             pages of their own for rows begin .. end - 1 (a shared page's rows before begin copied)
   c.append(latent, seq, row, ratio, cos, sin, rd)      (append_decode: the rows by the tokens' positions)
   o = sattn4(q, ring, c, idx, ...)       decode: fused2.sattn2 with the cache in the place of kv_c
   o = sparse_attn4(q, kv, c, sink, win_idxs, topk_idxs, scale)     prefill: kernels.sparse_attn with kv2 in 4 bits
@@ -175,8 +175,10 @@ class PagedKV4:
     # ---- pages
     def reserve(self, seq, begin, end) -> None:
         """Rows begin[i] .. end[i] - 1 of sequence seq[i] made writable: a page of its own wherever it has none or shares
-        one, the lowest free pages in the order of the arguments; where a shared page is replaced, its rows before
-        begin[i] are copied.  Distinct sequences, 4096 at most."""
+        one, the lowest free pages in the order of the arguments.  Where a shared page is replaced its rows before begin[i]
+        are copied, and no others: the sequence's rows from begin[i] to the end of the last replaced page are gone, those
+        from end[i] on too, and hold what the new page held until they are appended (a sequence that goes on reserves from
+        its length on).  Distinct sequences, 4096 at most."""
         n = _count(seq)
         if n > _MOST_ENTRIES:
             raise RuntimeError(f"kv4.reserve: {n} sequences (at most {_MOST_ENTRIES})")

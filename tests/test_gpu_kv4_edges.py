@@ -148,6 +148,27 @@ def test_compact_of_a_page_without_a_count():
         c.check()
 
 
+def test_reserve_keeps_the_rows_before_begin_alone():
+    """A shared page that is replaced keeps its rows before begin for the sequence; those from begin on are what the new
+    page held, until they are appended.  The other sequence's rows stay."""
+    from dsv41_amd.kv4 import PagedKV4
+    g = _gen(6)
+    c = PagedKV4.empty(8, 2, 64, 512, 32, DEV)
+    c.reserve([0], [0], [50])
+    x = _rows(g, 50, 512).to(DEV)
+    c.append(x, [0] * 50, list(range(50)), 1, None, None, 0)
+    was = c.read([0] * 50, list(range(50)))
+    c.fork([0], [1])
+    c.reserve([1], [10], [12])
+    y = _rows(g, 2, 512).to(DEV)
+    c.append(y, [1, 1], [10, 11], 1, None, None, 0)
+    got = c.read([1] * 50, list(range(50)))
+    assert torch.equal(got[:10], was[:10]) and torch.equal(got[32:], was[32:])  # (the second page is still shared)
+    assert torch.equal(got[10:12].double().cpu(), R.grid(y.double().cpu())[0]) and not got[12:32].any()
+    assert torch.equal(c.read([0] * 50, list(range(50))), was)
+    c.check()
+
+
 # ------------------------------------------------------------------------------------------------ views
 def test_windows_of_one_batch_row_and_of_none():
     """Window rows of one batch row (or ring) cut out of a wider buffer, whose batch stride is then any number; and a window
