@@ -193,6 +193,92 @@ def test_windows_of_one_batch_row_and_of_none():
     assert not sparse_attn4(q, none, c, sink, win, None, 0.04).any()
 
 
+# ------------------------------------------------------------------------------------------------ attention, row by row
+def _each(o, q, keys, sink, scale, splits=1):
+    """Every (row, head) by its own norm.  Probabilities in bf16 (2^-8 of each), partial results in bf16 where a row is split,
+    one rounding: 2^-8 |o| + splits 2^-8 sum p |v|; fp32 logits are off by 2^-20 of the largest, which adds that to every p.
+    keys[i]: the rows that query i sees, fp64."""
+    bad = 0
+    for i in range(len(q)):
+        x = torch.cat((q[i].double() @ keys[i].t() * scale, sink.double()[:, None]), 1)
+        p, v = x.softmax(1)[:, :-1], keys[i][:, :512]
+        ref = p @ v
+        rel = splits * 2.0 ** -8 + 2.0 ** -19 * x.abs().max()
+        bound = 2.0 ** -8 * ref.norm(dim=1) + rel * (p * v.norm(dim=1)).sum(1)
+        bad += int(((o[i].double().cpu() - ref).norm(dim=1) > bound).sum())
+    assert bad == 0
+
+
+@pytest.mark.parametrize("dim,heads,s,prior,t", [(576, 40, 530, 400, 256), (512, 16, 90, 900, 200), (576, 20, 40, 900, 100)])
+def test_prompt_row_by_row(dim, heads, s, prior, t):
+    """Sharp softmaxes, so that a few keys are most of each (row, head), at other places of the list for each: a wrong one
+    among them is more than the 2 % that its norm may be off by."""
+    from dsv41_amd.kv4 import sparse_attn4
+    g = _gen(s + heads)
+    n = (prior + s) // 4
+    c, (rows,) = _filled(g, [n], dim, 16)
+    q = torch.randn(1, s, heads, dim, generator=g).to(BF)
+    kv = (torch.randn(1, s, dim, generator=g) * 0.7).to(BF)
+    win = (torch.arange(s)[:, None] - torch.arange(100)).to(torch.int32)[None]
+    idx = torch.full((1, s, t), -1, dtype=torch.int32)
+    for i in range(s):
+        k = min(n, t)
+        idx[0, i, :k] = torch.randperm(n, generator=g)[:k].to(torch.int32)
+    sink = torch.randn(heads, generator=g)
+    o = sparse_attn4(q.to(DEV), kv.to(DEV), c, sink.to(DEV), win.clamp_min(-1).to(DEV), idx.to(DEV), 0.5)
+    keys = [torch.cat((kv[0].double()[win[0, i][win[0, i] >= 0].long()], rows[idx[0, i][idx[0, i] >= 0].long()])) for i in range(s)]
+    _each(o[0], q[0], keys, sink, 0.5, splits=2)
+
+
+@pytest.mark.parametrize("dim", [512, 576])
+def test_drafts_see_up_to_plim(dim):
+    """Rows of one sequence whose ring already holds later positions, each limited by its own plim: all of them, some, none."""
+    from dsv41_amd.kv4 import sattn4
+    g = _gen(dim + 5)
+    W, H, rd = 128, 20, 64 if dim == 512 else 0
+    c, rows = _filled(g, [260, 40], dim, 16)
+    pos = torch.tensor([600, 601, 602, 603, 90, 91, 127, 604])
+    seq = torch.tensor([0, 0, 0, 0, 1, 1, 1, 0])
+    pmax = torch.tensor([603, 603, 603, 603, 127, 127, 127, 603])
+    plim = torch.tensor([600, 601, 550, 603, 90, 40, -1, 500])
+    B = len(pos)
+    q = torch.randn(B, 1, H, dim, generator=g).to(BF)
+    ring = (torch.randn(2, W, dim, generator=g) * 0.7).to(BF)
+    idx = torch.stack([torch.randperm(40, generator=g)[:30] for _ in range(B)]).to(torch.int32).view(B, 1, 30)
+    sink = torch.randn(H, generator=g)
+    cos, sin = _angles(700)
+    D = lambda x: x.to(DEV)  # noqa: E731
+    call = lambda lim: sattn4(D(q), D(ring), c, D(idx), D(pos), D(sink), D(cos), D(sin), rd, 0.5, D(seq), D(pmax), lim)  # noqa: E731
+    o = call(D(plim))
+    keys, turned = [], o[:, 0].double().cpu()
+    for b in range(B):
+        e = int(seq[b])
+        seen = R.ring_slots(int(pos[b]), int(pmax[b]), int(plim[b]), W)
+        keys.append(torch.cat((ring[e][seen].double(), rows[e][idx[b, 0].long()])))
+        if rd:  # (turned back: a rotation keeps the norm that is looked at)
+            turned[b] = R.rotate(turned[b], cos, sin, int(pos[b]), rd)
+    assert len({len(k) for k in keys}) > 4
+    _each(turned, q[:, 0], keys, sink, 0.5)
+    assert torch.equal(call(None), call(D(pos))) and torch.equal(call(D(plim.to(torch.int32))), o)
+
+
+def test_positions_outside_the_rope_tables():
+    """The rotated columns of a row whose position has no angle are NaN; its others and the other rows are what they are."""
+    from dsv41_amd.kv4 import sattn4
+    g = _gen(17)
+    c, _ = _filled(g, [80], 512, 16)
+    q = torch.randn(4, 1, 16, 512, generator=g).to(BF).to(DEV)
+    ring = torch.randn(1, 128, 512, generator=g).to(BF).to(DEV)
+    idx = torch.randint(0, 80, (4, 1, 70), generator=g, dtype=torch.int32).to(DEV)
+    pos = torch.tensor([199, 200, 198, 1 << 30], device=DEV)
+    zero, sink = torch.zeros(4, dtype=torch.int64, device=DEV), torch.zeros(16, device=DEV)
+    run = lambda n: sattn4(q, ring, c, idx, pos, sink, *(t.to(DEV) for t in _angles(n)), 64, 0.04, zero, zero + 199)  # noqa: E731
+    o, plain = run(200)[:, 0], run(201)[:, 0]
+    assert torch.equal(torch.isnan(o).any(1).any(1).cpu(), torch.tensor([False, True, False, True]))
+    assert torch.isnan(o[[1, 3], :, 448:]).all() and torch.equal(o[..., :448], plain[..., :448])
+    assert torch.equal(o[[0, 2]], plain[[0, 2]]) and torch.isfinite(plain[1]).all()
+
+
 # ------------------------------------------------------------------------------------------------ in the layer
 def test_attention_layer_forks_a_sequence():
     """A sequence of the layer forked as its documentation says -- the pages by fork, the other tables' rows copied -- and

@@ -43,3 +43,20 @@ def test_launches_of_too_many_lanes_are_refused():
             h._span, other._span = (0, 10), (10, 20)
             with pytest.raises(RuntimeError, match="at most"):
                 call()
+
+
+# (rows, heads, list, window, rows of the cache's tables) of prompts whose cache is decoded first, and of some just short of it
+FIRST = [(530, 33, 256, 100, 256), (530, 64, 256, 1, 256), (530, 80, 250, 37, 256), (531, 64, 257, 128, 2016), (130, 64, 1025, 128, 2304),
+         (68, 128, 2000, 64, 2176), (520, 40, 260, 0, 416)]
+DIRECT = [(530, 32, 256, 100, 256), (150, 33, 512, 128, 650), (15, 64, 9000, 128, 416), (530, 64, 256, 100, 40000), (65529, 64, 256, 1, 256)]
+
+
+@pytest.mark.parametrize("first,args", [(True, a) for a in FIRST] + [(False, a) for a in DIRECT])
+def test_which_prompts_are_decoded_first(first, args):
+    """More than 32 heads, 16 to 65528 query rows, 2^18 keys of 16 heads, and each row of the cache's tables listed four times: the
+    workspace then holds the tables' rows in bf16 (else the splits' partial results, of few rows)."""
+    rows, heads, t, w, held = args
+    c = ctypes.byref(_struct(dim=576, page=16, pages=4096, slots=1, cols=held // 16))
+    n = _lib.lib().dsv41_kv4_attn_workspace_bytes(c, rows, heads, w, t, 1)
+    decoded = held // 16 * 16 * 576 * 2
+    assert n >= decoded + rows * (w + t) * 4 if first else n % (4 * rows * heads * 514) == 0
