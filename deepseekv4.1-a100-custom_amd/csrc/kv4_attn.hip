@@ -11,7 +11,8 @@
 // at most, a logit by less than fp32's own rounding of a sum with that one).  Window rows have bf16's range, so they stay
 // in bf16.
 // Sums, the softmax's maximum and sum and O are fp32; the reference maximum moves only for a score 2^8 above it; the
-// probabilities are rounded to fp16 (bf16 for window rows), the operand type, and the output once, after the rotation.
+// probabilities are rounded to fp16 (2^-11 of each; bf16 for window rows, whose values need its range: 2^-8), the operand type
+// of the products, and the output once, after the rotation.
 // Of a cache's rows the reference is 2^7 under the maximum, so that the largest probability is 2^7 to 2^15 and fp16's last
 // bit, 2^-24, is 2^-31 of it or less: n keys of a long flat rest are off by n 2^-32 of the peak's weight together (with the
 // maximum as the reference weights under 2^-25 were lost, 2^18 of them 0.5 % of the numerator).
@@ -418,8 +419,9 @@ Plan plan_of(int R, int H, int wt, int t, int dim, long rows) {
   p.tiles = p.wtiles + (t + 63) / 64;
   if (p.tiles == 0) p.tiles = 1;  // (no key at all: zeros)
   // Splits until each of the card's CUs has a workgroup, two where one would have more than 12 tiles: before, two cost more
-  // in partial results than they hide (64 heads, 34 tiles: 4 sequences 18.4 us and 20.6, 16 27.9 and 29.9, 32 42.1 and 37.7).
-  // Of more than 16 tiles no split has a single one (1 sequence 15.3 us for 17.8; 10 tiles 12.3 for 11.7).
+  // in partial results than they hide (64 heads, 34 tiles: 4 sequences 17.3 us and 20.0, 16 27.1 and 29.0, 32 41.8 and 37.9).
+  // Of more than 16 tiles no split has a single one (1 sequence 14.7 us for 16.2; 10 tiles 11.7 for 10.8).
+  // (rows: what the tables have room for, whether or not pages are there: how many are is known on the device alone.)
   const long units = (long)R * p.groups, most = p.tiles > 16 ? (p.tiles + 1) / 2 : p.tiles;
   long ns = (256 + units - 1) / units;
   if (p.tiles > 12 * ns) ns = (512 + units - 1) / units;

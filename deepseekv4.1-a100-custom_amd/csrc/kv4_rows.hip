@@ -33,10 +33,10 @@ struct RowsArgs {
 
 // The grid's scale of 16 values and the codes of this lane's eight.  bf16 values over a 4-bit significand often lie on a
 // border of the grid, where the even code is right, so a quotient may not be off there.  Quotients are products with a
-// reciprocal (two fp32 roundings) rounded to bf16: one that is a border comes out as the border, which has 3 bits (the
-// scale's 5); any other is at least 2^-8 of itself away from one -- two integers of at most 8 bits that differ -- and bf16
-// moves it by 2^-9.  The conversions round to even and saturate: the scale at 448, the codes at 6.  A group with an
-// infinity or a NaN reads back as NaN (scale 0x7f).
+// reciprocal (off by 2^-22 of themselves) rounded to bf16: one that is a border comes out as the border, which has 3 bits (the
+// scale's 5).  Any other is at least 1/254 of a border away from it: the value, and the border times the divisor (of 7 bits,
+// so even at 8), are two integers of 8 bits that differ; bf16 moves it by 2^-8 of the border at most.  The conversions round
+// to even and saturate: the scale at 448, the codes at 6.  A group with an infinity or a NaN reads back as NaN (scale 0x7f).
 DSV41_DEV uint32_t kv4_encode(const float* v, uint8_t* scale) {
   uint32_t top = 0;  // the largest magnitude's bits: a NaN's are above an infinity's
 #pragma unroll

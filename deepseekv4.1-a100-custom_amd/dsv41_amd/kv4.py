@@ -16,8 +16,12 @@ values and 336 a row of 576 instead of 1024 and 1152, in pages that sequences sh
 
 Every call is asynchronous on the current stream, synchronises with nothing and may be captured; calls on one cache must
 be stream-ordered.  Index arguments are tensors or lists (captured calls: tensors on the GPU); host memory may be filled
-anew when a call returns.  What a call cannot do on the device -- too few free pages, an index out of range, a row without a page --
-it leaves out and notes in the cache's error word, which check() raises for (every call does with DSV41_CHECK_ERRORS=1).
+anew when a call returns.  What a call that writes (append, reserve, fork, release, compact, copy_pages) cannot do on the
+device -- too few free pages, an index out of range, a row without a page -- it leaves out and notes in the cache's error
+word, which check() raises for (every such call does with DSV41_CHECK_ERRORS=1).  To read and to the attentions a row that
+is not there is none: zeros, no key, no note.
+
+A PagedKV4 is a handle to keep: making one checks its tensors and clears an error word (a few launches' time).
 
 Forward only, as everything here."""
 from __future__ import annotations
@@ -339,7 +343,9 @@ def sparse_attn4(q, kv, cache: PagedKV4, attn_sink, win_idxs, topk_idxs, softmax
 
     q [b, s, h, dim] bf16; kv [b, n, dim] bf16 window rows and win_idxs [b, s, w] into them; topk_idxs [b, s, t] rows of the
     cache's sequence seq[i] of batch row i (None: i); -1 (or past the end, or without a page) is none, and either list may
-    be None.  Returns [b, s, h, 512] bf16, rounded once; a query that sees no key is zeros."""
+    be None.  Returns [b, s, h, 512] bf16, rounded once; a query that sees no key is zeros.  Where many queries of more than
+    32 heads list more than four times the rows that the b sequences' tables have room for, these are decoded to bf16 first, in
+    a workspace of 2 * dim bytes a row, mapped or not."""
     b, s, h, d = q.shape
     _values_of("sparse_attn4", d_v)
     index, q, sink = _operands("sparse_attn4", q, cache, attn_sink, h, kv)

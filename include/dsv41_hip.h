@@ -416,7 +416,9 @@ int dsv41_kv4_copy(const dsv41_kv4* c, const dsv41_kv4* other, const long* src, 
                    long ws_bytes, void* stream);
 
 /* Workspace of the two attention calls: R query rows, H heads, wt window (or ring) rows and t cache rows a query, b batch
- * rows of dsv41_sparse_attn4 (0 for dsv41_sattn4).  Needs no zeroing and no life beyond the call; 16-byte aligned. */
+ * rows of dsv41_sparse_attn4 (0 for dsv41_sattn4): the splits' partial results, or, where many queries have the cache decoded
+ * first (H > 32, R * t >= 4 rows of the tables), the lists and b * cols * page rows in bf16, mapped or not: a table for 262144
+ * rows takes 320 MB of 2048 queries, one for 16960 37 MB.  Needs no zeroing and no life beyond the call; 16-byte aligned. */
 long dsv41_kv4_attn_workspace_bytes(const dsv41_kv4* c, int R, int H, int wt, int t, int b);
 
 /* dsv41_sattn2 over a 4-bit cache: query row b at position pos[b] of sequence seq[b] over the ring kv_win[seq] (bf16
