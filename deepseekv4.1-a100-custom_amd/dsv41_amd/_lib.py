@@ -182,11 +182,12 @@ def as_i64(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
 
 
 def to_i64(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
-    """t as contiguous int64 on GPU dev, asynchronously.  A copy out of pinned memory is still to come when the call
-    returns, and its owner may fill it for the next step by then: its entries go by way of other host memory, which the
-    runtime has read when a copy returns.  (A captured copy reads the pinned memory at every replay, as it is meant to.)"""
+    """t as contiguous int64 on GPU dev.  A copy out of pinned memory is still to come when the call returns, and its owner
+    may fill it for the next step by then: its entries go by way of pinned memory of torch's, which keeps it until the copy
+    is done.  (A captured copy reads the owner's at every replay, as it is meant to.)  Out of other host memory the runtime
+    has copied when the call returns; for many entries it waits for the stream."""
     if not t.is_cuda and t.is_pinned() and not torch.cuda.is_current_stream_capturing():
-        t = t.clone()
+        t = torch.empty(t.shape, dtype=torch.int64, pin_memory=True).copy_(t)
     return t.to(device=dev, dtype=torch.int64, non_blocking=True).contiguous()
 
 

@@ -16,10 +16,10 @@ values and 336 a row of 576 instead of 1024 and 1152, in pages that sequences sh
 
 Every call is asynchronous on the current stream, synchronises with nothing and may be captured; calls on one cache must
 be stream-ordered.  Index arguments are tensors or lists (captured calls: tensors on the GPU); host memory may be filled
-anew when a call returns.  What a call that writes (append, reserve, fork, release, compact, copy_pages) cannot do on the
-device -- too few free pages, an index out of range, a row without a page -- it leaves out and notes in the cache's error
-word, which check() raises for (every such call does with DSV41_CHECK_ERRORS=1).  To read and to the attentions a row that
-is not there is none: zeros, no key, no note.
+anew when a call returns (many entries that are not in pinned memory are waited for).  What a call that writes (append,
+reserve, fork, release, compact, copy_pages) cannot do on the device -- too few free pages, an index out of range, a row
+without a page -- it leaves out and notes in the cache's error word, which check() raises for (every such call does with
+DSV41_CHECK_ERRORS=1).  To read and to the attentions a row that is not there is none: zeros, no key, no note.
 
 A PagedKV4 is a handle to keep: making one checks its tensors and clears an error word (a few launches' time).
 

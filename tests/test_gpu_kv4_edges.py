@@ -43,6 +43,22 @@ def test_rows_go_where_a_pinned_index_said():
     assert c.read([0, 0, 0, 0], [3, 20, 40, 41]).eq(6).all(1).tolist() == [True, True, False, False]
 
 
+def test_pinned_indices_of_queued_calls_stay_apart():
+    """Many calls queued behind a busy stream, from one pinned buffer: asynchronous, and each has its own entries."""
+    from dsv41_amd.kv4 import PagedKV4
+    c = PagedKV4.empty(2, 1, 32, 512, 16, DEV)
+    busy, t = torch.randn(4096, 4096, device=DEV), torch.empty(1 << 16, dtype=torch.int64).pin_memory()
+    c._i64("x", t, len(t))
+    torch.cuda.synchronize()
+    for _ in range(300):
+        busy @ busy
+    done = torch.cuda.Event()
+    done.record()
+    got = [c._i64("x", t.fill_(k), len(t)) for k in range(8)]
+    assert not done.query()  # (none of them waited)
+    assert [(int(g.min()), int(g.max())) for g in got] == [(k, k) for k in range(8)]
+
+
 @pytest.mark.parametrize("dtype", [torch.int64, torch.int16, torch.int8, torch.uint8])
 def test_attention_takes_any_integer_list(dtype):
     from dsv41_amd.kv4 import sparse_attn4
