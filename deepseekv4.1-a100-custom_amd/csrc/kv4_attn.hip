@@ -405,6 +405,7 @@ Plan plan_of(int R, int H, int wt, int t, int dim, long rows) {
   // keys: 64 heads 183 us for 303, 33 heads 180 for 229, 32 heads 180 for 158), from 2^18 keys of 16 heads each on (602
   // query rows of 512 keys: 64 heads 99 us for 118, 48 and 33 heads 96 for 94; 150 rows, 64 heads 37.3 for 41.6, 33 heads 35.7
   // for 27.8; 32 rows of 2048 39.6 for 40.6, 16 of them 36.7 for 27.5) and with each row of the cache listed four times.
+  // (rows: what the tables have room for, whether or not pages are there: how many are is known on the device alone.)
   // (From 16 query rows on the bf16 kernel joins its splits by a kernel of its own; its grid ends at 65535.)
   p.groups = (H + 15) / 16;
   p.many = rows > 0 && H > 32 && R >= 16 && R <= 65528 && (long)R * t * p.groups >= 1L << 18 && (long)R * t >= 4 * rows &&
@@ -421,7 +422,6 @@ Plan plan_of(int R, int H, int wt, int t, int dim, long rows) {
   // Splits until each of the card's CUs has a workgroup, two where one would have more than 12 tiles: before, two cost more
   // in partial results than they hide (64 heads, 34 tiles: 4 sequences 17.3 us and 20.0, 16 27.1 and 29.0, 32 41.8 and 37.9).
   // Of more than 16 tiles no split has a single one (1 sequence 14.7 us for 16.2; 10 tiles 11.7 for 10.8).
-  // (rows: what the tables have room for, whether or not pages are there: how many are is known on the device alone.)
   const long units = (long)R * p.groups, most = p.tiles > 16 ? (p.tiles + 1) / 2 : p.tiles;
   long ns = (256 + units - 1) / units;
   if (p.tiles > 12 * ns) ns = (512 + units - 1) / units;

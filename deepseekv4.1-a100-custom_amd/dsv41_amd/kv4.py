@@ -180,9 +180,8 @@ class PagedKV4:
     def reserve(self, seq, begin, end) -> None:
         """Rows begin[i] .. end[i] - 1 of sequence seq[i] made writable: a page of its own wherever it has none or shares
         one, the lowest free pages in the order of the arguments.  Where a shared page is replaced its rows before begin[i]
-        are copied, and no others: the sequence's rows from begin[i] to the end of the last replaced page are gone, those
-        from end[i] on too, and hold what the new page held until they are appended (a sequence that goes on reserves from
-        its length on).  Distinct sequences, 4096 at most."""
+        are copied, and no others: the rest of the page, from end[i] on too, holds what the new page held until rows are
+        appended there (a sequence that goes on reserves from its length on).  Distinct sequences, 4096 at most."""
         n = _count(seq)
         if n > _MOST_ENTRIES:
             raise RuntimeError(f"kv4.reserve: {n} sequences (at most {_MOST_ENTRIES})")
