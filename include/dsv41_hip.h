@@ -399,7 +399,8 @@ int dsv41_kv4_release(const dsv41_kv4* c, const long* seq, const long* rows, int
 
 /* Rows begin[i] .. end[i] - 1 of sequence seq[i] made writable: a page of its own wherever it has none or shares one (by
  * the counts at the call), the lowest free pages in the order of the arguments; what a replaced first page held before
- * begin[i] is copied, nothing else: the rest of a replaced page, behind end[i] too, is what the new page held.  Up to 4096 entries a call, distinct sequences (a repeated one is left out). */
+ * begin[i] is copied, nothing else: the rest of a replaced page, behind end[i] too, is what the new page held.  Up to 4096
+ * entries a call, distinct sequences (a repeated one is left out). */
 long dsv41_kv4_reserve_workspace_bytes(const dsv41_kv4* c, int n);
 int dsv41_kv4_reserve(const dsv41_kv4* c, const long* seq, const long* begin, const long* end, int n, void* ws,
                       long ws_bytes, void* stream);
